@@ -14,7 +14,8 @@ A page holds, for each layer and head of dk dimensions (32, 64, 96 or 128), a re
 
 A half byte is a sign (8) and one of the eight levels 0, 1/2, 1, 3/2, 2, 3, 4, 6, times the scale of its frame and head:
 the least bfloat16 whose six-fold is no less than the largest magnitude. The nearest level is taken, of two as near the
-one with the even code. A head that holds a NaN or an infinity, or nothing of 2^-121 or more, is kept as zeros.
+one with the even code. A head that holds a NaN or anything of 2^127 or more, or nothing of 2^-121 or more, is kept as
+zeros.
 
 The attention is the encoder's: frame i at position pos_i scores frame j by
 
@@ -213,7 +214,7 @@ def _rounded(x, dk):
     """The values that x's heads of dk are kept as."""
     a = x.reshape(x.shape[0], -1, dk)
     top = a.abs().amax(-1, keepdim=True)
-    fine = torch.isfinite(a).all(-1, keepdim=True) & (top >= 2.0 ** -121)
+    fine = (top >= 2.0 ** -121) & (top < 2.0 ** 127)
     top = torch.where(fine, top, 1.0)
     d = (top / 6).view(torch.int32) & -65536        # a bfloat16 no more than a step from the scale; the least that holds
     d = torch.where(6 * d.view(torch.float32) >= top, d - 65536, d)
