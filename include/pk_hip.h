@@ -12,7 +12,7 @@
  * This library computes both on the GPU with the reference's bits: the int8
  * activations, their scales and every fp32 output are those of the
  * reference's scalar ref backend (backend/ref/kernels.c:24-86) on the same
- * inputs. The entry points come in five groups:
+ * inputs. The entry points come in six groups:
  *
  *   1. the drop-in: pk_hip_quantize and pk_hip_gemm_q8 take host pointers and
  *      the arguments of the table's quantize and gemm_q8, and return with the
@@ -26,7 +26,11 @@
  *      between its products, fused with their quantizes, and a whole layer
  *      in one call (core/encoder.c:108-368);
  *   5. the decoder's token steps: its T = 1 products fused into one launch a
- *      step (core/decoder.c:54-101).
+ *      step (core/decoder.c:54-101);
+ *   6. the cache of keys and values, for streams of live audio: the encoder's
+ *      attention over frames kept in 4 bits between calls. Its outputs are
+ *      computed in 32 bits, not held to a bit pattern (the reference has no
+ *      cache).
  *
  * Every function returns PK_HIP_OK or an error code (pk_hip_strerror names it,
  * pk_hip_last_error gives the calling thread's last message); nothing falls
@@ -390,6 +394,133 @@ typedef struct {
 size_t pk_hip_search_workspace(const pk_hip_decoder *d, uint32_t cap);
 int pk_hip_search_dev(const pk_hip_decoder *d, const float *f, uint32_t T, int32_t *toks, uint32_t cap,
                       uint32_t *ntoks, void *ws, size_t ws_bytes, uint32_t spin_limit, void *stream);
+
+/* ------------------------------------- the cache of keys and values --- */
+
+/* A stream of live audio is encoded a chunk of frames at a time, and each
+ * chunk attends to the frames before it, whose keys and values are kept here
+ * between the calls, in 4 bits and in pages. The reference has no counterpart
+ * (it encodes a segment in one piece, core/encoder.c:280-327); the attention
+ * is that one's, restricted to a window and run over many streams in a call.
+ *
+ * A page holds PK_HIP_CACHE_PAGE frames of one stream, in every layer and
+ * head; which page holds which frames is the caller's table (one table a
+ * stream serves all layers). The pool of pages is the caller's device memory,
+ * 16-byte aligned, pk_hip_cache_bytes long, its contents of no matter before
+ * they are written: layers x pages x heads records of 64 dk + 256 bytes, dk =
+ * 32, 64, 96 or 128 (csrc/cache_layout.h has a record's layout). heads is the
+ * number of kept heads; an attention of H heads, H a multiple of it, shares
+ * each among H / heads consecutive ones.
+ *
+ * A kept value is one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 with a sign, times the
+ * scale of its frame and head: the least bfloat16 whose six-fold is no less
+ * than the head's largest magnitude. The nearest one is kept (of two as near,
+ * the one with the even code). A head with a NaN, an infinity or a magnitude
+ * of 2^127 or more, or with none of 2^-121 or more, is kept as zeros. */
+#define PK_HIP_CACHE_PAGE 64
+typedef struct {
+    void     *data;
+    uint32_t  layers, pages, heads, dk;
+} pk_hip_cache;
+/* 0 for sizes that are not taken */
+size_t pk_hip_cache_bytes(uint32_t layers, uint32_t pages, uint32_t heads, uint32_t dk);
+
+/* The streams of a call, B of them, with the call's rows of all streams one
+ * after another. Device memory, read when the kernels run, so that a captured
+ * graph follows the streams as they grow:
+ *   table  [B][max_pages]: page of the stream's frames [64 i, 64 i + 64) in
+ *          entry i. An entry outside [0, pages) is a hole: its frames are not
+ *          written, read as zeros and not attended (a page given up for a
+ *          limited context).
+ *   len    [B]: the stream's frames before this call's
+ *   row0   [B + 1]: stream b's rows are [row0[b], row0[b + 1]), its frames
+ *          [len[b], len[b] + T) with T = row0[b + 1] - row0[b], which may be 0
+ * rows is the call's number of rows and max_T at least the longest stream's T
+ * (rows a stream has beyond max_T or beyond rows take no part, and frames
+ * past 64 max_pages have no page). Rows of no stream are left as they were.
+ * No two streams of a call may write one page. max_pages up to 2^24, B up to
+ * 65535, rows up to 2^22. */
+typedef struct {
+    const int32_t *table, *len, *row0;
+    uint32_t B, max_pages, rows, max_T;
+} pk_hip_streams;
+
+/* Writes the rows' keys and values, k and v [rows][heads * dk] (row r at k + r
+ * ks, v + r vs), as the streams' frames [len, len + T) of one layer. k and v
+ * 16-byte aligned, ks and vs multiples of 4. The other frames of a page keep
+ * their values. */
+int pk_hip_cache_append_dev(const pk_hip_cache *c, uint32_t layer, const float *k, size_t ks, const float *v,
+                            size_t vs, const pk_hip_streams *st, void *stream);
+
+/* The values kept for the streams' frames [len, len + T), into k and v (as
+ * above): zeros for a hole's frames. */
+int pk_hip_cache_read_dev(const pk_hip_cache *c, uint32_t layer, float *k, size_t ks, float *v, size_t vs,
+                          const pk_hip_streams *st, void *stream);
+
+/* The attention's positions: p [n][H * dk], the projected position of
+ * distance r = (row's frame - attended frame) in row center - r (the encoder's
+ * order, center T - 1 for a segment of T, core/encoder.c:280-327), and the
+ * biases u and w [H * dk] of the content and the position scores. Device
+ * pointers, 16-byte aligned. */
+typedef struct {
+    const float *p, *bias_u, *bias_w;
+    uint32_t n, center;
+} pk_hip_positions;
+
+#define PK_HIP_UNLIMITED 0xffffffffu
+
+/* The attention of the call's rows, q [rows][H * dk] (row r at q + r qs), to
+ * the frames kept for their streams in one layer, their own among them (append
+ * them first), o likewise. The row of frame t attends frames [t - left, t +
+ * right] of those its stream has, [0, len + T): right 0 is causal,
+ * PK_HIP_UNLIMITED the whole chunk. Scores are
+ *   ((q + u) . k + (q + w) . p[center - (t - j)]) / sqrt(dk)
+ * or q . k / sqrt(dk) with pos NULL. With pos, distances that p has no row for
+ * are not attended: left is at most center, right at most n - 1 - center. A
+ * row that attends nothing is zeros. o and q 16-byte aligned, os and qs
+ * multiples of 4; o may be q with os = qs. ws: pk_hip_attention_cache_workspace(...) bytes of device
+ * memory (of the same cache, streams' counts, H, pos, left and right),
+ * 16-byte aligned, of no matter before and after; calls that overlap in time
+ * need workspaces of their own. Products and sums in 32 bits. */
+size_t pk_hip_attention_cache_workspace(const pk_hip_cache *c, const pk_hip_streams *st, uint32_t H,
+                                        const pk_hip_positions *pos, uint32_t left, uint32_t right);
+int pk_hip_attention_cache_dev(float *o, size_t os, const float *q, size_t qs, const pk_hip_cache *c, uint32_t layer,
+                               const pk_hip_streams *st, uint32_t H, const pk_hip_positions *pos, uint32_t left,
+                               uint32_t right, void *ws, size_t ws_bytes, void *stream);
+
+/* Copies pages in every layer: pairs (host, 2 n) of a page of src and the page
+ * of dst it goes to; src and dst have the same layers, heads and dk and may be
+ * one cache. A fork copies a stream's last page, a compaction moves pages
+ * down. With table (device, entries of it), entries that name a page moved
+ * become the page it went to, as a compaction's streams need (src and dst one
+ * cache, then). Refused: ids outside the pools, a page copied to twice, a page
+ * both copied from and to, and with a table a page moved twice. */
+int pk_hip_cache_move_dev(const pk_hip_cache *dst, const pk_hip_cache *src, const int32_t *pairs, uint32_t n,
+                          int32_t *table, size_t entries, void *stream);
+
+/* Which pages of a pool are in use, on the host (no device needed): each page
+ * has a count of the streams that hold it. Safe from several threads.
+ *   alloc    n pages nobody holds, the lowest, into ids; PK_HIP_ENOMEM and
+ *            nothing taken if fewer are free
+ *   share    one more holder for each of ids (a fork's whole pages)
+ *   release  one fewer; a page without holders is free. Ids that are not held
+ *            are refused, and then nothing is changed (an id may be named as
+ *            often as it has holders)
+ *   holders  a page's count; 0 for a free page or an id outside the pool
+ *   compact  the pairs (from, to) that move every page in use below the
+ *            number in use, at most cap of them; the pool's own counts move at
+ *            once, so the caller's next calls are pk_hip_cache_move_dev with
+ *            them and the tables (in stream order before any later write).
+ *            Returns how many in *n. */
+typedef struct pk_hip_pool pk_hip_pool;
+int pk_hip_pool_create(pk_hip_pool **pool, uint32_t pages);
+void pk_hip_pool_destroy(pk_hip_pool *pool);
+uint32_t pk_hip_pool_free_pages(const pk_hip_pool *pool);
+int pk_hip_pool_alloc(pk_hip_pool *pool, int32_t *ids, uint32_t n);
+int pk_hip_pool_share(pk_hip_pool *pool, const int32_t *ids, uint32_t n);
+int pk_hip_pool_release(pk_hip_pool *pool, const int32_t *ids, uint32_t n);
+uint32_t pk_hip_pool_holders(const pk_hip_pool *pool, int32_t id);
+int pk_hip_pool_compact(pk_hip_pool *pool, int32_t *pairs, uint32_t cap, uint32_t *n);
 
 /* Measurement aids, with no counterpart in the reference: the floors a
  * small product's time is read against. pk_hip_empty_dev launches an empty

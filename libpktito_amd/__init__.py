@@ -71,6 +71,28 @@ class Decoder(ctypes.Structure):
                 ("jpred_b", ctypes.c_void_p), ("jout_b", ctypes.c_void_p)]
 
 
+class Cache(ctypes.Structure):
+    """pk_hip_cache: a pool of pages of keys and values in 4 bits."""
+    _fields_ = [("data", ctypes.c_void_p), ("layers", ctypes.c_uint32), ("pages", ctypes.c_uint32),
+                ("heads", ctypes.c_uint32), ("dk", ctypes.c_uint32)]
+
+
+class Streams(ctypes.Structure):
+    """pk_hip_streams: the streams of a call on a cache."""
+    _fields_ = [("table", ctypes.c_void_p), ("len", ctypes.c_void_p), ("row0", ctypes.c_void_p),
+                ("B", ctypes.c_uint32), ("max_pages", ctypes.c_uint32), ("rows", ctypes.c_uint32),
+                ("max_T", ctypes.c_uint32)]
+
+
+class Positions(ctypes.Structure):
+    """pk_hip_positions: an attention's projected positions and biases."""
+    _fields_ = [("p", ctypes.c_void_p), ("bias_u", ctypes.c_void_p), ("bias_w", ctypes.c_void_p),
+                ("n", ctypes.c_uint32), ("center", ctypes.c_uint32)]
+
+
+CACHE_PAGE = 64
+UNLIMITED = 0xffffffff
+
 _F32P = ctypes.c_void_p
 LAYER_VECTORS = ("ff1_nw", "ff1_nb", "att_nw", "att_nb", "conv_nw", "conv_nb", "ff2_nw", "ff2_nb", "out_nw",
                  "out_nb")
@@ -161,6 +183,32 @@ _SIGS = {
     "pk_hip_search_dev": (ctypes.c_int, [ctypes.POINTER(Decoder), ctypes.c_void_p, ctypes.c_uint32,
                                          ctypes.c_void_p, ctypes.c_uint32, ctypes.POINTER(ctypes.c_uint32),
                                          ctypes.c_void_p, ctypes.c_size_t, ctypes.c_uint32, ctypes.c_void_p]),
+    "pk_hip_cache_bytes": (ctypes.c_size_t, [ctypes.c_uint32] * 4),
+    "pk_hip_cache_append_dev": (ctypes.c_int, [ctypes.POINTER(Cache), ctypes.c_uint32, ctypes.c_void_p,
+                                               ctypes.c_size_t, ctypes.c_void_p, ctypes.c_size_t,
+                                               ctypes.POINTER(Streams), ctypes.c_void_p]),
+    "pk_hip_cache_read_dev": (ctypes.c_int, [ctypes.POINTER(Cache), ctypes.c_uint32, ctypes.c_void_p,
+                                             ctypes.c_size_t, ctypes.c_void_p, ctypes.c_size_t,
+                                             ctypes.POINTER(Streams), ctypes.c_void_p]),
+    "pk_hip_attention_cache_workspace": (ctypes.c_size_t, [ctypes.POINTER(Cache), ctypes.POINTER(Streams),
+                                                           ctypes.c_uint32, ctypes.POINTER(Positions),
+                                                           ctypes.c_uint32, ctypes.c_uint32]),
+    "pk_hip_attention_cache_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_size_t,
+                                                  ctypes.POINTER(Cache), ctypes.c_uint32, ctypes.POINTER(Streams),
+                                                  ctypes.c_uint32, ctypes.POINTER(Positions), ctypes.c_uint32,
+                                                  ctypes.c_uint32, ctypes.c_void_p, ctypes.c_size_t,
+                                                  ctypes.c_void_p]),
+    "pk_hip_cache_move_dev": (ctypes.c_int, [ctypes.POINTER(Cache), ctypes.POINTER(Cache), ctypes.c_void_p,
+                                             ctypes.c_uint32, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "pk_hip_pool_create": (ctypes.c_int, [ctypes.POINTER(ctypes.c_void_p), ctypes.c_uint32]),
+    "pk_hip_pool_destroy": (None, [ctypes.c_void_p]),
+    "pk_hip_pool_free_pages": (ctypes.c_uint32, [ctypes.c_void_p]),
+    "pk_hip_pool_alloc": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32]),
+    "pk_hip_pool_share": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32]),
+    "pk_hip_pool_release": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32]),
+    "pk_hip_pool_holders": (ctypes.c_uint32, [ctypes.c_void_p, ctypes.c_int32]),
+    "pk_hip_pool_compact": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32,
+                                           ctypes.POINTER(ctypes.c_uint32)]),
     "pk_hip_joint_dev": (ctypes.c_int, [ctypes.c_void_p] * 6 + [ctypes.c_uint32, ctypes.c_uint32, ctypes.c_void_p]),
     "pk_hip_layer_dev": (ctypes.c_int, [ctypes.POINTER(LayerW), ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p,
                                         ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p, ctypes.c_size_t,
@@ -635,3 +683,194 @@ class DeviceDecoder:
         for m in self.m.values():
             m.release()
         self.m = {}
+
+
+# --------------------------------------------- the cache of keys and values ---
+
+def cache_bytes(layers, pages, heads, dk):
+    """Bytes of a pool of pages (pk_hip_cache_bytes)."""
+    return lib().pk_hip_cache_bytes(layers, pages, heads, dk)
+
+
+def _is(t, dtype, what):
+    """Refuses a tensor that a kernel would misread: another type, or one that
+    is on the host."""
+    if str(t.dtype) != dtype or not t.is_cuda:
+        raise PkHipError(PK_HIP_EINVAL, f"{what}: a device tensor of {dtype[6:]}, not {t.dtype} on {t.device}")
+
+
+def _rows(t, n, width, what):
+    """A float32 matrix's address and row stride, its rows dense."""
+    _is(t, "torch.float32", what)
+    if t.dim() != 2 or t.shape[0] != n or t.shape[1] != width or (width > 1 and t.stride(1) != 1):
+        raise PkHipError(PK_HIP_EINVAL, f"{what}: [{n}, {width}] with dense rows, not {tuple(t.shape)} strides "
+                                        f"{tuple(t.stride())}")
+    return t.data_ptr(), t.stride(0) if n > 1 else width
+
+
+class CacheStreams:
+    """The streams of a call on a cache (pk_hip_streams): int32 device tensors
+    table [B, max_pages], len [B] and row0 [B + 1], the call's number of rows
+    and its longest stream's. The tensors are read when kernels run: a program
+    keeps them and updates them in place between steps."""
+
+    def __init__(self, table, len, row0, rows, max_T):
+        for t, what in ((table, "table"), (len, "len"), (row0, "row0")):
+            _is(t, "torch.int32", what)
+            if not t.is_contiguous():
+                raise PkHipError(PK_HIP_EINVAL, f"{what} is not contiguous")
+        if table.dim() != 2 or tuple(len.shape) != (table.shape[0],) or tuple(row0.shape) != (table.shape[0] + 1,):
+            raise PkHipError(PK_HIP_EINVAL, "streams: table [B, max_pages], len [B], row0 [B + 1]")
+        self.table, self.len, self.row0 = table, len, row0
+        self.rows, self.max_T = int(rows), int(max_T)
+        self.st = Streams(table.data_ptr(), len.data_ptr(), row0.data_ptr(), table.shape[0], table.shape[1],
+                          self.rows, self.max_T)
+
+
+class DeviceCache:
+    """Keys and values of streams of live audio, kept in 4 bits in pages of
+    CACHE_PAGE frames (pk_hip_cache): data a contiguous uint8 device tensor of
+    cache_bytes(layers, pages, heads, dk)."""
+
+    def __init__(self, data, layers, pages, heads, dk):
+        _is(data, "torch.uint8", "cache")
+        if not data.is_contiguous() or data.numel() < max(1, cache_bytes(layers, pages, heads, dk)):
+            raise PkHipError(PK_HIP_EINVAL, f"cache: {cache_bytes(layers, pages, heads, dk)} contiguous bytes (heads of "
+                                            "32, 64, 96 or 128 dimensions)")
+        self.data, self.heads, self.dk = data, int(heads), int(dk)
+        self.st = Cache(data.data_ptr(), layers, pages, heads, dk)
+
+    def append(self, layer, k, v, streams, stream=None):
+        """Writes the rows' keys and values [rows, heads * dk] as the streams'
+        frames [len, len + T) (pk_hip_cache_append_dev)."""
+        n, w = streams.rows, self.heads * self.dk
+        _check(lib().pk_hip_cache_append_dev(ctypes.byref(self.st), layer, *_rows(k, n, w, "k"), *_rows(v, n, w, "v"),
+                                             ctypes.byref(streams.st), _stream(stream)))
+
+    def read(self, layer, k, v, streams, stream=None):
+        """The values kept for the streams' frames [len, len + T), into k and v
+        [rows, heads * dk] (pk_hip_cache_read_dev)."""
+        n, w = streams.rows, self.heads * self.dk
+        _check(lib().pk_hip_cache_read_dev(ctypes.byref(self.st), layer, *_rows(k, n, w, "k"), *_rows(v, n, w, "v"),
+                                           ctypes.byref(streams.st), _stream(stream)))
+
+    def attention_workspace(self, streams, H, positions, left=None, right=None):
+        """Bytes of workspace an attention takes; positions as for attention,
+        or True for a table that reaches as far as left and right do."""
+        if positions is True:
+            pos = Positions(16, 16, 16, 0xffffffff, 0x7fffffff)
+        else:
+            pos = self._positions(positions, H)
+        return lib().pk_hip_attention_cache_workspace(ctypes.byref(self.st), ctypes.byref(streams.st), H,
+                                                      ctypes.byref(pos) if pos else None,
+                                                      UNLIMITED if left is None else left,
+                                                      UNLIMITED if right is None else right)
+
+    def _positions(self, positions, H):
+        if not positions:
+            return None
+        p, center, u, w = positions
+        for t, what in ((p, "p"), (u, "bias_u"), (w, "bias_w")):
+            _is(t, "torch.float32", what)
+            if not t.is_contiguous() or t.numel() % (H * self.dk) or (what != "p" and t.numel() != H * self.dk):
+                raise PkHipError(PK_HIP_EINVAL, f"positions: p [n, {H * self.dk}] and biases [{H * self.dk}], contiguous")
+        return Positions(p.data_ptr(), u.data_ptr(), w.data_ptr(), p.numel() // (H * self.dk), center)
+
+    def attention(self, o, layer, q, streams, H, ws, positions=None, left=None, right=None, stream=None):
+        """The attention of the rows q [rows, H * dk] to their streams' kept
+        frames, into o (pk_hip_attention_cache_dev); ws a uint8 tensor of
+        attention_workspace(...) bytes, positions (p [n, H * dk], center,
+        bias_u, bias_w) or None, left and right the frames attended behind and
+        ahead (None: all)."""
+        n, w = streams.rows, H * self.dk
+        pos = self._positions(positions, H)
+        _check(lib().pk_hip_attention_cache_dev(*_rows(o, n, w, "o"), *_rows(q, n, w, "q"), ctypes.byref(self.st),
+                                                layer, ctypes.byref(streams.st), H, ctypes.byref(pos) if pos else None,
+                                                UNLIMITED if left is None else left,
+                                                UNLIMITED if right is None else right,
+                                                _dptr(ws), ws.numel() if ws is not None else 0, _stream(stream)))
+
+    def move(self, pairs, table=None, source=None, stream=None):
+        """Copies pages in every layer: pairs [(from, to), ...], from a page of
+        source (this cache by default), to one of this cache; with table, an
+        int32 device tensor, its entries that name a page moved follow it
+        (pk_hip_cache_move_dev)."""
+        flat = np.ascontiguousarray(pairs, dtype=np.int32).reshape(-1)
+        if table is not None:
+            _is(table, "torch.int32", "table")
+            if not table.is_contiguous():
+                raise PkHipError(PK_HIP_EINVAL, "table is not contiguous")
+        _check(lib().pk_hip_cache_move_dev(ctypes.byref(self.st), ctypes.byref((source or self).st), _ptr(flat),
+                                           flat.size // 2, _dptr(table), table.numel() if table is not None else 0,
+                                           _stream(stream)))
+
+
+class PagePool:
+    """Which pages of a cache are in use, with a count of holders each, on the
+    host (pk_hip_pool_*)."""
+
+    def __init__(self, pages):
+        self.handle = ctypes.c_void_p()
+        _check(lib().pk_hip_pool_create(ctypes.byref(self.handle), pages))
+
+    def __del__(self):
+        if getattr(self, "handle", None):
+            lib().pk_hip_pool_destroy(self.handle)
+            self.handle = None
+
+    @property
+    def free_pages(self):
+        return lib().pk_hip_pool_free_pages(self.handle)
+
+    def holders(self, page):
+        """How many hold the page (0: free)."""
+        return lib().pk_hip_pool_holders(self.handle, page)
+
+    def alloc(self, n):
+        """n pages nobody holds, as a list; raises if fewer are free."""
+        ids = (ctypes.c_int32 * max(1, n))()
+        _check(lib().pk_hip_pool_alloc(self.handle, ids, n))
+        return list(ids[:n])
+
+    def _ids(self, ids):
+        return (ctypes.c_int32 * max(1, len(ids)))(*ids), len(ids)
+
+    def share(self, ids):
+        """One more holder for each page."""
+        _check(lib().pk_hip_pool_share(self.handle, *self._ids(ids)))
+
+    def release(self, ids):
+        """One holder fewer for each page; free without any."""
+        _check(lib().pk_hip_pool_release(self.handle, *self._ids(ids)))
+
+    def fork(self, cache, ids, frames, stream=None):
+        """A second stream over the pages ids of one of `frames` frames: its
+        whole pages shared, a page that the next frame goes into copied. Returns
+        the new stream's pages."""
+        whole = ids[:frames // CACHE_PAGE]
+        rest = ids[len(whole):]
+        copies = self.alloc(len(rest))
+        try:
+            self.share(whole)
+            try:
+                if rest:
+                    cache.move(list(zip(rest, copies)), stream=stream)
+            except Exception:
+                self.release(whole)
+                raise
+        except Exception:
+            self.release(copies)
+            raise
+        return list(whole) + copies
+
+    def compact(self, cache, table, most=None, stream=None):
+        """Moves the pages in use below the number in use (at most `most` of
+        them), table's entries with them; returns the pairs moved."""
+        cap = cache.st.pages if most is None else most
+        pairs = (ctypes.c_int32 * max(2, 2 * cap))()
+        n = ctypes.c_uint32(0)
+        _check(lib().pk_hip_pool_compact(self.handle, pairs, cap, ctypes.byref(n)))
+        moved = [(pairs[2 * i], pairs[2 * i + 1]) for i in range(n.value)]
+        if moved:
+            cache.move(moved, table, stream=stream)
+        return moved

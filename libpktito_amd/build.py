@@ -5,8 +5,9 @@
 hipcc for gfx950, each source compiled apart (in parallel) and linked into one
 shared library: the kernels (csrc/q8_kernels.hip, the quantizer, repack and
 products; csrc/layer_kernels.hip, the device-resident layer's float kernels;
-csrc/dec_kernels.hip, the decoder's fused per-token launches) and the runtime
-(csrc/pk_hip.cpp). The flags are part of the path's contract:
+csrc/dec_kernels.hip, the decoder's fused per-token launches;
+csrc/cache_kernels.hip, the 4-bit cache of keys and values and its attention)
+and the runtime (csrc/pk_hip.cpp). The flags are part of the path's contract:
   -ffp-contract=off    no multiply and add the code writes apart is fused: the
                        epilogue's operations are the reference's, one rounding
                        each (its Makefile builds with the same flag);
@@ -30,7 +31,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libpkhip.so")
 SOURCES = [os.path.join(HERE, "csrc", n)
-           for n in ("q8_kernels.hip", "q8_stream.hip", "layer_kernels.hip", "dec_kernels.hip", "diag_kernels.hip", "pk_hip.cpp")]
+           for n in ("q8_kernels.hip", "q8_stream.hip", "layer_kernels.hip", "dec_kernels.hip", "cache_kernels.hip",
+                       "diag_kernels.hip", "pk_hip.cpp")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 FLAGS = [

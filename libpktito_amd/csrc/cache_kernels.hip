@@ -1,0 +1,521 @@
+/* The 4-bit cache of keys and values (cache_layout.h has its layout): the
+ * write of a chunk's keys and values, their read-back, the attention of a
+ * chunk's rows to everything kept, and the move of pages. */
+#include "cache_layout.h"
+#include "q8_device.h"
+#include "q8_internal.h"
+
+#include <hip/hip_runtime.h>
+
+#pragma clang fp contract(off)
+
+namespace pkq8 {
+
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v4f_u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ CacheSpan span_of(const CacheStreams &s, uint32_t b) {
+    return cache_span(s, s.row0[b], s.row0[b + 1], s.len[b]);
+}
+
+/* ---------------------------------------------------------------- write --- */
+
+/* A workgroup writes one page's part of a stream's new frames for one kept
+ * head. A wave takes a frame at a time, a lane two dimensions: the largest
+ * magnitude over the wave, the scale, a byte of two codes. Keys go straight
+ * to their rows. Values go through LDS and are gathered into dwords of eight
+ * frames; a dword that the chunk covers in part keeps its other frames'
+ * codes (read, merged, stored by one thread, so a frame that shares a byte
+ * with the one before it is no race). */
+__global__ __launch_bounds__(256) void cache_write_kernel(uint8_t *data, uint32_t pages, uint32_t G, uint32_t dk,
+                                                          CacheStreams st, const float *__restrict__ k, uint64_t ks,
+                                                          const float *__restrict__ v, uint64_t vs) {
+    const uint32_t g = blockIdx.x, b = blockIdx.z;
+    const CacheSpan sp = span_of(st, b);
+    const int32_t pg = sp.len / (int32_t)kPage + (int32_t)blockIdx.y;
+    if (pg * (int32_t)kPage >= sp.total)
+        return;
+    const int32_t id = st.table[(uint64_t)b * st.max_pages + pg];
+    if (!cache_page_ok(id, pages))
+        return;
+    uint8_t *rec = data + ((uint64_t)id * G + g) * cache_record(dk);
+    const int32_t base = pg * (int32_t)kPage;
+    const int32_t f0 = max(sp.len - base, 0), f1 = min(sp.total - base, (int32_t)kPage);
+    __shared__ uint8_t code[kPage][kMaxCacheDk / 2];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool in = 2 * lane < dk;
+    for (int32_t f = f0 + (int32_t)wave; f < f1; f += 4) {
+        const uint64_t row = (uint64_t)(sp.r0 + base + f - sp.len);
+#pragma unroll
+        for (int which = 0; which < 2; which++) {
+            const float *src = which ? v + row * vs : k + row * ks;
+            float2 x = make_float2(0.0f, 0.0f);
+            if (in)
+                x = *(const float2 *)(src + g * dk + 2 * lane);
+            const uint32_t bf = cache_scale((uint32_t)wave_max_nonneg(max(mag_bits(x.x), mag_bits(x.y))));
+            const float d = cache_scale_value(bf);
+            const uint32_t c = bf ? cache_code(x.x, d) | cache_code(x.y, d) << 4 : 0;
+            if (in) {
+                if (which)
+                    code[f][lane] = (uint8_t)c;
+                else
+                    rec[cache_key_at(dk, f) + lane] = (uint8_t)c;
+            }
+            if (lane == 0)
+                *(uint16_t *)(rec + (which ? cache_value_scale_at(dk, f) : cache_key_scale_at(dk, f))) = (uint16_t)bf;
+        }
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < 8 * dk; i += 256) {
+        const uint32_t c = i % dk, gg = i / dk / 4, w = i / dk % 4;
+        uint32_t val = 0, mask = 0;
+#pragma unroll
+        for (uint32_t n = 0; n < 8; n++) {
+            const int32_t f = (int32_t)cache_frame_of(gg, w, n);
+            if (f >= f0 && f < f1) {
+                val |= (code[f][c / 2] >> 4 * (c % 2) & 15u) << 4 * n;
+                mask |= 15u << 4 * n;
+            }
+        }
+        if (mask == 0)
+            continue;
+        uint32_t *at = (uint32_t *)(rec + cache_values_at(dk) + cache_value_dword(c, gg, w));
+        *at = mask == 0xffffffffu ? val : (*at & ~mask) | val;
+    }
+}
+
+/* ----------------------------------------------------------------- read --- */
+
+/* A workgroup reads back one page's part of a stream's frames [len, len + T)
+ * for one kept head, a thread a value at a time. Frames of a hole read as
+ * zeros, and so do frames past the table. */
+__global__ __launch_bounds__(256) void cache_read_kernel(const uint8_t *__restrict__ data, uint32_t pages, uint32_t G,
+                                                         uint32_t dk, CacheStreams st, float *__restrict__ k,
+                                                         uint64_t ks, float *__restrict__ v, uint64_t vs) {
+    const uint32_t g = blockIdx.x, b = blockIdx.z;
+    const CacheSpan sp = span_of(st, b);
+    const int32_t pg = sp.len / (int32_t)kPage + (int32_t)blockIdx.y;
+    const int32_t base = pg * (int32_t)kPage;
+    const int32_t f0 = max(sp.len - base, 0), f1 = min(sp.len + sp.T - base, (int32_t)kPage);
+    if (f0 >= f1)
+        return;
+    const int32_t id = pg < (int32_t)st.max_pages ? st.table[(uint64_t)b * st.max_pages + pg] : -1;
+    const bool ok = cache_page_ok(id, pages);
+    const uint8_t *rec = data + ((uint64_t)(ok ? id : 0) * G + g) * cache_record(dk);
+    for (uint32_t i = threadIdx.x; i < (uint32_t)(f1 - f0) * dk; i += 256) {
+        const uint32_t f = (uint32_t)f0 + i / dk, c = i % dk;
+        const uint64_t row = (uint64_t)(sp.r0 + base + (int32_t)f - sp.len);
+        float kv = 0.0f, vv = 0.0f;
+        if (ok) {
+            const uint32_t gg = f / 32, w = f / 4 % 4, n = 4 * (f / 16 % 2) + f % 4;
+            const uint32_t kb = rec[cache_key_at(dk, f) + c / 2] >> 4 * (c % 2) & 15u;
+            const uint32_t vb = rec[cache_values_at(dk) + cache_value_dword(c, gg, w) + n / 2] >> 4 * (n % 2) & 15u;
+            kv = cache_level(kb) * cache_scale_value(*(const uint16_t *)(rec + cache_key_scale_at(dk, f)));
+            vv = cache_level(vb) * cache_scale_value(*(const uint16_t *)(rec + cache_value_scale_at(dk, f)));
+        }
+        k[row * ks + g * dk + c] = kv;
+        v[row * vs + g * dk + c] = vv;
+    }
+}
+
+/* ------------------------------------------------------------ attention --- */
+
+/* Products in 32 bits on the bfloat16 matrix cores. A level has 2 significant
+ * bits, so it is a bfloat16 as it stands; the other operand (a query, a
+ * probability times its value's scale) is a float cut into three bfloat16 of
+ * 8 bits each, whose sum is the float exactly (truncation leaves 16 bits
+ * after the first piece and 8 after the second). Three products of exact
+ * terms, added in 32 bits: what an fp32 product of the same values gives, at
+ * a third of the bfloat16 rate, five times the fp32 matrix rate. */
+struct Pieces {
+    v8bf p[3];
+};
+
+__device__ __forceinline__ Pieces cut(const float (&x)[8]) {
+    Pieces r;
+    uint32_t w[3][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+        for (int n = 0; n < 3; n++) {
+            const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+            w[n][i] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+            a -= __uint_as_float(ua & 0xffff0000u);
+            b -= __uint_as_float(ub & 0xffff0000u);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < 3; n++)
+        r.p[n] = __builtin_bit_cast(v8bf, v4u{ w[n][0], w[n][1], w[n][2], w[n][3] });
+    return r;
+}
+
+/* eight codes as bfloat16 levels */
+__device__ __forceinline__ v8bf levels(uint32_t w) {
+    const v2bf a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 0);
+    const v2bf b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 1);
+    const v2bf c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 2);
+    const v2bf d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 3);
+    return v8bf{ a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y };
+}
+
+__device__ __forceinline__ v4f mfma(v8bf a, v8bf b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+struct CacheAttention {
+    float *o;
+    const float *q;
+    uint64_t os, qs;
+    const uint8_t *data;                    /* the layer's records */
+    uint32_t pages, G, H, dk;
+    CacheStreams st;
+    int32_t left, right;                    /* clipped to what can occur */
+    float scale;                            /* 1 / sqrt(dk) */
+    /* positions (p NULL: none): row place0 is distance left's */
+    const float *p, *bias_u, *bias_w;
+    float *place;                           /* [rows][H][place_stride(bw)] */
+    uint32_t bw;
+};
+
+/* The position scores (q + w) . p of every row at every distance that it
+ * needs, into the workspace: the same rows of p serve every stream, so this
+ * is one product of all rows by the table, read once, where the attention
+ * reads its own stream's pages only. A workgroup takes 64 rows of a head,
+ * their pieces as the matrix instruction's operands in LDS, and walks tiles
+ * of 16 distances, a wave each; both operands are floats, so six of the nine
+ * products of pieces are taken (the other three are under 2^-24 of the
+ * whole). */
+constexpr int kPlaceRows = 64, kPlaceTiles = 4;
+template <int NS>
+__global__ __launch_bounds__(256) void cache_place_kernel(CacheAttention a) {
+    __shared__ v4u frag[kPlaceRows / 16][NS][3][64];
+    __shared__ int32_t need_lo, need_hi;
+    const uint32_t h = blockIdx.y, n0 = blockIdx.z * kPlaceRows;
+    const int32_t x0 = (int32_t)blockIdx.x * (64 * kPlaceTiles);
+    const uint32_t dk = 32 * NS, stride = place_stride(a.bw);
+    if (threadIdx.x == 0)
+        need_lo = INT32_MAX, need_hi = INT32_MIN;
+    __syncthreads();
+    int32_t lo = INT32_MAX, hi = INT32_MIN;
+    for (uint32_t b = threadIdx.x; b < a.st.B; b += 256) {
+        const CacheSpan sp = span_of(a.st, b);
+        const int32_t r0 = max(sp.r0, (int32_t)n0), r1 = min(sp.r0 + sp.T, (int32_t)(n0 + kPlaceRows));
+        if (r0 >= r1)
+            continue;
+        const int32_t p0 = sp.len + r0 - sp.r0, p1 = sp.len + r1 - 1 - sp.r0;
+        lo = min(lo, a.left - p1);
+        hi = max(hi, a.left + sp.total - 1 - p0);
+    }
+    if (lo <= hi) {
+        atomicMin(&need_lo, lo);
+        atomicMax(&need_hi, hi);
+    }
+    __syncthreads();
+    if (need_lo >= x0 + 64 * kPlaceTiles || need_hi < x0)
+        return;
+    const uint32_t rows = min((uint32_t)kPlaceRows, a.st.rows - n0);
+    for (uint32_t i = threadIdx.x; i < kPlaceRows * 4 * NS; i += 256) {
+        const uint32_t row = i / (4 * NS), part = i % (4 * NS);       /* eight dimensions */
+        float x[8] = {};
+        if (row < rows) {
+            const v4f *src = (const v4f *)(a.q + (uint64_t)(n0 + row) * a.qs + h * dk + 8 * part);
+            const v4f *bias = (const v4f *)(a.bias_w + h * dk + 8 * part);
+            const v4f s0 = src[0] + bias[0], s1 = src[1] + bias[1];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                x[j] = s0[j], x[4 + j] = s1[j];
+        }
+        const Pieces c = cut(x);
+#pragma unroll
+        for (int n = 0; n < 3; n++)
+            frag[row / 16][part / 4][n][16 * (part % 4) + row % 16] = __builtin_bit_cast(v4u, c.p[n]);
+    }
+    __syncthreads();
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = lane / 16;
+#pragma unroll 1
+    for (int t = 0; t < kPlaceTiles; t++) {
+        const int32_t x = x0 + 64 * t + 16 * (int32_t)wave;
+        if (x >= (int32_t)a.bw || need_lo >= x + 16 || need_hi < x)
+            continue;
+        const uint32_t m = min((uint32_t)x + lane % 16, a.bw - 1);
+        Pieces p[NS];
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            const v4f *src = (const v4f *)(a.p + (uint64_t)m * (a.H * dk) + h * dk + 32 * s + 8 * w);
+            const v4f s0 = src[0], s1 = src[1];
+            const float xs[8] = { s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3] };
+            p[s] = cut(xs);
+        }
+        for (uint32_t rt = 0; 16 * rt < rows; rt++) {
+            v4f acc = { 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                v8bf q[3];
+#pragma unroll
+                for (int n = 0; n < 3; n++)
+                    q[n] = __builtin_bit_cast(v8bf, frag[rt][s][n][lane]);
+                acc = mfma(p[s].p[2], q[0], acc);
+                acc = mfma(p[s].p[1], q[1], acc);
+                acc = mfma(p[s].p[0], q[2], acc);
+                acc = mfma(p[s].p[1], q[0], acc);
+                acc = mfma(p[s].p[0], q[1], acc);
+                acc = mfma(p[s].p[0], q[0], acc);
+            }
+            const uint32_t row = 16 * rt + lane % 16;
+            if (row < rows)
+                *(v4f *)(a.place + ((uint64_t)(n0 + row) * a.H + h) * stride + kPlacePad + x + 4 * w) = acc;
+        }
+    }
+}
+
+/* A workgroup attends for 16 rows of a stream and kept head (a row is a frame
+ * and one of the H / G heads that share the kept one), its four waves a page
+ * each in turn with the running maximum and sum of a softmax, their sums met
+ * in LDS at the end. */
+template <int NS>
+__global__ __launch_bounds__(256) void cache_attention_kernel(CacheAttention a, uint32_t tiles) {
+    constexpr uint32_t dk = 32 * NS, record = kPage * dk + 4 * kPage;
+    const uint32_t g = blockIdx.x % a.G, tile = blockIdx.x / a.G % tiles, b = blockIdx.x / a.G / tiles;
+    const CacheSpan sp = span_of(a.st, b);
+    const uint32_t grp = a.H / a.G;
+    const int32_t nrows = sp.T * (int32_t)grp, rr0 = (int32_t)tile * 16;
+    if (rr0 >= nrows)
+        return;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = lane / 16;
+    const int32_t rr = min(rr0 + (int32_t)(lane % 16), nrows - 1);
+    const int32_t t = rr / (int32_t)grp;
+    const uint32_t h = g * grp + (uint32_t)rr % grp;
+    const uint64_t row = (uint64_t)(sp.r0 + t);
+    const int32_t pos = sp.len + t;
+    const int32_t lo = cache_lo(pos, a.left), hi = cache_hi(pos, a.right, sp.total);
+
+    Pieces q[NS];
+#pragma unroll
+    for (int s = 0; s < NS; s++) {
+        const uint32_t c = h * dk + w * (8 * NS) + 8 * s;
+        const v4f *src = (const v4f *)(a.q + row * a.qs + c);
+        v4f s0 = src[0], s1 = src[1];
+        if (a.p) {
+            const v4f *bias = (const v4f *)(a.bias_u + c);
+            s0 += bias[0], s1 += bias[1];
+        }
+        const float x[8] = { s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3] };
+        q[s] = cut(x);
+    }
+    const float *place = nullptr;
+    if (a.p)
+        place = a.place + (row * a.H + h) * place_stride(a.bw) + kPlacePad + (a.left - pos);
+
+    /* the pages of any of the tile's rows */
+    const int32_t t1 = min(rr0 + 15, nrows - 1) / (int32_t)grp;
+    const int32_t j0 = cache_lo(sp.len + rr0 / (int32_t)grp, a.left), j1 = cache_hi(sp.len + t1, a.right, sp.total);
+    const float c2 = a.scale * 1.44269504088896340736f;     /* scores in powers of 2 */
+    float top = -INFINITY, sum = 0.0f;
+    v4f o[2 * NS] = {};
+    for (int32_t pg = j0 / (int32_t)kPage + (int32_t)wave; pg * (int32_t)kPage <= j1; pg += 4) {
+        const int32_t id = a.st.table[(uint64_t)b * a.st.max_pages + pg];
+        if (!cache_page_ok(id, a.pages))
+            continue;
+        const uint8_t *rec = a.data + ((uint64_t)id * a.G + g) * record;
+        float s[4][4], best = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < 4; kt++) {
+            const uint32_t *kp = (const uint32_t *)(rec + cache_key_at(dk, 16 * kt + lane % 16) + w * (4 * NS));
+            v4f acc = { 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+            for (int st = 0; st < NS; st++) {
+                const v8bf k = levels(kp[st]);
+                acc = mfma(k, q[st].p[2], acc);
+                acc = mfma(k, q[st].p[1], acc);
+                acc = mfma(k, q[st].p[0], acc);
+            }
+            const uint32_t f = 16 * kt + 4 * w;
+            const v2u ks = *(const v2u *)(rec + cache_key_scale_at(dk, f));
+            const int32_t j = pg * (int32_t)kPage + (int32_t)f;
+            v4f add = { 0.0f, 0.0f, 0.0f, 0.0f };
+            if (a.p)
+                add = *(const v4f_u *)(place + j);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float d = __uint_as_float(r % 2 ? ks[r / 2] & 0xffff0000u : ks[r / 2] << 16);
+                const float v = (acc[r] * d + add[r]) * c2;
+                s[kt][r] = j + r >= lo && j + r <= hi ? v : -INFINITY;
+                best = fmaxf(best, s[kt][r]);
+            }
+        }
+        best = fmaxf(best, __shfl_xor(best, 16));
+        best = fmaxf(best, __shfl_xor(best, 32));
+        const float now = fmaxf(top, best), base = now == -INFINITY ? 0.0f : now;
+        const float scale = __builtin_amdgcn_exp2f(top - base);
+        top = now;
+        sum *= scale;
+#pragma unroll
+        for (int i = 0; i < 2 * NS; i++)
+            o[i] *= scale;
+#pragma unroll
+        for (int gg = 0; gg < 2; gg++) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int kt = 2 * gg + i / 4, r = i % 4;
+                const uint32_t f = 16 * kt + 4 * w;
+                const v2u vs = *(const v2u *)(rec + cache_value_scale_at(dk, f));
+                const float d = __uint_as_float(r % 2 ? vs[r / 2] & 0xffff0000u : vs[r / 2] << 16);
+                const float e = __builtin_amdgcn_exp2f(s[kt][r] - base);
+                sum += e;
+                /* a frame that is not attended may have a scale that was never written */
+                x[i] = s[kt][r] == -INFINITY ? 0.0f : e * d;
+            }
+            const Pieces pr = cut(x);
+#pragma unroll
+            for (int dt = 0; dt < 2 * NS; dt++) {
+                const v8bf val = levels(*(const uint32_t *)(rec + cache_values_at(dk) + 1024 * (dt / 2) + 16 * lane +
+                                                            8 * (dt % 2) + 4 * gg));
+                o[dt] = mfma(val, pr.p[2], o[dt]);
+                o[dt] = mfma(val, pr.p[1], o[dt]);
+                o[dt] = mfma(val, pr.p[0], o[dt]);
+            }
+        }
+    }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+
+    __shared__ float part[4][16][dk + 4], tops[4][16], sums[4][16];
+    if (w == 0) {
+        tops[wave][lane % 16] = top;
+        sums[wave][lane % 16] = sum;
+    }
+#pragma unroll
+    for (int dt = 0; dt < 2 * NS; dt++)
+        *(v4f *)&part[wave][lane % 16][16 * dt + 4 * w] = o[dt];
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < 16 * dk / 4; i += 256) {
+        const uint32_t r = i / (dk / 4), c = i % (dk / 4) * 4;
+        if (rr0 + (int32_t)r >= nrows)
+            continue;
+        float m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+            m = fmaxf(m, tops[n][r]);
+        const float base = m == -INFINITY ? 0.0f : m;
+        v4f y = { 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+            const float e = __builtin_amdgcn_exp2f(tops[n][r] - base);
+            l += sums[n][r] * e;
+            y += *(const v4f *)&part[n][r][c] * e;
+        }
+        y = l == 0.0f ? v4f{ 0.0f, 0.0f, 0.0f, 0.0f } : y / l;      /* nothing attended: zeros; a NaN stays one */
+        const int32_t ro = rr0 + (int32_t)r;
+        *(v4f *)(a.o + (uint64_t)(sp.r0 + ro / (int32_t)grp) * a.os + (g * grp + (uint32_t)ro % grp) * dk + c) = y;
+    }
+}
+
+/* ----------------------------------------------------------------- move --- */
+
+/* Pairs (from, to) of pages by value, so that a call needs no device memory
+ * of its own; more take several launches. */
+constexpr int kMovePairs = 256;
+struct MovePairs {
+    int32_t from[kMovePairs], to[kMovePairs];
+};
+
+/* a page of a layer is one contiguous run of G records */
+__global__ __launch_bounds__(256) void cache_move_kernel(uint8_t *__restrict__ dst, uint64_t dlayer,
+                                                         const uint8_t *__restrict__ src, uint64_t slayer,
+                                                         uint32_t page_bytes, MovePairs m) {
+    const v4u *from = (const v4u *)(src + blockIdx.z * slayer + (uint64_t)m.from[blockIdx.y] * page_bytes);
+    v4u *to = (v4u *)(dst + blockIdx.z * dlayer + (uint64_t)m.to[blockIdx.y] * page_bytes);
+    const uint32_t n = page_bytes / 16;
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256)
+        to[i] = from[i];
+}
+
+__global__ __launch_bounds__(256) void cache_follow_kernel(int32_t *table, uint64_t entries, MovePairs m,
+                                                           uint32_t pairs) {
+    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const int32_t old = i < entries ? table[i] : -1;
+    int32_t now = old;
+    for (uint32_t p = 0; p < pairs; p++)
+        if (m.from[p] == old)
+            now = m.to[p];
+    if (now != old)
+        table[i] = now;
+}
+
+/* ------------------------------------------------------------- launches --- */
+
+int launch_cache_write(uint8_t *data, uint32_t pages, uint32_t G, uint32_t dk, const CacheStreams &st, const float *k,
+                       uint64_t ks, const float *v, uint64_t vs, hipStream_t s) {
+    const dim3 grid(G, (st.max_T + kPage - 2) / kPage + 1, st.B);
+    cache_write_kernel<<<grid, 256, 0, s>>>(data, pages, G, dk, st, k, ks, v, vs);
+    return hipPeekAtLastError() == hipSuccess ? 0 : -1;
+}
+
+int launch_cache_read(const uint8_t *data, uint32_t pages, uint32_t G, uint32_t dk, const CacheStreams &st, float *k,
+                      uint64_t ks, float *v, uint64_t vs, hipStream_t s) {
+    const dim3 grid(G, (st.max_T + kPage - 2) / kPage + 1, st.B);
+    cache_read_kernel<<<grid, 256, 0, s>>>(data, pages, G, dk, st, k, ks, v, vs);
+    return hipPeekAtLastError() == hipSuccess ? 0 : -1;
+}
+
+size_t cache_attention_workspace(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, bool positions,
+                                 int32_t left, int32_t right) {
+    (void)G, (void)dk;
+    return positions ? (size_t)st.rows * H * place_stride((uint32_t)left + (uint32_t)right + 1) * sizeof(float) : 0;
+}
+
+template <int NS>
+static void attend(const CacheAttention &a, hipStream_t s) {
+    if (a.p) {
+        const dim3 grid((a.bw + 64 * kPlaceTiles - 1) / (64 * kPlaceTiles), a.H, (a.st.rows + kPlaceRows - 1) / kPlaceRows);
+        cache_place_kernel<NS><<<grid, 256, 0, s>>>(a);
+    }
+    const uint32_t tiles = (a.st.max_T * (a.H / a.G) + 15) / 16;
+    cache_attention_kernel<NS><<<a.G * tiles * a.st.B, 256, 0, s>>>(a, tiles);
+}
+
+int launch_cache_attention(const CacheAttentionCall &c, hipStream_t s) {
+    CacheAttention a = {};
+    a.o = c.o, a.os = c.os, a.q = c.q, a.qs = c.qs;
+    a.data = c.data, a.pages = c.pages, a.G = c.G, a.H = c.H, a.dk = c.dk;
+    a.st = c.st;
+    a.left = c.left, a.right = c.right;
+    a.scale = 1.0f / sqrtf((float)c.dk);
+    a.p = c.p, a.bias_u = c.bias_u, a.bias_w = c.bias_w;
+    a.place = (float *)c.ws;
+    a.bw = (uint32_t)c.left + (uint32_t)c.right + 1;
+    switch (c.dk / 32) {
+    case 1: attend<1>(a, s); break;
+    case 2: attend<2>(a, s); break;
+    case 3: attend<3>(a, s); break;
+    case 4: attend<4>(a, s); break;
+    default: return -2;
+    }
+    return hipPeekAtLastError() == hipSuccess ? 0 : -1;
+}
+
+int launch_cache_move(uint8_t *dst, uint64_t dlayer, const uint8_t *src, uint64_t slayer, uint32_t layers,
+                      uint32_t page_bytes, const int32_t *pairs, uint32_t n, int32_t *table, uint64_t entries,
+                      hipStream_t s) {
+    for (uint32_t p0 = 0; p0 < n; p0 += kMovePairs) {
+        const uint32_t m = n - p0 < (uint32_t)kMovePairs ? n - p0 : (uint32_t)kMovePairs;
+        MovePairs mp = {};
+        for (uint32_t i = 0; i < m; i++) {
+            mp.from[i] = pairs[2 * (p0 + i)];
+            mp.to[i] = pairs[2 * (p0 + i) + 1];
+        }
+        cache_move_kernel<<<dim3(4, m, layers), 256, 0, s>>>(dst, dlayer, src, slayer, page_bytes, mp);
+        if (table && entries)
+            cache_follow_kernel<<<(uint32_t)((entries + 255) / 256), 256, 0, s>>>(table, entries, mp, m);
+    }
+    return hipPeekAtLastError() == hipSuccess ? 0 : -1;
+}
+
+}  // namespace pkq8

@@ -11,6 +11,7 @@
  * share one and no call waits for another's.
  */
 #include "pk_hip.h"
+#include "page_pool.h"
 #include "q8_internal.h"
 
 #include <algorithm>
@@ -1543,6 +1544,267 @@ int pk_hip_search_dev(const pk_hip_decoder *d, const float *f, uint32_t T, int32
     if (res[0] > nhead)
         PK_TRY(hipMemcpy(toks + 3 * nhead, a.toks + 3 * nhead, (size_t)(res[0] - nhead) * 12, hipMemcpyDeviceToHost));
     *ntoks = res[0];
+    return PK_HIP_OK;
+}
+
+/* ------------------------------------- the cache of keys and values --- */
+
+/* The arguments are checked before the device is opened, so that a refusal
+ * is the same with and without one. */
+
+static int check_cache(const pk_hip_cache *c, const char *who) {
+    if (!c || !c->data || ((uintptr_t)c->data & 15) ||
+        !pk_hip_cache_bytes(c->layers, c->pages, c->heads, c->dk))
+        return fail(PK_HIP_EINVAL, "%s: a cache of 16-byte aligned memory, at least one layer, page and head, heads of "
+                                   "32, 64, 96 or 128 dimensions", who);
+    return PK_HIP_OK;
+}
+
+static int check_streams(const pk_hip_streams *st, const char *who) {
+    if (!st || !st->table || !st->len || !st->row0 || st->max_pages == 0 || st->max_pages > 1u << 24 || st->B > 65535 ||
+        st->rows > 1u << 22 || st->max_T > st->rows)
+        return fail(PK_HIP_EINVAL, "%s: streams with their table, len and row0, 1 to 2^24 pages a stream, up to 65535 "
+                                   "streams and 2^22 rows, max_T up to rows", who);
+    return PK_HIP_OK;
+}
+
+static int check_rows(const float *p, size_t stride, uint64_t width, uint32_t rows, const char *who, const char *what) {
+    if (!p || ((uintptr_t)p & 15) || stride % 4 || (rows > 1 && stride < width))
+        return fail(PK_HIP_EINVAL, "%s: %s 16-byte aligned, its stride a multiple of 4 and at least %llu", who, what,
+                    (unsigned long long)width);
+    return PK_HIP_OK;
+}
+
+static pkq8::CacheStreams streams_of(const pk_hip_streams *st) {
+    pkq8::CacheStreams s;
+    s.table = st->table, s.len = st->len, s.row0 = st->row0;
+    s.B = st->B, s.max_pages = st->max_pages, s.rows = st->rows, s.max_T = st->max_T;
+    return s;
+}
+
+static uint64_t cache_layer_bytes(const pk_hip_cache *c) {
+    return (uint64_t)c->pages * c->heads * pkq8::cache_record(c->dk);
+}
+
+size_t pk_hip_cache_bytes(uint32_t layers, uint32_t pages, uint32_t heads, uint32_t dk) {
+    if (layers == 0 || layers > 65535 || pages == 0 || pages > 1u << 30 || heads == 0 || heads > 1024 ||
+        !pkq8::cache_dk_ok(dk))
+        return 0;
+    return (size_t)layers * pages * heads * pkq8::cache_record(dk);
+}
+
+int pk_hip_cache_append_dev(const pk_hip_cache *c, uint32_t layer, const float *k, size_t ks, const float *v,
+                            size_t vs, const pk_hip_streams *st, void *stream) {
+    int e;
+    if ((e = check_cache(c, "cache_append_dev")) || (e = check_streams(st, "cache_append_dev")))
+        return e;
+    if (layer >= c->layers)
+        return fail(PK_HIP_EINVAL, "cache_append_dev: layer %u of %u", layer, c->layers);
+    const uint64_t width = (uint64_t)c->heads * c->dk;
+    if (st->rows && ((e = check_rows(k, ks, width, st->rows, "cache_append_dev", "k")) ||
+                     (e = check_rows(v, vs, width, st->rows, "cache_append_dev", "v"))))
+        return e;
+    if ((e = pk_hip_init()))
+        return e;
+    if (st->B == 0 || st->max_T == 0)
+        return PK_HIP_OK;
+    PK_LAUNCH(pkq8::launch_cache_write((uint8_t *)c->data + layer * cache_layer_bytes(c), c->pages, c->heads, c->dk,
+                                       streams_of(st), k, ks, v, vs, (hipStream_t)stream),
+              "cache write launch");
+    g_kernel = "cache_write";
+    return PK_HIP_OK;
+}
+
+int pk_hip_cache_read_dev(const pk_hip_cache *c, uint32_t layer, float *k, size_t ks, float *v, size_t vs,
+                          const pk_hip_streams *st, void *stream) {
+    int e;
+    if ((e = check_cache(c, "cache_read_dev")) || (e = check_streams(st, "cache_read_dev")))
+        return e;
+    if (layer >= c->layers)
+        return fail(PK_HIP_EINVAL, "cache_read_dev: layer %u of %u", layer, c->layers);
+    const uint64_t width = (uint64_t)c->heads * c->dk;
+    if (st->rows && ((e = check_rows(k, ks, width, st->rows, "cache_read_dev", "k")) ||
+                     (e = check_rows(v, vs, width, st->rows, "cache_read_dev", "v"))))
+        return e;
+    if ((e = pk_hip_init()))
+        return e;
+    if (st->B == 0 || st->max_T == 0)
+        return PK_HIP_OK;
+    PK_LAUNCH(pkq8::launch_cache_read((const uint8_t *)c->data + layer * cache_layer_bytes(c), c->pages, c->heads,
+                                      c->dk, streams_of(st), k, ks, v, vs, (hipStream_t)stream),
+              "cache read launch");
+    g_kernel = "cache_read";
+    return PK_HIP_OK;
+}
+
+/* The window that an attention's rows have: the asked one, no wider than a
+ * stream can be or than the positions' table reaches. */
+static int attention_window(const pk_hip_cache *c, const pk_hip_streams *st, uint32_t H, const pk_hip_positions *pos,
+                            uint32_t left, uint32_t right, const char *who, int32_t *l, int32_t *r) {
+    int e;
+    if ((e = check_streams(st, who)))
+        return e;
+    if (!c || c->heads == 0 || c->heads > 1024 || !pkq8::cache_dk_ok(c->dk) || H == 0 || H > 65535 || H % c->heads ||
+        (uint64_t)st->max_T * (H / c->heads) > 0x3fffffff)
+        return fail(PK_HIP_EINVAL, "%s: H = %u heads of 32, 64, 96 or 128 dimensions, a multiple of the kept ones, at "
+                                   "most 2^30 rows of a kept head a stream", who, H);
+    uint32_t lo = std::min(left, st->max_pages * pkq8::kPage - 1), hi = std::min(right, st->max_T ? st->max_T - 1 : 0);
+    if (pos) {
+        if (!pos->p || !pos->bias_u || !pos->bias_w || (((uintptr_t)pos->p | (uintptr_t)pos->bias_u |
+            (uintptr_t)pos->bias_w) & 15) || pos->center >= pos->n)
+            return fail(PK_HIP_EINVAL, "%s: positions with p and both biases 16-byte aligned, the center one of the "
+                                       "rows", who);
+        lo = std::min(lo, pos->center);
+        hi = std::min(hi, pos->n - 1 - pos->center);
+    }
+    *l = (int32_t)lo;
+    *r = (int32_t)hi;
+    return PK_HIP_OK;
+}
+
+size_t pk_hip_attention_cache_workspace(const pk_hip_cache *c, const pk_hip_streams *st, uint32_t H,
+                                        const pk_hip_positions *pos, uint32_t left, uint32_t right) {
+    int32_t l, r;
+    if (attention_window(c, st, H, pos, left, right, "attention_cache_workspace", &l, &r))
+        return 0;
+    return pkq8::cache_attention_workspace(streams_of(st), c->heads, H, c->dk, pos != nullptr, l, r);
+}
+
+int pk_hip_attention_cache_dev(float *o, size_t os, const float *q, size_t qs, const pk_hip_cache *c, uint32_t layer,
+                               const pk_hip_streams *st, uint32_t H, const pk_hip_positions *pos, uint32_t left,
+                               uint32_t right, void *ws, size_t ws_bytes, void *stream) {
+    int e;
+    pkq8::CacheAttentionCall a = {};
+    if ((e = check_cache(c, "attention_cache_dev")) ||
+        (e = attention_window(c, st, H, pos, left, right, "attention_cache_dev", &a.left, &a.right)))
+        return e;
+    if (layer >= c->layers)
+        return fail(PK_HIP_EINVAL, "attention_cache_dev: layer %u of %u", layer, c->layers);
+    const uint64_t width = (uint64_t)H * c->dk;
+    if (st->rows && ((e = check_rows(o, os, width, st->rows, "attention_cache_dev", "o")) ||
+                     (e = check_rows(q, qs, width, st->rows, "attention_cache_dev", "q"))))
+        return e;
+    if ((const float *)o == q && os != qs)
+        return fail(PK_HIP_EINVAL, "attention_cache_dev: an output over its queries has their stride");
+    a.st = streams_of(st);
+    const size_t need = pkq8::cache_attention_workspace(a.st, c->heads, H, c->dk, pos != nullptr, a.left, a.right);
+    if (need && (!ws || ((uintptr_t)ws & 15) || ws_bytes < need))
+        return fail(PK_HIP_EINVAL, "attention_cache_dev: 16-byte aligned workspace of %zu bytes, %zu needed", ws_bytes,
+                    need);
+    if ((e = pk_hip_init()))
+        return e;
+    if (st->B == 0 || st->max_T == 0)
+        return PK_HIP_OK;
+    a.o = o, a.os = os, a.q = q, a.qs = qs;
+    a.data = (const uint8_t *)c->data + layer * cache_layer_bytes(c);
+    a.pages = c->pages, a.G = c->heads, a.H = H, a.dk = c->dk;
+    if (pos) {
+        a.p = pos->p + (pos->center - (uint32_t)a.left) * width;
+        a.bias_u = pos->bias_u, a.bias_w = pos->bias_w;
+    }
+    a.ws = ws;
+    PK_LAUNCH(pkq8::launch_cache_attention(a, (hipStream_t)stream), "cache attention launch");
+    g_kernel = "cache_attention";
+    return PK_HIP_OK;
+}
+
+int pk_hip_cache_move_dev(const pk_hip_cache *dst, const pk_hip_cache *src, const int32_t *pairs, uint32_t n,
+                          int32_t *table, size_t entries, void *stream) {
+    int e;
+    if ((e = check_cache(dst, "cache_move_dev")) || (e = check_cache(src, "cache_move_dev")))
+        return e;
+    if (dst->layers != src->layers || dst->heads != src->heads || dst->dk != src->dk)
+        return fail(PK_HIP_EINVAL, "cache_move_dev: caches of the same layers, heads and dk");
+    const bool same = dst->data == src->data;
+    const char *d0 = (const char *)dst->data, *s0 = (const char *)src->data;
+    if (same ? dst->pages != src->pages
+             : d0 < s0 + src->layers * cache_layer_bytes(src) && s0 < d0 + dst->layers * cache_layer_bytes(dst))
+        return fail(PK_HIP_EINVAL, "cache_move_dev: caches that overlap are one cache");
+    if ((n && !pairs) || (table && !same) || entries > (size_t)1 << 38)
+        return fail(PK_HIP_EINVAL, "cache_move_dev: pairs set, and a table only where src and dst are one cache");
+    if (n > dst->pages)
+        return fail(PK_HIP_EINVAL, "cache_move_dev: %u pairs onto %u pages: one is copied to twice", n, dst->pages);
+    try {
+        /* bit 0: copied to, bit 1: copied from (of src, which is dst where it matters) */
+        std::vector<uint8_t> seen(same ? src->pages : std::max(src->pages, dst->pages), 0);
+        for (uint32_t i = 0; i < n; i++) {
+            const uint32_t f = (uint32_t)pairs[2 * i], t = (uint32_t)pairs[2 * i + 1];
+            if (f >= src->pages || t >= dst->pages)
+                return fail(PK_HIP_EINVAL, "cache_move_dev: pair %u is pages %d and %d, of %u and %u", i, (int)f, (int)t,
+                            src->pages, dst->pages);
+            if (seen[t] & 1)
+                return fail(PK_HIP_EINVAL, "cache_move_dev: page %u is copied to twice", t);
+            seen[t] |= 1;
+            if (table && (seen[f] & 2))
+                return fail(PK_HIP_EINVAL, "cache_move_dev: page %u moves to two places", f);
+            seen[f] |= 2;
+        }
+        if (same)
+            for (uint32_t i = 0; i < n; i++)
+                if (seen[(uint32_t)pairs[2 * i]] & 1)
+                    return fail(PK_HIP_EINVAL, "cache_move_dev: page %d is copied from and to", (int)pairs[2 * i]);
+    } catch (...) {
+        return fail(PK_HIP_ENOMEM, "cache_move_dev: host memory for %u pages", dst->pages);
+    }
+    if ((e = pk_hip_init()))
+        return e;
+    if (n == 0)
+        return PK_HIP_OK;
+    PK_LAUNCH(pkq8::launch_cache_move((uint8_t *)dst->data, cache_layer_bytes(dst), (const uint8_t *)src->data,
+                                      cache_layer_bytes(src), src->layers, src->heads * pkq8::cache_record(src->dk),
+                                      pairs, n, table, entries, (hipStream_t)stream),
+              "cache move launch");
+    g_kernel = "cache_move";
+    return PK_HIP_OK;
+}
+
+struct pk_hip_pool {
+    pkq8::PagePool pages;
+    explicit pk_hip_pool(uint32_t n) : pages(n) {}
+};
+
+int pk_hip_pool_create(pk_hip_pool **pool, uint32_t pages) {
+    if (!pool || pages == 0 || pages > 1u << 30)
+        return fail(PK_HIP_EINVAL, "pool_create: 1 to 2^30 pages");
+    try {
+        *pool = new pk_hip_pool(pages);
+    } catch (...) {
+        *pool = nullptr;
+        return fail(PK_HIP_ENOMEM, "pool_create: host memory for %u pages", pages);
+    }
+    return PK_HIP_OK;
+}
+
+void pk_hip_pool_destroy(pk_hip_pool *pool) { delete pool; }
+
+uint32_t pk_hip_pool_free_pages(const pk_hip_pool *pool) { return pool ? pool->pages.free_pages() : 0; }
+
+uint32_t pk_hip_pool_holders(const pk_hip_pool *pool, int32_t id) { return pool ? pool->pages.holders(id) : 0; }
+
+int pk_hip_pool_alloc(pk_hip_pool *pool, int32_t *ids, uint32_t n) {
+    if (!pool || (n && !ids))
+        return fail(PK_HIP_EINVAL, "pool_alloc: pool and ids set");
+    if (!pool->pages.alloc(ids, n))
+        return fail(PK_HIP_ENOMEM, "pool_alloc: %u pages asked for, fewer free", n);
+    return PK_HIP_OK;
+}
+
+int pk_hip_pool_share(pk_hip_pool *pool, const int32_t *ids, uint32_t n) {
+    if (!pool || (n && !ids) || !pool->pages.share(ids, n))
+        return fail(PK_HIP_EINVAL, "pool_share: ids of pages in use");
+    return PK_HIP_OK;
+}
+
+int pk_hip_pool_release(pk_hip_pool *pool, const int32_t *ids, uint32_t n) {
+    if (!pool || (n && !ids) || !pool->pages.release(ids, n))
+        return fail(PK_HIP_EINVAL, "pool_release: ids of pages in use, each at most as often as it has holders");
+    return PK_HIP_OK;
+}
+
+int pk_hip_pool_compact(pk_hip_pool *pool, int32_t *pairs, uint32_t cap, uint32_t *n) {
+    if (!pool || !n || (cap && !pairs))
+        return fail(PK_HIP_EINVAL, "pool_compact: pool, pairs and n set");
+    *n = pool->pages.compact(pairs, cap);
     return PK_HIP_OK;
 }
 

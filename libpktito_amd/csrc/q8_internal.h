@@ -3,6 +3,8 @@
 #ifndef PK_Q8_INTERNAL_H
 #define PK_Q8_INTERNAL_H
 
+#include "cache_layout.h"
+
 #include <hip/hip_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -208,6 +210,34 @@ int launch_search(SearchArgs &a, void *ws, hipStream_t s, const char **name);
 /* tests: false makes the search load its panels each token where they
  * would fit resident; returns the previous setting */
 bool set_search_resident(bool on);
+
+/* The 4-bit cache of keys and values (cache_kernels.hip; data at a layer's
+ * records). Arguments checked by the caller; 0, -2 for shapes no kernel
+ * takes, -1 for a failed launch. */
+int launch_cache_write(uint8_t *data, uint32_t pages, uint32_t G, uint32_t dk, const CacheStreams &st, const float *k,
+                       uint64_t ks, const float *v, uint64_t vs, hipStream_t s);
+int launch_cache_read(const uint8_t *data, uint32_t pages, uint32_t G, uint32_t dk, const CacheStreams &st, float *k,
+                      uint64_t ks, float *v, uint64_t vs, hipStream_t s);
+/* the attention: left and right clipped to what can occur, p at distance
+ * left's row (NULL: content scores alone) */
+struct CacheAttentionCall {
+    float *o;
+    const float *q;
+    uint64_t os, qs;
+    const uint8_t *data;
+    uint32_t pages, G, H, dk;
+    CacheStreams st;
+    int32_t left, right;
+    const float *p, *bias_u, *bias_w;
+    void *ws;
+};
+size_t cache_attention_workspace(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, bool positions,
+                                 int32_t left, int32_t right);
+int launch_cache_attention(const CacheAttentionCall &c, hipStream_t s);
+/* n pairs (from, to) of pages, in every layer (dlayer, slayer bytes a layer) */
+int launch_cache_move(uint8_t *dst, uint64_t dlayer, const uint8_t *src, uint64_t slayer, uint32_t layers,
+                      uint32_t page_bytes, const int32_t *pairs, uint32_t n, int32_t *table, uint64_t entries,
+                      hipStream_t s);
 
 /* Measurement aids (diag_kernels.hip): an empty launch; a streaming read of
  * bytes (a multiple of 16) at p, 16-byte aligned. */

@@ -1,0 +1,300 @@
+"""The 4-bit cache of keys and values without a GPU: the layout's arithmetic (the
+header the kernels take every address and bound from, compiled for the host),
+the pool of pages, and what the entries refuse."""
+import ctypes
+import os
+import random
+import subprocess
+
+import numpy as np
+import pytest
+
+import cache_ref as cr
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+DKS = (32, 64, 96, 128)
+
+
+@pytest.fixture(scope="module")
+def layout(tmp_path_factory):
+    so = str(tmp_path_factory.mktemp("layout") / "layout.so")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-ffp-contract=off", "-shared", "-fPIC",
+                    "-fsanitize=undefined", "-fno-sanitize-recover=all", "-I",
+                    os.path.join(ROOT, "libpktito_amd", "csrc"), os.path.join(ROOT, "tests", "cache_layout_host.cpp"),
+                    "-o", so], check=True)
+    l = ctypes.CDLL(so)
+    f, u, i = ctypes.c_float, ctypes.c_uint32, ctypes.c_int32
+    for name, res, args in (("t_scale", u, [f]), ("t_code", u, [f, f]), ("t_level", f, [u]), ("t_record", u, [u]),
+                            ("t_key_at", u, [u, u]), ("t_value_dword", u, [u] * 4), ("t_frame_of", u, [u] * 3),
+                            ("t_key_scale_at", u, [u, u]), ("t_value_scale_at", u, [u, u]),
+                            ("t_page_ok", ctypes.c_int, [i, u]), ("t_place_stride", u, [u]), ("t_place_pad", u, []),
+                            ("t_lo", i, [i, i]), ("t_hi", i, [i, i, i]),
+                            ("t_span", None, [u, u, u, i, i, i, ctypes.POINTER(i)])):
+        getattr(l, name).restype, getattr(l, name).argtypes = res, args
+    return l
+
+
+def test_scale_is_the_least_that_holds(layout):
+    g = np.random.default_rng(1)
+    tops = np.concatenate([g.standard_normal(3000).astype(np.float32), np.float32(2.0) ** g.uniform(-121, 126.9, 3000),
+                           [2.0 ** -121, np.nextafter(np.float32(2.0 ** 127), np.float32(0)), 6.0, 1.5, 0.75,
+                            np.nextafter(np.float32(6), np.float32(7))]]).astype(np.float32)
+    for top in np.abs(tops):
+        got = layout.t_scale(float(top))
+        want = cr.scale_of(float(top))
+        assert np.uint32(got << 16).view(np.float32) == np.float32(want), top
+        if want:
+            assert 6 * want >= top > 6 * float(np.uint32((got - 1) << 16).view(np.float32))
+    for top in (0.0, np.nextafter(np.float32(2.0 ** -121), np.float32(0)), 2.0 ** 127, 3.4e38, np.inf, np.nan):
+        assert layout.t_scale(float(top)) == 0
+
+
+def test_code_is_the_nearest_level(layout):
+    g = np.random.default_rng(2)
+    for _ in range(40):
+        d = cr.scale_of(float(np.float32(abs(g.standard_normal()) * 10.0 ** g.uniform(-30, 30))))
+        mid = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0]) * d
+        x = np.concatenate([g.uniform(-6, 6, 200) * d, mid, -mid, cr.LEVELS * d, [0.0, -0.0]]).astype(np.float32)
+        x = np.concatenate([x, np.nextafter(x, np.float32(np.inf)), np.nextafter(x, np.float32(-np.inf))])
+        x = x[np.abs(x) <= 6 * d]
+        want = cr.codes_of(x, d)
+        got = np.array([layout.t_code(float(v), d) for v in x], np.uint8)
+        assert np.array_equal(got, want)
+    for c in range(16):
+        assert layout.t_level(c) == cr.LEVELS[c & 7] * (-1 if c & 8 else 1)
+
+
+@pytest.mark.parametrize("dk", DKS)
+def test_record_holds_each_value_once(layout, dk):
+    """Every nibble of a record belongs to one (which, frame, dimension), every
+    scale to one frame; nothing lies outside the record; dwords are aligned."""
+    n = layout.t_record(dk)
+    assert n == cr.record_bytes(dk) and n % 16 == 0
+    used = np.zeros(2 * n, int)
+    for f in range(64):
+        for c in range(dk):
+            used[2 * (layout.t_key_at(dk, f) + c // 2) + c % 2] += 1
+        for at in (layout.t_key_scale_at(dk, f), layout.t_value_scale_at(dk, f)):
+            assert at % 2 == 0
+            used[2 * at:2 * at + 4] += 1
+    pool = cr.Pool(1, 1, 1, dk)
+    for c in range(dk):
+        for g in range(2):
+            for w in range(4):
+                at = layout.t_value_dword(dk, c, g, w)
+                assert at % 4 == 0
+                for i in range(8):
+                    used[2 * (at + i // 2) + i % 2] += 1
+                    byte, shift = pool._value_at(layout.t_frame_of(g, w, i), c)
+                    assert (byte, shift) == (at + i // 2, 4 * (i % 2))
+    assert (used == 1).all()
+
+
+def test_spans_stay_in_bounds(layout):
+    """Whatever the arrays hold: rows in the call, frames in the table, and the
+    position scores' reads in a row's pads."""
+    r = random.Random(3)
+    odd = [0, 1, -1, 2 ** 31 - 1, -2 ** 31, 63, 64, 65, 1000]
+    out = (ctypes.c_int32 * 4)()
+    for _ in range(20000):
+        max_pages = r.choice([1, 2, 3, 100, 1 << 24])
+        rows = r.choice([0, 1, 5, 300, 1 << 22])
+        max_T = r.randint(0, rows)
+        pick = lambda: r.choice(odd) if r.random() < 0.3 else r.randint(0, 400)
+        layout.t_span(max_pages, rows, max_T, pick(), pick(), pick(), out)
+        r0, T, ln, total = out
+        assert 0 <= r0 and 0 <= T <= max_T and r0 + T <= rows
+        assert 0 <= ln <= total <= 64 * max_pages and total <= ln + T
+        left, right = min(r.choice(odd[:1] + odd[5:]), 64 * max_pages - 1), min(r.choice([0, 3, 1000]), max(0, max_T - 1))
+        bw = left + right + 1
+        if T == 0:
+            continue
+        t0 = r.randint(0, T - 1)
+        t1 = min(T - 1, t0 + r.randint(0, 15))
+        j0, j1 = layout.t_lo(ln + t0, left), layout.t_hi(ln + t1, right, total)
+        for pg in {j0 // 64, max(j0 // 64, j1 // 64)}:
+            if 64 * pg > j1:
+                continue
+            assert 0 <= pg < max_pages
+            for pos in (ln + t0, ln + t1):
+                first = layout.t_place_pad() + 64 * pg - (pos - left)
+                assert 0 <= first and first + 64 <= layout.t_place_stride(bw), (pos, left, right, pg)
+    for id, pages, ok in ((0, 1, 1), (1, 1, 0), (-1, 5, 0), (-2 ** 31, 5, 0), (4, 5, 1), (2 ** 31 - 1, 1 << 30, 0)):
+        assert bool(layout.t_page_ok(id, pages)) == bool(ok)
+
+
+# ------------------------------------------------------------------ pool --
+
+def test_pool_counts_holders():
+    import libpktito_amd as pk
+    p = pk.PagePool(130)
+    assert p.free_pages == 130
+    a = p.alloc(3)
+    assert a == [0, 1, 2] and p.free_pages == 127
+    p.share([1, 1])
+    assert [p.holders(i) for i in (0, 1, 2, 3, -1, 130)] == [1, 3, 1, 0, 0, 0]
+    p.release([1, 0, 1])
+    assert p.free_pages == 128 and p.holders(1) == 1 and p.alloc(1) == [0]
+    with pytest.raises(pk.PkHipError) as e:
+        p.alloc(128)
+    assert e.value.code == pk.PK_HIP_ENOMEM and p.free_pages == 127
+    for bad in ([3], [-1], [130], [2, 2]):
+        with pytest.raises(pk.PkHipError) as e:
+            p.release(bad)
+        assert e.value.code == pk.PK_HIP_EINVAL
+        assert [p.holders(i) for i in (0, 1, 2)] == [1, 1, 1]
+    with pytest.raises(pk.PkHipError):
+        p.share([0, 7])
+    assert p.holders(0) == 1
+    p.share([2])
+    p.release([2, 2])                   # both holders in one call: free once
+    assert p.free_pages == 128
+    with pytest.raises(pk.PkHipError):
+        pk.PagePool(0)
+
+
+def test_pool_against_a_model():
+    import libpktito_amd as pk
+    r = random.Random(4)
+    for pages in (1, 63, 64, 200):
+        p, model = pk.PagePool(pages), {}
+        for _ in range(400):
+            what = r.random()
+            free = [i for i in range(pages) if i not in model]
+            if what < 0.4:
+                n = r.randint(0, 5)
+                if n <= len(free):
+                    assert p.alloc(n) == free[:n]
+                    model.update({i: 1 for i in free[:n]})
+                else:
+                    with pytest.raises(pk.PkHipError):
+                        p.alloc(n)
+            elif what < 0.6 and model:
+                ids = r.choices(sorted(model), k=r.randint(1, 3))
+                p.share(ids)
+                for i in ids:
+                    model[i] += 1
+            elif what < 0.9 and model:
+                i = r.choice(sorted(model))
+                p.release([i])
+                model[i] -= 1
+                model = {k: v for k, v in model.items() if v}
+            else:
+                cap = r.choice([0, 1, 2, pages])
+                pairs = (ctypes.c_int32 * (2 * pages + 2))()
+                n = ctypes.c_uint32()
+                assert pk.lib().pk_hip_pool_compact(p.handle, pairs, cap, ctypes.byref(n)) == 0
+                moves = [(pairs[2 * i], pairs[2 * i + 1]) for i in range(n.value)]
+                want = sum(i >= len(model) for i in model)
+                assert len(moves) == min(cap, want)
+                assert len({t for _, t in moves} | {f for f, _ in moves}) == 2 * len(moves)
+                for f, t in moves:
+                    assert f in model and t not in model and t < f
+                    model[t] = model.pop(f)
+                if cap == pages:
+                    assert sorted(model) == list(range(len(model)))
+            assert p.free_pages == pages - len(model)
+            assert [p.holders(i) for i in range(pages)] == [model.get(i, 0) for i in range(pages)]
+
+
+# -------------------------------------------------------------- refusals --
+
+def _calls(pk, **change):
+    """Each entry's return for a call that is in order but for `change` (all have
+    one, so nothing is launched: the pointers stand for device memory)."""
+    v = dict(data=4096, layers=2, pages=8, heads=4, dk=64, table=4096, len=4096, row0=4096, B=2, max_pages=4, rows=5,
+             max_T=3, layer=1, k=4096, ks=256, v=4096, vs=256, o=4096, os=512, q=8192, qs=512, H=8, p=4096, bu=4096,
+             bw=4096, n=9, center=4, ws=4096, ws_bytes=1 << 40)
+    v.update(change)
+    c = pk.Cache(v["data"], v["layers"], v["pages"], v["heads"], v["dk"])
+    st = pk.Streams(v["table"], v["len"], v["row0"], v["B"], v["max_pages"], v["rows"], v["max_T"])
+    pos = pk.Positions(v["p"], v["bu"], v["bw"], v["n"], v["center"])
+    l, r = pk.lib(), ctypes.byref
+    return {
+        "append": lambda: l.pk_hip_cache_append_dev(r(c), v["layer"], v["k"], v["ks"], v["v"], v["vs"], r(st), None),
+        "read": lambda: l.pk_hip_cache_read_dev(r(c), v["layer"], v["k"], v["ks"], v["v"], v["vs"], r(st), None),
+        "attention": lambda: l.pk_hip_attention_cache_dev(v["o"], v["os"], v["q"], v["qs"], r(c), v["layer"], r(st),
+                                                          v["H"], r(pos), 10, 10, v["ws"], v["ws_bytes"], None),
+    }
+
+
+BOTH = ("append", "read")
+ALL = BOTH + ("attention",)
+
+
+@pytest.mark.parametrize("entries,change", [
+    (ALL, {"data": None}), (ALL, {"data": 4100}), (ALL, {"layers": 0}), (ALL, {"pages": 0}), (ALL, {"heads": 0}),
+    (ALL, {"dk": 48}), (ALL, {"dk": 0}), (ALL, {"dk": 160}), (ALL, {"dk": 256}), (ALL, {"pages": 1 << 31}),
+    (ALL, {"layer": 2}), (ALL, {"table": None}), (ALL, {"len": None}), (ALL, {"row0": None}), (ALL, {"max_pages": 0}),
+    (ALL, {"max_pages": (1 << 24) + 1}), (ALL, {"B": 65536}), (ALL, {"rows": (1 << 22) + 1}), (ALL, {"max_T": 6}),
+    (BOTH, {"k": None}), (BOTH, {"v": None}), (BOTH, {"k": 4104}), (BOTH, {"v": 4100}), (BOTH, {"ks": 252}),
+    (BOTH, {"vs": 0}), (BOTH, {"ks": 258}), (BOTH, {"vs": 257}),
+    (("attention",), {"o": None}), (("attention",), {"q": None}), (("attention",), {"o": 4104}),
+    (("attention",), {"q": 4104}), (("attention",), {"os": 508}), (("attention",), {"qs": 508}),
+    (("attention",), {"qs": 514}), (("attention",), {"H": 0}), (("attention",), {"H": 6}),
+    (("attention",), {"p": None}), (("attention",), {"bu": None}), (("attention",), {"bw": None}),
+    (("attention",), {"p": 4104}), (("attention",), {"center": 9}), (("attention",), {"n": 0, "center": 0}),
+    (("attention",), {"ws": None}), (("attention",), {"ws": 4104}), (("attention",), {"ws_bytes": 100}),
+    (("attention",), {"q": 4096, "qs": 516}),
+], ids=lambda v: "-".join(f"{k}={x}" for k, x in v.items()) if isinstance(v, dict) else "")
+def test_refusals(entries, change):
+    import libpktito_amd as pk
+    calls = _calls(pk, **change)
+    for e in entries:
+        assert calls[e]() == pk.PK_HIP_EINVAL, e
+        assert pk.lib().pk_hip_last_error()
+
+
+@pytest.mark.parametrize("pairs,change", [
+    ([(0, 8)], {}), ([(8, 0)], {}), ([(-1, 0)], {}), ([(0, -1)], {}),
+    ([(0, 1), (2, 1)], {}),                     # copied to twice
+    ([(0, 1), (1, 2)], {}), ([(3, 3)], {}),     # copied from and to
+    ([(0, 1), (0, 2)], {"table": 4096}),        # moves to two places
+    ([(i, 4) for i in range(9)], {}),           # more pairs than pages
+    ([(0, 1)], {"dst": dict(dk=32)}), ([(0, 1)], {"dst": dict(heads=2)}), ([(0, 1)], {"dst": dict(layers=1)}),
+    ([(0, 1)], {"dst": dict(pages=4)}),         # one memory, two sizes
+    ([(0, 1)], {"dst": dict(data=8192)}),       # memories that overlap
+    ([(0, 1)], {"dst": dict(data=1 << 30), "table": 4096}),
+])
+def test_move_refusals(pairs, change):
+    import libpktito_amd as pk
+    base = dict(data=4096, layers=2, pages=8, heads=4, dk=64)
+    src = pk.Cache(**base)
+    dst = pk.Cache(**(base | change.get("dst", {})))
+    flat = np.array(pairs, np.int32).reshape(-1)
+    assert pk.lib().pk_hip_cache_move_dev(ctypes.byref(dst), ctypes.byref(src), flat.ctypes.data, len(pairs),
+                                          change.get("table"), 16, None) == pk.PK_HIP_EINVAL
+    assert pk.lib().pk_hip_last_error()
+
+
+def test_sizes():
+    import libpktito_amd as pk
+    for dk in DKS:
+        assert pk.cache_bytes(3, 5, 7, dk) == 3 * 5 * 7 * cr.record_bytes(dk)
+    for bad in ((0, 1, 1, 64), (1, 0, 1, 64), (1, 1, 0, 64), (1, 1, 1, 16), (1, 1, 1025, 64)):
+        assert pk.cache_bytes(*bad) == 0
+
+
+def test_host_tensors_are_refused():
+    import torch
+    import libpktito_amd as pk
+    z = torch.zeros(2, 4, dtype=torch.int32)
+    with pytest.raises(pk.PkHipError, match="device tensor"):
+        pk.CacheStreams(z, z[0, :2], z[0, :3], 4, 2)
+    with pytest.raises(pk.PkHipError, match="device tensor"):
+        pk.DeviceCache(torch.zeros(1 << 20, dtype=torch.uint8), 1, 1, 1, 64)
+
+
+def test_reference_round_trip():
+    """The host model of a pool keeps what its own quantizer gives."""
+    g = np.random.default_rng(5)
+    for dk in DKS:
+        pool = cr.Pool(1, 2, 2, dk)
+        x = g.standard_normal((64, 2, 2 * dk)).astype(np.float32)
+        for f in range(64):
+            pool.write(0, 1, f, x[f, 0], x[f, 1])
+        for h in range(2):
+            for which in range(2):
+                want, _, _ = cr.kept(x[:, which], 2)
+                got = pool.read(0, 1, h)[which]
+                assert np.array_equal(got, want[:, h * dk:(h + 1) * dk])

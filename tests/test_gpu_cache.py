@@ -1,0 +1,617 @@
+"""The 4-bit cache of keys and values on the GPU: writes, reads and moves byte for
+byte against the host model, the attention against 64 bits within the bound
+that 32-bit arithmetic gives (cache_ref.attend), and a stream's life through
+all of them."""
+import random
+import sys
+
+import numpy as np
+import pytest
+
+import cache_ref as cr
+
+pytestmark = pytest.mark.gpu
+DKS = (32, 64, 96, 128)
+
+
+def say(*a):
+    print("[case]", *a, flush=True)
+    sys.stdout.flush()
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    assert torch.cuda.is_available()
+    return torch
+
+
+class World:
+    """A cache on the device and its model on the host, with some streams."""
+
+    def __init__(self, pk, torch, lens, Ts, G, dk, seed=0, layers=1, layer=0, first=0, tail=0, spare=2, max_pages=None,
+                 slack_T=0):
+        self.pk, self.torch, self.layer = pk, torch, layer
+        self.g = np.random.default_rng(seed)
+        self.G, self.dk, self.lens, self.Ts = G, dk, list(lens), list(Ts)
+        B = len(lens)
+        held = [-(-(a + t) // 64) for a, t in zip(lens, Ts)]
+        mp = max_pages or max(1, max(held, default=1))
+        ids = self.g.permutation(sum(held) + spare)
+        self.table = np.full((B, mp), -1, np.int32)
+        at = 0
+        for b, h in enumerate(held):
+            h = min(h, mp)
+            self.table[b, :h] = ids[at:at + h]
+            at += h
+        self.row0 = np.cumsum([first] + self.Ts).astype(np.int32)
+        self.rows = int(self.row0[-1]) + tail
+        self.pool = cr.Pool(layers, len(ids), G, dk)
+        self.max_T = min(self.rows, max(self.Ts, default=0) + slack_T)
+        self.upload()
+
+    def dev(self, a):
+        return self.torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+    def upload(self):
+        d = self.pool.data
+        self.data = self.dev(d)
+        self.cache = self.pk.DeviceCache(self.data, *d.shape[:3], self.dk)
+        self.streams = self.pk.CacheStreams(self.dev(self.table), self.dev(np.array(self.lens, np.int32)),
+                                            self.dev(self.row0), self.rows, self.max_T)
+
+    def fill(self, upto=None, scale=1.0):
+        """Random keys and values for every frame of every stream, on the host;
+        frames of no stream keep bytes that are NaN as scales."""
+        for b in range(len(self.lens)):
+            total = self.lens[b] + self.Ts[b] if upto is None else upto[b]
+            for f in range(min(total, 64 * self.table.shape[1])):
+                pg = self.table[b, f // 64]
+                if 0 <= pg < self.pool.data.shape[1]:
+                    x = scale * self.g.standard_normal((2, self.G * self.dk))
+                    self.pool.write(self.layer, pg, f % 64, *x.astype(np.float32))
+        self.upload()
+
+    def positions(self, H, back, ahead, biased=True):
+        n = back + ahead + 1
+        p = self.g.standard_normal((n, H * self.dk)).astype(np.float32)
+        u, w = (0.3 * self.g.standard_normal((2, H * self.dk))).astype(np.float32)
+        return p, back, u, w
+
+    def attend(self, q, H, positions=None, left=None, right=None, layer=None):
+        """The device's attention of q, into rows that hold a mark before."""
+        torch = self.torch
+        layer = self.layer if layer is None else layer
+        pos = None if positions is None else (self.dev(positions[0]), positions[1], self.dev(positions[2]),
+                                              self.dev(positions[3]))
+        o = torch.full((self.rows, H * self.dk), 7.25, device="cuda")
+        need = self.cache.attention_workspace(self.streams, H, pos, left, right)
+        ws = torch.full((max(1, need),), 0xff, dtype=torch.uint8, device="cuda")
+        self.cache.attention(o, layer, self.dev(q), self.streams, H, ws, pos, left, right)
+        torch.cuda.synchronize()
+        return o.cpu().numpy()
+
+    def check(self, H, positions=None, left=None, right=None, qscale=1.0, q=None):
+        if q is None:
+            q = (qscale * self.g.standard_normal((self.rows, H * self.dk))).astype(np.float32)
+        got = self.attend(q, H, positions, left, right)
+        want, bound = cr.attend(self.pool, self.layer, self.table, self.lens, self.row0, self.rows, q, H, positions,
+                                left, right)
+        none = np.isnan(want)
+        assert (got[none] == 7.25).all()            # rows of no stream: as they were
+        off = np.abs(np.where(none, 0, got - np.where(none, 0, want)))
+        assert np.isfinite(got).all()
+        assert (off <= bound + none).all(), (off.max(), bound[off > bound].min())
+        ref = np.linalg.norm(want[~none])
+        assert np.linalg.norm(off[~none]) <= 1e-5 * ref + 1e-30
+        return got
+
+
+# ----------------------------------------------------------- write, read --
+
+@pytest.mark.parametrize("dk", DKS)
+@pytest.mark.parametrize("G", [1, 3])
+def test_write_bytes(hip, torch, dk, G):
+    """Streams that begin and end anywhere in a page: the bytes are the model's,
+    and every byte that is not the call's keeps what it held."""
+    say("write", dk, G)
+    lens, Ts = [0, 1, 63, 64, 50, 0, 127, 3], [1, 2, 3, 64, 90, 0, 1, 130]
+    w = World(hip, torch, lens, Ts, G, dk, seed=dk + G, layers=2, layer=1, first=2, tail=3)
+    x = w.g.standard_normal((2, w.rows, G * dk)).astype(np.float32)
+    x[0, 2, :5] = [0.0, -0.0, 1e-30, -1e-30, 2.0]
+    x[:, 3] = 0.0
+    x[0, 4, 0], x[1, 5, dk - 1], x[0, 6, 1] = np.nan, np.inf, -np.inf
+    x[1, 7, 0] = 2.0 ** 127
+    x[0, 8] *= np.float32(2.0 ** -124)
+    w.cache.append(1, w.dev(x[0]), w.dev(x[1]), w.streams)
+    ko, vo = (torch.full((w.rows, G * dk), 7.25, device="cuda") for _ in range(2))
+    w.cache.read(1, ko, vo, w.streams)
+    torch.cuda.synchronize()
+    for b in range(len(lens)):
+        for t in range(Ts[b]):
+            f, r = lens[b] + t, w.row0[b] + t
+            w.pool.write(1, w.table[b, f // 64], f % 64, x[0, r], x[1, r])
+    assert np.array_equal(w.data.cpu().numpy(), w.pool.data)
+    for got, which in ((ko, 0), (vo, 1)):
+        got = got.cpu().numpy()
+        want, _, _ = cr.kept(x[which], G)
+        assert np.array_equal(got[2:w.row0[-1]], want[2:w.row0[-1]].astype(np.float32))
+        assert (got[:2] == 7.25).all() and (got[w.row0[-1]:] == 7.25).all()
+
+
+@pytest.mark.parametrize("T", [1, 2, 31, 64, 65, 200])
+def test_write_in_pieces(hip, torch, T):
+    """The same frames written in one call and in chunks of T: the same bytes."""
+    say("pieces", T)
+    G, dk, n = 2, 64, 201
+    w = World(hip, torch, [0], [n], G, dk, seed=T)
+    x = w.g.standard_normal((2, n, G * dk)).astype(np.float32)
+    k, v = w.dev(x[0]), w.dev(x[1])
+    w.cache.append(0, k, v, w.streams)
+    whole = w.data.clone()
+    w.data.fill_(0xff)
+    length = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for a in range(0, n, T):
+        m = min(T, n - a)
+        st = hip.CacheStreams(w.streams.table, length, w.dev(np.array([0, m], np.int32)), m, m)
+        w.cache.append(0, k[a:a + m], v[a:a + m], st)
+        length += m
+    assert torch.equal(w.data, whole)
+
+
+def test_write_strides_and_holes(hip, torch):
+    """Rows at strides, a table with entries outside the pool, frames past the
+    table, a stream with more rows than max_T: nothing else is touched."""
+    say("strides")
+    G, dk = 2, 32
+    w = World(hip, torch, [60, 10, 100], [80, 20, 70], G, dk, seed=3, max_pages=2)
+    w.table[0, 1] = w.pool.data.shape[1]            # one past the pool
+    w.table[2, 0] = -5
+    w.max_T = 70
+    w.upload()
+    x = w.g.standard_normal((2, w.rows, G * dk + 12)).astype(np.float32)
+    k, v = w.dev(x[0]), w.dev(x[1])
+    w.cache.append(0, k[:, 4:4 + G * dk], v[:, 8:8 + G * dk], w.streams)
+    for b in range(3):
+        for t in range(min(70, w.Ts[b])):
+            f, r = w.lens[b] + t, w.row0[b] + t
+            if f < 128 and 0 <= w.table[b, f // 64] < w.pool.data.shape[1]:
+                w.pool.write(0, w.table[b, f // 64], f % 64, x[0, r, 4:4 + G * dk], x[1, r, 8:8 + G * dk])
+    assert np.array_equal(w.data.cpu().numpy(), w.pool.data)
+    out = torch.full((2, w.rows, G * dk + 4), 7.25, device="cuda")
+    w.cache.read(0, out[0, :, :G * dk], out[1, :, :G * dk], w.streams)
+    got = out.cpu().numpy()
+    assert (got[:, :, G * dk:] == 7.25).all()
+    for which, cut in ((0, 4), (1, 8)):
+        want, _, _ = cr.kept(x[which][:, cut:cut + G * dk], G)
+        for b in range(3):
+            for t in range(w.Ts[b]):
+                f, r = w.lens[b] + t, w.row0[b] + t
+                if t >= 70:
+                    assert (got[which, r, :G * dk] == 7.25).all()
+                elif f < 128 and 0 <= w.table[b, f // 64] < w.pool.data.shape[1]:
+                    assert np.array_equal(got[which, r, :G * dk], want[r].astype(np.float32))
+                else:
+                    assert (got[which, r, :G * dk] == 0).all()
+
+
+# ------------------------------------------------------------- attention --
+
+@pytest.mark.parametrize("dk", DKS)
+@pytest.mark.parametrize("H,G", [(1, 1), (4, 4), (6, 2), (3, 1)])
+@pytest.mark.parametrize("with_positions", [False, True])
+def test_attention(hip, torch, dk, H, G, with_positions):
+    """Ragged streams from nothing to a few pages, a row gap at both ends."""
+    say("attention", dk, H, G, with_positions)
+    w = World(hip, torch, [0, 1, 63, 64, 130, 200, 0, 5], [1, 1, 1, 2, 17, 0, 40, 3], G, dk, seed=dk + H, first=1, tail=2)
+    w.fill()
+    pos = w.positions(H, 210, 60) if with_positions else None
+    w.check(H, pos)
+
+
+@pytest.mark.parametrize("left,right", [(0, 0), (3, 0), (None, 0), (0, None), (64, 5), (70, 63), (1 << 30, 1 << 30)])
+@pytest.mark.parametrize("with_positions", [False, True])
+def test_windows(hip, torch, left, right, with_positions):
+    say("window", left, right, with_positions)
+    w = World(hip, torch, [0, 90, 64, 150], [70, 33, 1, 2], 2, 64, seed=11)
+    w.fill()
+    w.check(4, w.positions(4, 160, 75) if with_positions else None, left, right)
+
+
+@pytest.mark.parametrize("back,ahead", [(0, 0), (7, 0), (0, 9), (40, 3), (300, 200)])
+def test_positions_table_bounds_the_window(hip, torch, back, ahead):
+    """Distances that the table has no row for are not attended; rows of it
+    that no frame needs may hold anything."""
+    say("table", back, ahead)
+    w = World(hip, torch, [100, 3], [20, 50], 2, 32, seed=12)
+    w.fill()
+    p, c, u, v = w.positions(2, back, ahead)
+    if back >= 300:
+        p[:c - 119] = np.nan
+        p[c + 50:] = np.inf
+    w.check(2, (p, c, u, v))
+
+
+def test_single_frames(hip, torch):
+    """One row a stream, many streams of every length around the pages."""
+    say("single")
+    lens = list(range(0, 140, 3)) + [320]
+    w = World(hip, torch, lens, [1] * len(lens), 2, 128, seed=13)
+    w.fill()
+    w.check(2, w.positions(2, 320, 0))
+    w.check(8)
+
+
+def test_long_stream(hip, torch):
+    """One row against 70 pages, and chunks against them."""
+    say("long")
+    for T in (1, 3, 30):
+        w = World(hip, torch, [4470], [T], 1, 64, seed=14 + T)
+        w.fill()
+        w.check(1, w.positions(1, 4500, 30))
+        w.check(4, left=2000)
+
+
+def test_rows_that_attend_nothing(hip, torch):
+    """Holes in the table (given up pages, ids outside the pool, of every size):
+    their frames are skipped, and a row with nothing else is zeros."""
+    say("holes")
+    w = World(hip, torch, [200, 64, 10, 128], [3, 2, 4, 20], 2, 64, seed=15)
+    w.fill()
+    w.table[0, :2] = -1
+    w.table[1] = [-1, 2 ** 31 - 1, -2 ** 31, w.pool.data.shape[1]]
+    w.table[2] = -7
+    w.upload()
+    for pos in (None, w.positions(4, 210, 20)):
+        for left in (None, 5):
+            got = w.check(4, pos, left)
+            assert (got[3:9] == 0).all()
+
+
+def test_single_dimension_precision(hip, torch):
+    """A query with one dimension set scores with one term, so little is rounded:
+    a score's product by its key's level is exact (8 + 8 + 8 bits), then a
+    rounding each for the key's scale, the scale to powers of two and the
+    exponential's argument, relative to the score; the output's few terms are
+    positive. Third pieces that went missing would be 2^-16."""
+    say("precision")
+    dk = 64
+    w = World(hip, torch, [9], [1], 1, dk, seed=16)
+    w.fill(scale=1.0)
+    for i in range(200):
+        q = np.zeros((1, dk), np.float32)
+        q[0, i % dk] = np.float32(w.g.uniform(-8, 8))
+        got = w.attend(q, 1)[0]
+        k, v = (a[:10] for a in w.pool.read(0, w.table[0, 0], 0))
+        s = k @ q[0].astype(np.float64) / np.sqrt(dk)
+        e = np.exp(s - s.max())
+        want = e @ v / e.sum()
+        tol = (8 + 8 * (np.abs(s).max() + 1) + 3 * 10 + 8) * 2.0 ** -24 * (e @ np.abs(v)) / e.sum()
+        assert (np.abs(got - want) <= tol).all(), (np.abs(got - want) / tol).max()
+
+
+@pytest.mark.parametrize("kscale,qscale", [(1e-18, 1e18), (1e18, 1e-18), (1e-30, 1e30), (3.0, 8.0)])
+def test_magnitudes(hip, torch, kscale, qscale):
+    """Keys and queries far from one, and peaked softmaxes."""
+    say("magnitudes", kscale, qscale)
+    w = World(hip, torch, [100, 7], [5, 2], 1, 128, seed=17)
+    w.fill(scale=kscale)
+    w.check(1, None, qscale=qscale)
+
+
+def test_bad_values_stay_in_their_row(hip, torch):
+    """A query that holds a NaN makes its own head's row NaN and no other."""
+    say("nan rows")
+    w = World(hip, torch, [70, 5], [20, 4], 2, 64, seed=18)
+    w.fill()
+    q = w.g.standard_normal((24, 4 * 64)).astype(np.float32)
+    for pos in (None, w.positions(4, 100, 30)):
+        clean = w.attend(q, 4, pos)
+        bad = q.copy()
+        bad[5, 70], bad[22, 0] = np.nan, np.inf
+        got = w.attend(bad, 4, pos)
+        assert np.isnan(got[5, 64:128]).all() and np.isnan(got[22, :64]).all()
+        clean[5, 64:128] = clean[22, :64] = got[5, 64:128] = got[22, :64] = 0
+        assert np.array_equal(clean, got)
+
+
+def test_strided_and_in_place(hip, torch):
+    """Queries inside wider rows, outputs into wider rows, and over the queries."""
+    say("strides")
+    w = World(hip, torch, [100, 30], [9, 40], 2, 64, seed=19)
+    w.fill()
+    H, n = 4, 49
+    q = w.g.standard_normal((n, H * 64)).astype(np.float32)
+    pos = w.positions(H, 140, 40)
+    dpos = (w.dev(pos[0]), pos[1], w.dev(pos[2]), w.dev(pos[3]))
+    want = w.attend(q, H, pos)
+    ws = torch.empty(w.cache.attention_workspace(w.streams, H, dpos), dtype=torch.uint8, device="cuda")
+    wide = torch.full((n, H * 64 + 20), 7.25, device="cuda")
+    wide[:, 8:8 + H * 64] = w.dev(q)
+    out = torch.full((n, H * 64 + 4), 7.25, device="cuda")
+    w.cache.attention(out[:, :H * 64], 0, wide[:, 8:8 + H * 64], w.streams, H, ws, dpos)
+    assert np.array_equal(out[:, :H * 64].cpu().numpy(), want) and (out[:, H * 64:] == 7.25).all()
+    w.cache.attention(wide[:, 8:8 + H * 64], 0, wide[:, 8:8 + H * 64], w.streams, H, ws, dpos)
+    assert np.array_equal(wide[:, 8:8 + H * 64].cpu().numpy(), want)
+    assert (wide[:, :8] == 7.25).all() and (wide[:, 8 + H * 64:] == 7.25).all()
+
+
+def test_descriptors_out_of_range(hip, torch):
+    """Lengths and rows that no stream can have are cut to the call's and the
+    table's bounds: the kernels' other rows are right and nothing else moves."""
+    say("descriptors")
+    w = World(hip, torch, [30, 20, 10], [4, 5, 6], 1, 32, seed=20, tail=4)
+    w.fill(upto=[34, 26, 16])               # one frame more of stream 1, which its longer rows then attend
+    q = w.g.standard_normal((w.rows, 32)).astype(np.float32)
+    good = w.attend(q, 1)
+    w.streams.len[0] = -9                   # as 0
+    w.streams.row0[2] = 2 ** 31 - 1         # stream 1's rows to the end (max_T of them), stream 2 without any
+    got = w.attend(q, 1)
+    lens, row0 = [0, 20, 10], np.array([0, 4, 10, 10])
+    want, bound = cr.attend(w.pool, 0, w.table, lens, row0, w.rows, q, 1)
+    assert (np.abs(got[:10] - want[:10]) <= bound[:10]).all()
+    assert (got[10:] == 7.25).all()
+    assert not np.array_equal(good[:4], got[:4])
+
+
+def test_ids_and_offsets_past_32_bits(hip, torch):
+    """A pool of more than 4 GiB: its last pages."""
+    say("large pool")
+    G, dk, pages = 8, 128, 66000
+    n = hip.cache_bytes(1, pages, G, dk)
+    assert n > 1 << 32
+    data = torch.zeros(n, dtype=torch.uint8, device="cuda")
+    cache = hip.DeviceCache(data, 1, pages, G, dk)
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    st = hip.CacheStreams(i32([pages - 1, pages - 2]), i32(60), i32(0, 10), 10, 10)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v, q = (torch.randn(10, G * dk, device="cuda", generator=g) for _ in range(3))
+    cache.append(0, k, v, st)
+    small = hip.DeviceCache(torch.zeros(hip.cache_bytes(1, 2, G, dk), dtype=torch.uint8, device="cuda"), 1, 2, G, dk)
+    st2 = hip.CacheStreams(i32([1, 0]), st.len, st.row0, 10, 10)
+    small.append(0, k, v, st2)
+    rec = G * cr.record_bytes(dk)
+    assert torch.equal(data[-2 * rec:], small.data) and small.data.any()
+    o, o2 = torch.empty_like(q), torch.empty_like(q)
+    need = cache.attention_workspace(st, G, None)
+    ws = torch.empty(max(16, need), dtype=torch.uint8, device="cuda")
+    cache.attention(o, 0, q, st, G, ws)
+    small.attention(o2, 0, q, st2, G, ws)
+    assert torch.equal(o, o2) and torch.isfinite(o).all()
+    cache.move([(pages - 1, 0)])
+    assert torch.equal(data[:rec], data[-rec:])
+
+
+# ------------------------------------------------------------------ move --
+
+@pytest.mark.parametrize("dk,G,layers,n", [(32, 1, 1, 1), (128, 8, 3, 2), (96, 3, 2, 5), (64, 4, 1, 300)])
+def test_move(hip, torch, dk, G, layers, n):
+    say("move", dk, G, layers, n)
+    pages = 2 * n + 3
+    r = random.Random(n)
+    g = torch.Generator(device="cuda").manual_seed(n)
+    shape = (layers, pages, G, cr.record_bytes(dk))
+    data = torch.randint(0, 256, shape, dtype=torch.uint8, device="cuda", generator=g)
+    before = data.cpu().numpy()
+    ids = r.sample(range(pages), 2 * n)
+    pairs = list(zip(ids[:n], ids[n:]))
+    cache = hip.DeviceCache(data, layers, pages, G, dk)
+    table = torch.randint(-1, pages, (7, 11), dtype=torch.int32, device="cuda", generator=g)
+    want = table.cpu().numpy()
+    cache.move(pairs, table)
+    to = dict(pairs)
+    assert np.array_equal(table.cpu().numpy(), np.vectorize(lambda i: to.get(i, i))(want))
+    after = before.copy()
+    for f, t in pairs:
+        after[:, t] = before[:, f]
+    assert np.array_equal(data.cpu().numpy(), after)
+    # to another cache, of another size; one page to several places
+    other = torch.zeros(layers, pages + 5, G, cr.record_bytes(dk), dtype=torch.uint8, device="cuda")
+    hip.DeviceCache(other, layers, pages + 5, G, dk).move([(0, pages + 4), (0, 1), (2, 0)], source=cache)
+    got = other.cpu().numpy()
+    assert np.array_equal(got[:, pages + 4], after[:, 0]) and np.array_equal(got[:, 1], after[:, 0])
+    assert np.array_equal(got[:, 0], after[:, 2]) and not got[:, 2:pages + 4].any()
+    cache.move([])
+
+
+# ------------------------------------------------------ a stream's life --
+
+def _segment_attention(hip, torch, q, k, v, p, u, w, T, D, H):
+    """The library's whole-segment attention over the same float inputs."""
+    o = torch.empty(T, D, device="cuda")
+    ws = torch.empty(hip.attention_workspace(T, H), dtype=torch.uint8, device="cuda")
+    hip.attention_dev(o, q, k, v, p, u, w, T, D, H, ws)
+    return o
+
+
+def test_whole_segment_is_the_encoders_attention(hip, torch):
+    """A segment written at once and attended whole, its kept values given to the
+    encoder's own attention: the same function. Both are within their 32-bit
+    bounds of the same value; the bound is the cache's, twice."""
+    say("segment")
+    T, H, dk = 137, 2, 64
+    D = H * dk
+    w = World(hip, torch, [0], [T], H, dk, seed=21)
+    k, v, q = (w.dev(w.g.standard_normal((T, D)).astype(np.float32)) for _ in range(3))
+    p, c, u, b = w.positions(H, T - 1, T - 1)
+    w.cache.append(0, k, v, w.streams)
+    ko, vo = torch.empty_like(k), torch.empty_like(v)
+    w.cache.read(0, ko, vo, w.streams)
+    dp, du, db = w.dev(p), w.dev(u), w.dev(b)
+    want = _segment_attention(hip, torch, q, ko, vo, dp, du, db, T, D, H).cpu().numpy()
+    got = w.attend(q.cpu().numpy(), H, (p, c, u, b))
+    w.pool.data = w.data.cpu().numpy()
+    _, bound = cr.attend(w.pool, 0, w.table, w.lens, w.row0, T, q.cpu().numpy(), H, (p, c, u, b))
+    assert (np.abs(got - want) <= 2 * bound).all()
+
+
+def test_stream_in_chunks_is_the_segment(hip, torch):
+    """Audio heard a chunk at a time, two streams side by side, one forked on the
+    way and the pool compacted under them: each step's causal outputs are the
+    rows of one causal pass over all the frames."""
+    say("life")
+    H, dk, n = 2, 64, 150
+    D = H * dk
+    g = torch.Generator(device="cuda").manual_seed(22)
+    x = torch.randn(3, 2, n, D, device="cuda", generator=g)      # q, k, v of two streams
+    p = torch.randn(n, D, device="cuda", generator=g)
+    u, b = 0.1 * torch.randn(2, D, device="cuda", generator=g)
+    pos = (p, n - 1, u, b)
+    pages = 16
+    cache = hip.DeviceCache(torch.zeros(hip.cache_bytes(1, pages, H, dk), dtype=torch.uint8, device="cuda"), 1, pages, H, dk)
+    pool = hip.PagePool(pages)
+    pool.alloc(2)                                                # someone else's, freed later
+    table = torch.full((3, 3), -1, dtype=torch.int32, device="cuda")
+    length = torch.zeros(3, dtype=torch.int32, device="cuda")
+    ids, have = [[], [], []], [0, 0, 0]
+
+    def hold(s, frames):
+        while 64 * len(ids[s]) < frames:
+            ids[s] += pool.alloc(1)
+            table[s, len(ids[s]) - 1] = ids[s][-1]
+
+    def step(who, T):
+        """T more frames of the streams `who` ((stream, whose audio) pairs)"""
+        rows = [0, 0, 0, 0]
+        for s in range(3):
+            rows[s + 1] = rows[s] + (T if s in dict(who) else 0)
+            if s in dict(who):
+                hold(s, have[s] + T)
+        qkv = [torch.cat([x[i, a, have[s]:have[s] + T] for s, a in who]).contiguous() for i in range(3)]
+        st = hip.CacheStreams(table, length, torch.tensor(rows, dtype=torch.int32, device="cuda"), rows[3], T)
+        cache.append(0, qkv[1], qkv[2], st)
+        o = torch.empty_like(qkv[0])
+        ws = torch.empty(cache.attention_workspace(st, H, pos, None, 0), dtype=torch.uint8, device="cuda")
+        cache.attention(o, 0, qkv[0], st, H, ws, pos, None, 0)
+        for i, (s, a) in enumerate(who):
+            outs[s].append(o[i * T:(i + 1) * T])
+            have[s] += T
+            length[s] += T
+
+    outs = [[], [], []]
+    for T in (1, 13, 1, 40, 15):                                 # 70 frames of both
+        step([(0, 0), (1, 1)], T)
+    ids[2] = pool.fork(cache, ids[0], have[0])
+    assert ids[2][0] == ids[0][0] and ids[2][1] != ids[0][1] and pool.holders(ids[0][0]) == 2
+    table[2, :2] = torch.tensor(ids[2], dtype=torch.int32)
+    have[2], length[2] = have[0], have[0]
+    outs[2] = list(outs[0])
+    for T in (20, 1, 9):                                         # 100 of all three; the fork hears stream 1's audio
+        step([(0, 0), (1, 1), (2, 1)], T)
+    pool.release([0, 1])
+    moved = pool.compact(cache, table)
+    assert moved and pool.free_pages == pages - 5
+    ids = [[i for i in row if i >= 0] for row in table.cpu().tolist()]
+    assert max(map(max, ids)) == 4
+    for T in (28, 22):
+        step([(0, 0), (1, 1), (2, 1)], T)
+    k2, v2 = (torch.cat([x[i, 0, :70], x[i, 1, 70:]]) for i in (1, 2))
+    q2 = torch.cat([x[0, 0, :70], x[0, 1, 70:]])
+    st = hip.CacheStreams(torch.tensor([[0, 1, 2]], dtype=torch.int32, device="cuda"),
+                          torch.zeros(1, dtype=torch.int32, device="cuda"),
+                          torch.tensor([0, n], dtype=torch.int32, device="cuda"), n, n)
+    other = hip.DeviceCache(torch.zeros(hip.cache_bytes(1, 3, H, dk), dtype=torch.uint8, device="cuda"), 1, 3, H, dk)
+    ws = torch.empty(other.attention_workspace(st, H, pos, None, 0), dtype=torch.uint8, device="cuda")
+    for s, (q, k, v) in enumerate(((x[0, 0], x[1, 0], x[2, 0]), (x[0, 1], x[1, 1], x[2, 1]), (q2, k2, v2))):
+        other.append(0, k.contiguous(), v.contiguous(), st)
+        o = torch.empty(n, D, device="cuda")
+        other.attention(o, 0, q.contiguous(), st, H, ws, pos, None, 0)
+        host = cr.Pool(1, 3, H, dk)
+        host.data = other.data.cpu().numpy().reshape(host.data.shape)
+        _, bound = cr.attend(host, 0, np.array([[0, 1, 2]]), [0], [0, n], n, q.cpu().numpy(), H,
+                             (p.cpu().numpy(), n - 1, u.cpu().numpy(), b.cpu().numpy()), None, 0)
+        off = np.abs((torch.cat(outs[s]) - o).cpu().numpy())
+        assert (off <= 2 * bound).all(), (s, (off / bound).max())
+
+
+def test_graph_follows_the_streams(hip, torch):
+    """A step captured once and replayed as the streams grow (their lengths and
+    tables updated in place, the program's own work between replays) gives what
+    eager steps give."""
+    say("graph")
+    H, dk, T, steps = 2, 64, 3, 6
+    D = H * dk
+    g = torch.Generator(device="cuda").manual_seed(23)
+    x = torch.randn(steps, 3, 2 * T, D, device="cuda", generator=g)
+    p = torch.randn(200, D, device="cuda", generator=g)
+    pos = (p, 190, torch.zeros(D, device="cuda"), torch.zeros(D, device="cuda"))
+    row0 = torch.tensor([0, T, 2 * T], dtype=torch.int32, device="cuda")
+
+    def world():
+        cache = hip.DeviceCache(torch.zeros(hip.cache_bytes(1, 6, H, dk), dtype=torch.uint8, device="cuda"), 1, 6, H, dk)
+        table = torch.tensor([[0, 2, 4], [1, 3, 5]], dtype=torch.int32, device="cuda")
+        length = torch.tensor([60, 125], dtype=torch.int32, device="cuda")
+        st = hip.CacheStreams(table, length, row0, 2 * T, T)
+        ws = torch.empty(cache.attention_workspace(st, H, pos), dtype=torch.uint8, device="cuda")
+        return cache, st, ws, torch.empty(2 * T, D, device="cuda")
+
+    def step(c, st, ws, o, a):
+        c.append(0, a[1], a[2], st)
+        c.attention(o, 0, a[0], st, H, ws, pos)
+
+    eager = world()
+    want = []
+    for i in range(steps):
+        step(*eager, x[i])
+        eager[1].len.add_(T)
+        want.append(eager[3].clone())
+    c = world()
+    a = x[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(*c, a)
+    c[0].data.zero_()
+    for i in range(steps):
+        a.copy_(x[i])
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(c[3], want[i]), i
+        c[1].len.add_(T)
+        (torch.randn(512, 512, device="cuda") @ torch.randn(512, 512, device="cuda")).sum().item()
+    assert torch.equal(c[0].data, eager[0].data)
+
+
+def test_two_streams_of_work(hip, torch):
+    """Calls on two streams at once, a workspace each."""
+    say("two streams")
+    w = World(hip, torch, [300, 200], [4, 30], 2, 64, seed=24)
+    w.fill()
+    H = 4
+    q = [w.dev(w.g.standard_normal((34, H * 64)).astype(np.float32)) for _ in range(2)]
+    want = [w.attend(a.cpu().numpy(), H) for a in q]
+    need = max(16, w.cache.attention_workspace(w.streams, H, None))
+    ws = [torch.empty(need, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    ss = [torch.cuda.Stream() for _ in range(2)]
+    o = [torch.empty_like(a) for a in q]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, s in enumerate(ss):
+            with torch.cuda.stream(s):
+                w.cache.attention(o[i], 0, q[i], w.streams, H, ws[i])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert np.array_equal(o[i].cpu().numpy(), want[i])
+
+
+def test_same_call_same_bits(hip, torch):
+    say("repeat")
+    w = World(hip, torch, [700, 20, 64], [2, 50, 1], 2, 128, seed=25)
+    w.fill()
+    q = w.g.standard_normal((53, 256)).astype(np.float32)
+    pos = w.positions(2, 720, 60)
+    first = w.attend(q, 2, pos)
+    for _ in range(5):
+        assert np.array_equal(w.attend(q, 2, pos), first)
+
+
+def test_nothing_to_do(hip, torch):
+    say("empty")
+    w = World(hip, torch, [10, 20], [0, 0], 2, 64, seed=26, tail=2)
+    w.fill()
+    q = w.g.standard_normal((2, 128)).astype(np.float32)
+    assert (w.attend(q, 2) == 7.25).all()
+    z = torch.zeros(0, dtype=torch.int32, device="cuda")
+    st = hip.CacheStreams(z.reshape(0, 1), z, torch.zeros(1, dtype=torch.int32, device="cuda"), 0, 0)
+    e = torch.empty(0, 128, device="cuda")
+    assert w.cache.attention_workspace(st, 2, None) == 0
