@@ -7,6 +7,9 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <cmath>
+
 #pragma clang fp contract(off)
 
 namespace pkq8 {
@@ -181,6 +184,9 @@ struct CacheAttention {
     const float *p, *bias_u, *bias_w;
     float *place;                           /* [rows][H][place_stride(bw)] */
     uint32_t bw;
+    /* a stream's tiles of rows a kept head, workgroups that share a tile's pages, what they leave each other */
+    uint32_t tiles, splits;
+    float *parts;
 };
 
 /* The position scores (q + w) . p of every row at every distance that it
@@ -274,23 +280,327 @@ __global__ __launch_bounds__(256) void cache_place_kernel(CacheAttention a) {
     }
 }
 
-/* A workgroup attends for 16 rows of a stream and kept head (a row is a frame
- * and one of the H / G heads that share the kept one), its four waves a page
- * each in turn with the running maximum and sum of a softmax, their sums met
- * in LDS at the end. */
-template <int NS>
-__global__ __launch_bounds__(256) void cache_attention_kernel(CacheAttention a, uint32_t tiles) {
-    constexpr uint32_t dk = 32 * NS, record = kPage * dk + 4 * kPage;
-    const uint32_t g = blockIdx.x % a.G, tile = blockIdx.x / a.G % tiles, b = blockIdx.x / a.G / tiles;
-    const CacheSpan sp = span_of(a.st, b);
-    const uint32_t grp = a.H / a.G;
-    const int32_t nrows = sp.T * (int32_t)grp, rr0 = (int32_t)tile * 16;
-    if (rr0 >= nrows)
+/* Which rows of a stream and kept head a workgroup attends for, and which of
+ * their pages: a stream's rows for a kept head are its frames, each with the
+ * H / G heads that share the kept one; `splits` workgroups share a tile's
+ * pages in runs. */
+struct Share {
+    CacheSpan sp;
+    uint32_t g, b, grp, split;
+    int32_t nrows, rr0;                     /* the stream's rows, the tile's first */
+    int32_t pa, pb;                         /* pages [pa, pb) of the stream */
+    uint64_t unit;                          /* the tile among all of the call's */
+};
+
+template <int R>
+__device__ __forceinline__ bool share_of(const CacheAttention &a, Share &s, uint32_t splits) {
+    uint32_t i = blockIdx.x;
+    s.g = i % a.G, i /= a.G;
+    s.split = i % splits, i /= splits;
+    const uint32_t tile = i % a.tiles;
+    s.b = i / a.tiles;
+    s.sp = span_of(a.st, s.b);
+    s.grp = a.H / a.G;
+    s.nrows = s.sp.T * (int32_t)s.grp;
+    s.rr0 = (int32_t)tile * R;
+    if (s.rr0 >= s.nrows)
+        return false;
+    const int32_t t0 = s.rr0 / (int32_t)s.grp, t1 = min(s.rr0 + R - 1, s.nrows - 1) / (int32_t)s.grp;
+    const int32_t j0 = cache_lo(s.sp.len + t0, a.left), j1 = cache_hi(s.sp.len + t1, a.right, s.sp.total);
+    const int32_t p0 = j0 / (int32_t)kPage, p1 = j1 < j0 ? p0 : j1 / (int32_t)kPage + 1;
+    const int32_t each = (p1 - p0 + (int32_t)splits - 1) / (int32_t)splits;
+    s.pa = min(p0 + (int32_t)s.split * each, p1);
+    s.pb = min(s.pa + each, p1);
+    s.unit = ((uint64_t)s.b * a.tiles + tile) * a.G + s.g;
+    return true;
+}
+
+/* the pages of a wave, 64 at a time: page `first + 4 i` is lane i's, and a bit
+ * of the mask is set where the table has one */
+__device__ __forceinline__ uint64_t page_ids(const CacheAttention &a, const Share &s, int32_t first, int32_t &id) {
+    const int32_t pg = first + 4 * (int32_t)(threadIdx.x & 63);
+    id = pg < s.pb ? a.st.table[(uint64_t)s.b * a.st.max_pages + pg] : -1;
+    return __ballot(cache_page_ok(id, a.pages));
+}
+
+__device__ __forceinline__ float bf_lo(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float bf_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+__device__ __forceinline__ float bf_of(v2u u, int r) { return r % 2 ? bf_hi(u[r / 2]) : bf_lo(u[r / 2]); }
+
+/* The maximum and the sum over each 16 lanes, in all of them. */
+__device__ __forceinline__ float row_max(float v) {
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, false)));
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xF, 0xF, false)));
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, false)));
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xF, 0xF, false)));
+}
+__device__ __forceinline__ float row_sum(float v) {
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, false));
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xF, 0xF, false));
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, false));
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xF, 0xF, false));
+}
+
+/* Parts of softmaxes over disjoint frames, n of them with their maxima and
+ * sums, as one: sum(part e^(top - m)) / sum(sum e^(top - m)). Parts that
+ * attended nothing have a maximum of -infinity and a sum of 0; a NaN among
+ * the scores is in the sum and stays. */
+template <int N, typename P>
+__device__ __forceinline__ v4f joined(int n, P part, float &m, float &l) {
+    m = -INFINITY;
+    l = 0.0f;
+    float top, sum;
+    v4f y = { 0.0f, 0.0f, 0.0f, 0.0f }, o;
+#pragma unroll N
+    for (int i = 0; i < n; i++) {
+        part(i, top, sum, nullptr);
+        m = fmaxf(m, top);
+    }
+    const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll N
+    for (int i = 0; i < n; i++) {
+        part(i, top, sum, &o);
+        const float e = __builtin_amdgcn_exp2f(top - base);
+        l += sum * e;
+        y += o * e;
+    }
+    return y;
+}
+
+__device__ __forceinline__ v4f normal(v4f y, float l) {
+    return l == 0.0f ? v4f{ 0.0f, 0.0f, 0.0f, 0.0f } : y / l;
+}
+
+/* The workgroup's waves met: into the outputs, or with several splits into
+ * the workspace (R rows of dk sums, then R pairs of maximum and sum). */
+template <int R, int NS>
+__device__ __forceinline__ void finish(const CacheAttention &a, const Share &s, float (*part)[R][32 * NS + 4],
+                                       float (*tops)[R], float (*sums)[R]) {
+    constexpr uint32_t dk = 32 * NS;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < R * dk / 4; i += 256) {
+        const uint32_t r = i / (dk / 4), c = i % (dk / 4) * 4;
+        const int32_t rr = s.rr0 + (int32_t)r;
+        if (rr >= s.nrows)
+            continue;
+        float m, l;
+        const v4f y = joined<4>(4, [&](int n, float &top, float &sum, v4f *o) {
+            top = tops[n][r], sum = sums[n][r];
+            if (o)
+                *o = *(const v4f *)&part[n][r][c];
+        }, m, l);
+        if (a.splits == 1) {
+            const uint64_t row = (uint64_t)(s.sp.r0 + rr / (int32_t)s.grp);
+            *(v4f *)(a.o + row * a.os + (s.g * s.grp + (uint32_t)rr % s.grp) * dk + c) = normal(y, l);
+        } else {
+            float *w = a.parts + (s.unit * a.splits + s.split) * (R * (dk + 2));
+            *(v4f *)(w + r * dk + c) = y;
+            if (c == 0) {
+                w[R * dk + 2 * r] = m;
+                w[R * dk + 2 * r + 1] = l;
+            }
+        }
+    }
+}
+
+/* The splits of each tile met, a workgroup a tile. */
+template <int R, int NS>
+__global__ __launch_bounds__(256) void cache_join_kernel(CacheAttention a) {
+    constexpr uint32_t dk = 32 * NS;
+    Share s;
+    if (!share_of<R>(a, s, 1))
         return;
+    const float *w = a.parts + s.unit * a.splits * (R * (dk + 2));
+    for (uint32_t i = threadIdx.x; i < R * dk / 4; i += 256) {
+        const uint32_t r = i / (dk / 4), c = i % (dk / 4) * 4;
+        const int32_t rr = s.rr0 + (int32_t)r;
+        if (rr >= s.nrows)
+            continue;
+        float m, l;
+        const v4f y = joined<8>((int)a.splits, [&](int n, float &top, float &sum, v4f *o) {
+            const float *p = w + (uint64_t)n * (R * (dk + 2));
+            top = p[R * dk + 2 * r], sum = p[R * dk + 2 * r + 1];
+            if (o)
+                *o = *(const v4f *)(p + r * dk + c);
+        }, m, l);
+        const uint64_t row = (uint64_t)(s.sp.r0 + rr / (int32_t)s.grp);
+        *(v4f *)(a.o + row * a.os + (s.g * s.grp + (uint32_t)rr % s.grp) * dk + c) = normal(y, l);
+    }
+}
+
+/* Up to four rows of a stream and kept head (a step of a frame or a few), where
+ * the cache's bytes are what takes time. A row's three pieces are three rows
+ * of the matrix instruction's 16 (row 4 i + n piece n of query i), so one
+ * product takes them all, and the keys are its columns: a lane's four sums
+ * are one query's pieces of one key, added in place, and every lane has
+ * scores of its own to make a softmax of (of the columns' other use, queries,
+ * each would be made four times over). Tile kt's column c is key 4 c + kt, so
+ * a lane's four scores are neighbours in memory: their scales and position
+ * scores are one load each. The probabilities cross lanes once, cut, through
+ * LDS, to be the second product's rows as the queries were the first's. */
+template <int NS>
+__global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
+    constexpr uint32_t dk = 32 * NS, record = kPage * dk + 4 * kPage;
+    constexpr uint32_t kRow = 72;           /* bfloat16 a row of pieces: 64 and a pad against bank conflicts */
+    __shared__ float part[4][4][dk + 4], tops[4][4], sums[4][4];
+    __shared__ __attribute__((aligned(16))) uint16_t prob[4][12][kRow];
+    Share s;
+    if (!share_of<4>(a, s, a.splits))
+        return;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = lane / 16, c = lane % 16;
+
+    v8bf q[NS];
+    {
+        const int32_t i = (int32_t)(c / 4);
+        const uint32_t n = c % 4;
+        const uint32_t m1 = n >= 1 ? 0xffff0000u : 0, m2 = n >= 2 ? 0xffff0000u : 0;
+        const bool live = i < s.nrows && n < 3;
+        const int32_t ic = min(i, s.nrows - 1);
+        const uint64_t row = (uint64_t)(s.sp.r0 + ic / (int32_t)s.grp);
+        const uint32_t h = s.g * s.grp + (uint32_t)ic % s.grp;
+#pragma unroll
+        for (int st = 0; st < NS; st++) {
+            const uint32_t d = h * dk + w * (8 * NS) + 8 * st;
+            const v4f *src = (const v4f *)(a.q + row * a.qs + d);
+            v4f s0 = src[0], s1 = src[1];
+            if (a.p) {
+                const v4f *bias = (const v4f *)(a.bias_u + d);
+                s0 += bias[0], s1 += bias[1];
+            }
+            uint32_t u[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                float x = j < 4 ? s0[j % 4] : s1[j % 4];
+                x -= __uint_as_float(__float_as_uint(x) & m1);
+                x -= __uint_as_float(__float_as_uint(x) & m2);
+                u[j] = live ? __float_as_uint(x) : 0;
+            }
+            v4u packed;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                packed[j] = __builtin_amdgcn_perm(u[2 * j + 1], u[2 * j], 0x07060302u);
+            q[st] = __builtin_bit_cast(v8bf, packed);
+        }
+    }
+    /* the lane's query in the softmax */
+    const bool mine = (int32_t)w < s.nrows;
+    const int32_t wi = min((int32_t)w, s.nrows - 1);
+    const int32_t pos = s.sp.len + wi / (int32_t)s.grp;
+    const int32_t lo = cache_lo(pos, a.left), hi = mine ? cache_hi(pos, a.right, s.sp.total) : -1;
+    const float *place = nullptr;
+    if (a.p)
+        place = a.place + ((uint64_t)(s.sp.r0 + wi / (int32_t)s.grp) * a.H + s.g * s.grp + (uint32_t)wi % s.grp) *
+                              place_stride(a.bw) + kPlacePad + (a.left - pos);
+
+    const float c2 = a.scale * 1.44269504088896340736f;     /* scores in powers of 2 */
+    float top = -INFINITY, sum = 0.0f;
+    v4f o[2 * NS] = {};
+    for (int32_t first = s.pa + (int32_t)wave; first < s.pb; first += 4 * 64) {
+        int32_t ids;
+        uint64_t left = page_ids(a, s, first, ids);
+        while (left) {
+            const int at = __builtin_ctzll(left);
+            left &= left - 1;
+            const int32_t pg = first + 4 * at, id = __builtin_amdgcn_readlane(ids, at);
+            const uint8_t *rec = a.data + ((uint64_t)(uint32_t)id * a.G + s.g) * record;
+            uint32_t kw[4][NS];
+            v4u vw[NS];
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+                for (int st = 0; st < NS; st++)
+                    kw[kt][st] = ((const uint32_t *)(rec + cache_key_at(dk, 4 * c + kt) + w * (4 * NS)))[st];
+            const v2u ks = *(const v2u *)(rec + cache_key_scale_at(dk, 4 * c));
+            const v2u vs = *(const v2u *)(rec + cache_value_scale_at(dk, 4 * c));
+            const int32_t j = pg * (int32_t)kPage + 4 * (int32_t)c;
+            v4f add = { 0.0f, 0.0f, 0.0f, 0.0f };
+            if (a.p)
+                add = *(const v4f_u *)(place + j);
+#pragma unroll
+            for (int i = 0; i < NS; i++)
+                vw[i] = *(const v4u *)(rec + cache_values_at(dk) + 1024 * i + 16 * lane);
+
+            float x[4], best = -INFINITY;
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++) {
+                v4f acc = { 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+                for (int st = 0; st < NS; st++)
+                    acc = mfma(q[st], levels(kw[kt][st]), acc);
+                const float v = (((acc[2] + acc[1]) + acc[0]) * bf_of(ks, kt) + add[kt]) * c2;
+                x[kt] = j + kt >= lo && j + kt <= hi ? v : -INFINITY;
+                best = fmaxf(best, x[kt]);
+            }
+            best = row_max(best);
+            if (__any(best > top)) {
+                const float now = fmaxf(top, best);
+                const float scale = __builtin_amdgcn_exp2f(top - (now == -INFINITY ? 0.0f : now));
+                top = now;
+                sum *= scale;
+#pragma unroll
+                for (int i = 0; i < 2 * NS; i++)
+                    o[i] *= scale;
+            }
+            const float base = top == -INFINITY ? 0.0f : top;
+            uint32_t u[3][4];
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++) {
+                const float e = __builtin_amdgcn_exp2f(x[kt] - base);
+                sum += e;
+                /* a frame that is not attended may have a scale that was never written */
+                float y = x[kt] == -INFINITY ? 0.0f : e * bf_of(vs, kt);
+#pragma unroll
+                for (int n = 0; n < 3; n++) {
+                    u[n][kt] = __float_as_uint(y);
+                    y -= __uint_as_float(u[n][kt] & 0xffff0000u);
+                }
+            }
+            /* key 4 c + kt = 32 g + 16 h + 4 w' + kt with c = 8 g + 4 h + w': the eight frames that quarter w' of the
+             * second product takes are in a row */
+#pragma unroll
+            for (int n = 0; n < 3; n++)
+                *(v2u *)&prob[wave][3 * w + n][32 * (c / 8) + 8 * (c % 4) + 4 * (c / 4 % 2)] =
+                    v2u{ __builtin_amdgcn_perm(u[n][1], u[n][0], 0x07060302u),
+                         __builtin_amdgcn_perm(u[n][3], u[n][2], 0x07060302u) };
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int gg = 0; gg < 2; gg++) {
+                const v8bf pr = __builtin_bit_cast(v8bf, *(const v4u *)&prob[wave][3 * (c / 4) + min(c % 4, 2u)][32 * gg + 8 * w]);
+#pragma unroll
+                for (int dt = 0; dt < 2 * NS; dt++)
+                    o[dt] = mfma(pr, levels(vw[dt / 2][2 * (dt % 2) + gg]), o[dt]);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+    sum = row_sum(sum);
+    if (c == 0) {
+        tops[wave][w] = top;
+        sums[wave][w] = sum;
+    }
+#pragma unroll
+    for (int dt = 0; dt < 2 * NS; dt++)
+        part[wave][w][16 * dt + c] = (o[dt][2] + o[dt][1]) + o[dt][0];
+    finish<4, NS>(a, s, part, tops, sums);
+}
+
+/* More rows: 16 a workgroup, its four waves a page each in turn with the
+ * running maximum and sum of a softmax, a query a column and its pieces three
+ * products one after another. */
+template <int NS>
+__global__ __launch_bounds__(256) void cache_many_kernel(CacheAttention a) {
+    constexpr uint32_t dk = 32 * NS, record = kPage * dk + 4 * kPage;
+    __shared__ float part[4][16][dk + 4], tops[4][16], sums[4][16];
+    Share sh;
+    if (!share_of<16>(a, sh, a.splits))
+        return;
+    const CacheSpan &sp = sh.sp;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = lane / 16;
-    const int32_t rr = min(rr0 + (int32_t)(lane % 16), nrows - 1);
-    const int32_t t = rr / (int32_t)grp;
-    const uint32_t h = g * grp + (uint32_t)rr % grp;
+    const int32_t rr = min(sh.rr0 + (int32_t)(lane % 16), sh.nrows - 1);
+    const int32_t t = rr / (int32_t)sh.grp;
+    const uint32_t h = sh.g * sh.grp + (uint32_t)rr % sh.grp;
     const uint64_t row = (uint64_t)(sp.r0 + t);
     const int32_t pos = sp.len + t;
     const int32_t lo = cache_lo(pos, a.left), hi = cache_hi(pos, a.right, sp.total);
@@ -312,81 +622,77 @@ __global__ __launch_bounds__(256) void cache_attention_kernel(CacheAttention a, 
     if (a.p)
         place = a.place + (row * a.H + h) * place_stride(a.bw) + kPlacePad + (a.left - pos);
 
-    /* the pages of any of the tile's rows */
-    const int32_t t1 = min(rr0 + 15, nrows - 1) / (int32_t)grp;
-    const int32_t j0 = cache_lo(sp.len + rr0 / (int32_t)grp, a.left), j1 = cache_hi(sp.len + t1, a.right, sp.total);
     const float c2 = a.scale * 1.44269504088896340736f;     /* scores in powers of 2 */
     float top = -INFINITY, sum = 0.0f;
     v4f o[2 * NS] = {};
-    for (int32_t pg = j0 / (int32_t)kPage + (int32_t)wave; pg * (int32_t)kPage <= j1; pg += 4) {
-        const int32_t id = a.st.table[(uint64_t)b * a.st.max_pages + pg];
-        if (!cache_page_ok(id, a.pages))
-            continue;
-        const uint8_t *rec = a.data + ((uint64_t)id * a.G + g) * record;
-        float s[4][4], best = -INFINITY;
+    for (int32_t first = sh.pa + (int32_t)wave; first < sh.pb; first += 4 * 64) {
+        int32_t ids;
+        uint64_t left = page_ids(a, sh, first, ids);
+        while (left) {
+            const int at = __builtin_ctzll(left);
+            left &= left - 1;
+            const int32_t pg = first + 4 * at, id = __builtin_amdgcn_readlane(ids, at);
+            const uint8_t *rec = a.data + ((uint64_t)(uint32_t)id * a.G + sh.g) * record;
+            float s[4][4], best = -INFINITY;
 #pragma unroll
-        for (int kt = 0; kt < 4; kt++) {
-            const uint32_t *kp = (const uint32_t *)(rec + cache_key_at(dk, 16 * kt + lane % 16) + w * (4 * NS));
-            v4f acc = { 0.0f, 0.0f, 0.0f, 0.0f };
+            for (int kt = 0; kt < 4; kt++) {
+                const uint32_t *kp = (const uint32_t *)(rec + cache_key_at(dk, 16 * kt + lane % 16) + w * (4 * NS));
+                v4f acc = { 0.0f, 0.0f, 0.0f, 0.0f };
 #pragma unroll
-            for (int st = 0; st < NS; st++) {
-                const v8bf k = levels(kp[st]);
-                acc = mfma(k, q[st].p[2], acc);
-                acc = mfma(k, q[st].p[1], acc);
-                acc = mfma(k, q[st].p[0], acc);
-            }
-            const uint32_t f = 16 * kt + 4 * w;
-            const v2u ks = *(const v2u *)(rec + cache_key_scale_at(dk, f));
-            const int32_t j = pg * (int32_t)kPage + (int32_t)f;
-            v4f add = { 0.0f, 0.0f, 0.0f, 0.0f };
-            if (a.p)
-                add = *(const v4f_u *)(place + j);
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float d = __uint_as_float(r % 2 ? ks[r / 2] & 0xffff0000u : ks[r / 2] << 16);
-                const float v = (acc[r] * d + add[r]) * c2;
-                s[kt][r] = j + r >= lo && j + r <= hi ? v : -INFINITY;
-                best = fmaxf(best, s[kt][r]);
-            }
-        }
-        best = fmaxf(best, __shfl_xor(best, 16));
-        best = fmaxf(best, __shfl_xor(best, 32));
-        const float now = fmaxf(top, best), base = now == -INFINITY ? 0.0f : now;
-        const float scale = __builtin_amdgcn_exp2f(top - base);
-        top = now;
-        sum *= scale;
-#pragma unroll
-        for (int i = 0; i < 2 * NS; i++)
-            o[i] *= scale;
-#pragma unroll
-        for (int gg = 0; gg < 2; gg++) {
-            float x[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int kt = 2 * gg + i / 4, r = i % 4;
+                for (int st = 0; st < NS; st++) {
+                    const v8bf k = levels(kp[st]);
+                    acc = mfma(k, q[st].p[2], acc);
+                    acc = mfma(k, q[st].p[1], acc);
+                    acc = mfma(k, q[st].p[0], acc);
+                }
                 const uint32_t f = 16 * kt + 4 * w;
-                const v2u vs = *(const v2u *)(rec + cache_value_scale_at(dk, f));
-                const float d = __uint_as_float(r % 2 ? vs[r / 2] & 0xffff0000u : vs[r / 2] << 16);
-                const float e = __builtin_amdgcn_exp2f(s[kt][r] - base);
-                sum += e;
-                /* a frame that is not attended may have a scale that was never written */
-                x[i] = s[kt][r] == -INFINITY ? 0.0f : e * d;
-            }
-            const Pieces pr = cut(x);
+                const v2u ks = *(const v2u *)(rec + cache_key_scale_at(dk, f));
+                const int32_t j = pg * (int32_t)kPage + (int32_t)f;
+                v4f add = { 0.0f, 0.0f, 0.0f, 0.0f };
+                if (a.p)
+                    add = *(const v4f_u *)(place + j);
 #pragma unroll
-            for (int dt = 0; dt < 2 * NS; dt++) {
-                const v8bf val = levels(*(const uint32_t *)(rec + cache_values_at(dk) + 1024 * (dt / 2) + 16 * lane +
-                                                            8 * (dt % 2) + 4 * gg));
-                o[dt] = mfma(val, pr.p[2], o[dt]);
-                o[dt] = mfma(val, pr.p[1], o[dt]);
-                o[dt] = mfma(val, pr.p[0], o[dt]);
+                for (int r = 0; r < 4; r++) {
+                    const float v = (acc[r] * bf_of(ks, r) + add[r]) * c2;
+                    s[kt][r] = j + r >= lo && j + r <= hi ? v : -INFINITY;
+                    best = fmaxf(best, s[kt][r]);
+                }
+            }
+            best = fmaxf(best, __shfl_xor(best, 16));
+            best = fmaxf(best, __shfl_xor(best, 32));
+            const float now = fmaxf(top, best), base = now == -INFINITY ? 0.0f : now;
+            const float scale = __builtin_amdgcn_exp2f(top - base);
+            top = now;
+            sum *= scale;
+#pragma unroll
+            for (int i = 0; i < 2 * NS; i++)
+                o[i] *= scale;
+#pragma unroll
+            for (int gg = 0; gg < 2; gg++) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int kt = 2 * gg + i / 4, r = i % 4;
+                    const v2u vs = *(const v2u *)(rec + cache_value_scale_at(dk, 16 * kt + 4 * w));
+                    const float e = __builtin_amdgcn_exp2f(s[kt][r] - base);
+                    sum += e;
+                    /* a frame that is not attended may have a scale that was never written */
+                    x[i] = s[kt][r] == -INFINITY ? 0.0f : e * bf_of(vs, r);
+                }
+                const Pieces pr = cut(x);
+#pragma unroll
+                for (int dt = 0; dt < 2 * NS; dt++) {
+                    const v8bf val = levels(*(const uint32_t *)(rec + cache_values_at(dk) + 1024 * (dt / 2) + 16 * lane +
+                                                                8 * (dt % 2) + 4 * gg));
+                    o[dt] = mfma(val, pr.p[2], o[dt]);
+                    o[dt] = mfma(val, pr.p[1], o[dt]);
+                    o[dt] = mfma(val, pr.p[0], o[dt]);
+                }
             }
         }
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
-
-    __shared__ float part[4][16][dk + 4], tops[4][16], sums[4][16];
     if (w == 0) {
         tops[wave][lane % 16] = top;
         sums[wave][lane % 16] = sum;
@@ -394,27 +700,7 @@ __global__ __launch_bounds__(256) void cache_attention_kernel(CacheAttention a, 
 #pragma unroll
     for (int dt = 0; dt < 2 * NS; dt++)
         *(v4f *)&part[wave][lane % 16][16 * dt + 4 * w] = o[dt];
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < 16 * dk / 4; i += 256) {
-        const uint32_t r = i / (dk / 4), c = i % (dk / 4) * 4;
-        if (rr0 + (int32_t)r >= nrows)
-            continue;
-        float m = -INFINITY, l = 0.0f;
-#pragma unroll
-        for (int n = 0; n < 4; n++)
-            m = fmaxf(m, tops[n][r]);
-        const float base = m == -INFINITY ? 0.0f : m;
-        v4f y = { 0.0f, 0.0f, 0.0f, 0.0f };
-#pragma unroll
-        for (int n = 0; n < 4; n++) {
-            const float e = __builtin_amdgcn_exp2f(tops[n][r] - base);
-            l += sums[n][r] * e;
-            y += *(const v4f *)&part[n][r][c] * e;
-        }
-        y = l == 0.0f ? v4f{ 0.0f, 0.0f, 0.0f, 0.0f } : y / l;      /* nothing attended: zeros; a NaN stays one */
-        const int32_t ro = rr0 + (int32_t)r;
-        *(v4f *)(a.o + (uint64_t)(sp.r0 + ro / (int32_t)grp) * a.os + (g * grp + (uint32_t)ro % grp) * dk + c) = y;
-    }
+    finish<16, NS>(a, sh, part, tops, sums);
 }
 
 /* ----------------------------------------------------------------- move --- */
@@ -465,20 +751,55 @@ int launch_cache_read(const uint8_t *data, uint32_t pages, uint32_t G, uint32_t 
     return hipPeekAtLastError() == hipSuccess ? 0 : -1;
 }
 
+/* How a call's rows are dealt: tiles of four rows where a stream has at most
+ * four a kept head, else of 16; and enough splits of a tile's pages that the
+ * chip has work, none of them under four pages (one a wave). */
+struct Deal {
+    uint32_t rows, tiles, splits;
+    uint64_t units;
+};
+
+static Deal deal(const CacheStreams &st, uint32_t G, uint32_t H, int32_t left, int32_t right) {
+    Deal d;
+    const uint32_t rows = st.max_T * (H / G);
+    d.rows = rows <= 4 ? 4 : 16;
+    d.tiles = (rows + d.rows - 1) / d.rows;
+    d.units = (uint64_t)st.B * G * d.tiles;
+    const uint64_t reach = (uint64_t)left + (uint64_t)right + st.max_T;
+    const uint64_t pages = std::min<uint64_t>(st.max_pages, reach / kPage + 2);
+    const uint64_t want = d.units ? (1024 + d.units - 1) / d.units : 1;
+    d.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({ want, (pages + 3) / 4, 128 }));
+    return d;
+}
+
+static size_t place_bytes(const CacheStreams &st, uint32_t H, int32_t left, int32_t right) {
+    return (size_t)st.rows * H * place_stride((uint32_t)left + (uint32_t)right + 1) * sizeof(float);
+}
+
 size_t cache_attention_workspace(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, bool positions,
                                  int32_t left, int32_t right) {
-    (void)G, (void)dk;
-    return positions ? (size_t)st.rows * H * place_stride((uint32_t)left + (uint32_t)right + 1) * sizeof(float) : 0;
+    const Deal d = deal(st, G, H, left, right);
+    return (positions ? place_bytes(st, H, left, right) : 0) +
+           (d.splits > 1 ? d.units * d.splits * d.rows * (dk + 2) * sizeof(float) : 0);
 }
 
 template <int NS>
-static void attend(const CacheAttention &a, hipStream_t s) {
+static void attend(const CacheAttention &a, const Deal &d, hipStream_t s) {
     if (a.p) {
         const dim3 grid((a.bw + 64 * kPlaceTiles - 1) / (64 * kPlaceTiles), a.H, (a.st.rows + kPlaceRows - 1) / kPlaceRows);
         cache_place_kernel<NS><<<grid, 256, 0, s>>>(a);
     }
-    const uint32_t tiles = (a.st.max_T * (a.H / a.G) + 15) / 16;
-    cache_attention_kernel<NS><<<a.G * tiles * a.st.B, 256, 0, s>>>(a, tiles);
+    const uint32_t grid = (uint32_t)(d.units * d.splits);
+    if (d.rows == 4)
+        cache_few_kernel<NS><<<grid, 256, 0, s>>>(a);
+    else
+        cache_many_kernel<NS><<<grid, 256, 0, s>>>(a);
+    if (d.splits > 1) {
+        if (d.rows == 4)
+            cache_join_kernel<4, NS><<<grid / d.splits, 256, 0, s>>>(a);
+        else
+            cache_join_kernel<16, NS><<<grid / d.splits, 256, 0, s>>>(a);
+    }
 }
 
 int launch_cache_attention(const CacheAttentionCall &c, hipStream_t s) {
@@ -491,11 +812,16 @@ int launch_cache_attention(const CacheAttentionCall &c, hipStream_t s) {
     a.p = c.p, a.bias_u = c.bias_u, a.bias_w = c.bias_w;
     a.place = (float *)c.ws;
     a.bw = (uint32_t)c.left + (uint32_t)c.right + 1;
+    const Deal d = deal(c.st, c.G, c.H, c.left, c.right);
+    if (d.units * d.splits > 0x7fffffff)
+        return -2;
+    a.tiles = d.tiles, a.splits = d.splits;
+    a.parts = (float *)((char *)c.ws + (c.p ? place_bytes(c.st, c.H, c.left, c.right) : 0));
     switch (c.dk / 32) {
-    case 1: attend<1>(a, s); break;
-    case 2: attend<2>(a, s); break;
-    case 3: attend<3>(a, s); break;
-    case 4: attend<4>(a, s); break;
+    case 1: attend<1>(a, d, s); break;
+    case 2: attend<2>(a, d, s); break;
+    case 3: attend<3>(a, d, s); break;
+    case 4: attend<4>(a, d, s); break;
     default: return -2;
     }
     return hipPeekAtLastError() == hipSuccess ? 0 : -1;
