@@ -189,25 +189,76 @@ struct CacheAttention {
     float *parts;
 };
 
-/* The position scores (q + w) . p of every row at every distance that it
- * needs, into the workspace: the same rows of p serve every stream, so this
- * is one product of all rows by the table, read once, where the attention
- * reads its own stream's pages only. A workgroup takes 64 rows of a head,
- * their pieces as the matrix instruction's operands in LDS, and walks tiles
- * of 16 distances, a wave each; both operands are floats, so six of the nine
- * products of pieces are taken (the other three are under 2^-24 of the
- * whole). */
-constexpr int kPlaceRows = 64, kPlaceTiles = 4;
+/* A row of floats cut in two float16 for a product of floats with floats: times
+ * the power of two that puts the row's largest magnitude into [2^14, 2^15),
+ * its nearest float16 and the nearest of what is left, so that every value is
+ * kept to 2^-22 of itself, or of 2^-17 of the row's largest where that is more
+ * (float16's own last places). Three products of pieces are taken, and the
+ * exponents of both rows put back at the end. */
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+struct Halves {
+    v8h hi, lo;
+};
+
+/* the exponent e with 2^e <= top < 2^(e + 1), kept where 2^(14 - e) is a normal number (0 for a row of zeros, or
+ * with a NaN or an infinity, which its products then are too) */
+__device__ __forceinline__ int row_exponent(uint32_t top_bits) {
+    const int e = (int)(top_bits >> 23) - 127;
+    return e == 128 || top_bits == 0 ? 0 : max(e, -112);
+}
+
+__device__ __forceinline__ Halves halve(const float (&x)[8], int e) {
+    const float s = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+    Halves r;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float v = x[i] * s;
+        r.hi[i] = (_Float16)v;
+        r.lo[i] = (_Float16)(v - (float)r.hi[i]);
+    }
+    return r;
+}
+
+__device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+/* The position scores (q + w) . p, scaled as the softmax takes them (in powers
+ * of 2), of every row at every distance that it needs, into the workspace:
+ * the same rows of p serve every stream, so this is one product of all rows by
+ * the table, read once, where the attention reads its own stream's pages only.
+ * A workgroup takes 64 rows of a head, halved into the matrix instruction's
+ * operands in LDS, and walks `steps` runs of 128 distances; a wave takes 32 of
+ * each, two tiles, so that an operand read from LDS serves two. */
+constexpr int kPlaceRows = 64, kPlaceRun = 128;
 template <int NS>
-__global__ __launch_bounds__(256) void cache_place_kernel(CacheAttention a) {
-    __shared__ v4u frag[kPlaceRows / 16][NS][3][64];
-    __shared__ int32_t need_lo, need_hi;
+__global__ __launch_bounds__(256) void cache_place_kernel(CacheAttention a, int32_t steps) {
+    __shared__ v8h frag[kPlaceRows / 16][NS][2][64];
+    __shared__ int32_t need_lo, need_hi, expo[kPlaceRows];
     const uint32_t h = blockIdx.y, n0 = blockIdx.z * kPlaceRows;
-    const int32_t x0 = (int32_t)blockIdx.x * (64 * kPlaceTiles);
+    const int32_t x0 = (int32_t)blockIdx.x * (kPlaceRun * steps), x1 = min(x0 + kPlaceRun * steps, (int32_t)a.bw);
     const uint32_t dk = 32 * NS, stride = place_stride(a.bw);
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = lane / 16;
+    const uint32_t rows = min((uint32_t)kPlaceRows, a.st.rows - n0);
+
+    v4f p[2][NS][2];
+    auto load = [&](int32_t x) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint32_t m = min((uint32_t)x + 16 * i + lane % 16, a.bw - 1);
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                const v4f *src = (const v4f *)(a.p + (uint64_t)m * (a.H * dk) + h * dk + 32 * s + 8 * w);
+                p[i][s][0] = src[0], p[i][s][1] = src[1];
+            }
+        }
+    };
+    load(x0 + 32 * (int32_t)wave);
     if (threadIdx.x == 0)
         need_lo = INT32_MAX, need_hi = INT32_MIN;
     __syncthreads();
+    /* the distances that any of the rows needs */
     int32_t lo = INT32_MAX, hi = INT32_MIN;
     for (uint32_t b = threadIdx.x; b < a.st.B; b += 256) {
         const CacheSpan sp = span_of(a.st, b);
@@ -222,14 +273,11 @@ __global__ __launch_bounds__(256) void cache_place_kernel(CacheAttention a) {
         atomicMin(&need_lo, lo);
         atomicMax(&need_hi, hi);
     }
-    __syncthreads();
-    if (need_lo >= x0 + 64 * kPlaceTiles || need_hi < x0)
-        return;
-    const uint32_t rows = min((uint32_t)kPlaceRows, a.st.rows - n0);
-    for (uint32_t i = threadIdx.x; i < kPlaceRows * 4 * NS; i += 256) {
-        const uint32_t row = i / (4 * NS), part = i % (4 * NS);       /* eight dimensions */
+#pragma unroll
+    for (uint32_t i = threadIdx.x; i < kPlaceRows * 16; i += 256) {
+        const uint32_t row = i / 16, part = i % 16;                 /* eight dimensions */
         float x[8] = {};
-        if (row < rows) {
+        if (row < rows && part < 4 * NS) {
             const v4f *src = (const v4f *)(a.q + (uint64_t)(n0 + row) * a.qs + h * dk + 8 * part);
             const v4f *bias = (const v4f *)(a.bias_w + h * dk + 8 * part);
             const v4f s0 = src[0] + bias[0], s1 = src[1] + bias[1];
@@ -237,45 +285,80 @@ __global__ __launch_bounds__(256) void cache_place_kernel(CacheAttention a) {
             for (int j = 0; j < 4; j++)
                 x[j] = s0[j], x[4 + j] = s1[j];
         }
-        const Pieces c = cut(x);
+        int top = 0;
 #pragma unroll
-        for (int n = 0; n < 3; n++)
-            frag[row / 16][part / 4][n][16 * (part % 4) + row % 16] = __builtin_bit_cast(v4u, c.p[n]);
+        for (int j = 0; j < 8; j++)
+            top = max(top, mag_bits(x[j]));
+        const int e = row_exponent((uint32_t)group_max_nonneg<16>(top));
+        const Halves c = halve(x, e);
+        if (part < 4 * NS) {
+            frag[row / 16][part / 4][0][16 * (part % 4) + row % 16] = c.hi;
+            frag[row / 16][part / 4][1][16 * (part % 4) + row % 16] = c.lo;
+        }
+        if (part == 0)
+            expo[row] = e;
     }
     __syncthreads();
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = lane / 16;
+    const int32_t from = need_lo, to = need_hi;
+    const float c2 = a.scale * 1.44269504088896340736f;
 #pragma unroll 1
-    for (int t = 0; t < kPlaceTiles; t++) {
-        const int32_t x = x0 + 64 * t + 16 * (int32_t)wave;
-        if (x >= (int32_t)a.bw || need_lo >= x + 16 || need_hi < x)
+    for (int32_t x = x0 + 32 * (int32_t)wave; x < x1; x += kPlaceRun) {
+        if (from >= x + 32 || to < x) {
+            if (to < x)
+                break;
+            load(x + kPlaceRun);
             continue;
-        const uint32_t m = min((uint32_t)x + lane % 16, a.bw - 1);
-        Pieces p[NS];
-#pragma unroll
-        for (int s = 0; s < NS; s++) {
-            const v4f *src = (const v4f *)(a.p + (uint64_t)m * (a.H * dk) + h * dk + 32 * s + 8 * w);
-            const v4f s0 = src[0], s1 = src[1];
-            const float xs[8] = { s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3] };
-            p[s] = cut(xs);
         }
-        for (uint32_t rt = 0; 16 * rt < rows; rt++) {
-            v4f acc = { 0.0f, 0.0f, 0.0f, 0.0f };
+        Halves ph[2][NS];
+        int pe[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            int top = 0;
+#pragma unroll
+            for (int s = 0; s < NS; s++)
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    top = max(top, mag_bits(p[i][s][j / 4][j % 4]));
+            top = max(top, __shfl_xor(top, 16));
+            top = max(top, __shfl_xor(top, 32));
+            const int e = row_exponent((uint32_t)top);
 #pragma unroll
             for (int s = 0; s < NS; s++) {
-                v8bf q[3];
+                const float xs[8] = { p[i][s][0][0], p[i][s][0][1], p[i][s][0][2], p[i][s][0][3],
+                                      p[i][s][1][0], p[i][s][1][1], p[i][s][1][2], p[i][s][1][3] };
+                ph[i][s] = halve(xs, e);
+            }
 #pragma unroll
-                for (int n = 0; n < 3; n++)
-                    q[n] = __builtin_bit_cast(v8bf, frag[rt][s][n][lane]);
-                acc = mfma(p[s].p[2], q[0], acc);
-                acc = mfma(p[s].p[1], q[1], acc);
-                acc = mfma(p[s].p[0], q[2], acc);
-                acc = mfma(p[s].p[1], q[0], acc);
-                acc = mfma(p[s].p[0], q[1], acc);
-                acc = mfma(p[s].p[0], q[0], acc);
+            for (int r = 0; r < 4; r++)
+                pe[i][r] = __shfl(e, 4 * w + r) - 28;
+        }
+        load(x + kPlaceRun);
+#pragma unroll 1
+        for (uint32_t rt = 0; 16 * rt < rows; rt++) {
+            v4f acc[2] = {};
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                const v8h qh = frag[rt][s][0][lane], ql = frag[rt][s][1][lane];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    acc[i] = mfma(ph[i][s].lo, qh, acc[i]);
+                    acc[i] = mfma(ph[i][s].hi, ql, acc[i]);
+                    acc[i] = mfma(ph[i][s].hi, qh, acc[i]);
+                }
             }
             const uint32_t row = 16 * rt + lane % 16;
-            if (row < rows)
-                *(v4f *)(a.place + ((uint64_t)(n0 + row) * a.H + h) * stride + kPlacePad + x + 4 * w) = acc;
+            const int qe = expo[row];
+            if (row < rows) {
+                float *to_row = a.place + ((uint64_t)(n0 + row) * a.H + h) * stride + kPlacePad + x + 4 * w;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    v4f y;
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        y[r] = __builtin_ldexpf(acc[i][r], pe[i][r] + qe) * c2;
+                    *(v4f *)(to_row + 16 * i) = y;
+                }
+            }
         }
     }
 }
@@ -315,13 +398,33 @@ __device__ __forceinline__ bool share_of(const CacheAttention &a, Share &s, uint
     return true;
 }
 
-/* the pages of a wave, 64 at a time: page `first + 4 i` is lane i's, and a bit
- * of the mask is set where the table has one */
-__device__ __forceinline__ uint64_t page_ids(const CacheAttention &a, const Share &s, int32_t first, int32_t &id) {
-    const int32_t pg = first + 4 * (int32_t)(threadIdx.x & 63);
-    id = pg < s.pb ? a.st.table[(uint64_t)s.b * a.st.max_pages + pg] : -1;
-    return __ballot(cache_page_ok(id, a.pages));
-}
+/* The pages that a wave takes, every fourth of its workgroup's: 64 table
+ * entries at a time, one a lane, those that are no page of the pool passed
+ * over. */
+struct Walk {
+    int32_t first, ids;
+    uint64_t left;
+
+    __device__ __forceinline__ Walk(const CacheAttention &a, const Share &s)
+        : first(s.pa + (int32_t)(threadIdx.x >> 6) - 4 * 64), ids(0), left(0) {}
+
+    /* the next page and its place in the pool; false, and pg and id as they were, after the last */
+    __device__ __forceinline__ bool next(const CacheAttention &a, const Share &s, int32_t &pg, int32_t &id) {
+        while (left == 0) {
+            if (first + 4 * 64 >= s.pb)
+                return false;
+            first += 4 * 64;
+            const int32_t mine = first + 4 * (int32_t)(threadIdx.x & 63);
+            ids = mine < s.pb ? a.st.table[(uint64_t)s.b * a.st.max_pages + mine] : -1;
+            left = __ballot(cache_page_ok(ids, a.pages));
+        }
+        const int at = __builtin_ctzll(left);
+        left &= left - 1;
+        pg = first + 4 * at;
+        id = __builtin_amdgcn_readlane(ids, at);
+        return true;
+    }
+};
 
 __device__ __forceinline__ float bf_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
@@ -403,29 +506,43 @@ __device__ __forceinline__ void finish(const CacheAttention &a, const Share &s, 
     }
 }
 
-/* The splits of each tile met, a workgroup a tile. */
+/* The splits of each tile met, a workgroup a row: its threads in groups of
+ * dk / 4, a group every so many splits, four dimensions a thread. */
 template <int R, int NS>
 __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttention a) {
-    constexpr uint32_t dk = 32 * NS;
+    constexpr uint32_t dk = 32 * NS, kCols = dk / 4, kGroups = 256 / kCols;
+    __shared__ v4f part[kGroups][kCols];
+    __shared__ float tops[kGroups], sums[kGroups];
     Share s;
     if (!share_of<R>(a, s, 1))
         return;
+    const uint32_t r = blockIdx.y, group = threadIdx.x / kCols, c = threadIdx.x % kCols;
+    const int32_t rr = s.rr0 + (int32_t)r;
+    if (rr >= s.nrows)
+        return;
     const float *w = a.parts + s.unit * a.splits * (R * (dk + 2));
-    for (uint32_t i = threadIdx.x; i < R * dk / 4; i += 256) {
-        const uint32_t r = i / (dk / 4), c = i % (dk / 4) * 4;
-        const int32_t rr = s.rr0 + (int32_t)r;
-        if (rr >= s.nrows)
-            continue;
-        float m, l;
-        const v4f y = joined<8>((int)a.splits, [&](int n, float &top, float &sum, v4f *o) {
-            const float *p = w + (uint64_t)n * (R * (dk + 2));
+    float m, l;
+    if (group < kGroups) {
+        const int n = group < a.splits ? (int)((a.splits - group + kGroups - 1) / kGroups) : 0;
+        part[group][c] = joined<4>(n, [&](int i, float &top, float &sum, v4f *o) {
+            const float *p = w + (uint64_t)(group + (uint32_t)i * kGroups) * (R * (dk + 2));
             top = p[R * dk + 2 * r], sum = p[R * dk + 2 * r + 1];
             if (o)
-                *o = *(const v4f *)(p + r * dk + c);
+                *o = *(const v4f *)(p + r * dk + 4 * c);
         }, m, l);
-        const uint64_t row = (uint64_t)(s.sp.r0 + rr / (int32_t)s.grp);
-        *(v4f *)(a.o + row * a.os + (s.g * s.grp + (uint32_t)rr % s.grp) * dk + c) = normal(y, l);
+        if (c == 0)
+            tops[group] = m, sums[group] = l;
     }
+    __syncthreads();
+    if (group)
+        return;
+    const v4f y = joined<(int)kGroups>((int)kGroups, [&](int i, float &top, float &sum, v4f *o) {
+        top = tops[i], sum = sums[i];
+        if (o)
+            *o = part[i][c];
+    }, m, l);
+    const uint64_t row = (uint64_t)(s.sp.r0 + rr / (int32_t)s.grp);
+    *(v4f *)(a.o + row * a.os + (s.g * s.grp + (uint32_t)rr % s.grp) * dk + 4 * c) = normal(y, l);
 }
 
 /* Up to four rows of a stream and kept head (a step of a frame or a few), where
@@ -495,85 +612,97 @@ __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
     const float c2 = a.scale * 1.44269504088896340736f;     /* scores in powers of 2 */
     float top = -INFINITY, sum = 0.0f;
     v4f o[2 * NS] = {};
-    for (int32_t first = s.pa + (int32_t)wave; first < s.pb; first += 4 * 64) {
-        int32_t ids;
-        uint64_t left = page_ids(a, s, first, ids);
-        while (left) {
-            const int at = __builtin_ctzll(left);
-            left &= left - 1;
-            const int32_t pg = first + 4 * at, id = __builtin_amdgcn_readlane(ids, at);
-            const uint8_t *rec = a.data + ((uint64_t)(uint32_t)id * a.G + s.g) * record;
-            uint32_t kw[4][NS];
-            v4u vw[NS];
-#pragma unroll
-            for (int kt = 0; kt < 4; kt++)
-#pragma unroll
-                for (int st = 0; st < NS; st++)
-                    kw[kt][st] = ((const uint32_t *)(rec + cache_key_at(dk, 4 * c + kt) + w * (4 * NS)))[st];
-            const v2u ks = *(const v2u *)(rec + cache_key_scale_at(dk, 4 * c));
-            const v2u vs = *(const v2u *)(rec + cache_value_scale_at(dk, 4 * c));
-            const int32_t j = pg * (int32_t)kPage + 4 * (int32_t)c;
-            v4f add = { 0.0f, 0.0f, 0.0f, 0.0f };
-            if (a.p)
-                add = *(const v4f_u *)(place + j);
-#pragma unroll
-            for (int i = 0; i < NS; i++)
-                vw[i] = *(const v4u *)(rec + cache_values_at(dk) + 1024 * i + 16 * lane);
 
-            float x[4], best = -INFINITY;
+    /* a page's keys, and its values: the next page's are loaded as soon as this one's have been used, into the
+     * registers that they leave (after the last page, once more its own) */
+    uint32_t kw[4][NS];
+    v4u vw[NS];
+    v2u ks, vs;
+    v4f add = { 0.0f, 0.0f, 0.0f, 0.0f };
+    auto record_of = [&](int32_t id) { return a.data + ((uint64_t)(uint32_t)id * a.G + s.g) * record; };
+    auto load_keys = [&](const uint8_t *rec, int32_t pg) {
 #pragma unroll
-            for (int kt = 0; kt < 4; kt++) {
-                v4f acc = { 0.0f, 0.0f, 0.0f, 0.0f };
+        for (int kt = 0; kt < 4; kt++)
 #pragma unroll
-                for (int st = 0; st < NS; st++)
-                    acc = mfma(q[st], levels(kw[kt][st]), acc);
-                const float v = (((acc[2] + acc[1]) + acc[0]) * bf_of(ks, kt) + add[kt]) * c2;
-                x[kt] = j + kt >= lo && j + kt <= hi ? v : -INFINITY;
-                best = fmaxf(best, x[kt]);
-            }
-            best = row_max(best);
-            if (__any(best > top)) {
-                const float now = fmaxf(top, best);
-                const float scale = __builtin_amdgcn_exp2f(top - (now == -INFINITY ? 0.0f : now));
-                top = now;
-                sum *= scale;
+            for (int st = 0; st < NS; st++)
+                kw[kt][st] = ((const uint32_t *)(rec + cache_key_at(dk, 4 * c + kt) + w * (4 * NS)))[st];
+        ks = *(const v2u *)(rec + cache_key_scale_at(dk, 4 * c));
+        if (a.p)
+            add = *(const v4f_u *)(place + pg * (int32_t)kPage + 4 * (int32_t)c);
+    };
+    auto load_values = [&](const uint8_t *rec) {
 #pragma unroll
-                for (int i = 0; i < 2 * NS; i++)
-                    o[i] *= scale;
-            }
-            const float base = top == -INFINITY ? 0.0f : top;
-            uint32_t u[3][4];
+        for (int i = 0; i < NS; i++)
+            vw[i] = *(const v4u *)(rec + cache_values_at(dk) + 1024 * i + 16 * lane);
+        vs = *(const v2u *)(rec + cache_value_scale_at(dk, 4 * c));
+    };
+
+    Walk walk(a, s);
+    int32_t pg = 0, id = 0;
+    bool more = walk.next(a, s, pg, id);
+    if (more) {
+        load_keys(record_of(id), pg);
+        load_values(record_of(id));
+    }
+    while (more) {
+        float x[4], best = -INFINITY;
+        const int32_t j = pg * (int32_t)kPage + 4 * (int32_t)c;
 #pragma unroll
-            for (int kt = 0; kt < 4; kt++) {
-                const float e = __builtin_amdgcn_exp2f(x[kt] - base);
-                sum += e;
-                /* a frame that is not attended may have a scale that was never written */
-                float y = x[kt] == -INFINITY ? 0.0f : e * bf_of(vs, kt);
+        for (int kt = 0; kt < 4; kt++) {
+            v4f acc = { 0.0f, 0.0f, 0.0f, 0.0f };
 #pragma unroll
-                for (int n = 0; n < 3; n++) {
-                    u[n][kt] = __float_as_uint(y);
-                    y -= __uint_as_float(u[n][kt] & 0xffff0000u);
-                }
-            }
-            /* key 4 c + kt = 32 g + 16 h + 4 w' + kt with c = 8 g + 4 h + w': the eight frames that quarter w' of the
-             * second product takes are in a row */
-#pragma unroll
-            for (int n = 0; n < 3; n++)
-                *(v2u *)&prob[wave][3 * w + n][32 * (c / 8) + 8 * (c % 4) + 4 * (c / 4 % 2)] =
-                    v2u{ __builtin_amdgcn_perm(u[n][1], u[n][0], 0x07060302u),
-                         __builtin_amdgcn_perm(u[n][3], u[n][2], 0x07060302u) };
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int gg = 0; gg < 2; gg++) {
-                const v8bf pr = __builtin_bit_cast(v8bf, *(const v4u *)&prob[wave][3 * (c / 4) + min(c % 4, 2u)][32 * gg + 8 * w]);
-#pragma unroll
-                for (int dt = 0; dt < 2 * NS; dt++)
-                    o[dt] = mfma(pr, levels(vw[dt / 2][2 * (dt % 2) + gg]), o[dt]);
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+            for (int st = 0; st < NS; st++)
+                acc = mfma(q[st], levels(kw[kt][st]), acc);
+            const float v = __builtin_fmaf((acc[2] + acc[1]) + acc[0], bf_of(ks, kt) * c2, add[kt]);
+            x[kt] = j + kt >= lo && j + kt <= hi ? v : -INFINITY;
+            best = fmaxf(best, x[kt]);
         }
+        more = walk.next(a, s, pg, id);
+        const uint8_t *rec = record_of(id);
+        load_keys(rec, pg);
+        best = row_max(best);
+        if (__any(best > top)) {
+            const float now = fmaxf(top, best);
+            const float scale = __builtin_amdgcn_exp2f(top - (now == -INFINITY ? 0.0f : now));
+            top = now;
+            sum *= scale;
+#pragma unroll
+            for (int i = 0; i < 2 * NS; i++)
+                o[i] *= scale;
+        }
+        const float base = top == -INFINITY ? 0.0f : top;
+        uint32_t u[3][4];
+#pragma unroll
+        for (int kt = 0; kt < 4; kt++) {
+            const float e = __builtin_amdgcn_exp2f(x[kt] - base);
+            sum += e;
+            /* a frame that is not attended may have a scale that was never written */
+            float y = x[kt] == -INFINITY ? 0.0f : e * bf_of(vs, kt);
+#pragma unroll
+            for (int n = 0; n < 3; n++) {
+                u[n][kt] = __float_as_uint(y);
+                y -= __uint_as_float(u[n][kt] & 0xffff0000u);
+            }
+        }
+        /* key 4 c + kt = 32 g + 16 h + 4 w' + kt with c = 8 g + 4 h + w': the eight frames that quarter w' of the
+         * second product takes are in a row */
+#pragma unroll
+        for (int n = 0; n < 3; n++)
+            *(v2u *)&prob[wave][3 * w + n][32 * (c / 8) + 8 * (c % 4) + 4 * (c / 4 % 2)] =
+                v2u{ __builtin_amdgcn_perm(u[n][1], u[n][0], 0x07060302u),
+                     __builtin_amdgcn_perm(u[n][3], u[n][2], 0x07060302u) };
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int gg = 0; gg < 2; gg++) {
+            const v8bf pr = __builtin_bit_cast(v8bf, *(const v4u *)&prob[wave][3 * (c / 4) + min(c % 4, 2u)][32 * gg + 8 * w]);
+#pragma unroll
+            for (int dt = 0; dt < 2 * NS; dt++)
+                o[dt] = mfma(pr, levels(vw[dt / 2][2 * (dt % 2) + gg]), o[dt]);
+        }
+        load_values(rec);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
     sum = row_sum(sum);
     if (c == 0) {
@@ -622,74 +751,116 @@ __global__ __launch_bounds__(256) void cache_many_kernel(CacheAttention a) {
     if (a.p)
         place = a.place + (row * a.H + h) * place_stride(a.bw) + kPlacePad + (a.left - pos);
 
+    /* frames that every row of the tile attends */
+    const int32_t t1 = min(sh.rr0 + 15, sh.nrows - 1) / (int32_t)sh.grp;
+    const int32_t all_lo = cache_lo(sp.len + t1, a.left);
+    const int32_t all_hi = cache_hi(sp.len + sh.rr0 / (int32_t)sh.grp, a.right, sp.total);
     const float c2 = a.scale * 1.44269504088896340736f;     /* scores in powers of 2 */
     float top = -INFINITY, sum = 0.0f;
     v4f o[2 * NS] = {};
-    for (int32_t first = sh.pa + (int32_t)wave; first < sh.pb; first += 4 * 64) {
-        int32_t ids;
-        uint64_t left = page_ids(a, sh, first, ids);
-        while (left) {
-            const int at = __builtin_ctzll(left);
-            left &= left - 1;
-            const int32_t pg = first + 4 * at, id = __builtin_amdgcn_readlane(ids, at);
-            const uint8_t *rec = a.data + ((uint64_t)(uint32_t)id * a.G + sh.g) * record;
-            float s[4][4], best = -INFINITY;
+
+    /* loads ahead as in cache_few_kernel */
+    uint32_t kw[4][NS];
+    v4u vw[NS];
+    v2u ks[4], vs[4];
+    v4f add[4] = {};
+    auto record_of = [&](int32_t id) { return a.data + ((uint64_t)(uint32_t)id * a.G + sh.g) * record; };
+    auto load_keys = [&](const uint8_t *rec, int32_t pg) {
 #pragma unroll
-            for (int kt = 0; kt < 4; kt++) {
-                const uint32_t *kp = (const uint32_t *)(rec + cache_key_at(dk, 16 * kt + lane % 16) + w * (4 * NS));
-                v4f acc = { 0.0f, 0.0f, 0.0f, 0.0f };
+        for (int kt = 0; kt < 4; kt++) {
 #pragma unroll
-                for (int st = 0; st < NS; st++) {
-                    const v8bf k = levels(kp[st]);
-                    acc = mfma(k, q[st].p[2], acc);
-                    acc = mfma(k, q[st].p[1], acc);
-                    acc = mfma(k, q[st].p[0], acc);
-                }
-                const uint32_t f = 16 * kt + 4 * w;
-                const v2u ks = *(const v2u *)(rec + cache_key_scale_at(dk, f));
-                const int32_t j = pg * (int32_t)kPage + (int32_t)f;
-                v4f add = { 0.0f, 0.0f, 0.0f, 0.0f };
-                if (a.p)
-                    add = *(const v4f_u *)(place + j);
+            for (int st = 0; st < NS; st++)
+                kw[kt][st] = ((const uint32_t *)(rec + cache_key_at(dk, 16 * kt + lane % 16) + w * (4 * NS)))[st];
+            ks[kt] = *(const v2u *)(rec + cache_key_scale_at(dk, 16 * kt + 4 * w));
+            if (a.p)
+                add[kt] = *(const v4f_u *)(place + pg * (int32_t)kPage + 16 * kt + 4 * (int32_t)w);
+        }
+    };
+    auto load_values = [&](const uint8_t *rec) {
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float v = (acc[r] * bf_of(ks, r) + add[r]) * c2;
-                    s[kt][r] = j + r >= lo && j + r <= hi ? v : -INFINITY;
-                    best = fmaxf(best, s[kt][r]);
-                }
+        for (int i = 0; i < NS; i++)
+            vw[i] = *(const v4u *)(rec + cache_values_at(dk) + 1024 * i + 16 * lane);
+#pragma unroll
+        for (int kt = 0; kt < 4; kt++)
+            vs[kt] = *(const v2u *)(rec + cache_value_scale_at(dk, 16 * kt + 4 * w));
+    };
+
+    Walk walk(a, sh);
+    int32_t pg = 0, id = 0;
+    bool more = walk.next(a, sh, pg, id);
+    if (more) {
+        load_keys(record_of(id), pg);
+        load_values(record_of(id));
+    }
+    while (more) {
+        float s[4][4], best = -INFINITY;
+        const int32_t j = pg * (int32_t)kPage + 4 * (int32_t)w;
+        const bool inside = pg * (int32_t)kPage >= all_lo && pg * (int32_t)kPage + (int32_t)kPage - 1 <= all_hi;
+#pragma unroll
+        for (int kt = 0; kt < 4; kt++) {
+            v4f acc = { 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+            for (int st = 0; st < NS; st++) {
+                const v8bf k = levels(kw[kt][st]);
+                acc = mfma(k, q[st].p[2], acc);
+                acc = mfma(k, q[st].p[1], acc);
+                acc = mfma(k, q[st].p[0], acc);
             }
-            best = fmaxf(best, __shfl_xor(best, 16));
-            best = fmaxf(best, __shfl_xor(best, 32));
-            const float now = fmaxf(top, best), base = now == -INFINITY ? 0.0f : now;
-            const float scale = __builtin_amdgcn_exp2f(top - base);
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                s[kt][r] = __builtin_fmaf(acc[r], bf_of(ks[kt], r) * c2, add[kt][r]);
+        }
+        if (!inside) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int32_t f = j + 16 * (i / 4) + i % 4;
+                s[i / 4][i % 4] = f >= lo && f <= hi ? s[i / 4][i % 4] : -INFINITY;
+            }
+        }
+        more = walk.next(a, sh, pg, id);
+        const uint8_t *rec = record_of(id);
+        load_keys(rec, pg);
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            best = fmaxf(best, s[i / 4][i % 4]);
+        best = fmaxf(best, __shfl_xor(best, 16));
+        best = fmaxf(best, __shfl_xor(best, 32));
+        if (__any(best > top)) {
+            const float now = fmaxf(top, best);
+            const float scale = __builtin_amdgcn_exp2f(top - (now == -INFINITY ? 0.0f : now));
             top = now;
             sum *= scale;
 #pragma unroll
             for (int i = 0; i < 2 * NS; i++)
                 o[i] *= scale;
+        }
+        const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-            for (int gg = 0; gg < 2; gg++) {
-                float x[8];
+        for (int gg = 0; gg < 2; gg++) {
+            float x[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int kt = 2 * gg + i / 4, r = i % 4;
-                    const v2u vs = *(const v2u *)(rec + cache_value_scale_at(dk, 16 * kt + 4 * w));
-                    const float e = __builtin_amdgcn_exp2f(s[kt][r] - base);
-                    sum += e;
-                    /* a frame that is not attended may have a scale that was never written */
-                    x[i] = s[kt][r] == -INFINITY ? 0.0f : e * bf_of(vs, r);
-                }
-                const Pieces pr = cut(x);
+            for (int i = 0; i < 8; i++) {
+                const int kt = 2 * gg + i / 4, r = i % 4;
+                const float e = __builtin_amdgcn_exp2f(s[kt][r] - base);
+                sum += e;
+                x[i] = e * bf_of(vs[kt], r);
+            }
+            if (!inside) {
+                /* a frame that is not attended may have a scale that was never written */
 #pragma unroll
-                for (int dt = 0; dt < 2 * NS; dt++) {
-                    const v8bf val = levels(*(const uint32_t *)(rec + cache_values_at(dk) + 1024 * (dt / 2) + 16 * lane +
-                                                                8 * (dt % 2) + 4 * gg));
-                    o[dt] = mfma(val, pr.p[2], o[dt]);
-                    o[dt] = mfma(val, pr.p[1], o[dt]);
-                    o[dt] = mfma(val, pr.p[0], o[dt]);
-                }
+                for (int i = 0; i < 8; i++)
+                    x[i] = s[2 * gg + i / 4][i % 4] == -INFINITY ? 0.0f : x[i];
+            }
+            const Pieces pr = cut(x);
+#pragma unroll
+            for (int dt = 0; dt < 2 * NS; dt++) {
+                const v8bf val = levels(vw[dt / 2][2 * (dt % 2) + gg]);
+                o[dt] = mfma(val, pr.p[2], o[dt]);
+                o[dt] = mfma(val, pr.p[1], o[dt]);
+                o[dt] = mfma(val, pr.p[0], o[dt]);
             }
         }
+        load_values(rec);
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
@@ -786,8 +957,10 @@ size_t cache_attention_workspace(const CacheStreams &st, uint32_t G, uint32_t H,
 template <int NS>
 static void attend(const CacheAttention &a, const Deal &d, hipStream_t s) {
     if (a.p) {
-        const dim3 grid((a.bw + 64 * kPlaceTiles - 1) / (64 * kPlaceTiles), a.H, (a.st.rows + kPlaceRows - 1) / kPlaceRows);
-        cache_place_kernel<NS><<<grid, 256, 0, s>>>(a);
+        /* runs one after another where there are workgroups enough without: the rows' operands are made once for all */
+        const uint32_t runs = (a.bw + kPlaceRun - 1) / kPlaceRun, blocks = (a.st.rows + kPlaceRows - 1) / kPlaceRows;
+        const uint32_t steps = std::min(8u, std::max(1u, (uint32_t)((uint64_t)runs * a.H * blocks / 1024)));
+        cache_place_kernel<NS><<<dim3((runs + steps - 1) / steps, a.H, blocks), 256, 0, s>>>(a, (int32_t)steps);
     }
     const uint32_t grid = (uint32_t)(d.units * d.splits);
     if (d.rows == 4)
@@ -796,9 +969,9 @@ static void attend(const CacheAttention &a, const Deal &d, hipStream_t s) {
         cache_many_kernel<NS><<<grid, 256, 0, s>>>(a);
     if (d.splits > 1) {
         if (d.rows == 4)
-            cache_join_kernel<4, NS><<<grid / d.splits, 256, 0, s>>>(a);
+            cache_join_kernel<4, NS><<<dim3(grid / d.splits, std::min(d.rows, a.st.max_T * (a.H / a.G))), 256, 0, s>>>(a);
         else
-            cache_join_kernel<16, NS><<<grid / d.splits, 256, 0, s>>>(a);
+            cache_join_kernel<16, NS><<<dim3(grid / d.splits, std::min(d.rows, a.st.max_T * (a.H / a.G))), 256, 0, s>>>(a);
     }
 }
 
