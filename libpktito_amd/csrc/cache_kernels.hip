@@ -182,12 +182,18 @@ struct CacheAttention {
     float scale;                            /* 1 / sqrt(dk) */
     /* positions (p NULL: none): row place0 is distance left's */
     const float *p, *bias_u, *bias_w;
-    float *place;                           /* [rows][H][place_stride(bw)] */
+    float *place;                           /* the position scores, [rows][H][place_stride(bw)] */
     uint32_t bw;
+    void *halved;                           /* the table's operands, [H][tiles of 16][steps][2][64 lanes], and its exponents */
+    int32_t *halved_expo;
     /* a stream's tiles of rows a kept head, workgroups that share a tile's pages, what they leave each other */
     uint32_t tiles, splits;
     float *parts;
 };
+
+__device__ __forceinline__ uint64_t unit_of(const CacheAttention &a, uint32_t b, uint32_t tile, uint32_t g) {
+    return ((uint64_t)b * a.tiles + tile) * a.G + g;
+}
 
 /* A row of floats cut in two float16 for a product of floats with floats: times
  * the power of two that puts the row's largest magnitude into [2^14, 2^15),
@@ -208,6 +214,15 @@ __device__ __forceinline__ int row_exponent(uint32_t top_bits) {
     return e == 128 || top_bits == 0 ? 0 : max(e, -112);
 }
 
+/* the largest magnitude, NaNs passed over (they are in the pieces) */
+__device__ __forceinline__ float largest(const float (&x)[8]) {
+    float m = fmaxf(fabsf(x[0]), fabsf(x[1]));
+#pragma unroll
+    for (int i = 2; i < 8; i++)
+        m = fmaxf(m, fabsf(x[i]));
+    return m;
+}
+
 __device__ __forceinline__ Halves halve(const float (&x)[8], int e) {
     const float s = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
     Halves r;
@@ -224,45 +239,100 @@ __device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+/* Sixteen rows of the positions' table for one head as the matrix
+ * instruction's operand: lane l has dimensions 32 s + 8 (l / 16) of row l % 16
+ * in step s, and that row's exponent. */
+template <int NS>
+struct PlaceTile {
+    v4f p[NS][2];
+
+    __device__ __forceinline__ void load(const CacheAttention &a, uint32_t h, uint32_t x) {
+        const uint32_t lane = threadIdx.x & 63, dk = 32 * NS;
+        const v4f *src = (const v4f *)(a.p + (uint64_t)min(x + lane % 16, a.bw - 1) * (a.H * dk) + h * dk + lane / 16 * 8);
+#pragma unroll
+        for (int s = 0; s < NS; s++)
+            p[s][0] = src[8 * s], p[s][1] = src[8 * s + 1];
+    }
+
+    __device__ __forceinline__ int halves(Halves (&out)[NS]) const {
+        float x[NS][8], most = 0.0f;
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                x[s][j] = p[s][j / 4][j % 4];
+            most = fmaxf(most, largest(x[s]));
+        }
+        int top = mag_bits(most);
+        top = max(top, __shfl_xor(top, 16));
+        top = max(top, __shfl_xor(top, 32));
+        const int e = row_exponent((uint32_t)top);
+#pragma unroll
+        for (int s = 0; s < NS; s++)
+            out[s] = halve(x[s], e);
+        return e;
+    }
+};
+
+/* The table halved once for a call whose rows would do it many times over: a
+ * wave a tile of a head, its operands 1 KB in a row each, then the exponents. */
+template <int NS>
+__global__ __launch_bounds__(256) void cache_halve_kernel(CacheAttention a) {
+    const uint32_t tiles = (a.bw + 15) / 16, lane = threadIdx.x & 63;
+    const uint32_t h = blockIdx.y, tile = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (tile >= tiles)
+        return;
+    PlaceTile<NS> t;
+    t.load(a, h, 16 * tile);
+    Halves ph[NS];
+    const int e = t.halves(ph);
+    v8h *to = (v8h *)a.halved + ((uint64_t)h * tiles + tile) * (NS * 2 * 64) + lane;
+#pragma unroll
+    for (int s = 0; s < NS; s++)
+        to[128 * s] = ph[s].hi, to[128 * s + 64] = ph[s].lo;
+    if (lane < 16)
+        a.halved_expo[((uint64_t)h * tiles + tile) * 16 + lane] = e;
+}
+
 /* The position scores (q + w) . p, scaled as the softmax takes them (in powers
  * of 2), of every row at every distance that it needs, into the workspace:
  * the same rows of p serve every stream, so this is one product of all rows by
  * the table, read once, where the attention reads its own stream's pages only.
- * A workgroup takes 64 rows of a head, halved into the matrix instruction's
- * operands in LDS, and walks `steps` runs of 128 distances; a wave takes 32 of
- * each, two tiles, so that an operand read from LDS serves two. */
-constexpr int kPlaceRows = 64, kPlaceRun = 128;
-template <int NS>
-__global__ __launch_bounds__(256) void cache_place_kernel(CacheAttention a, int32_t steps) {
-    __shared__ v8h frag[kPlaceRows / 16][NS][2][64];
-    __shared__ int32_t need_lo, need_hi, expo[kPlaceRows];
-    const uint32_t h = blockIdx.y, n0 = blockIdx.z * kPlaceRows;
-    const int32_t x0 = (int32_t)blockIdx.x * (kPlaceRun * steps), x1 = min(x0 + kPlaceRun * steps, (int32_t)a.bw);
+ * A workgroup of RT waves takes 16 RT rows of a head, halved into the matrix
+ * instruction's operands in LDS, and walks `steps` runs of 32 RT distances; a
+ * wave takes 32 of each, two tiles, so that an operand read from LDS serves
+ * two. */
+template <int NS, int RT, int W, int MT, bool PRE>
+__global__ __launch_bounds__(64 * W, 4) void cache_place_kernel(CacheAttention a, int32_t steps) {
+    constexpr int kRows = 16 * RT, kRun = 16 * MT * W, kThreads = 64 * W, kFill = kRows * 16 / kThreads;
+    __shared__ v8h frag[RT][NS][2][64];
+    __shared__ int32_t need_lo, need_hi, expo[kRows];
+    const uint32_t h = blockIdx.y, n0 = blockIdx.z * kRows;
+    const int32_t x0 = (int32_t)blockIdx.x * (kRun * steps), x1 = min(x0 + kRun * steps, (int32_t)a.bw);
     const uint32_t dk = 32 * NS, stride = place_stride(a.bw);
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = lane / 16;
-    const uint32_t rows = min((uint32_t)kPlaceRows, a.st.rows - n0);
+    const uint32_t rows = min((uint32_t)kRows, a.st.rows - n0);
 
-    v4f p[2][NS][2];
-    auto load = [&](int32_t x) {
+    /* the rows' queries, 16 lanes a row: in flight while the streams are looked through */
+    const uint32_t part = threadIdx.x % 16, row_a = threadIdx.x / 16;
+    v4f qv[kFill][2] = {}, bias[2] = {};
+    if (part < 4 * NS) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint32_t m = min((uint32_t)x + 16 * i + lane % 16, a.bw - 1);
-#pragma unroll
-            for (int s = 0; s < NS; s++) {
-                const v4f *src = (const v4f *)(a.p + (uint64_t)m * (a.H * dk) + h * dk + 32 * s + 8 * w);
-                p[i][s][0] = src[0], p[i][s][1] = src[1];
-            }
+        for (int i = 0; i < kFill; i++) {
+            const v4f *src = (const v4f *)(a.q + (uint64_t)(n0 + min(row_a + 4 * W * i, rows - 1)) * a.qs + h * dk + 8 * part);
+            qv[i][0] = src[0], qv[i][1] = src[1];
         }
-    };
-    load(x0 + 32 * (int32_t)wave);
+        const v4f *b = (const v4f *)(a.bias_w + h * dk + 8 * part);
+        bias[0] = b[0], bias[1] = b[1];
+    }
     if (threadIdx.x == 0)
         need_lo = INT32_MAX, need_hi = INT32_MIN;
     __syncthreads();
     /* the distances that any of the rows needs */
     int32_t lo = INT32_MAX, hi = INT32_MIN;
-    for (uint32_t b = threadIdx.x; b < a.st.B; b += 256) {
+    for (uint32_t b = threadIdx.x; b < a.st.B; b += kThreads) {
         const CacheSpan sp = span_of(a.st, b);
-        const int32_t r0 = max(sp.r0, (int32_t)n0), r1 = min(sp.r0 + sp.T, (int32_t)(n0 + kPlaceRows));
+        const int32_t r0 = max(sp.r0, (int32_t)n0), r1 = min(sp.r0 + sp.T, (int32_t)(n0 + kRows));
         if (r0 >= r1)
             continue;
         const int32_t p0 = sp.len + r0 - sp.r0, p1 = sp.len + r1 - 1 - sp.r0;
@@ -273,74 +343,65 @@ __global__ __launch_bounds__(256) void cache_place_kernel(CacheAttention a, int3
         atomicMin(&need_lo, lo);
         atomicMax(&need_hi, hi);
     }
+    const float c2 = a.scale * 1.44269504088896340736f;     /* scores in powers of 2 */
 #pragma unroll
-    for (uint32_t i = threadIdx.x; i < kPlaceRows * 16; i += 256) {
-        const uint32_t row = i / 16, part = i % 16;                 /* eight dimensions */
-        float x[8] = {};
-        if (row < rows && part < 4 * NS) {
-            const v4f *src = (const v4f *)(a.q + (uint64_t)(n0 + row) * a.qs + h * dk + 8 * part);
-            const v4f *bias = (const v4f *)(a.bias_w + h * dk + 8 * part);
-            const v4f s0 = src[0] + bias[0], s1 = src[1] + bias[1];
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                x[j] = s0[j], x[4 + j] = s1[j];
-        }
-        int top = 0;
+    for (int i = 0; i < kFill; i++) {
+        const uint32_t row = row_a + 4 * W * i;
+        float x[8];
 #pragma unroll
         for (int j = 0; j < 8; j++)
-            top = max(top, mag_bits(x[j]));
-        const int e = row_exponent((uint32_t)group_max_nonneg<16>(top));
+            x[j] = (qv[i][j / 4][j % 4] + bias[j / 4][j % 4]) * c2;
+        const int e = row_exponent((uint32_t)group_max_nonneg<16>(mag_bits(largest(x))));
         const Halves c = halve(x, e);
-        if (part < 4 * NS) {
-            frag[row / 16][part / 4][0][16 * (part % 4) + row % 16] = c.hi;
-            frag[row / 16][part / 4][1][16 * (part % 4) + row % 16] = c.lo;
+        if (part < 4 * NS) {                /* a row's parts in different banks */
+            frag[row / 16][part / 4][0][16 * (part % 4) + (row % 16 ^ part)] = c.hi;
+            frag[row / 16][part / 4][1][16 * (part % 4) + (row % 16 ^ part)] = c.lo;
         }
         if (part == 0)
             expo[row] = e;
     }
     __syncthreads();
     const int32_t from = need_lo, to = need_hi;
-    const float c2 = a.scale * 1.44269504088896340736f;
 #pragma unroll 1
-    for (int32_t x = x0 + 32 * (int32_t)wave; x < x1; x += kPlaceRun) {
-        if (from >= x + 32 || to < x) {
-            if (to < x)
-                break;
-            load(x + kPlaceRun);
+    for (int32_t x = x0 + 16 * MT * (int32_t)wave; x < x1 && x <= to; x += kRun) {
+        if (from >= x + 16 * MT)
             continue;
-        }
-        Halves ph[2][NS];
-        int pe[2][4];
+        Halves ph[MT][NS];
+        int pe[MT][4];
+        if constexpr (PRE) {
+            const uint32_t tiles = (a.bw + 15) / 16;
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            int top = 0;
+            for (int i = 0; i < MT; i++) {
+                const uint32_t tile = min((uint32_t)x / 16 + i, tiles - 1);
+                const v8h *src = (const v8h *)a.halved + ((uint64_t)h * tiles + tile) * (NS * 2 * 64) + lane;
 #pragma unroll
-            for (int s = 0; s < NS; s++)
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    top = max(top, mag_bits(p[i][s][j / 4][j % 4]));
-            top = max(top, __shfl_xor(top, 16));
-            top = max(top, __shfl_xor(top, 32));
-            const int e = row_exponent((uint32_t)top);
-#pragma unroll
-            for (int s = 0; s < NS; s++) {
-                const float xs[8] = { p[i][s][0][0], p[i][s][0][1], p[i][s][0][2], p[i][s][0][3],
-                                      p[i][s][1][0], p[i][s][1][1], p[i][s][1][2], p[i][s][1][3] };
-                ph[i][s] = halve(xs, e);
+                for (int s = 0; s < NS; s++)
+                    ph[i][s].hi = src[128 * s], ph[i][s].lo = src[128 * s + 64];
+                const int4 e = *(const int4 *)(a.halved_expo + ((uint64_t)h * tiles + tile) * 16 + 4 * w);
+                pe[i][0] = e.x, pe[i][1] = e.y, pe[i][2] = e.z, pe[i][3] = e.w;
             }
+        } else {
+            PlaceTile<NS> t[MT];
 #pragma unroll
-            for (int r = 0; r < 4; r++)
-                pe[i][r] = __shfl(e, 4 * w + r) - 28;
+            for (int i = 0; i < MT; i++)
+                t[i].load(a, h, (uint32_t)x + 16 * i);
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+                const int e = t[i].halves(ph[i]);
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    pe[i][r] = __shfl(e, 4 * w + r);
+            }
         }
-        load(x + kPlaceRun);
 #pragma unroll 1
         for (uint32_t rt = 0; 16 * rt < rows; rt++) {
-            v4f acc[2] = {};
+            v4f acc[MT] = {};
 #pragma unroll
             for (int s = 0; s < NS; s++) {
-                const v8h qh = frag[rt][s][0][lane], ql = frag[rt][s][1][lane];
+                const uint32_t at = 16 * w + (lane % 16 ^ (4 * s + w));
+                const v8h qh = frag[rt][s][0][at], ql = frag[rt][s][1][at];
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
+                for (int i = 0; i < MT; i++) {
                     acc[i] = mfma(ph[i][s].lo, qh, acc[i]);
                     acc[i] = mfma(ph[i][s].hi, ql, acc[i]);
                     acc[i] = mfma(ph[i][s].hi, qh, acc[i]);
@@ -348,15 +409,15 @@ __global__ __launch_bounds__(256) void cache_place_kernel(CacheAttention a, int3
             }
             const uint32_t row = 16 * rt + lane % 16;
             const int qe = expo[row];
+            float *to_row = a.place + ((uint64_t)(n0 + row) * a.H + h) * stride + kPlacePad + x + 4 * w;
             if (row < rows) {
-                float *to_row = a.place + ((uint64_t)(n0 + row) * a.H + h) * stride + kPlacePad + x + 4 * w;
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
+                for (int i = 0; i < MT; i++) {
                     v4f y;
 #pragma unroll
                     for (int r = 0; r < 4; r++)
-                        y[r] = __builtin_ldexpf(acc[i][r], pe[i][r] + qe) * c2;
-                    *(v4f *)(to_row + 16 * i) = y;
+                        y[r] = __builtin_ldexpf(acc[i][r], pe[i][r] + qe - 28);
+                    __builtin_nontemporal_store(y, (v4f *)(to_row + 16 * i));
                 }
             }
         }
@@ -371,7 +432,7 @@ struct Share {
     CacheSpan sp;
     uint32_t g, b, grp, split;
     int32_t nrows, rr0;                     /* the stream's rows, the tile's first */
-    int32_t pa, pb;                         /* pages [pa, pb) of the stream */
+    int32_t pa, pb;                         /* the workgroup's pages, [pa, pb) of the stream */
     uint64_t unit;                          /* the tile among all of the call's */
 };
 
@@ -394,9 +455,12 @@ __device__ __forceinline__ bool share_of(const CacheAttention &a, Share &s, uint
     const int32_t each = (p1 - p0 + (int32_t)splits - 1) / (int32_t)splits;
     s.pa = min(p0 + (int32_t)s.split * each, p1);
     s.pb = min(s.pa + each, p1);
-    s.unit = ((uint64_t)s.b * a.tiles + tile) * a.G + s.g;
+    s.unit = unit_of(a, s.b, tile, s.g);
     return true;
 }
+
+/* the wave's number in its workgroup, known to be the same in all its lanes */
+__device__ __forceinline__ uint32_t wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 /* The pages that a wave takes, every fourth of its workgroup's: 64 table
  * entries at a time, one a lane, those that are no page of the pool passed
@@ -406,7 +470,7 @@ struct Walk {
     uint64_t left;
 
     __device__ __forceinline__ Walk(const CacheAttention &a, const Share &s)
-        : first(s.pa + (int32_t)(threadIdx.x >> 6) - 4 * 64), ids(0), left(0) {}
+        : first(s.pa + (int32_t)wave_id() - 4 * 64), ids(0), left(0) {}
 
     /* the next page and its place in the pool; false, and pg and id as they were, after the last */
     __device__ __forceinline__ bool next(const CacheAttention &a, const Share &s, int32_t &pg, int32_t &id) {
@@ -555,7 +619,7 @@ __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttention a) {
  * a lane's four scores are neighbours in memory: their scales and position
  * scores are one load each. The probabilities cross lanes once, cut, through
  * LDS, to be the second product's rows as the queries were the first's. */
-template <int NS>
+template <int NS, bool POS>
 __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
     constexpr uint32_t dk = 32 * NS, record = kPage * dk + 4 * kPage;
     constexpr uint32_t kRow = 72;           /* bfloat16 a row of pieces: 64 and a pad against bank conflicts */
@@ -564,8 +628,9 @@ __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
     Share s;
     if (!share_of<4>(a, s, a.splits))
         return;
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = lane / 16, c = lane % 16;
+    const uint32_t lane = threadIdx.x & 63, wave = wave_id(), w = lane / 16, c = lane % 16;
 
+    const float c2 = a.scale * 1.44269504088896340736f;     /* scores in powers of 2 */
     v8bf q[NS];
     {
         const int32_t i = (int32_t)(c / 4);
@@ -580,14 +645,14 @@ __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
             const uint32_t d = h * dk + w * (8 * NS) + 8 * st;
             const v4f *src = (const v4f *)(a.q + row * a.qs + d);
             v4f s0 = src[0], s1 = src[1];
-            if (a.p) {
+            if constexpr (POS) {
                 const v4f *bias = (const v4f *)(a.bias_u + d);
                 s0 += bias[0], s1 += bias[1];
             }
             uint32_t u[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                float x = j < 4 ? s0[j % 4] : s1[j % 4];
+                float x = (j < 4 ? s0[j % 4] : s1[j % 4]) * c2;
                 x -= __uint_as_float(__float_as_uint(x) & m1);
                 x -= __uint_as_float(__float_as_uint(x) & m2);
                 u[j] = live ? __float_as_uint(x) : 0;
@@ -605,11 +670,10 @@ __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
     const int32_t pos = s.sp.len + wi / (int32_t)s.grp;
     const int32_t lo = cache_lo(pos, a.left), hi = mine ? cache_hi(pos, a.right, s.sp.total) : -1;
     const float *place = nullptr;
-    if (a.p)
+    if constexpr (POS)
         place = a.place + ((uint64_t)(s.sp.r0 + wi / (int32_t)s.grp) * a.H + s.g * s.grp + (uint32_t)wi % s.grp) *
-                              place_stride(a.bw) + kPlacePad + (a.left - pos);
+                              place_stride(a.bw) + kPlacePad + (a.left - pos) + 4 * c;
 
-    const float c2 = a.scale * 1.44269504088896340736f;     /* scores in powers of 2 */
     float top = -INFINITY, sum = 0.0f;
     v4f o[2 * NS] = {};
 
@@ -627,13 +691,13 @@ __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
             for (int st = 0; st < NS; st++)
                 kw[kt][st] = ((const uint32_t *)(rec + cache_key_at(dk, 4 * c + kt) + w * (4 * NS)))[st];
         ks = *(const v2u *)(rec + cache_key_scale_at(dk, 4 * c));
-        if (a.p)
-            add = *(const v4f_u *)(place + pg * (int32_t)kPage + 4 * (int32_t)c);
+        if constexpr (POS)
+            add = *(const v4f_u *)(place + pg * (int32_t)kPage);
     };
     auto load_values = [&](const uint8_t *rec) {
 #pragma unroll
         for (int i = 0; i < NS; i++)
-            vw[i] = *(const v4u *)(rec + cache_values_at(dk) + 1024 * i + 16 * lane);
+            vw[i] = __builtin_nontemporal_load((const v4u *)(rec + cache_values_at(dk) + 1024 * i + 16 * lane));
         vs = *(const v2u *)(rec + cache_value_scale_at(dk, 4 * c));
     };
 
@@ -647,13 +711,15 @@ __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
     while (more) {
         float x[4], best = -INFINITY;
         const int32_t j = pg * (int32_t)kPage + 4 * (int32_t)c;
+        v4f acc[4] = {};                    /* four chains side by side: a product waits for the one before it in its own */
+#pragma unroll
+        for (int st = 0; st < NS; st++)
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++)
+                acc[kt] = mfma(q[st], levels(kw[kt][st]), acc[kt]);
 #pragma unroll
         for (int kt = 0; kt < 4; kt++) {
-            v4f acc = { 0.0f, 0.0f, 0.0f, 0.0f };
-#pragma unroll
-            for (int st = 0; st < NS; st++)
-                acc = mfma(q[st], levels(kw[kt][st]), acc);
-            const float v = __builtin_fmaf((acc[2] + acc[1]) + acc[0], bf_of(ks, kt) * c2, add[kt]);
+            const float v = __builtin_fmaf((acc[kt][2] + acc[kt][1]) + acc[kt][0], bf_of(ks, kt), add[kt]);
             x[kt] = j + kt >= lo && j + kt <= hi ? v : -INFINITY;
             best = fmaxf(best, x[kt]);
         }
@@ -718,7 +784,7 @@ __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
 /* More rows: 16 a workgroup, its four waves a page each in turn with the
  * running maximum and sum of a softmax, a query a column and its pieces three
  * products one after another. */
-template <int NS>
+template <int NS, bool POS>
 __global__ __launch_bounds__(256) void cache_many_kernel(CacheAttention a) {
     constexpr uint32_t dk = 32 * NS, record = kPage * dk + 4 * kPage;
     __shared__ float part[4][16][dk + 4], tops[4][16], sums[4][16];
@@ -726,7 +792,7 @@ __global__ __launch_bounds__(256) void cache_many_kernel(CacheAttention a) {
     if (!share_of<16>(a, sh, a.splits))
         return;
     const CacheSpan &sp = sh.sp;
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = lane / 16;
+    const uint32_t lane = threadIdx.x & 63, wave = wave_id(), w = lane / 16;
     const int32_t rr = min(sh.rr0 + (int32_t)(lane % 16), sh.nrows - 1);
     const int32_t t = rr / (int32_t)sh.grp;
     const uint32_t h = sh.g * sh.grp + (uint32_t)rr % sh.grp;
@@ -734,28 +800,29 @@ __global__ __launch_bounds__(256) void cache_many_kernel(CacheAttention a) {
     const int32_t pos = sp.len + t;
     const int32_t lo = cache_lo(pos, a.left), hi = cache_hi(pos, a.right, sp.total);
 
+    const float c2 = a.scale * 1.44269504088896340736f;     /* scores in powers of 2 */
     Pieces q[NS];
 #pragma unroll
     for (int s = 0; s < NS; s++) {
         const uint32_t c = h * dk + w * (8 * NS) + 8 * s;
         const v4f *src = (const v4f *)(a.q + row * a.qs + c);
         v4f s0 = src[0], s1 = src[1];
-        if (a.p) {
+        if constexpr (POS) {
             const v4f *bias = (const v4f *)(a.bias_u + c);
             s0 += bias[0], s1 += bias[1];
         }
+        s0 *= c2, s1 *= c2;
         const float x[8] = { s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3] };
         q[s] = cut(x);
     }
     const float *place = nullptr;
-    if (a.p)
-        place = a.place + (row * a.H + h) * place_stride(a.bw) + kPlacePad + (a.left - pos);
+    if constexpr (POS)
+        place = a.place + (row * a.H + h) * place_stride(a.bw) + kPlacePad + (a.left - pos) + 4 * w;
 
     /* frames that every row of the tile attends */
     const int32_t t1 = min(sh.rr0 + 15, sh.nrows - 1) / (int32_t)sh.grp;
     const int32_t all_lo = cache_lo(sp.len + t1, a.left);
     const int32_t all_hi = cache_hi(sp.len + sh.rr0 / (int32_t)sh.grp, a.right, sp.total);
-    const float c2 = a.scale * 1.44269504088896340736f;     /* scores in powers of 2 */
     float top = -INFINITY, sum = 0.0f;
     v4f o[2 * NS] = {};
 
@@ -772,8 +839,8 @@ __global__ __launch_bounds__(256) void cache_many_kernel(CacheAttention a) {
             for (int st = 0; st < NS; st++)
                 kw[kt][st] = ((const uint32_t *)(rec + cache_key_at(dk, 16 * kt + lane % 16) + w * (4 * NS)))[st];
             ks[kt] = *(const v2u *)(rec + cache_key_scale_at(dk, 16 * kt + 4 * w));
-            if (a.p)
-                add[kt] = *(const v4f_u *)(place + pg * (int32_t)kPage + 16 * kt + 4 * (int32_t)w);
+            if constexpr (POS)
+                add[kt] = *(const v4f_u *)(place + pg * (int32_t)kPage + 16 * kt);
         }
     };
     auto load_values = [&](const uint8_t *rec) {
@@ -796,20 +863,22 @@ __global__ __launch_bounds__(256) void cache_many_kernel(CacheAttention a) {
         float s[4][4], best = -INFINITY;
         const int32_t j = pg * (int32_t)kPage + 4 * (int32_t)w;
         const bool inside = pg * (int32_t)kPage >= all_lo && pg * (int32_t)kPage + (int32_t)kPage - 1 <= all_hi;
+        v4f acc[4] = {};                    /* four chains side by side: a product waits for the one before it in its own */
 #pragma unroll
-        for (int kt = 0; kt < 4; kt++) {
-            v4f acc = { 0.0f, 0.0f, 0.0f, 0.0f };
+        for (int st = 0; st < NS; st++) {
+            v8bf k[4];
 #pragma unroll
-            for (int st = 0; st < NS; st++) {
-                const v8bf k = levels(kw[kt][st]);
-                acc = mfma(k, q[st].p[2], acc);
-                acc = mfma(k, q[st].p[1], acc);
-                acc = mfma(k, q[st].p[0], acc);
-            }
+            for (int kt = 0; kt < 4; kt++)
+                k[kt] = levels(kw[kt][st]);
 #pragma unroll
-            for (int r = 0; r < 4; r++)
-                s[kt][r] = __builtin_fmaf(acc[r], bf_of(ks[kt], r) * c2, add[kt][r]);
+            for (int n = 2; n >= 0; n--)
+#pragma unroll
+                for (int kt = 0; kt < 4; kt++)
+                    acc[kt] = mfma(k[kt], q[st].p[n], acc[kt]);
         }
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            s[i / 4][i % 4] = __builtin_fmaf(acc[i / 4][i % 4], bf_of(ks[i / 4], i % 4), add[i / 4][i % 4]);
         if (!inside) {
 #pragma unroll
             for (int i = 0; i < 16; i++) {
@@ -852,13 +921,15 @@ __global__ __launch_bounds__(256) void cache_many_kernel(CacheAttention a) {
                     x[i] = s[2 * gg + i / 4][i % 4] == -INFINITY ? 0.0f : x[i];
             }
             const Pieces pr = cut(x);
+            v8bf val[2 * NS];
 #pragma unroll
-            for (int dt = 0; dt < 2 * NS; dt++) {
-                const v8bf val = levels(vw[dt / 2][2 * (dt % 2) + gg]);
-                o[dt] = mfma(val, pr.p[2], o[dt]);
-                o[dt] = mfma(val, pr.p[1], o[dt]);
-                o[dt] = mfma(val, pr.p[0], o[dt]);
-            }
+            for (int dt = 0; dt < 2 * NS; dt++)
+                val[dt] = levels(vw[dt / 2][2 * (dt % 2) + gg]);
+#pragma unroll
+            for (int n = 2; n >= 0; n--)
+#pragma unroll
+                for (int dt = 0; dt < 2 * NS; dt++)
+                    o[dt] = mfma(val[dt], pr.p[n], o[dt]);
         }
         load_values(rec);
     }
@@ -926,7 +997,8 @@ int launch_cache_read(const uint8_t *data, uint32_t pages, uint32_t G, uint32_t 
  * four a kept head, else of 16; and enough splits of a tile's pages that the
  * chip has work, none of them under four pages (one a wave). */
 struct Deal {
-    uint32_t rows, tiles, splits;
+    uint32_t rows, tiles, splits;           /* rows a tile, a stream's tiles a kept head, a tile's splits */
+    uint32_t pages;                         /* pages a tile can reach */
     uint64_t units;
 };
 
@@ -936,37 +1008,76 @@ static Deal deal(const CacheStreams &st, uint32_t G, uint32_t H, int32_t left, i
     d.rows = rows <= 4 ? 4 : 16;
     d.tiles = (rows + d.rows - 1) / d.rows;
     d.units = (uint64_t)st.B * G * d.tiles;
-    const uint64_t reach = (uint64_t)left + (uint64_t)right + st.max_T;
-    const uint64_t pages = std::min<uint64_t>(st.max_pages, reach / kPage + 2);
+    d.pages = cache_tile_pages(st.max_pages, left, right);
     const uint64_t want = d.units ? (1024 + d.units - 1) / d.units : 1;
-    d.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({ want, (pages + 3) / 4, 128 }));
+    d.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({ want, (d.pages + 3) / 4, 128 }));
     return d;
 }
 
-static size_t place_bytes(const CacheStreams &st, uint32_t H, int32_t left, int32_t right) {
-    return (size_t)st.rows * H * place_stride((uint32_t)left + (uint32_t)right + 1) * sizeof(float);
+/* From this many rows on, the position scores are made of a table halved
+ * beforehand, 128 rows a workgroup: with 2624 rows by 3750 distances 10 + 91
+ * us, without 128; with 384 by 767 4 + 8, without 12. */
+static bool place_halved(uint32_t rows) { return rows >= 512; }
+
+static size_t halved_bytes(uint32_t H, uint32_t bw, uint32_t dk) {
+    return (size_t)H * ((bw + 15) / 16) * 16 * (4 * dk + 4);
+}
+
+/* The workspace's parts, in bytes, one after another (each a multiple of 16). */
+struct Space {
+    size_t place, halved, parts;
+};
+
+static Space space(const CacheStreams &st, uint32_t H, uint32_t dk, bool positions, uint32_t bw, const Deal &d) {
+    Space s = { 0, 0, 0 };
+    if (positions) {
+        s.place = (size_t)st.rows * H * place_stride(bw) * sizeof(float);
+        s.halved = place_halved(st.rows) ? halved_bytes(H, bw, dk) : 0;
+    }
+    if (d.splits > 1)
+        s.parts = (size_t)d.units * d.splits * d.rows * (dk + 2) * sizeof(float);
+    return s;
 }
 
 size_t cache_attention_workspace(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, bool positions,
                                  int32_t left, int32_t right) {
-    const Deal d = deal(st, G, H, left, right);
-    return (positions ? place_bytes(st, H, left, right) : 0) +
-           (d.splits > 1 ? d.units * d.splits * d.rows * (dk + 2) * sizeof(float) : 0);
+    const Space s = space(st, H, dk, positions, (uint32_t)left + (uint32_t)right + 1, deal(st, G, H, left, right));
+    return s.place + s.halved + s.parts;
+}
+
+template <int NS, int RT, int W, int MT, bool PRE>
+static void place(const CacheAttention &a, hipStream_t s) {
+    /* runs one after another where there are workgroups enough without: the rows' operands are made once for all */
+    constexpr uint32_t kRun = 16 * MT * W;
+    const uint32_t runs = (a.bw + kRun - 1) / kRun, blocks = (a.st.rows + 16 * RT - 1) / (16 * RT);
+    const uint32_t steps = std::min(8u, std::max(1u, (uint32_t)((uint64_t)runs * a.H * blocks * W / 8192)));
+    cache_place_kernel<NS, RT, W, MT, PRE><<<dim3((runs + steps - 1) / steps, a.H, blocks), 64 * W, 0, s>>>(a, (int32_t)steps);
 }
 
 template <int NS>
 static void attend(const CacheAttention &a, const Deal &d, hipStream_t s) {
     if (a.p) {
-        /* runs one after another where there are workgroups enough without: the rows' operands are made once for all */
-        const uint32_t runs = (a.bw + kPlaceRun - 1) / kPlaceRun, blocks = (a.st.rows + kPlaceRows - 1) / kPlaceRows;
-        const uint32_t steps = std::min(8u, std::max(1u, (uint32_t)((uint64_t)runs * a.H * blocks / 1024)));
-        cache_place_kernel<NS><<<dim3((runs + steps - 1) / steps, a.H, blocks), 256, 0, s>>>(a, (int32_t)steps);
+        if (place_halved(a.st.rows)) {
+            cache_halve_kernel<NS><<<dim3(((a.bw + 15) / 16 + 3) / 4, a.H), 256, 0, s>>>(a);
+            place<NS, 8, 8, 2, true>(a, s);
+        } else if ((uint64_t)((a.st.rows + 15) / 16) * ((a.bw + 15) / 16) * a.H <= 8192) {
+            /* up to eight tiles of 16 by 16 a SIMD: one workgroup's pass from the table's rows to the last store is what
+             * takes time, and 16 rows have the shortest (128 rows by 751 distances 8.1 us, with 64 rows 10.7; 256 by
+             * 4500 58 and 30) */
+            place<NS, 1, 4, 1, false>(a, s);
+        } else {
+            place<NS, 4, 4, 2, false>(a, s);
+        }
     }
     const uint32_t grid = (uint32_t)(d.units * d.splits);
-    if (d.rows == 4)
-        cache_few_kernel<NS><<<grid, 256, 0, s>>>(a);
+    if (d.rows == 4 && a.p)
+        cache_few_kernel<NS, true><<<grid, 256, 0, s>>>(a);
+    else if (d.rows == 4)
+        cache_few_kernel<NS, false><<<grid, 256, 0, s>>>(a);
+    else if (a.p)
+        cache_many_kernel<NS, true><<<grid, 256, 0, s>>>(a);
     else
-        cache_many_kernel<NS><<<grid, 256, 0, s>>>(a);
+        cache_many_kernel<NS, false><<<grid, 256, 0, s>>>(a);
     if (d.splits > 1) {
         if (d.rows == 4)
             cache_join_kernel<4, NS><<<dim3(grid / d.splits, std::min(d.rows, a.st.max_T * (a.H / a.G))), 256, 0, s>>>(a);
@@ -983,13 +1094,16 @@ int launch_cache_attention(const CacheAttentionCall &c, hipStream_t s) {
     a.left = c.left, a.right = c.right;
     a.scale = 1.0f / sqrtf((float)c.dk);
     a.p = c.p, a.bias_u = c.bias_u, a.bias_w = c.bias_w;
-    a.place = (float *)c.ws;
     a.bw = (uint32_t)c.left + (uint32_t)c.right + 1;
     const Deal d = deal(c.st, c.G, c.H, c.left, c.right);
     if (d.units * d.splits > 0x7fffffff)
         return -2;
     a.tiles = d.tiles, a.splits = d.splits;
-    a.parts = (float *)((char *)c.ws + (c.p ? place_bytes(c.st, c.H, c.left, c.right) : 0));
+    const Space sp = space(c.st, c.H, c.dk, c.p != nullptr, a.bw, d);
+    a.place = (float *)c.ws;
+    a.halved = (char *)c.ws + sp.place;
+    a.halved_expo = (int32_t *)((char *)a.halved + (size_t)c.H * ((a.bw + 15) / 16) * 16 * 4 * c.dk);
+    a.parts = (float *)((char *)c.ws + sp.place + sp.halved);
     switch (c.dk / 32) {
     case 1: attend<1>(a, d, s); break;
     case 2: attend<2>(a, d, s); break;

@@ -157,11 +157,20 @@ PK_HD int32_t cache_hi(int32_t pos, int32_t right, int32_t total) {
     return h < (int64_t)total - 1 ? (int32_t)h : total - 1;
 }
 
+/* The pages that a tile of rows reaches, at most: its rows' positions are up
+ * to 15 apart, so its frames are at most left + right + 16 in a row, which
+ * touch one page more than they fill. */
+PK_HD uint32_t cache_tile_pages(uint32_t max_pages, int32_t left, int32_t right) {
+    const uint64_t n = ((uint64_t)left + (uint64_t)right + 16 + kPage - 2) / kPage + 1;
+    return n < max_pages ? (uint32_t)n : max_pages;
+}
+
 /* The position scores' workspace: a row's bw + 2 kPlacePad floats a head,
  * score of distance x at kPlacePad + x, x = frame - (pos - left). A tile of
  * 16 rows reads whole pages for all of them: a page's first frame is up to 63
  * before the first row's lo and the rows' positions up to 15 apart, so x runs
- * from -78 to bw + 77, inside the row's pads. */
+ * from -78 to bw + 77, inside the row's pads. They are written 32 at a time,
+ * up to 31 past bw. */
 constexpr uint32_t kPlacePad = 80;
 PK_HD uint32_t place_stride(uint32_t bw) { return (bw + 2 * kPlacePad + 15) / 16 * 16; }
 

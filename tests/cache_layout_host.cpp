@@ -17,6 +17,7 @@ uint32_t t_frame_of(uint32_t g, uint32_t w, uint32_t i) { return cache_frame_of(
 uint32_t t_key_scale_at(uint32_t dk, uint32_t f) { return cache_key_scale_at(dk, f); }
 uint32_t t_value_scale_at(uint32_t dk, uint32_t f) { return cache_value_scale_at(dk, f); }
 int t_page_ok(int32_t id, uint32_t pages) { return cache_page_ok(id, pages); }
+uint32_t t_tile_pages(uint32_t max_pages, int32_t left, int32_t right) { return cache_tile_pages(max_pages, left, right); }
 uint32_t t_place_stride(uint32_t bw) { return place_stride(bw); }
 uint32_t t_place_pad(void) { return kPlacePad; }
 int32_t t_lo(int32_t pos, int32_t left) { return cache_lo(pos, left); }

@@ -27,7 +27,8 @@ def layout(tmp_path_factory):
     for name, res, args in (("t_scale", u, [f]), ("t_code", u, [f, f]), ("t_level", f, [u]), ("t_record", u, [u]),
                             ("t_key_at", u, [u, u]), ("t_value_dword", u, [u] * 4), ("t_frame_of", u, [u] * 3),
                             ("t_key_scale_at", u, [u, u]), ("t_value_scale_at", u, [u, u]),
-                            ("t_page_ok", ctypes.c_int, [i, u]), ("t_place_stride", u, [u]), ("t_place_pad", u, []),
+                            ("t_page_ok", ctypes.c_int, [i, u]), ("t_tile_pages", u, [u, i, i]), ("t_place_stride", u, [u]),
+                            ("t_place_pad", u, []),
                             ("t_lo", i, [i, i]), ("t_hi", i, [i, i, i]),
                             ("t_span", None, [u, u, u, i, i, i, ctypes.POINTER(i)])):
         getattr(l, name).restype, getattr(l, name).argtypes = res, args
@@ -91,8 +92,8 @@ def test_record_holds_each_value_once(layout, dk):
 
 
 def test_spans_stay_in_bounds(layout):
-    """Whatever the arrays hold: rows in the call, frames in the table, and the
-    position scores' reads in a row's pads."""
+    """Whatever the arrays hold: rows in the call, frames in the table, and a
+    tile's pages and position scores where they are counted."""
     r = random.Random(3)
     odd = [0, 1, -1, 2 ** 31 - 1, -2 ** 31, 63, 64, 65, 1000]
     out = (ctypes.c_int32 * 4)()
@@ -106,7 +107,6 @@ def test_spans_stay_in_bounds(layout):
         assert 0 <= r0 and 0 <= T <= max_T and r0 + T <= rows
         assert 0 <= ln <= total <= 64 * max_pages and total <= ln + T
         left, right = min(r.choice(odd[:1] + odd[5:]), 64 * max_pages - 1), min(r.choice([0, 3, 1000]), max(0, max_T - 1))
-        bw = left + right + 1
         if T == 0:
             continue
         t0 = r.randint(0, T - 1)
@@ -116,9 +116,10 @@ def test_spans_stay_in_bounds(layout):
             if 64 * pg > j1:
                 continue
             assert 0 <= pg < max_pages
+            assert pg - j0 // 64 < layout.t_tile_pages(max_pages, left, right), (left, right, j0, j1)
             for pos in (ln + t0, ln + t1):
                 first = layout.t_place_pad() + 64 * pg - (pos - left)
-                assert 0 <= first and first + 64 <= layout.t_place_stride(bw), (pos, left, right, pg)
+                assert 0 <= first and first + 64 <= layout.t_place_stride(left + right + 1), (pos, left, right, pg)
     for id, pages, ok in ((0, 1, 1), (1, 1, 0), (-1, 5, 0), (-2 ** 31, 5, 0), (4, 5, 1), (2 ** 31 - 1, 1 << 30, 0)):
         assert bool(layout.t_page_ok(id, pages)) == bool(ok)
 
