@@ -692,20 +692,29 @@ def cache_bytes(layers, pages, heads, dk):
     return lib().pk_hip_cache_bytes(layers, pages, heads, dk)
 
 
+_dtypes = {}
+
+
 def _is(t, dtype, what):
     """Refuses a tensor that a kernel would misread: another type, or one that
     is on the host."""
-    if str(t.dtype) != dtype or not t.is_cuda:
-        raise PkHipError(PK_HIP_EINVAL, f"{what}: a device tensor of {dtype[6:]}, not {t.dtype} on {t.device}")
+    want = _dtypes.get(dtype)
+    if want is None:
+        import torch
+        want = _dtypes[dtype] = getattr(torch, dtype)
+    if t.dtype is not want or not t.is_cuda:
+        raise PkHipError(PK_HIP_EINVAL, f"{what}: a device tensor of {dtype}, not {t.dtype} on {t.device}")
 
 
 def _rows(t, n, width, what):
     """A float32 matrix's address and row stride, its rows dense."""
-    _is(t, "torch.float32", what)
-    if t.dim() != 2 or t.shape[0] != n or t.shape[1] != width or (width > 1 and t.stride(1) != 1):
-        raise PkHipError(PK_HIP_EINVAL, f"{what}: [{n}, {width}] with dense rows, not {tuple(t.shape)} strides "
-                                        f"{tuple(t.stride())}")
-    return t.data_ptr(), t.stride(0) if n > 1 else width
+    _is(t, "float32", what)
+    if t.shape != (n, width):
+        raise PkHipError(PK_HIP_EINVAL, f"{what}: [{n}, {width}], not {tuple(t.shape)}")
+    rs, cs = t.stride()
+    if cs != 1 and width > 1:
+        raise PkHipError(PK_HIP_EINVAL, f"{what}: rows that are dense, not strides {(rs, cs)}")
+    return t.data_ptr(), rs if n > 1 else width
 
 
 class CacheStreams:
@@ -716,7 +725,7 @@ class CacheStreams:
 
     def __init__(self, table, len, row0, rows, max_T):
         for t, what in ((table, "table"), (len, "len"), (row0, "row0")):
-            _is(t, "torch.int32", what)
+            _is(t, "int32", what)
             if not t.is_contiguous():
                 raise PkHipError(PK_HIP_EINVAL, f"{what} is not contiguous")
         if table.dim() != 2 or tuple(len.shape) != (table.shape[0],) or tuple(row0.shape) != (table.shape[0] + 1,):
@@ -733,7 +742,7 @@ class DeviceCache:
     cache_bytes(layers, pages, heads, dk)."""
 
     def __init__(self, data, layers, pages, heads, dk):
-        _is(data, "torch.uint8", "cache")
+        _is(data, "uint8", "cache")
         if not data.is_contiguous() or data.numel() < max(1, cache_bytes(layers, pages, heads, dk)):
             raise PkHipError(PK_HIP_EINVAL, f"cache: {cache_bytes(layers, pages, heads, dk)} contiguous bytes (heads of "
                                             "32, 64, 96 or 128 dimensions)")
@@ -760,21 +769,25 @@ class DeviceCache:
         if positions is True:
             pos = Positions(16, 16, 16, 0xffffffff, 0x7fffffff)
         else:
-            pos = self._positions(positions, H)
+            pos = self._positions(positions or None, H)
         return lib().pk_hip_attention_cache_workspace(ctypes.byref(self.st), ctypes.byref(streams.st), H,
                                                       ctypes.byref(pos) if pos else None,
                                                       UNLIMITED if left is None else left,
                                                       UNLIMITED if right is None else right)
 
     def _positions(self, positions, H):
-        if not positions:
+        if positions is None:
             return None
         p, center, u, w = positions
-        for t, what in ((p, "p"), (u, "bias_u"), (w, "bias_w")):
-            _is(t, "torch.float32", what)
-            if not t.is_contiguous() or t.numel() % (H * self.dk) or (what != "p" and t.numel() != H * self.dk):
-                raise PkHipError(PK_HIP_EINVAL, f"positions: p [n, {H * self.dk}] and biases [{H * self.dk}], contiguous")
-        return Positions(p.data_ptr(), u.data_ptr(), w.data_ptr(), p.numel() // (H * self.dk), center)
+        n = H * self.dk
+        _is(p, "float32", "p")
+        _is(u, "float32", "bias_u")
+        _is(w, "float32", "bias_w")
+        rows, rest = divmod(p.numel(), n)
+        if rest or u.numel() != n or w.numel() != n or not (p.is_contiguous() and u.is_contiguous() and
+                                                            w.is_contiguous()):
+            raise PkHipError(PK_HIP_EINVAL, f"positions: p [n, {n}] and biases [{n}], contiguous")
+        return Positions(p.data_ptr(), u.data_ptr(), w.data_ptr(), rows, center)
 
     def attention(self, o, layer, q, streams, H, ws, positions=None, left=None, right=None, stream=None):
         """The attention of the rows q [rows, H * dk] to their streams' kept
@@ -795,14 +808,17 @@ class DeviceCache:
         source (this cache by default), to one of this cache; with table, an
         int32 device tensor, its entries that name a page moved follow it
         (pk_hip_cache_move_dev)."""
-        flat = np.ascontiguousarray(pairs, dtype=np.int32).reshape(-1)
+        flat = [i for pair in pairs for i in pair]
+        n = len(flat)
+        if n != 2 * len(pairs):
+            raise PkHipError(PK_HIP_EINVAL, "pairs of pages (from, to)")
         if table is not None:
-            _is(table, "torch.int32", "table")
+            _is(table, "int32", "table")
             if not table.is_contiguous():
                 raise PkHipError(PK_HIP_EINVAL, "table is not contiguous")
-        _check(lib().pk_hip_cache_move_dev(ctypes.byref(self.st), ctypes.byref((source or self).st), _ptr(flat),
-                                           flat.size // 2, _dptr(table), table.numel() if table is not None else 0,
-                                           _stream(stream)))
+        _check(lib().pk_hip_cache_move_dev(ctypes.byref(self.st), ctypes.byref((source or self).st),
+                                           (ctypes.c_int32 * max(1, n))(*flat), n // 2, _dptr(table),
+                                           table.numel() if table is not None else 0, _stream(stream)))
 
 
 class PagePool:

@@ -18,6 +18,7 @@ typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v4f_u __attribute__((ext_vector_type(4), aligned(4)));
+typedef float v2f_c __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
@@ -25,103 +26,239 @@ __device__ __forceinline__ CacheSpan span_of(const CacheStreams &s, uint32_t b) 
     return cache_span(s, s.row0[b], s.row0[b + 1], s.len[b]);
 }
 
+/* An 8 x 8 square of codes turned over: dword i's nibble n and dword n's
+ * nibble i change places. Eight frames' codes of eight dimensions become eight
+ * dimensions' codes of eight frames, and back. */
+__device__ __forceinline__ void turn(uint32_t (&a)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t t = (a[i] >> 16 ^ a[i + 4]) & 0x0000ffffu;
+        a[i + 4] ^= t, a[i] ^= t << 16;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (!(i & 2)) {
+            const uint32_t t = (a[i] >> 8 ^ a[i + 2]) & 0x00ff00ffu;
+            a[i + 2] ^= t, a[i] ^= t << 8;
+        }
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const uint32_t t = (a[i] >> 4 ^ a[i + 1]) & 0x0f0f0f0fu;
+        a[i + 1] ^= t, a[i] ^= t << 4;
+    }
+}
+
+/* Eight values' codes at scale d. The hardware's rounding to e2m1 takes x / d
+ * only as a rounded product with 1 / d, off by up to 2^-23 of itself; where it
+ * gives one code a little below and a little above, that is the code, and
+ * elsewhere (one value in 10^5, every tie among them) the exact comparisons
+ * decide: 5 instructions a value in place of 18. */
+__device__ __forceinline__ uint32_t codes(v4f a, v4f b, float d) {
+    const float id = 1.0f / d;
+    uint32_t c[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const float s = id * (i ? 1.0f + 0x1p-20f : 1.0f - 0x1p-20f);
+        const v4f x = a * s, y = b * s;
+        c[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x[0], x[1], 1.0f, 0);
+        c[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c[i], x[2], x[3], 1.0f, 1);
+        c[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c[i], y[0], y[1], 1.0f, 2);
+        c[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c[i], y[2], y[3], 1.0f, 3);
+    }
+    if (c[0] != c[1]) {
+        c[0] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            c[0] |= cache_code(a[j], d) << 4 * j | cache_code(b[j], d) << (16 + 4 * j);
+    }
+    /* no sign without a magnitude */
+    const uint32_t some = (c[0] | c[0] >> 1 | c[0] >> 2) & 0x11111111u;
+    return c[0] & (0x77777777u | some << 3);
+}
+
+/* The part of a stream's frames [len, len + T) that a workgroup has: page pg of
+ * the stream, frames [f0, f1) of it, the page's record if it has one. */
+struct PagePart {
+    CacheSpan sp;
+    int32_t base, f0, f1, id;
+    uint8_t *rec;
+};
+
+__device__ __forceinline__ bool part_of(uint8_t *data, uint32_t pages, uint32_t G, uint32_t dk, const CacheStreams &st,
+                                        PagePart &p) {
+    const uint32_t g = blockIdx.x, b = blockIdx.z;
+    p.sp = span_of(st, b);
+    const int32_t pg = p.sp.len / (int32_t)kPage + (int32_t)blockIdx.y;
+    p.base = pg * (int32_t)kPage;
+    p.f0 = max(p.sp.len - p.base, 0), p.f1 = min(p.sp.len + p.sp.T - p.base, (int32_t)kPage);
+    if (p.f0 >= p.f1)
+        return false;
+    p.id = pg < (int32_t)st.max_pages ? st.table[(uint64_t)b * st.max_pages + pg] : -1;
+    p.rec = cache_page_ok(p.id, pages) ? data + ((uint64_t)p.id * G + g) * cache_record(dk) : nullptr;
+    return true;
+}
+
+constexpr uint32_t kCodeRow = kMaxCacheDk / 8 + 1;  /* dwords of a frame's codes in LDS, and one against bank conflicts */
+
 /* ---------------------------------------------------------------- write --- */
 
 /* A workgroup writes one page's part of a stream's new frames for one kept
- * head. A wave takes a frame at a time, a lane two dimensions: the largest
- * magnitude over the wave, the scale, a byte of two codes. Keys go straight
- * to their rows. Values go through LDS and are gathered into dwords of eight
- * frames; a dword that the chunk covers in part keeps its other frames'
- * codes (read, merged, stored by one thread, so a frame that shares a byte
- * with the one before it is no race). */
+ * head: 16 lanes a frame, eight dimensions a lane, so that a frame's largest
+ * magnitude is four steps over its lanes and its codes a dword a lane. Every
+ * load is issued before the first code is made. Keys go straight to their
+ * rows. Values are turned over in LDS, eight frames by eight dimensions a
+ * thread, into the record's own order, and stored 16 bytes a lane; what a
+ * chunk covers in part keeps its other frames' codes (a lane's 16 bytes read,
+ * merged and stored by it alone, so a frame that shares a byte with the one
+ * before it is no race). */
 __global__ __launch_bounds__(256) void cache_write_kernel(uint8_t *data, uint32_t pages, uint32_t G, uint32_t dk,
                                                           CacheStreams st, const float *__restrict__ k, uint64_t ks,
                                                           const float *__restrict__ v, uint64_t vs) {
-    const uint32_t g = blockIdx.x, b = blockIdx.z;
-    const CacheSpan sp = span_of(st, b);
-    const int32_t pg = sp.len / (int32_t)kPage + (int32_t)blockIdx.y;
-    if (pg * (int32_t)kPage >= sp.total)
+    __shared__ uint32_t code[kPage][kCodeRow];
+    __shared__ v4u image[kPage * kMaxCacheDk / 2 / 16];
+    PagePart p;
+    if (!part_of(data, pages, G, dk, st, p))
         return;
-    const int32_t id = st.table[(uint64_t)b * st.max_pages + pg];
-    if (!cache_page_ok(id, pages))
+    const uint32_t part = threadIdx.x % 16, g = blockIdx.x;
+    const bool in = part < dk / 8;
+    const int32_t fa = p.f0 + (int32_t)(threadIdx.x / 16);
+    v4f x[2][4][2] = {};
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (in && fa + 16 * i < p.f1) {
+            const uint64_t row = (uint64_t)(p.sp.r0 + p.base + fa + 16 * i - p.sp.len);
+            const v4f *kp = (const v4f *)(k + row * ks + g * dk + 8 * part);
+            const v4f *vp = (const v4f *)(v + row * vs + g * dk + 8 * part);
+            x[0][i][0] = __builtin_nontemporal_load(kp), x[0][i][1] = __builtin_nontemporal_load(kp + 1);
+            x[1][i][0] = __builtin_nontemporal_load(vp), x[1][i][1] = __builtin_nontemporal_load(vp + 1);
+        }
+    if (!p.rec)
         return;
-    uint8_t *rec = data + ((uint64_t)id * G + g) * cache_record(dk);
-    const int32_t base = pg * (int32_t)kPage;
-    const int32_t f0 = max(sp.len - base, 0), f1 = min(sp.total - base, (int32_t)kPage);
-    __shared__ uint8_t code[kPage][kMaxCacheDk / 2];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const bool in = 2 * lane < dk;
-    for (int32_t f = f0 + (int32_t)wave; f < f1; f += 4) {
-        const uint64_t row = (uint64_t)(sp.r0 + base + f - sp.len);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int32_t f = fa + 16 * i;
+        if (f - (int32_t)(threadIdx.x / 16) >= p.f1)
+            break;                          /* all of the workgroup's, so the lanes stay together */
 #pragma unroll
         for (int which = 0; which < 2; which++) {
-            const float *src = which ? v + row * vs : k + row * ks;
-            float2 x = make_float2(0.0f, 0.0f);
-            if (in)
-                x = *(const float2 *)(src + g * dk + 2 * lane);
-            const uint32_t bf = cache_scale((uint32_t)wave_max_nonneg(max(mag_bits(x.x), mag_bits(x.y))));
+            const v4f a = x[which][i][0], b = x[which][i][1];
+            int top = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                top = max(top, max(mag_bits(a[j]), mag_bits(b[j])));
+            const uint32_t bf = cache_scale((uint32_t)group_max_nonneg<16>(top));
             const float d = cache_scale_value(bf);
-            const uint32_t c = bf ? cache_code(x.x, d) | cache_code(x.y, d) << 4 : 0;
-            if (in) {
-                if (which)
-                    code[f][lane] = (uint8_t)c;
-                else
-                    rec[cache_key_at(dk, f) + lane] = (uint8_t)c;
+            const uint32_t c = bf ? codes(a, b, d) : 0;
+            if (f < p.f1) {
+                if (in && which == 0)
+                    *(uint32_t *)(p.rec + cache_key_at(dk, f) + 4 * part) = c;
+                else if (in)
+                    code[f][part] = c;
+                if (part == 0)
+                    *(uint16_t *)(p.rec + (which ? cache_value_scale_at(dk, f) : cache_key_scale_at(dk, f))) =
+                        (uint16_t)bf;
             }
-            if (lane == 0)
-                *(uint16_t *)(rec + (which ? cache_value_scale_at(dk, f) : cache_key_scale_at(dk, f))) = (uint16_t)bf;
         }
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < 8 * dk; i += 256) {
-        const uint32_t c = i % dk, gg = i / dk / 4, w = i / dk % 4;
-        uint32_t val = 0, mask = 0;
+    /* a thread's square: dimensions 8 e to 8 e + 7 of the eight frames of (gg, w) */
+    if (threadIdx.x < dk) {
+        const uint32_t e = threadIdx.x / 8, gg = threadIdx.x % 2, w = threadIdx.x / 2 % 4;
+        uint32_t a[8];
 #pragma unroll
-        for (uint32_t n = 0; n < 8; n++) {
-            const int32_t f = (int32_t)cache_frame_of(gg, w, n);
-            if (f >= f0 && f < f1) {
-                val |= (code[f][c / 2] >> 4 * (c % 2) & 15u) << 4 * n;
-                mask |= 15u << 4 * n;
-            }
+        for (uint32_t n = 0; n < 8; n++)
+            a[n] = code[cache_frame_of(gg, w, n)][e];       /* frames that are not the call's: never kept below */
+        turn(a);
+#pragma unroll
+        for (uint32_t n = 0; n < 8; n++)
+            ((uint32_t *)image)[cache_value_dword(8 * e + n, gg, w) / 4] = a[n];
+    }
+    __syncthreads();
+    /* a lane's 16 bytes: dimensions c and c + 16, frames of (0, w) and (1, w) */
+    if (threadIdx.x < 2 * dk) {
+        const uint32_t w = threadIdx.x / 16 % 4;
+        uint32_t mask[2] = { 0, 0 };
+#pragma unroll
+        for (uint32_t n = 0; n < 16; n++) {
+            const int32_t f = (int32_t)cache_frame_of(n / 8, w, n % 8);
+            mask[n / 8] |= f >= p.f0 && f < p.f1 ? 15u << 4 * (n % 8) : 0;
         }
-        if (mask == 0)
-            continue;
-        uint32_t *at = (uint32_t *)(rec + cache_values_at(dk) + cache_value_dword(c, gg, w));
-        *at = mask == 0xffffffffu ? val : (*at & ~mask) | val;
+        if (mask[0] | mask[1]) {
+            v4u *at = (v4u *)(p.rec + cache_values_at(dk)) + threadIdx.x;
+            v4u now = image[threadIdx.x];
+            if (~mask[0] | ~mask[1]) {
+                const v4u old = *at;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    now[i] = (now[i] & mask[i % 2]) | (old[i] & ~mask[i % 2]);
+            }
+            *at = now;
+        }
     }
 }
 
 /* ----------------------------------------------------------------- read --- */
 
-/* A workgroup reads back one page's part of a stream's frames [len, len + T)
- * for one kept head, a thread a value at a time. Frames of a hole read as
- * zeros, and so do frames past the table. */
-__global__ __launch_bounds__(256) void cache_read_kernel(const uint8_t *__restrict__ data, uint32_t pages, uint32_t G,
-                                                         uint32_t dk, CacheStreams st, float *__restrict__ k,
-                                                         uint64_t ks, float *__restrict__ v, uint64_t vs) {
-    const uint32_t g = blockIdx.x, b = blockIdx.z;
-    const CacheSpan sp = span_of(st, b);
-    const int32_t pg = sp.len / (int32_t)kPage + (int32_t)blockIdx.y;
-    const int32_t base = pg * (int32_t)kPage;
-    const int32_t f0 = max(sp.len - base, 0), f1 = min(sp.len + sp.T - base, (int32_t)kPage);
-    if (f0 >= f1)
+/* The write's way back: a workgroup reads one page's part of a stream's frames
+ * [len, len + T) for one kept head. Frames of a hole read as zeros, and so do
+ * frames past the table. */
+__global__ __launch_bounds__(256) void cache_read_kernel(uint8_t *data, uint32_t pages, uint32_t G, uint32_t dk,
+                                                         CacheStreams st, float *__restrict__ k, uint64_t ks,
+                                                         float *__restrict__ v, uint64_t vs) {
+    __shared__ uint32_t code[kPage][kCodeRow];
+    __shared__ v4u image[kPage * kMaxCacheDk / 2 / 16];
+    PagePart p;
+    if (!part_of(data, pages, G, dk, st, p))
         return;
-    const int32_t id = pg < (int32_t)st.max_pages ? st.table[(uint64_t)b * st.max_pages + pg] : -1;
-    const bool ok = cache_page_ok(id, pages);
-    const uint8_t *rec = data + ((uint64_t)(ok ? id : 0) * G + g) * cache_record(dk);
-    for (uint32_t i = threadIdx.x; i < (uint32_t)(f1 - f0) * dk; i += 256) {
-        const uint32_t f = (uint32_t)f0 + i / dk, c = i % dk;
-        const uint64_t row = (uint64_t)(sp.r0 + base + (int32_t)f - sp.len);
-        float kv = 0.0f, vv = 0.0f;
-        if (ok) {
-            const uint32_t gg = f / 32, w = f / 4 % 4, n = 4 * (f / 16 % 2) + f % 4;
-            const uint32_t kb = rec[cache_key_at(dk, f) + c / 2] >> 4 * (c % 2) & 15u;
-            const uint32_t vb = rec[cache_values_at(dk) + cache_value_dword(c, gg, w) + n / 2] >> 4 * (n % 2) & 15u;
-            kv = cache_level(kb) * cache_scale_value(*(const uint16_t *)(rec + cache_key_scale_at(dk, f)));
-            vv = cache_level(vb) * cache_scale_value(*(const uint16_t *)(rec + cache_value_scale_at(dk, f)));
+    const uint32_t part = threadIdx.x % 16, g = blockIdx.x;
+    const int32_t fa = p.f0 + (int32_t)(threadIdx.x / 16);
+    uint32_t kc[4] = {}, ks_bf[4] = {}, vs_bf[4] = {};
+    if (p.rec) {
+        if (threadIdx.x < 2 * dk)
+            image[threadIdx.x] = ((const v4u *)(p.rec + cache_values_at(dk)))[threadIdx.x];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int32_t f = fa + 16 * i;
+            if (part < dk / 8 && f < p.f1) {
+                kc[i] = *(const uint32_t *)(p.rec + cache_key_at(dk, f) + 4 * part);
+                ks_bf[i] = *(const uint16_t *)(p.rec + cache_key_scale_at(dk, f));
+                vs_bf[i] = *(const uint16_t *)(p.rec + cache_value_scale_at(dk, f));
+            }
         }
-        k[row * ks + g * dk + c] = kv;
-        v[row * vs + g * dk + c] = vv;
+        __syncthreads();
+        if (threadIdx.x < dk) {
+            const uint32_t e = threadIdx.x / 8, gg = threadIdx.x % 2, w = threadIdx.x / 2 % 4;
+            uint32_t a[8];
+#pragma unroll
+            for (uint32_t n = 0; n < 8; n++)
+                a[n] = ((const uint32_t *)image)[cache_value_dword(8 * e + n, gg, w) / 4];
+            turn(a);
+#pragma unroll
+            for (uint32_t n = 0; n < 8; n++)
+                code[cache_frame_of(gg, w, n)][e] = a[n];
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int32_t f = fa + 16 * i;
+        if (part >= dk / 8 || f >= p.f1)
+            continue;
+        const uint64_t row = (uint64_t)(p.sp.r0 + p.base + f - p.sp.len);
+        const uint32_t vc = p.rec ? code[f][part] : 0;
+        const float kd = cache_scale_value(ks_bf[i]), vd = cache_scale_value(vs_bf[i]);
+#pragma unroll
+        for (int which = 0; which < 2; which++) {
+            const uint32_t c = which ? vc : kc[i];
+            const float d = which ? vd : kd;
+            const v2f_c y0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0);
+            const v2f_c y1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1);
+            const v2f_c y2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 2);
+            const v2f_c y3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 3);
+            v4f *to = (v4f *)((which ? v + row * vs : k + row * ks) + g * dk + 8 * part);
+            to[0] = v4f{ y0.x * d, y0.y * d, y1.x * d, y1.y * d };
+            to[1] = v4f{ y2.x * d, y2.y * d, y3.x * d, y3.y * d };
+        }
     }
 }
 
@@ -294,6 +431,17 @@ __global__ __launch_bounds__(256) void cache_halve_kernel(CacheAttention a) {
         a.halved_expo[((uint64_t)h * tiles + tile) * 16 + lane] = e;
 }
 
+/* The maximum over the wave, in every lane (all of them active). */
+__device__ __forceinline__ int wave_max(int v) {
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x142, 0xA, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x143, 0xC, 0xF, false));
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
 /* The position scores (q + w) . p, scaled as the softmax takes them (in powers
  * of 2), of every row at every distance that it needs, into the workspace:
  * the same rows of p serve every stream, so this is one product of all rows by
@@ -306,7 +454,7 @@ template <int NS, int RT, int W, int MT, bool PRE>
 __global__ __launch_bounds__(64 * W, 4) void cache_place_kernel(CacheAttention a, int32_t steps) {
     constexpr int kRows = 16 * RT, kRun = 16 * MT * W, kThreads = 64 * W, kFill = kRows * 16 / kThreads;
     __shared__ v8h frag[RT][NS][2][64];
-    __shared__ int32_t need_lo, need_hi, expo[kRows];
+    __shared__ int32_t need[W][2], expo[kRows];
     const uint32_t h = blockIdx.y, n0 = blockIdx.z * kRows;
     const int32_t x0 = (int32_t)blockIdx.x * (kRun * steps), x1 = min(x0 + kRun * steps, (int32_t)a.bw);
     const uint32_t dk = 32 * NS, stride = place_stride(a.bw);
@@ -325,11 +473,8 @@ __global__ __launch_bounds__(64 * W, 4) void cache_place_kernel(CacheAttention a
         const v4f *b = (const v4f *)(a.bias_w + h * dk + 8 * part);
         bias[0] = b[0], bias[1] = b[1];
     }
-    if (threadIdx.x == 0)
-        need_lo = INT32_MAX, need_hi = INT32_MIN;
-    __syncthreads();
     /* the distances that any of the rows needs */
-    int32_t lo = INT32_MAX, hi = INT32_MIN;
+    int32_t lo = INT32_MAX, hi = -INT32_MAX;
     for (uint32_t b = threadIdx.x; b < a.st.B; b += kThreads) {
         const CacheSpan sp = span_of(a.st, b);
         const int32_t r0 = max(sp.r0, (int32_t)n0), r1 = min(sp.r0 + sp.T, (int32_t)(n0 + kRows));
@@ -339,10 +484,9 @@ __global__ __launch_bounds__(64 * W, 4) void cache_place_kernel(CacheAttention a
         lo = min(lo, a.left - p1);
         hi = max(hi, a.left + sp.total - 1 - p0);
     }
-    if (lo <= hi) {
-        atomicMin(&need_lo, lo);
-        atomicMax(&need_hi, hi);
-    }
+    lo = -wave_max(-lo), hi = wave_max(hi);
+    if (lane == 0)
+        need[wave][0] = lo, need[wave][1] = hi;
     const float c2 = a.scale * 1.44269504088896340736f;     /* scores in powers of 2 */
 #pragma unroll
     for (int i = 0; i < kFill; i++) {
@@ -361,7 +505,10 @@ __global__ __launch_bounds__(64 * W, 4) void cache_place_kernel(CacheAttention a
             expo[row] = e;
     }
     __syncthreads();
-    const int32_t from = need_lo, to = need_hi;
+    int32_t from = need[0][0], to = need[0][1];
+#pragma unroll
+    for (int i = 1; i < W; i++)
+        from = min(from, need[i][0]), to = max(to, need[i][1]);
 #pragma unroll 1
     for (int32_t x = x0 + 16 * MT * (int32_t)wave; x < x1 && x <= to; x += kRun) {
         if (from >= x + 16 * MT)
@@ -948,33 +1095,60 @@ __global__ __launch_bounds__(256) void cache_many_kernel(CacheAttention a) {
 /* ----------------------------------------------------------------- move --- */
 
 /* Pairs (from, to) of pages by value, so that a call needs no device memory
- * of its own; more take several launches. */
-constexpr int kMovePairs = 256;
+ * of its own (a kernel's arguments are 4 KB at most); more take several
+ * launches. */
+constexpr int kMovePairs = 448;
 struct MovePairs {
     int32_t from[kMovePairs], to[kMovePairs];
 };
 
-/* a page of a layer is one contiguous run of G records */
+/* A page of a layer is one contiguous run of G records: kMoveParts workgroups a
+ * page and layer, eight 16-byte loads a lane in flight. The row of workgroups
+ * behind the last pair lets the tables follow, each entry against all pairs in
+ * LDS (a page is moved at most once, so at most one is its). */
+constexpr int kMoveParts = 2;
 __global__ __launch_bounds__(256) void cache_move_kernel(uint8_t *__restrict__ dst, uint64_t dlayer,
                                                          const uint8_t *__restrict__ src, uint64_t slayer,
-                                                         uint32_t page_bytes, MovePairs m) {
+                                                         uint32_t page_bytes, MovePairs m, uint32_t pairs,
+                                                         int32_t *__restrict__ table, uint64_t entries) {
+    if (blockIdx.y == pairs) {
+        __shared__ __attribute__((aligned(16))) int32_t from[kMovePairs], to[kMovePairs];
+        for (uint32_t i = threadIdx.x; i < kMovePairs; i += 256) {
+            from[i] = i < pairs ? m.from[i] : -1;
+            to[i] = m.to[i];
+        }
+        __syncthreads();
+        const uint64_t step = (uint64_t)gridDim.x * gridDim.z * 256;
+        for (uint64_t i = ((uint64_t)blockIdx.z * gridDim.x + blockIdx.x) * 256 + threadIdx.x; i < entries; i += step) {
+            const int32_t old = table[i];
+            int32_t at = -1;
+            if (old >= 0) {
+                for (uint32_t q = 0; q < pairs; q += 4) {
+                    const int4 f = *(const int4 *)&from[q];
+                    at = f.x == old ? (int32_t)q : f.y == old ? (int32_t)q + 1 : f.z == old ? (int32_t)q + 2
+                       : f.w == old ? (int32_t)q + 3 : at;
+                }
+            }
+            if (at >= 0)
+                table[i] = to[at];
+        }
+        return;
+    }
     const v4u *from = (const v4u *)(src + blockIdx.z * slayer + (uint64_t)m.from[blockIdx.y] * page_bytes);
     v4u *to = (v4u *)(dst + blockIdx.z * dlayer + (uint64_t)m.to[blockIdx.y] * page_bytes);
-    const uint32_t n = page_bytes / 16;
-    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256)
+    const uint32_t n = page_bytes / 16, step = kMoveParts * 256;
+    uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    for (; i + 7 * step < n; i += 8 * step) {
+        v4u x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            x[j] = __builtin_nontemporal_load(from + i + j * step);
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            __builtin_nontemporal_store(x[j], to + i + j * step);
+    }
+    for (; i < n; i += step)
         to[i] = from[i];
-}
-
-__global__ __launch_bounds__(256) void cache_follow_kernel(int32_t *table, uint64_t entries, MovePairs m,
-                                                           uint32_t pairs) {
-    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    const int32_t old = i < entries ? table[i] : -1;
-    int32_t now = old;
-    for (uint32_t p = 0; p < pairs; p++)
-        if (m.from[p] == old)
-            now = m.to[p];
-    if (now != old)
-        table[i] = now;
 }
 
 /* ------------------------------------------------------------- launches --- */
@@ -989,13 +1163,17 @@ int launch_cache_write(uint8_t *data, uint32_t pages, uint32_t G, uint32_t dk, c
 int launch_cache_read(const uint8_t *data, uint32_t pages, uint32_t G, uint32_t dk, const CacheStreams &st, float *k,
                       uint64_t ks, float *v, uint64_t vs, hipStream_t s) {
     const dim3 grid(G, (st.max_T + kPage - 2) / kPage + 1, st.B);
-    cache_read_kernel<<<grid, 256, 0, s>>>(data, pages, G, dk, st, k, ks, v, vs);
+    cache_read_kernel<<<grid, 256, 0, s>>>((uint8_t *)data, pages, G, dk, st, k, ks, v, vs);
     return hipPeekAtLastError() == hipSuccess ? 0 : -1;
 }
 
 /* How a call's rows are dealt: tiles of four rows where a stream has at most
- * four a kept head, else of 16; and enough splits of a tile's pages that the
- * chip has work, none of them under four pages (one a wave). */
+ * four a kept head, else of 16; and splits of a tile's pages where the tiles
+ * are fewer than two workgroups a CU and a wave would take eight pages or more
+ * one after another. Joining the splits costs 4 to 5 us, a wave's page about
+ * one: one frame against 704 pages takes 873 us unsplit, 17 over 64 splits a
+ * head (19 over 96, 22 over 128); 16 streams of 17 pages 11 unsplit, 15 over
+ * two; 512 tiles of 12 pages 11.7 unsplit, 19 over two. */
 struct Deal {
     uint32_t rows, tiles, splits;           /* rows a tile, a stream's tiles a kept head, a tile's splits */
     uint32_t pages;                         /* pages a tile can reach */
@@ -1009,8 +1187,8 @@ static Deal deal(const CacheStreams &st, uint32_t G, uint32_t H, int32_t left, i
     d.tiles = (rows + d.rows - 1) / d.rows;
     d.units = (uint64_t)st.B * G * d.tiles;
     d.pages = cache_tile_pages(st.max_pages, left, right);
-    const uint64_t want = d.units ? (1024 + d.units - 1) / d.units : 1;
-    d.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({ want, (d.pages + 3) / 4, 128 }));
+    const uint64_t want = d.units ? 512 / d.units : 1;
+    d.splits = d.pages < 32 ? 1 : (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({ want, (d.pages + 7) / 8, 128 }));
     return d;
 }
 
@@ -1047,10 +1225,14 @@ size_t cache_attention_workspace(const CacheStreams &st, uint32_t G, uint32_t H,
 
 template <int NS, int RT, int W, int MT, bool PRE>
 static void place(const CacheAttention &a, hipStream_t s) {
-    /* runs one after another where there are workgroups enough without: the rows' operands are made once for all */
-    constexpr uint32_t kRun = 16 * MT * W;
+    /* Two runs one after another in a workgroup, whose rows' operands are then made once for both, where that takes
+     * fewer steps in a row over the rounds of workgroups that the chip holds, those operands counted as a step (36 runs
+     * by 32: in one round of two steps 28 us, in two of one 33; 2624 rows by 3750 in steps of one, two and five 97, 92
+     * and 103: lengths differ, and longer steps even them out less). */
+    constexpr uint32_t kRun = 16 * MT * W, kHeld = 256 * 16 / W;
     const uint32_t runs = (a.bw + kRun - 1) / kRun, blocks = (a.st.rows + 16 * RT - 1) / (16 * RT);
-    const uint32_t steps = std::min(8u, std::max(1u, (uint32_t)((uint64_t)runs * a.H * blocks * W / 8192)));
+    auto rounds = [&](uint32_t n) { return ((uint64_t)((runs + n - 1) / n) * a.H * blocks + kHeld - 1) / kHeld * (n + 1); };
+    const uint32_t steps = rounds(2) < rounds(1) ? 2 : 1;
     cache_place_kernel<NS, RT, W, MT, PRE><<<dim3((runs + steps - 1) / steps, a.H, blocks), 64 * W, 0, s>>>(a, (int32_t)steps);
 }
 
@@ -1060,8 +1242,8 @@ static void attend(const CacheAttention &a, const Deal &d, hipStream_t s) {
         if (place_halved(a.st.rows)) {
             cache_halve_kernel<NS><<<dim3(((a.bw + 15) / 16 + 3) / 4, a.H), 256, 0, s>>>(a);
             place<NS, 8, 8, 2, true>(a, s);
-        } else if ((uint64_t)((a.st.rows + 15) / 16) * ((a.bw + 15) / 16) * a.H <= 8192) {
-            /* up to eight tiles of 16 by 16 a SIMD: one workgroup's pass from the table's rows to the last store is what
+        } else if (a.st.rows <= 16 || (uint64_t)((a.st.rows + 15) / 16) * ((a.bw + 15) / 16) * a.H <= 4096) {
+            /* up to four tiles of 16 by 16 a SIMD: one workgroup's pass from the table's rows to the last store is what
              * takes time, and 16 rows have the shortest (128 rows by 751 distances 8.1 us, with 64 rows 10.7; 256 by
              * 4500 58 and 30) */
             place<NS, 1, 4, 1, false>(a, s);
@@ -1124,9 +1306,9 @@ int launch_cache_move(uint8_t *dst, uint64_t dlayer, const uint8_t *src, uint64_
             mp.from[i] = pairs[2 * (p0 + i)];
             mp.to[i] = pairs[2 * (p0 + i) + 1];
         }
-        cache_move_kernel<<<dim3(4, m, layers), 256, 0, s>>>(dst, dlayer, src, slayer, page_bytes, mp);
-        if (table && entries)
-            cache_follow_kernel<<<(uint32_t)((entries + 255) / 256), 256, 0, s>>>(table, entries, mp, m);
+        const uint32_t follow = table && entries ? 1 : 0;
+        cache_move_kernel<<<dim3(kMoveParts, m + follow, layers), 256, 0, s>>>(dst, dlayer, src, slayer, page_bytes, mp,
+                                                                              m, table, entries);
     }
     return hipPeekAtLastError() == hipSuccess ? 0 : -1;
 }
