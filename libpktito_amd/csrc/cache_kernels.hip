@@ -756,6 +756,12 @@ __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttention a) {
     *(v4f *)(a.o + row * a.os + (s.g * s.grp + (uint32_t)rr % s.grp) * dk + 4 * c) = normal(y, l);
 }
 
+/* The maximum that a softmax's exponentials are taken against follows the
+ * scores only when one is over it by more than this many powers of two: until
+ * then no lane asks another, and sums reach 2^8 times what they would, which
+ * 32-bit floats hold as well. */
+constexpr float kSlack = 8.0f;
+
 /* Up to four rows of a stream and kept head (a step of a frame or a few), where
  * the cache's bytes are what takes time. A row's three pieces are three rows
  * of the matrix instruction's 16 (row 4 i + n piece n of query i), so one
@@ -765,8 +771,13 @@ __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttention a) {
  * each would be made four times over). Tile kt's column c is key 4 c + kt, so
  * a lane's four scores are neighbours in memory: their scales and position
  * scores are one load each. The probabilities cross lanes once, cut, through
- * LDS, to be the second product's rows as the queries were the first's. */
-template <int NS, bool POS>
+ * LDS, to be the second product's rows as the queries were the first's.
+ *
+ * Position scores come from the workspace, or with one row a stream and few
+ * streams (kOwn) from the table itself: a quarter of the lanes' dimensions
+ * each, four keys a lane, as 32-bit products. */
+enum { kNone, kMade, kOwn };
+template <int NS, int POS>
 __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
     constexpr uint32_t dk = 32 * NS, record = kPage * dk + 4 * kPage;
     constexpr uint32_t kRow = 72;           /* bfloat16 a row of pieces: 64 and a pad against bank conflicts */
@@ -792,7 +803,7 @@ __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
             const uint32_t d = h * dk + w * (8 * NS) + 8 * st;
             const v4f *src = (const v4f *)(a.q + row * a.qs + d);
             v4f s0 = src[0], s1 = src[1];
-            if constexpr (POS) {
+            if constexpr (POS != kNone) {
                 const v4f *bias = (const v4f *)(a.bias_u + d);
                 s0 += bias[0], s1 += bias[1];
             }
@@ -817,7 +828,7 @@ __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
     const int32_t pos = s.sp.len + wi / (int32_t)s.grp;
     const int32_t lo = cache_lo(pos, a.left), hi = mine ? cache_hi(pos, a.right, s.sp.total) : -1;
     const float *place = nullptr;
-    if constexpr (POS)
+    if constexpr (POS == kMade)
         place = a.place + ((uint64_t)(s.sp.r0 + wi / (int32_t)s.grp) * a.H + s.g * s.grp + (uint32_t)wi % s.grp) *
                               place_stride(a.bw) + kPlacePad + (a.left - pos) + 4 * c;
 
@@ -830,6 +841,14 @@ __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
     v4u vw[NS];
     v2u ks, vs;
     v4f add = { 0.0f, 0.0f, 0.0f, 0.0f };
+    v4f pw[4][2 * NS], own[2 * NS];
+    if constexpr (POS == kOwn) {
+#pragma unroll
+        for (int i = 0; i < 2 * NS; i++) {
+            const uint32_t d = s.g * dk + w * (8 * NS) + 4 * i;
+            own[i] = (*(const v4f *)(a.q + (uint64_t)s.sp.r0 * a.qs + d) + *(const v4f *)(a.bias_w + d)) * c2;
+        }
+    }
     auto record_of = [&](int32_t id) { return a.data + ((uint64_t)(uint32_t)id * a.G + s.g) * record; };
     auto load_keys = [&](const uint8_t *rec, int32_t pg) {
 #pragma unroll
@@ -838,8 +857,18 @@ __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
             for (int st = 0; st < NS; st++)
                 kw[kt][st] = ((const uint32_t *)(rec + cache_key_at(dk, 4 * c + kt) + w * (4 * NS)))[st];
         ks = *(const v2u *)(rec + cache_key_scale_at(dk, 4 * c));
-        if constexpr (POS)
+        if constexpr (POS == kMade)
             add = *(const v4f_u *)(place + pg * (int32_t)kPage);
+        if constexpr (POS == kOwn) {
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++) {
+                const int32_t x = min(max(pg * (int32_t)kPage + 4 * (int32_t)c + kt - pos + a.left, 0), (int32_t)a.bw - 1);
+                const v4f *src = (const v4f *)(a.p + (uint64_t)(uint32_t)x * (a.H * dk) + s.g * dk + w * (8 * NS));
+#pragma unroll
+                for (int i = 0; i < 2 * NS; i++)
+                    pw[kt][i] = src[i];
+            }
+        }
     };
     auto load_values = [&](const uint8_t *rec) {
 #pragma unroll
@@ -864,6 +893,17 @@ __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
 #pragma unroll
             for (int kt = 0; kt < 4; kt++)
                 acc[kt] = mfma(q[st], levels(kw[kt][st]), acc[kt]);
+        if constexpr (POS == kOwn) {
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++) {
+                float d = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8 * NS; i++)
+                    d = __builtin_fmaf(own[i / 4][i % 4], pw[kt][i / 4][i % 4], d);
+                d += __shfl_xor(d, 16);
+                add[kt] = d + __shfl_xor(d, 32);
+            }
+        }
 #pragma unroll
         for (int kt = 0; kt < 4; kt++) {
             const float v = __builtin_fmaf((acc[kt][2] + acc[kt][1]) + acc[kt][0], bf_of(ks, kt), add[kt]);
@@ -873,9 +913,8 @@ __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
         more = walk.next(a, s, pg, id);
         const uint8_t *rec = record_of(id);
         load_keys(rec, pg);
-        best = row_max(best);
-        if (__any(best > top)) {
-            const float now = fmaxf(top, best);
+        if (__any(best > top + kSlack)) {
+            const float now = fmaxf(top, row_max(best));
             const float scale = __builtin_amdgcn_exp2f(top - (now == -INFINITY ? 0.0f : now));
             top = now;
             sum *= scale;
@@ -1039,9 +1078,9 @@ __global__ __launch_bounds__(256) void cache_many_kernel(CacheAttention a) {
 #pragma unroll
         for (int i = 0; i < 16; i++)
             best = fmaxf(best, s[i / 4][i % 4]);
-        best = fmaxf(best, __shfl_xor(best, 16));
-        best = fmaxf(best, __shfl_xor(best, 32));
-        if (__any(best > top)) {
+        if (__any(best > top + kSlack)) {
+            best = fmaxf(best, __shfl_xor(best, 16));
+            best = fmaxf(best, __shfl_xor(best, 32));
             const float now = fmaxf(top, best);
             const float scale = __builtin_amdgcn_exp2f(top - (now == -INFINITY ? 0.0f : now));
             top = now;
@@ -1178,8 +1217,14 @@ struct Deal {
     uint32_t rows, tiles, splits;           /* rows a tile, a stream's tiles a kept head, a tile's splits */
     uint32_t pages;                         /* pages a tile can reach */
     uint64_t units;
+    bool own;                               /* a row's position scores made where they are used */
 };
 
+/* A row's position scores are made where they are used for single rows of few
+ * streams with a narrow window: a launch fewer. One row by 71 distances takes
+ * 7.2 us so and 8.9 with a launch of their own, by 181 10.0 and 9.0; 16 rows
+ * by 71 7.3 and 9.1, 64 rows 13.6 and 10.6 (each stream reads the table
+ * itself, in pieces of 16 bytes). */
 static Deal deal(const CacheStreams &st, uint32_t G, uint32_t H, int32_t left, int32_t right) {
     Deal d;
     const uint32_t rows = st.max_T * (H / G);
@@ -1188,6 +1233,7 @@ static Deal deal(const CacheStreams &st, uint32_t G, uint32_t H, int32_t left, i
     d.units = (uint64_t)st.B * G * d.tiles;
     d.pages = cache_tile_pages(st.max_pages, left, right);
     const uint64_t want = d.units ? 512 / d.units : 1;
+    d.own = rows == 1 && st.B <= 16 && left + right < 100;
     d.splits = d.pages < 32 ? 1 : (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({ want, (d.pages + 7) / 8, 128 }));
     return d;
 }
@@ -1208,7 +1254,7 @@ struct Space {
 
 static Space space(const CacheStreams &st, uint32_t H, uint32_t dk, bool positions, uint32_t bw, const Deal &d) {
     Space s = { 0, 0, 0 };
-    if (positions) {
+    if (positions && !d.own) {
         s.place = (size_t)st.rows * H * place_stride(bw) * sizeof(float);
         s.halved = place_halved(st.rows) ? halved_bytes(H, bw, dk) : 0;
     }
@@ -1238,7 +1284,7 @@ static void place(const CacheAttention &a, hipStream_t s) {
 
 template <int NS>
 static void attend(const CacheAttention &a, const Deal &d, hipStream_t s) {
-    if (a.p) {
+    if (a.p && !d.own) {
         if (place_halved(a.st.rows)) {
             cache_halve_kernel<NS><<<dim3(((a.bw + 15) / 16 + 3) / 4, a.H), 256, 0, s>>>(a);
             place<NS, 8, 8, 2, true>(a, s);
@@ -1252,10 +1298,12 @@ static void attend(const CacheAttention &a, const Deal &d, hipStream_t s) {
         }
     }
     const uint32_t grid = (uint32_t)(d.units * d.splits);
-    if (d.rows == 4 && a.p)
-        cache_few_kernel<NS, true><<<grid, 256, 0, s>>>(a);
+    if (d.rows == 4 && a.p && d.own)
+        cache_few_kernel<NS, kOwn><<<grid, 256, 0, s>>>(a);
+    else if (d.rows == 4 && a.p)
+        cache_few_kernel<NS, kMade><<<grid, 256, 0, s>>>(a);
     else if (d.rows == 4)
-        cache_few_kernel<NS, false><<<grid, 256, 0, s>>>(a);
+        cache_few_kernel<NS, kNone><<<grid, 256, 0, s>>>(a);
     else if (a.p)
         cache_many_kernel<NS, true><<<grid, 256, 0, s>>>(a);
     else

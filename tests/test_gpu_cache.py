@@ -242,6 +242,24 @@ def test_single_frames(hip, torch):
     w.check(8)
 
 
+@pytest.mark.parametrize("dk", DKS)
+@pytest.mark.parametrize("B", [1, 5, 16, 17])
+def test_single_frames_narrow(hip, torch, dk, B):
+    """One row a stream and a narrow window, whose position scores are made
+    where they are used (up to 16 streams, 100 distances), and on both sides
+    of that."""
+    say("narrow", dk, B)
+    w = World(hip, torch, [(37 * b) % 150 for b in range(B)], [1] * B, 2, dk, seed=30 + B, first=1, tail=1)
+    w.fill()
+    for left in (0, 20, 70, 99, 100):
+        w.check(2, w.positions(2, 160, 3), left, 0)
+    p, c, u, v = w.positions(2, 40, 0)
+    w.check(2, (p, c, u, v))
+    w.table[0, :] = -1
+    w.upload()
+    w.check(2, (p, c, u, v))
+
+
 def test_long_stream(hip, torch):
     """One row against 70 pages, and chunks against them."""
     say("long")
