@@ -438,8 +438,8 @@ size_t pk_hip_cache_bytes(uint32_t layers, uint32_t pages, uint32_t heads, uint3
  * rows is the call's number of rows and max_T at least the longest stream's T
  * (rows a stream has beyond max_T or beyond rows take no part, and frames
  * past 64 max_pages have no page). Rows of no stream are left as they were.
- * No two streams of a call may write one page. max_pages up to 2^24, B up to
- * 65535, rows up to 2^22. */
+ * No two streams of a call may have one row or write one page. max_pages up to 2^24, B up to
+ * 65535, rows up to 2^21. */
 typedef struct {
     const int32_t *table, *len, *row0;
     uint32_t B, max_pages, rows, max_T;
@@ -481,7 +481,11 @@ typedef struct {
  * multiples of 4; o may be q with os = qs. ws: pk_hip_attention_cache_workspace(...) bytes of device
  * memory (of the same cache, streams' counts, H, pos, left and right),
  * 16-byte aligned, of no matter before and after; calls that overlap in time
- * need workspaces of their own. Products and sums in 32 bits. */
+ * need workspaces of their own (0 bytes: none is needed, or the sizes are not
+ * taken). Products and sums in 32 bits: what enters them is not rounded below
+ * that, but for the position scores' factors, kept to 2^-22 of themselves, and
+ * for what of a query or of a value is under 2^-126, which may be dropped (of
+ * numbers under 2^-110, their last bits). */
 size_t pk_hip_attention_cache_workspace(const pk_hip_cache *c, const pk_hip_streams *st, uint32_t H,
                                         const pk_hip_positions *pos, uint32_t left, uint32_t right);
 int pk_hip_attention_cache_dev(float *o, size_t os, const float *q, size_t qs, const pk_hip_cache *c, uint32_t layer,

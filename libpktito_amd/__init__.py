@@ -826,7 +826,7 @@ class PagePool:
     host (pk_hip_pool_*)."""
 
     def __init__(self, pages):
-        self.handle = ctypes.c_void_p()
+        self.handle, self.pages = ctypes.c_void_p(), pages
         _check(lib().pk_hip_pool_create(ctypes.byref(self.handle), pages))
 
     def __del__(self):
@@ -859,12 +859,17 @@ class PagePool:
         """One holder fewer for each page; free without any."""
         _check(lib().pk_hip_pool_release(self.handle, *self._ids(ids)))
 
+    def _fits(self, cache):
+        if cache.st.pages != self.pages:
+            raise PkHipError(PK_HIP_EINVAL, f"a pool of {self.pages} pages for a cache of {cache.st.pages}")
+
     def fork(self, cache, ids, frames, stream=None):
         """A second stream over the pages ids of one of `frames` frames: its
         whole pages shared, a page that the next frame goes into copied. Returns
         the new stream's pages."""
+        self._fits(cache)
         whole = ids[:frames // CACHE_PAGE]
-        rest = ids[len(whole):]
+        rest = ids[len(whole):-(-frames // CACHE_PAGE)]
         copies = self.alloc(len(rest))
         try:
             self.share(whole)
@@ -882,7 +887,8 @@ class PagePool:
     def compact(self, cache, table, most=None, stream=None):
         """Moves the pages in use below the number in use (at most `most` of
         them), table's entries with them; returns the pairs moved."""
-        cap = cache.st.pages if most is None else most
+        self._fits(cache)
+        cap = self.pages if most is None else min(most, self.pages)
         pairs = (ctypes.c_int32 * max(2, 2 * cap))()
         n = ctypes.c_uint32(0)
         _check(lib().pk_hip_pool_compact(self.handle, pairs, cap, ctypes.byref(n)))

@@ -260,6 +260,37 @@ def test_single_frames_narrow(hip, torch, dk, B):
     w.check(2, (p, c, u, v))
 
 
+@pytest.mark.parametrize("rows,lens,dk,H,G", [
+    ([300, 240], [40, 0], 64, 2, 1),            # 540 rows: the table halved beforehand
+    ([200, 320, 100, 7], [0, 3, 70, 5], 128, 1, 1),
+    ([150, 20], [1300, 900], 32, 4, 2),         # many distances: 64 rows a workgroup
+    ([90, 16], [1500, 10], 96, 3, 3),
+])
+@pytest.mark.parametrize("windowed", [False, True])
+def test_many_rows_with_positions(hip, torch, rows, lens, dk, H, G, windowed):
+    """The ways the position scores are made, by the call's rows and the table's
+    reach."""
+    say("many rows", rows, dk, H, windowed)
+    w = World(hip, torch, lens, rows, G, dk, seed=40 + dk, first=3, tail=2)
+    w.fill()
+    far = max(a + t for a, t in zip(lens, rows))
+    w.check(H, w.positions(H, far, max(rows)), *((50, 9) if windowed else (None, None)))
+
+
+@pytest.mark.parametrize("qscale,pscale", [(1e-18, 1e18), (1e18, 1e-18), (1e-30, 1e30), (1e30, 1e-30)])
+@pytest.mark.parametrize("T", [1, 7])
+def test_position_magnitudes(hip, torch, qscale, pscale, T):
+    """Queries and positions far from one and from each other: the exponents of
+    their rows are put back at once."""
+    say("position magnitudes", qscale, pscale, T)
+    w = World(hip, torch, [100, 7], [T, T], 1, 64, seed=43)
+    w.fill(scale=0.1 / qscale)              # so that neither part of a score is lost beside the other
+    p, c, u, v = w.positions(1, 130, 10)
+    p = (p * np.float32(pscale)).astype(np.float32)
+    p[::3] *= np.float32(1e-3)
+    w.check(1, (p, c, 0 * u, 0 * v), qscale=qscale)
+
+
 def test_long_stream(hip, torch):
     """One row against 70 pages, and chunks against them."""
     say("long")
@@ -315,6 +346,24 @@ def test_magnitudes(hip, torch, kscale, qscale):
     w = World(hip, torch, [100, 7], [5, 2], 1, 128, seed=17)
     w.fill(scale=kscale)
     w.check(1, None, qscale=qscale)
+
+
+@pytest.mark.parametrize("T", [1, 7])
+def test_tiny_queries(hip, torch, T):
+    """Queries of 1e-36 against keys of 1e35: a query is taken in pieces of 8
+    bits, and pieces under 2^-126 may count as zeros, two of them at most a
+    dimension. So a score (in powers of 2, as the pieces are) is off by at most
+    2 x 2^-126 x sum |k|, and the softmax by the exponential of twice that."""
+    say("tiny", T)
+    w = World(hip, torch, [40, 7], [T, T], 1, 64, seed=44)
+    w.fill(scale=1e35)
+    q = (1e-36 * w.g.standard_normal((2 * T, 64))).astype(np.float32)
+    got = w.attend(q, 1)
+    want, bound = cr.attend(w.pool, 0, w.table, w.lens, w.row0, 2 * T, q, 1)
+    most_k = max(np.abs(w.pool.read(0, pg, 0)[0][:n]).sum(1).max() for pg, n in ((w.table[0, 0], 40 + T), (w.table[1, 0], 7 + T)))
+    most_v = max(np.abs(w.pool.read(0, pg, 0)[1][:n]).max() for pg, n in ((w.table[0, 0], 40 + T), (w.table[1, 0], 7 + T)))
+    extra = (np.exp(2 * np.log(2) * 2 * 2.0 ** -126 * most_k) - 1) * 2 * most_v
+    assert np.isfinite(got).all() and (np.abs(got - want) <= bound + extra).all()
 
 
 def test_bad_values_stay_in_their_row(hip, torch):
@@ -621,6 +670,53 @@ def test_same_call_same_bits(hip, torch):
     first = w.attend(q, 2, pos)
     for _ in range(5):
         assert np.array_equal(w.attend(q, 2, pos), first)
+
+
+def test_pool_refuses_another_cache(hip, torch):
+    cache = hip.DeviceCache(torch.zeros(hip.cache_bytes(1, 4, 1, 32), dtype=torch.uint8, device="cuda"), 1, 4, 1, 32)
+    table = torch.zeros(1, 4, dtype=torch.int32, device="cuda")
+    pool = hip.PagePool(5)
+    ids = pool.alloc(2)
+    for call in (lambda: pool.fork(cache, ids, 70), lambda: pool.compact(cache, table)):
+        with pytest.raises(hip.PkHipError):
+            call()
+    assert pool.free_pages == 3 and [pool.holders(i) for i in range(5)] == [1, 1, 0, 0, 0]
+    pool = hip.PagePool(4)
+    ids = pool.alloc(3)
+    assert pool.fork(cache, ids, 128) == ids[:2] and pool.free_pages == 1       # a page ahead of the frames is not shared
+    assert pool.fork(cache, ids, 0) == []
+    with pytest.raises(hip.PkHipError):
+        pool.fork(cache, pool.alloc(1), 10)                                     # no page left for the copy
+    assert [pool.holders(i) for i in range(4)] == [2, 2, 1, 1]
+
+
+def test_wrapper_refusals(hip, torch):
+    """Tensors that a kernel would misread are refused before anything runs."""
+    w = World(hip, torch, [3], [4], 2, 64, seed=27)
+    f = lambda *a, **k: torch.zeros(*a, device="cuda", **k)
+    good, ws = f(4, 128), f(1 << 16, dtype=torch.uint8)
+    for bad in (f(4, 128, dtype=torch.float16), f(4, 127), f(3, 128), f(128, 4).T, torch.zeros(4, 128), f(4, 258)[:, ::2]):
+        for call in (lambda: w.cache.append(0, bad, good, w.streams), lambda: w.cache.append(0, good, bad, w.streams),
+                     lambda: w.cache.read(0, good, bad, w.streams),
+                     lambda: w.cache.attention(good, 0, bad, w.streams, 2, ws),
+                     lambda: w.cache.attention(bad, 0, good, w.streams, 2, ws)):
+            with pytest.raises(hip.PkHipError):
+                call()
+    b = f(128)
+    for p in ((f(9, 128), 9, b, b), (f(9, 127), 4, b, b), (f(9, 256)[:, :128], 4, b, b), (f(9, 128), 4, f(64), b),
+              (f(9, 128), 4, b, b.double())):
+        with pytest.raises(hip.PkHipError):
+            w.cache.attention(good, 0, good.clone(), w.streams, 2, ws, p)
+    with pytest.raises(hip.PkHipError):
+        w.cache.attention(good, 0, good.clone(), w.streams, 2, ws[:16], (f(9, 128), 4, b, b))
+    with pytest.raises(hip.PkHipError):
+        w.cache.move([(0, 1, 2)])
+    with pytest.raises(hip.PkHipError):
+        hip.DeviceCache(w.data[..., :-1], *w.pool.data.shape[:3], 64)
+    with pytest.raises(hip.PkHipError):
+        hip.CacheStreams(w.streams.table.long(), w.streams.len, w.streams.row0, 4, 4)
+    with pytest.raises(hip.PkHipError):
+        hip.CacheStreams(w.streams.table, w.streams.len, w.streams.row0[:1], 4, 4)
 
 
 def test_nothing_to_do(hip, torch):
