@@ -110,7 +110,12 @@ constexpr uint32_t kCodeRow = kMaxCacheDk / 8 + 1;  /* dwords of a frame's codes
  * thread, into the record's own order, and stored 16 bytes a lane; what a
  * chunk covers in part keeps its other frames' codes (a lane's 16 bytes read,
  * merged and stored by it alone, so a frame that shares a byte with the one
- * before it is no race). */
+ * before it is no race).
+ *
+ * 48 segments of 250 to 384 frames, 142 MB: 36 us, 3.9 TB/s, a third of it the
+ * codes' instructions; a wave a frame and two dimensions a lane took 61, exact
+ * comparisons alone 41. 64 streams of two frames: 5 us, three round trips (the
+ * stream, its page and rows, the codes around the new ones). */
 __global__ __launch_bounds__(256) void cache_write_kernel(uint8_t *data, uint32_t pages, uint32_t G, uint32_t dk,
                                                           CacheStreams st, const float *__restrict__ k, uint64_t ks,
                                                           const float *__restrict__ v, uint64_t vs) {
@@ -201,7 +206,8 @@ __global__ __launch_bounds__(256) void cache_write_kernel(uint8_t *data, uint32_
 
 /* The write's way back: a workgroup reads one page's part of a stream's frames
  * [len, len + T) for one kept head. Frames of a hole read as zeros, and so do
- * frames past the table. */
+ * frames past the table. 48 segments, 142 MB: 26 us, 5.4 TB/s (57 with a value
+ * a thread). */
 __global__ __launch_bounds__(256) void cache_read_kernel(uint8_t *data, uint32_t pages, uint32_t G, uint32_t dk,
                                                          CacheStreams st, float *__restrict__ k, uint64_t ks,
                                                          float *__restrict__ v, uint64_t vs) {
@@ -317,7 +323,7 @@ struct CacheAttention {
     CacheStreams st;
     int32_t left, right;                    /* clipped to what can occur */
     float scale;                            /* 1 / sqrt(dk) */
-    /* positions (p NULL: none): row place0 is distance left's */
+    /* positions (p NULL: none), p's first row the distance left's */
     const float *p, *bias_u, *bias_w;
     float *place;                           /* the position scores, [rows][H][place_stride(bw)] */
     uint32_t bw;
@@ -338,7 +344,6 @@ __device__ __forceinline__ uint64_t unit_of(const CacheAttention &a, uint32_t b,
  * kept to 2^-22 of itself, or of 2^-17 of the row's largest where that is more
  * (float16's own last places). Three products of pieces are taken, and the
  * exponents of both rows put back at the end. */
-typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 struct Halves {
     v8h hi, lo;
@@ -446,10 +451,22 @@ __device__ __forceinline__ int wave_max(int v) {
  * of 2), of every row at every distance that it needs, into the workspace:
  * the same rows of p serve every stream, so this is one product of all rows by
  * the table, read once, where the attention reads its own stream's pages only.
- * A workgroup of RT waves takes 16 RT rows of a head, halved into the matrix
- * instruction's operands in LDS, and walks `steps` runs of 32 RT distances; a
- * wave takes 32 of each, two tiles, so that an operand read from LDS serves
- * two. */
+ * A workgroup of W waves takes 16 RT rows of a head, halved into the matrix
+ * instruction's operands in LDS, and walks `steps` runs of 16 MT W distances;
+ * a wave takes MT tiles of 16 of each, so that an operand read from LDS serves
+ * MT. PRE: the table's rows come halved.
+ *
+ * At 2624 rows by up to 3750 distances it takes 91 us (and the halving 10) for
+ * 280 MB of scores: 57 without its stores, which is its operands' and
+ * instructions' latency (the matrix cores are busy a third of it), the stores
+ * on top at the rate that memory takes them. At 256 rows by 4500 it takes 28
+ * us, and at few rows a chain of two memory round trips and a launch, 4.5.
+ * Measured and taken back: a lane's four scores stored at the frames' own
+ * places (16 bytes at any multiple of 4: each step twice as long), one float a
+ * lane stored there (as long as now, and the attention no faster), the next
+ * step's rows loaded ahead (registers: 12 -> 15 us at 128 rows by 751), and
+ * six products of three bfloat16 pieces (14 -> 16 us there, 142 at 2624 rows
+ * without the halving apart, against 124). */
 template <int NS, int RT, int W, int MT, bool PRE>
 __global__ __launch_bounds__(64 * W, 4) void cache_place_kernel(CacheAttention a, int32_t steps) {
     constexpr int kRows = 16 * RT, kRun = 16 * MT * W, kThreads = 64 * W, kFill = kRows * 16 / kThreads;
@@ -775,7 +792,14 @@ constexpr float kSlack = 8.0f;
  *
  * Position scores come from the workspace, or with one row a stream and few
  * streams (kOwn) from the table itself: a quarter of the lanes' dimensions
- * each, four keys a lane, as 32-bit products. */
+ * each, four keys a lane, as 32-bit products.
+ *
+ * 256 streams of 3000 to 4500 frames, 8 heads of 128: 172 us for 1.02 GB, 5.9
+ * TB/s of the 6.8 that reads reach (612 us with the kernel below, which makes
+ * each score for 16 columns). What else counts: values loaded past the caches
+ * (187 -> 172; the keys too 180), three waves a SIMD (four, at 128 registers,
+ * spill: 233). Short calls take 10 to 12 us whatever their bytes: a launch,
+ * the stream, its table, a page's loads and three pages a wave. */
 enum { kNone, kMade, kOwn };
 template <int NS, int POS>
 __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
@@ -969,7 +993,17 @@ __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
 
 /* More rows: 16 a workgroup, its four waves a page each in turn with the
  * running maximum and sum of a softmax, a query a column and its pieces three
- * products one after another. */
+ * products one after another. A lane's scores are a query's, and stay where
+ * the second product takes them.
+ *
+ * Four files of 500 to 750 rows after 2200 to 3000 frames, 8 heads of 128:
+ * 124 us, 265 TFLOP/s as an fp32 product counts them. Instructions bound it:
+ * 515 vector ones a page and 16 rows, 96 of them products, issue in three
+ * quarters of the cycles at two waves a SIMD (235 registers). Measured and no
+ * faster: a page's first product under the page before's softmax (130), the
+ * products at another wave priority (127, 129), the queries' pieces in LDS
+ * (126; for three waves, 250: spills), eight waves (147; 13.2 against 14.2 us
+ * where 16 streams of 14 rows leave half the CUs idle). */
 template <int NS, bool POS>
 __global__ __launch_bounds__(256) void cache_many_kernel(CacheAttention a) {
     constexpr uint32_t dk = 32 * NS, record = kPage * dk + 4 * kPage;
@@ -1144,7 +1178,10 @@ struct MovePairs {
 /* A page of a layer is one contiguous run of G records: kMoveParts workgroups a
  * page and layer, eight 16-byte loads a lane in flight. The row of workgroups
  * behind the last pair lets the tables follow, each entry against all pairs in
- * LDS (a page is moved at most once, so at most one is its). */
+ * LDS (a page is moved at most once, so at most one is its). 300 pages of 24
+ * layers, 973 MB read and written: 175 us, 5.6 TB/s, where torch's copy of 4
+ * GiB reaches 4.8 (four workgroups a page, one load in flight: 200, and 23 for
+ * the tables in a launch of their own). */
 constexpr int kMoveParts = 2;
 __global__ __launch_bounds__(256) void cache_move_kernel(uint8_t *__restrict__ dst, uint64_t dlayer,
                                                          const uint8_t *__restrict__ src, uint64_t slayer,
@@ -1205,6 +1242,9 @@ int launch_cache_read(const uint8_t *data, uint32_t pages, uint32_t G, uint32_t 
     cache_read_kernel<<<grid, 256, 0, s>>>((uint8_t *)data, pages, G, dk, st, k, ks, v, vs);
     return hipPeekAtLastError() == hipSuccess ? 0 : -1;
 }
+
+/* workgroups of 256 in a launch's first dimension, under 2^32 threads */
+constexpr uint64_t kMostGroups = (1u << 24) - 1;
 
 /* How a call's rows are dealt: tiles of four rows where a stream has at most
  * four a kept head, else of 16; and splits of a tile's pages where the tiles
@@ -1269,6 +1309,11 @@ size_t cache_attention_workspace(const CacheStreams &st, uint32_t G, uint32_t H,
     return s.place + s.halved + s.parts;
 }
 
+bool cache_attention_fits(const CacheStreams &st, uint32_t G, uint32_t H, int32_t left, int32_t right) {
+    const Deal d = deal(st, G, H, left, right);
+    return d.units <= kMostGroups / d.splits && ((uint32_t)left + (uint32_t)right) / 64 < kMostGroups;
+}
+
 template <int NS, int RT, int W, int MT, bool PRE>
 static void place(const CacheAttention &a, hipStream_t s) {
     /* Two runs one after another in a workgroup, whose rows' operands are then made once for both, where that takes
@@ -1326,8 +1371,6 @@ int launch_cache_attention(const CacheAttentionCall &c, hipStream_t s) {
     a.p = c.p, a.bias_u = c.bias_u, a.bias_w = c.bias_w;
     a.bw = (uint32_t)c.left + (uint32_t)c.right + 1;
     const Deal d = deal(c.st, c.G, c.H, c.left, c.right);
-    if (d.units * d.splits > 0x7fffffff)
-        return -2;
     a.tiles = d.tiles, a.splits = d.splits;
     const Space sp = space(c.st, c.H, c.dk, c.p != nullptr, a.bw, d);
     a.place = (float *)c.ws;

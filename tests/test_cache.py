@@ -237,6 +237,7 @@ ALL = BOTH + ("attention",)
     (("attention",), {"p": 4104}), (("attention",), {"center": 9}), (("attention",), {"n": 0, "center": 0}),
     (("attention",), {"ws": None}), (("attention",), {"ws": 4104}), (("attention",), {"ws_bytes": 100}),
     (("attention",), {"q": 4096, "qs": 516}),
+    (("attention",), {"B": 65535, "rows": 1 << 21, "max_T": 1 << 21}),      # more workgroups than a launch holds
 ], ids=lambda v: "-".join(f"{k}={x}" for k, x in v.items()) if isinstance(v, dict) else "")
 def test_refusals(entries, change):
     import libpktito_amd as pk
