@@ -301,6 +301,34 @@ def test_long_stream(hip, torch):
         w.check(4, left=2000)
 
 
+@pytest.mark.parametrize("seed", range(24))
+def test_any_call(hip, torch, seed):
+    """Calls drawn over the documented ranges: streams, lengths, rows, heads,
+    windows, holes, a table wider or narrower than the streams, the bound on a
+    stream's rows above them."""
+    r = random.Random(seed)
+    dk, (H, G) = r.choice(DKS), r.choice([(1, 1), (2, 2), (4, 1), (6, 3), (5, 5)])
+    B = r.choice([1, 2, 3, 7, 20])
+    Ts = [r.choice([0, 1, 1, 2, 3, r.randint(1, 40)]) for _ in range(B)]
+    if not sum(Ts):
+        Ts[0] = 1
+    lens = [r.choice([0, 1, 63, 64, 127, r.randint(0, 300), r.randint(0, 2500 // B)]) for _ in range(B)]
+    say("any", seed, dk, H, G, lens, Ts)
+    held = max(-(-(a + t) // 64) for a, t in zip(lens, Ts))
+    w = World(hip, torch, lens, Ts, G, dk, seed=seed, layers=2, layer=r.randint(0, 1), first=r.randint(0, 2),
+              tail=r.randint(0, 2), max_pages=held + r.randint(0, 3), slack_T=r.choice([0, 0, 5]))
+    if r.random() < 0.4:
+        for _ in range(r.randint(1, 4)):
+            w.table[r.randrange(B), r.randrange(w.table.shape[1])] = r.choice([-1, -2 ** 31, 10 ** 6])
+    w.fill(scale=r.choice([1.0, 0.01, 30.0]))
+    left, right = (r.choice([None, 0, 1, 70, r.randint(0, 400)]) for _ in range(2))
+    pos = None
+    if r.random() < 0.6:
+        far = max(a + t for a, t in zip(lens, Ts))
+        pos = w.positions(H, r.choice([far, far + 9, far // 2]), r.choice([max(Ts), max(Ts) // 2, 50]))
+    w.check(H, pos, left, right, qscale=r.choice([1.0, 0.1, 4.0]))
+
+
 def test_rows_that_attend_nothing(hip, torch):
     """Holes in the table (given up pages, ids outside the pool, of every size):
     their frames are skipped, and a row with nothing else is zeros."""
