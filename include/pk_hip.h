@@ -422,7 +422,7 @@ typedef struct {
     void     *data;
     uint32_t  layers, pages, heads, dk;
 } pk_hip_cache;
-/* 0 for sizes that are not taken */
+/* 0 for sizes that are not taken (2^48 bytes at most) */
 size_t pk_hip_cache_bytes(uint32_t layers, uint32_t pages, uint32_t heads, uint32_t dk);
 
 /* The streams of a call, B of them, with the call's rows of all streams one

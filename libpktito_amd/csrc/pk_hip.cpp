@@ -1590,7 +1590,8 @@ size_t pk_hip_cache_bytes(uint32_t layers, uint32_t pages, uint32_t heads, uint3
     if (layers == 0 || layers > 65535 || pages == 0 || pages > 1u << 30 || heads == 0 || heads > 1024 ||
         !pkq8::cache_dk_ok(dk))
         return 0;
-    return (size_t)layers * pages * heads * pkq8::cache_record(dk);
+    const uint64_t layer = (uint64_t)pages * heads * pkq8::cache_record(dk);       /* under 2^54 */
+    return layer <= (1ull << 48) / layers ? (size_t)layer * layers : 0;
 }
 
 int pk_hip_cache_append_dev(const pk_hip_cache *c, uint32_t layer, const float *k, size_t ks, const float *v,

@@ -277,6 +277,20 @@ def test_sizes():
         assert pk.cache_bytes(*bad) == 0
 
 
+def test_sizes_past_what_a_size_holds():
+    """Products that pass 64 bits are no size (41361 x 2^30 x 1024 x 8448 would
+    come out as a smaller one), and a cache of them is refused."""
+    import libpktito_amd as pk
+    assert pk.cache_bytes(24, 1 << 20, 8, 128) == 24 * (1 << 20) * 8 * cr.record_bytes(128)
+    for big in ((41361, 1 << 30, 1024, 128), (65535, 1 << 30, 1024, 32), (65535, (1 << 30) - 1, 1023, 96)):
+        n = big[0] * big[1] * big[2] * cr.record_bytes(big[3])
+        assert n > 2 ** 64 and pk.cache_bytes(*big) == 0
+        calls = _calls(pk, layers=big[0], pages=big[1], heads=big[2], dk=big[3], H=big[2], ks=1 << 20, vs=1 << 20,
+                       os=1 << 20, qs=1 << 20)
+        for e in ALL:
+            assert calls[e]() == pk.PK_HIP_EINVAL, e
+
+
 def test_host_tensors_are_refused():
     import torch
     import libpktito_amd as pk
