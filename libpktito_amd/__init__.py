@@ -717,6 +717,14 @@ def _rows(t, n, width, what):
     return t.data_ptr(), rs if n > 1 else width
 
 
+def _table(t):
+    """Refuses a table that pages' moves could not follow in."""
+    if t is not None:
+        _is(t, "int32", "table")
+        if not t.is_contiguous():
+            raise PkHipError(PK_HIP_EINVAL, "table is not contiguous")
+
+
 class CacheStreams:
     """The streams of a call on a cache (pk_hip_streams): int32 device tensors
     table [B, max_pages], len [B] and row0 [B + 1], the call's number of rows
@@ -812,10 +820,7 @@ class DeviceCache:
         n = len(flat)
         if n != 2 * len(pairs):
             raise PkHipError(PK_HIP_EINVAL, "pairs of pages (from, to)")
-        if table is not None:
-            _is(table, "int32", "table")
-            if not table.is_contiguous():
-                raise PkHipError(PK_HIP_EINVAL, "table is not contiguous")
+        _table(table)
         _check(lib().pk_hip_cache_move_dev(ctypes.byref(self.st), ctypes.byref((source or self).st),
                                            (ctypes.c_int32 * max(1, n))(*flat), n // 2, _dptr(table),
                                            table.numel() if table is not None else 0, _stream(stream)))
@@ -888,6 +893,9 @@ class PagePool:
         """Moves the pages in use below the number in use (at most `most` of
         them), table's entries with them; returns the pairs moved."""
         self._fits(cache)
+        if most is not None and most < 0:
+            raise PkHipError(PK_HIP_EINVAL, f"compact: at most {most} pages")
+        _table(table)                                   # refused before the pool's own counts have moved
         cap = self.pages if most is None else min(most, self.pages)
         pairs = (ctypes.c_int32 * max(2, 2 * cap))()
         n = ctypes.c_uint32(0)

@@ -198,6 +198,33 @@ def test_pool_against_a_model():
             assert [p.holders(i) for i in range(pages)] == [model.get(i, 0) for i in range(pages)]
 
 
+class _Moves:
+    """Stands for a cache: keeps the pairs that the pool would have moved."""
+    def __init__(self, pages):
+        self.st, self.pairs = type("St", (), {"pages": pages}), []
+
+    def move(self, pairs, table=None, source=None, stream=None):
+        self.pairs += pairs
+
+
+def test_compact_refuses_before_it_moves():
+    """A limit under 0 (which an unsigned count would take for all pages, more
+    than the pairs' array holds) and a table that cannot follow leave the pool
+    as it was."""
+    import torch
+    import libpktito_amd as pk
+    p, cache = pk.PagePool(8), _Moves(8)
+    p.release(p.alloc(5)[:3])
+    for table, most in ((None, -1), (None, -(1 << 32)), (torch.zeros(2, 4, dtype=torch.int32), None),
+                        (torch.zeros(2, 4, dtype=torch.int64), None)):
+        with pytest.raises(pk.PkHipError) as e:
+            p.compact(cache, table, most)
+        assert e.value.code == pk.PK_HIP_EINVAL
+        assert [p.holders(i) for i in range(8)] == [0, 0, 0, 1, 1, 0, 0, 0] and not cache.pairs
+    assert p.compact(cache, None, 0) == [] and p.compact(cache, None, 1) == [(4, 0)] == cache.pairs
+    assert p.compact(cache, None) == [(3, 1)] and [p.holders(i) for i in range(4)] == [1, 1, 0, 0]
+
+
 # -------------------------------------------------------------- refusals --
 
 def _calls(pk, **change):
