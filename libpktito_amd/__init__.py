@@ -870,24 +870,26 @@ class PagePool:
 
     def fork(self, cache, ids, frames, stream=None):
         """A second stream over the pages ids of one of `frames` frames: its
-        whole pages shared, a page that the next frame goes into copied. Returns
-        the new stream's pages."""
+        whole pages shared, a page that the next frame goes into copied; ids
+        outside the pool are holes and stay. Returns the new stream's pages."""
         self._fits(cache)
-        whole = ids[:frames // CACHE_PAGE]
-        rest = ids[len(whole):-(-frames // CACHE_PAGE)]
-        copies = self.alloc(len(rest))
+        if not 0 <= frames <= CACHE_PAGE * len(ids):
+            raise PkHipError(PK_HIP_EINVAL, f"fork: {frames} frames of {len(ids)} pages")
+        in_pool = lambda pages: [i for i in pages if 0 <= i < self.pages]
+        whole = list(ids[:frames // CACHE_PAGE])
+        last = list(ids[len(whole):-(-frames // CACHE_PAGE)])
+        shared, copied = in_pool(whole), in_pool(last)
+        self.share(shared + copied)                      # the copied page is held until its copy is on its way
+        copies = []
         try:
-            self.share(whole)
-            try:
-                if rest:
-                    cache.move(list(zip(rest, copies)), stream=stream)
-            except Exception:
-                self.release(whole)
-                raise
+            copies = self.alloc(len(copied))
+            if copied:
+                cache.move(list(zip(copied, copies)), stream=stream)
         except Exception:
-            self.release(copies)
+            self.release(shared + copied + copies)
             raise
-        return list(whole) + copies
+        self.release(copied)
+        return whole + (copies or last)
 
     def compact(self, cache, table, most=None, stream=None):
         """Moves the pages in use below the number in use (at most `most` of

@@ -225,6 +225,23 @@ def test_compact_refuses_before_it_moves():
     assert p.compact(cache, None) == [(3, 1)] and [p.holders(i) for i in range(4)] == [1, 1, 0, 0]
 
 
+def test_fork_takes_what_a_stream_has():
+    """Frames that the pages do not hold, and pages that nobody holds, are
+    refused with nothing taken; holes stay holes."""
+    import libpktito_amd as pk
+    p, cache = pk.PagePool(8), _Moves(8)
+    ids = p.alloc(3)
+    for pages, frames in ((ids, -1), (ids, 3 * 64 + 1), ([], 1), ([5], 64), ([5], 10), (ids + [5], 200), (ids + [5], 256)):
+        with pytest.raises(pk.PkHipError) as e:
+            p.fork(cache, pages, frames)
+        assert e.value.code == pk.PK_HIP_EINVAL and not cache.pairs
+        assert p.free_pages == 5 and [p.holders(i) for i in range(4)] == [1, 1, 1, 0]
+    assert p.fork(cache, [-1, 1, 2], 140) == [-1, 1, 3] and cache.pairs == [(2, 3)]
+    assert [p.holders(i) for i in range(4)] == [1, 2, 1, 1]
+    assert p.fork(cache, [0, 8], 100) == [0, 8] and p.fork(cache, [-1], 64) == [-1] and cache.pairs == [(2, 3)]
+    assert [p.holders(i) for i in range(4)] == [2, 2, 1, 1] and p.free_pages == 4
+
+
 # -------------------------------------------------------------- refusals --
 
 def _calls(pk, **change):
