@@ -692,6 +692,26 @@ def cache_bytes(layers, pages, heads, dk):
     return lib().pk_hip_cache_bytes(layers, pages, heads, dk)
 
 
+def _u32(v, what):
+    """A count as the C side takes it; ctypes would keep a greater or negative
+    one's last 32 bits."""
+    if not 0 <= v <= 0xffffffff:
+        raise PkHipError(PK_HIP_EINVAL, f"{what} {v}: from 0 to 2^32 - 1")
+    return v
+
+
+def _reach(v, what):
+    """A window's side: the frames attended, None for all."""
+    return UNLIMITED if v is None else _u32(v, what)
+
+
+def _page_ids(ids):
+    """Pages' ids as a C array, those that are none refused there."""
+    if ids and not (-0x80000000 <= min(ids) and max(ids) <= 0x7fffffff):
+        raise PkHipError(PK_HIP_EINVAL, "ids of pages in 32 bits")
+    return (ctypes.c_int32 * max(1, len(ids)))(*ids)
+
+
 _dtypes = {}
 
 
@@ -739,7 +759,7 @@ class CacheStreams:
         if table.dim() != 2 or tuple(len.shape) != (table.shape[0],) or tuple(row0.shape) != (table.shape[0] + 1,):
             raise PkHipError(PK_HIP_EINVAL, "streams: table [B, max_pages], len [B], row0 [B + 1]")
         self.table, self.len, self.row0 = table, len, row0
-        self.rows, self.max_T = int(rows), int(max_T)
+        self.rows, self.max_T = _u32(int(rows), "rows"), _u32(int(max_T), "max_T")
         self.st = Streams(table.data_ptr(), len.data_ptr(), row0.data_ptr(), table.shape[0], table.shape[1],
                           self.rows, self.max_T)
 
@@ -751,6 +771,8 @@ class DeviceCache:
 
     def __init__(self, data, layers, pages, heads, dk):
         _is(data, "uint8", "cache")
+        for v, what in ((layers, "layers"), (pages, "pages"), (heads, "heads"), (dk, "dk")):
+            _u32(v, what)
         if not data.is_contiguous() or data.numel() < max(1, cache_bytes(layers, pages, heads, dk)):
             raise PkHipError(PK_HIP_EINVAL, f"cache: {cache_bytes(layers, pages, heads, dk)} contiguous bytes (heads of "
                                             "32, 64, 96 or 128 dimensions)")
@@ -761,14 +783,14 @@ class DeviceCache:
         """Writes the rows' keys and values [rows, heads * dk] as the streams'
         frames [len, len + T) (pk_hip_cache_append_dev)."""
         n, w = streams.rows, self.heads * self.dk
-        _check(lib().pk_hip_cache_append_dev(ctypes.byref(self.st), layer, *_rows(k, n, w, "k"), *_rows(v, n, w, "v"),
+        _check(lib().pk_hip_cache_append_dev(ctypes.byref(self.st), _u32(layer, "layer"), *_rows(k, n, w, "k"), *_rows(v, n, w, "v"),
                                              ctypes.byref(streams.st), _stream(stream)))
 
     def read(self, layer, k, v, streams, stream=None):
         """The values kept for the streams' frames [len, len + T), into k and v
         [rows, heads * dk] (pk_hip_cache_read_dev)."""
         n, w = streams.rows, self.heads * self.dk
-        _check(lib().pk_hip_cache_read_dev(ctypes.byref(self.st), layer, *_rows(k, n, w, "k"), *_rows(v, n, w, "v"),
+        _check(lib().pk_hip_cache_read_dev(ctypes.byref(self.st), _u32(layer, "layer"), *_rows(k, n, w, "k"), *_rows(v, n, w, "v"),
                                            ctypes.byref(streams.st), _stream(stream)))
 
     def attention_workspace(self, streams, H, positions, left=None, right=None):
@@ -778,16 +800,15 @@ class DeviceCache:
             pos = Positions(16, 16, 16, 0xffffffff, 0x7fffffff)
         else:
             pos = self._positions(positions or None, H)
-        return lib().pk_hip_attention_cache_workspace(ctypes.byref(self.st), ctypes.byref(streams.st), H,
+        return lib().pk_hip_attention_cache_workspace(ctypes.byref(self.st), ctypes.byref(streams.st), _u32(H, "H"),
                                                       ctypes.byref(pos) if pos else None,
-                                                      UNLIMITED if left is None else left,
-                                                      UNLIMITED if right is None else right)
+                                                      _reach(left, "left"), _reach(right, "right"))
 
     def _positions(self, positions, H):
         if positions is None:
             return None
         p, center, u, w = positions
-        n = H * self.dk
+        n = max(1, _u32(H, "H")) * self.dk
         _is(p, "float32", "p")
         _is(u, "float32", "bias_u")
         _is(w, "float32", "bias_w")
@@ -795,7 +816,7 @@ class DeviceCache:
         if rest or u.numel() != n or w.numel() != n or not (p.is_contiguous() and u.is_contiguous() and
                                                             w.is_contiguous()):
             raise PkHipError(PK_HIP_EINVAL, f"positions: p [n, {n}] and biases [{n}], contiguous")
-        return Positions(p.data_ptr(), u.data_ptr(), w.data_ptr(), rows, center)
+        return Positions(p.data_ptr(), u.data_ptr(), w.data_ptr(), rows, _u32(center, "center"))
 
     def attention(self, o, layer, q, streams, H, ws, positions=None, left=None, right=None, stream=None):
         """The attention of the rows q [rows, H * dk] to their streams' kept
@@ -806,9 +827,9 @@ class DeviceCache:
         n, w = streams.rows, H * self.dk
         pos = self._positions(positions, H)
         _check(lib().pk_hip_attention_cache_dev(*_rows(o, n, w, "o"), *_rows(q, n, w, "q"), ctypes.byref(self.st),
-                                                layer, ctypes.byref(streams.st), H, ctypes.byref(pos) if pos else None,
-                                                UNLIMITED if left is None else left,
-                                                UNLIMITED if right is None else right,
+                                                _u32(layer, "layer"), ctypes.byref(streams.st), _u32(H, "H"),
+                                                ctypes.byref(pos) if pos else None,
+                                                _reach(left, "left"), _reach(right, "right"),
                                                 _dptr(ws), ws.numel() if ws is not None else 0, _stream(stream)))
 
     def move(self, pairs, table=None, source=None, stream=None):
@@ -822,7 +843,7 @@ class DeviceCache:
             raise PkHipError(PK_HIP_EINVAL, "pairs of pages (from, to)")
         _table(table)
         _check(lib().pk_hip_cache_move_dev(ctypes.byref(self.st), ctypes.byref((source or self).st),
-                                           (ctypes.c_int32 * max(1, n))(*flat), n // 2, _dptr(table),
+                                           _page_ids(flat), n // 2, _dptr(table),
                                            table.numel() if table is not None else 0, _stream(stream)))
 
 
@@ -832,7 +853,7 @@ class PagePool:
 
     def __init__(self, pages):
         self.handle, self.pages = ctypes.c_void_p(), pages
-        _check(lib().pk_hip_pool_create(ctypes.byref(self.handle), pages))
+        _check(lib().pk_hip_pool_create(ctypes.byref(self.handle), _u32(pages, "pages")))
 
     def __del__(self):
         if getattr(self, "handle", None):
@@ -845,16 +866,16 @@ class PagePool:
 
     def holders(self, page):
         """How many hold the page (0: free)."""
-        return lib().pk_hip_pool_holders(self.handle, page)
+        return lib().pk_hip_pool_holders(self.handle, page) if 0 <= page < self.pages else 0
 
     def alloc(self, n):
         """n pages nobody holds, as a list; raises if fewer are free."""
-        ids = (ctypes.c_int32 * max(1, n))()
+        ids = (ctypes.c_int32 * max(1, min(_u32(n, "pages"), self.pages)))()    # more are refused
         _check(lib().pk_hip_pool_alloc(self.handle, ids, n))
         return list(ids[:n])
 
     def _ids(self, ids):
-        return (ctypes.c_int32 * max(1, len(ids)))(*ids), len(ids)
+        return _page_ids(ids), len(ids)
 
     def share(self, ids):
         """One more holder for each page."""

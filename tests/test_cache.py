@@ -345,6 +345,66 @@ def test_host_tensors_are_refused():
         pk.DeviceCache(torch.zeros(1 << 20, dtype=torch.uint8), 1, 1, 1, 64)
 
 
+class _Device:
+    """Stands for a device tensor in calls that are refused before one is read."""
+    is_cuda = True
+
+    def __init__(self, dtype, *shape, dense=True):
+        self.dtype, self.shape, self.dense, self.device = dtype, shape, dense, "cuda:0"
+
+    def numel(self):
+        return int(np.prod(self.shape))
+
+    def dim(self):
+        return len(self.shape)
+
+    def is_contiguous(self):
+        return self.dense
+
+    def stride(self):
+        return self.shape[1], 1
+
+    def data_ptr(self):
+        return 4096
+
+
+def _wrapped(pk, torch):
+    i32 = lambda *s: _Device(torch.int32, *s)
+    return (pk.DeviceCache(_Device(torch.uint8, pk.cache_bytes(2, 8, 4, 64)), 2, 8, 4, 64),
+            pk.CacheStreams(i32(2, 4), i32(2), i32(3), 5, 3))
+
+
+@pytest.mark.parametrize("past", [-1, -(1 << 32), 1 << 32, (1 << 32) + 1])
+def test_numbers_past_32_bits_are_refused(past):
+    """A number whose last 32 bits would do is not taken for those."""
+    import torch
+    import libpktito_amd as pk
+    cache, st = _wrapped(pk, torch)
+    f = lambda n: _Device(torch.float32, 5, n)
+    kv, q, ws, b = f(256), f(512), _Device(torch.uint8, 1 << 24), _Device(torch.float32, 512)
+    at = lambda center: (_Device(torch.float32, 9, 512), center, b, b)
+    i32 = lambda *s: _Device(torch.int32, *s)
+    pool = pk.PagePool(8)
+    pool.alloc(2)
+    for call in (lambda: cache.append(past, kv, kv, st), lambda: cache.read(past, kv, kv, st),
+                 lambda: cache.attention(q, past, q, st, 8, ws), lambda: cache.attention(q, 0, q, st, 8, ws, left=past),
+                 lambda: cache.attention(q, 0, q, st, 8, ws, right=past), lambda: cache.attention(q, 0, q, st, 8, ws, at(past)),
+                 lambda: cache.attention_workspace(st, 8, None, past), lambda: cache.attention_workspace(st, 8, None, 1, past),
+                 lambda: cache.attention_workspace(st, past, None), lambda: cache.attention_workspace(st, past, at(4)),
+                 lambda: cache.move([(0, past)], stream=0), lambda: cache.move([(past, 0)], stream=0),
+                 lambda: pk.CacheStreams(i32(2, 4), i32(2), i32(3), past, 3),
+                 lambda: pk.CacheStreams(i32(2, 4), i32(2), i32(3), 5, past),
+                 lambda: pk.DeviceCache(_Device(torch.uint8, 1 << 40), past, 8, 4, 64),
+                 lambda: pk.DeviceCache(_Device(torch.uint8, 1 << 40), 2, past, 4, 64),
+                 lambda: pk.DeviceCache(_Device(torch.uint8, 1 << 40), 2, 8, past, 64),
+                 lambda: pool.alloc(past), lambda: pool.share([past]), lambda: pool.release([0, past]),
+                 lambda: pk.PagePool(past)):
+        with pytest.raises(pk.PkHipError) as e:
+            call()
+        assert e.value.code == pk.PK_HIP_EINVAL
+    assert pool.holders(past) == 0 and pool.holders(0) == 1 and pool.free_pages == 6
+
+
 def test_reference_round_trip():
     """The host model of a pool keeps what its own quantizer gives."""
     g = np.random.default_rng(5)
