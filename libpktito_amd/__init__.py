@@ -826,6 +826,10 @@ class DeviceCache:
         ahead (None: all)."""
         n, w = streams.rows, H * self.dk
         pos = self._positions(positions, H)
+        if ws is not None:
+            _is(ws, "uint8", "ws")
+            if not ws.is_contiguous():                   # an expanded one has fewer bytes than elements
+                raise PkHipError(PK_HIP_EINVAL, "ws is not contiguous")
         _check(lib().pk_hip_attention_cache_dev(*_rows(o, n, w, "o"), *_rows(q, n, w, "q"), ctypes.byref(self.st),
                                                 _u32(layer, "layer"), ctypes.byref(streams.st), _u32(H, "H"),
                                                 ctypes.byref(pos) if pos else None,

@@ -405,6 +405,18 @@ def test_numbers_past_32_bits_are_refused(past):
     assert pool.holders(past) == 0 and pool.holders(0) == 1 and pool.free_pages == 6
 
 
+def test_workspaces_that_are_none_are_refused():
+    import torch
+    import libpktito_amd as pk
+    cache, st = _wrapped(pk, torch)
+    q = _Device(torch.float32, 5, 512)
+    for ws in (torch.zeros(1 << 20, dtype=torch.uint8), _Device(torch.float32, 1 << 20),
+               _Device(torch.uint8, 1 << 20, dense=False)):
+        with pytest.raises(pk.PkHipError) as e:
+            cache.attention(q, 0, q, st, 8, ws, stream=0)
+        assert e.value.code == pk.PK_HIP_EINVAL and ("ws" in str(e.value))
+
+
 def test_reference_round_trip():
     """The host model of a pool keeps what its own quantizer gives."""
     g = np.random.default_rng(5)
