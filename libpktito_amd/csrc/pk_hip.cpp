@@ -1601,6 +1601,9 @@ int pk_hip_cache_append_dev(const pk_hip_cache *c, uint32_t layer, const float *
         return e;
     if (layer >= c->layers)
         return fail(PK_HIP_EINVAL, "cache_append_dev: layer %u of %u", layer, c->layers);
+    if (!pkq8::cache_span_fits(streams_of(st), c->heads))
+        return fail(PK_HIP_EINVAL, "cache_append_dev: %u streams of up to %u rows, %u heads: more than a launch holds", st->B,
+                    st->max_T, c->heads);
     const uint64_t width = (uint64_t)c->heads * c->dk;
     if (st->rows && ((e = check_rows(k, ks, width, st->rows, "cache_append_dev", "k")) ||
                      (e = check_rows(v, vs, width, st->rows, "cache_append_dev", "v"))))
@@ -1623,6 +1626,9 @@ int pk_hip_cache_read_dev(const pk_hip_cache *c, uint32_t layer, float *k, size_
         return e;
     if (layer >= c->layers)
         return fail(PK_HIP_EINVAL, "cache_read_dev: layer %u of %u", layer, c->layers);
+    if (!pkq8::cache_span_fits(streams_of(st), c->heads))
+        return fail(PK_HIP_EINVAL, "cache_read_dev: %u streams of up to %u rows, %u heads: more than a launch holds", st->B,
+                    st->max_T, c->heads);
     const uint64_t width = (uint64_t)c->heads * c->dk;
     if (st->rows && ((e = check_rows(k, ks, width, st->rows, "cache_read_dev", "k")) ||
                      (e = check_rows(v, vs, width, st->rows, "cache_read_dev", "v"))))

@@ -218,6 +218,8 @@ int launch_cache_write(uint8_t *data, uint32_t pages, uint32_t G, uint32_t dk, c
                        uint64_t ks, const float *v, uint64_t vs, hipStream_t s);
 int launch_cache_read(const uint8_t *data, uint32_t pages, uint32_t G, uint32_t dk, const CacheStreams &st, float *k,
                       uint64_t ks, float *v, uint64_t vs, hipStream_t s);
+/* whether a write or read of the streams is launched */
+bool cache_span_fits(const CacheStreams &st, uint32_t G);
 /* the attention: left and right clipped to what can occur, p at distance
  * left's row (NULL: content scores alone) */
 struct CacheAttentionCall {

@@ -405,6 +405,19 @@ def test_numbers_past_32_bits_are_refused(past):
     assert pool.holders(past) == 0 and pool.holders(0) == 1 and pool.free_pages == 6
 
 
+@pytest.mark.parametrize("B,max_T,heads,ok", [(65535, 1 << 21, 4, False), (65535, 2, 1024, True), (65535, 66, 1024, True),
+                                              (65535, 450, 1024, False), (2048, 1 << 20, 8, False), (2048, 1 << 20, 7, True)])
+def test_launches_past_what_is_run(B, max_T, heads, ok):
+    """Pages of all streams and heads, 2^28 at most. The calls that are in order
+    end at a null k, which is looked at after."""
+    import libpktito_amd as pk
+    assert ((max_T + 62) // 64 + 1) * B * heads <= 1 << 28 if ok else True
+    calls = _calls(pk, B=B, rows=1 << 21, max_T=max_T, heads=heads, ks=1 << 18, vs=1 << 18, k=None)
+    for e in BOTH:
+        assert calls[e]() == pk.PK_HIP_EINVAL
+        assert (b"launch holds" in pk.lib().pk_hip_last_error()) == (not ok)
+
+
 def test_workspaces_that_are_none_are_refused():
     import torch
     import libpktito_amd as pk
