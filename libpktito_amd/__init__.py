@@ -715,20 +715,34 @@ def _page_ids(ids):
 _dtypes = {}
 
 
-def _is(t, dtype, what):
+def _is(t, dtype, what, device):
     """Refuses a tensor that a kernel would misread: another type, or one that
-    is on the host."""
+    is on the host or on another device (None: any is right)."""
     want = _dtypes.get(dtype)
     if want is None:
         import torch
         want = _dtypes[dtype] = getattr(torch, dtype)
-    if t.dtype is not want or not t.is_cuda:
-        raise PkHipError(PK_HIP_EINVAL, f"{what}: a device tensor of {dtype}, not {t.dtype} on {t.device}")
+    if t.dtype is not want or (t.get_device() != device if device is not None else not t.is_cuda):
+        where = "" if device is None else f" on {device}"
+        raise PkHipError(PK_HIP_EINVAL, f"{what}: a device tensor of {dtype}{where}, not {t.dtype} on {t.device}")
 
 
-def _rows(t, n, width, what):
+_current_device = None
+
+
+def _device():
+    """torch's current device, where launches go."""
+    global _current_device
+    if _current_device is None:
+        import torch
+        torch.cuda.current_device()                     # torch's own initialisation and its errors
+        _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    return _current_device()
+
+
+def _rows(t, n, width, what, device):
     """A float32 matrix's address and row stride, its rows dense."""
-    _is(t, "float32", what)
+    _is(t, "float32", what, device)
     if t.shape != (n, width):
         raise PkHipError(PK_HIP_EINVAL, f"{what}: [{n}, {width}], not {tuple(t.shape)}")
     rs, cs = t.stride()
@@ -737,10 +751,10 @@ def _rows(t, n, width, what):
     return t.data_ptr(), rs if n > 1 else width
 
 
-def _table(t):
+def _table(t, device):
     """Refuses a table that pages' moves could not follow in."""
     if t is not None:
-        _is(t, "int32", "table")
+        _is(t, "int32", "table", device)
         if not t.is_contiguous():
             raise PkHipError(PK_HIP_EINVAL, "table is not contiguous")
 
@@ -753,12 +767,12 @@ class CacheStreams:
 
     def __init__(self, table, len, row0, rows, max_T):
         for t, what in ((table, "table"), (len, "len"), (row0, "row0")):
-            _is(t, "int32", what)
+            _is(t, "int32", what, None if t is table else table.get_device())
             if not t.is_contiguous():
                 raise PkHipError(PK_HIP_EINVAL, f"{what} is not contiguous")
         if table.dim() != 2 or tuple(len.shape) != (table.shape[0],) or tuple(row0.shape) != (table.shape[0] + 1,):
             raise PkHipError(PK_HIP_EINVAL, "streams: table [B, max_pages], len [B], row0 [B + 1]")
-        self.table, self.len, self.row0 = table, len, row0
+        self.table, self.len, self.row0, self.device = table, len, row0, table.get_device()
         self.rows, self.max_T = _u32(int(rows), "rows"), _u32(int(max_T), "max_T")
         self.st = Streams(table.data_ptr(), len.data_ptr(), row0.data_ptr(), table.shape[0], table.shape[1],
                           self.rows, self.max_T)
@@ -770,28 +784,38 @@ class DeviceCache:
     cache_bytes(layers, pages, heads, dk)."""
 
     def __init__(self, data, layers, pages, heads, dk):
-        _is(data, "uint8", "cache")
+        _is(data, "uint8", "cache", None)
         for v, what in ((layers, "layers"), (pages, "pages"), (heads, "heads"), (dk, "dk")):
             _u32(v, what)
         if not data.is_contiguous() or data.numel() < max(1, cache_bytes(layers, pages, heads, dk)):
             raise PkHipError(PK_HIP_EINVAL, f"cache: {cache_bytes(layers, pages, heads, dk)} contiguous bytes (heads of "
                                             "32, 64, 96 or 128 dimensions)")
-        self.data, self.heads, self.dk = data, int(heads), int(dk)
+        self.data, self.heads, self.dk, self.device = data, int(heads), int(dk), data.get_device()
         self.st = Cache(data.data_ptr(), layers, pages, heads, dk)
+
+    def _queue(self, stream, other):
+        """The stream to launch on; the cache, what else the call reads and
+        torch's current device are one device."""
+        if not _device() == self.device == other.device:
+            raise PkHipError(PK_HIP_EINVAL, f"a cache on device {self.device}, with {_device()} the current one and "
+                                            f"{other.device} that of the streams or the source")
+        return _stream(stream)
 
     def append(self, layer, k, v, streams, stream=None):
         """Writes the rows' keys and values [rows, heads * dk] as the streams'
         frames [len, len + T) (pk_hip_cache_append_dev)."""
         n, w = streams.rows, self.heads * self.dk
-        _check(lib().pk_hip_cache_append_dev(ctypes.byref(self.st), _u32(layer, "layer"), *_rows(k, n, w, "k"), *_rows(v, n, w, "v"),
-                                             ctypes.byref(streams.st), _stream(stream)))
+        _check(lib().pk_hip_cache_append_dev(ctypes.byref(self.st), _u32(layer, "layer"),
+                                             *_rows(k, n, w, "k", self.device), *_rows(v, n, w, "v", self.device),
+                                             ctypes.byref(streams.st), self._queue(stream, streams)))
 
     def read(self, layer, k, v, streams, stream=None):
         """The values kept for the streams' frames [len, len + T), into k and v
         [rows, heads * dk] (pk_hip_cache_read_dev)."""
         n, w = streams.rows, self.heads * self.dk
-        _check(lib().pk_hip_cache_read_dev(ctypes.byref(self.st), _u32(layer, "layer"), *_rows(k, n, w, "k"), *_rows(v, n, w, "v"),
-                                           ctypes.byref(streams.st), _stream(stream)))
+        _check(lib().pk_hip_cache_read_dev(ctypes.byref(self.st), _u32(layer, "layer"),
+                                           *_rows(k, n, w, "k", self.device), *_rows(v, n, w, "v", self.device),
+                                           ctypes.byref(streams.st), self._queue(stream, streams)))
 
     def attention_workspace(self, streams, H, positions, left=None, right=None):
         """Bytes of workspace an attention takes; positions as for attention,
@@ -809,9 +833,9 @@ class DeviceCache:
             return None
         p, center, u, w = positions
         n = max(1, _u32(H, "H")) * self.dk
-        _is(p, "float32", "p")
-        _is(u, "float32", "bias_u")
-        _is(w, "float32", "bias_w")
+        _is(p, "float32", "p", self.device)
+        _is(u, "float32", "bias_u", self.device)
+        _is(w, "float32", "bias_w", self.device)
         rows, rest = divmod(p.numel(), n)
         if rest or u.numel() != n or w.numel() != n or not (p.is_contiguous() and u.is_contiguous() and
                                                             w.is_contiguous()):
@@ -827,14 +851,16 @@ class DeviceCache:
         n, w = streams.rows, H * self.dk
         pos = self._positions(positions, H)
         if ws is not None:
-            _is(ws, "uint8", "ws")
+            _is(ws, "uint8", "ws", self.device)
             if not ws.is_contiguous():                   # an expanded one has fewer bytes than elements
                 raise PkHipError(PK_HIP_EINVAL, "ws is not contiguous")
-        _check(lib().pk_hip_attention_cache_dev(*_rows(o, n, w, "o"), *_rows(q, n, w, "q"), ctypes.byref(self.st),
+        _check(lib().pk_hip_attention_cache_dev(*_rows(o, n, w, "o", self.device), *_rows(q, n, w, "q", self.device),
+                                                ctypes.byref(self.st),
                                                 _u32(layer, "layer"), ctypes.byref(streams.st), _u32(H, "H"),
                                                 ctypes.byref(pos) if pos else None,
                                                 _reach(left, "left"), _reach(right, "right"),
-                                                _dptr(ws), ws.numel() if ws is not None else 0, _stream(stream)))
+                                                _dptr(ws), ws.numel() if ws is not None else 0,
+                                                self._queue(stream, streams)))
 
     def move(self, pairs, table=None, source=None, stream=None):
         """Copies pages in every layer: pairs [(from, to), ...], from a page of
@@ -845,10 +871,11 @@ class DeviceCache:
         n = len(flat)
         if n != 2 * len(pairs):
             raise PkHipError(PK_HIP_EINVAL, "pairs of pages (from, to)")
-        _table(table)
-        _check(lib().pk_hip_cache_move_dev(ctypes.byref(self.st), ctypes.byref((source or self).st),
+        _table(table, self.device)
+        source = source or self
+        _check(lib().pk_hip_cache_move_dev(ctypes.byref(self.st), ctypes.byref(source.st),
                                            _page_ids(flat), n // 2, _dptr(table),
-                                           table.numel() if table is not None else 0, _stream(stream)))
+                                           table.numel() if table is not None else 0, self._queue(stream, source)))
 
 
 class PagePool:
@@ -922,7 +949,7 @@ class PagePool:
         self._fits(cache)
         if most is not None and most < 0:
             raise PkHipError(PK_HIP_EINVAL, f"compact: at most {most} pages")
-        _table(table)                                   # refused before the pool's own counts have moved
+        _table(table, cache.device)                     # refused before the pool's own counts have moved
         cap = self.pages if most is None else min(most, self.pages)
         pairs = (ctypes.c_int32 * max(2, 2 * cap))()
         n = ctypes.c_uint32(0)

@@ -201,7 +201,7 @@ def test_pool_against_a_model():
 class _Moves:
     """Stands for a cache: keeps the pairs that the pool would have moved."""
     def __init__(self, pages):
-        self.st, self.pairs = type("St", (), {"pages": pages}), []
+        self.st, self.pairs, self.device = type("St", (), {"pages": pages}), [], 0
 
     def move(self, pairs, table=None, source=None, stream=None):
         self.pairs += pairs
@@ -349,8 +349,9 @@ class _Device:
     """Stands for a device tensor in calls that are refused before one is read."""
     is_cuda = True
 
-    def __init__(self, dtype, *shape, dense=True):
-        self.dtype, self.shape, self.dense, self.device = dtype, shape, dense, "cuda:0"
+    def __init__(self, dtype, *shape, dense=True, device=0):
+        self.dtype, self.shape, self.dense, self.device = dtype, shape, dense, f"cuda:{device}"
+        self.get_device = lambda: device
 
     def numel(self):
         return int(np.prod(self.shape))
@@ -375,10 +376,11 @@ def _wrapped(pk, torch):
 
 
 @pytest.mark.parametrize("past", [-1, -(1 << 32), 1 << 32, (1 << 32) + 1])
-def test_numbers_past_32_bits_are_refused(past):
+def test_numbers_past_32_bits_are_refused(monkeypatch, past):
     """A number whose last 32 bits would do is not taken for those."""
     import torch
     import libpktito_amd as pk
+    monkeypatch.setattr(pk, "_device", lambda: 0)
     cache, st = _wrapped(pk, torch)
     f = lambda n: _Device(torch.float32, 5, n)
     kv, q, ws, b = f(256), f(512), _Device(torch.uint8, 1 << 24), _Device(torch.float32, 512)
@@ -428,6 +430,44 @@ def test_workspaces_that_are_none_are_refused():
         with pytest.raises(pk.PkHipError) as e:
             cache.attention(q, 0, q, st, 8, ws, stream=0)
         assert e.value.code == pk.PK_HIP_EINVAL and ("ws" in str(e.value))
+
+
+def test_other_devices_are_refused(monkeypatch):
+    """Tensors on another device than the cache's, and a current device that is
+    another (where the launch would go)."""
+    import torch
+    import libpktito_amd as pk
+    cache, st = _wrapped(pk, torch)
+    other = pk.DeviceCache(_Device(torch.uint8, pk.cache_bytes(2, 8, 4, 64), device=1), 2, 8, 4, 64)
+    f = lambda *s, device=0: _Device(torch.float32, *s, device=device)
+    i32 = lambda *s, device=0: _Device(torch.int32, *s, device=device)
+    kv, q, b, ws = f(5, 256), f(5, 512), f(512), _Device(torch.uint8, 1 << 24)
+    kv1, q1, b1, ws1 = f(5, 256, device=1), f(5, 512, device=1), f(512, device=1), _Device(torch.uint8, 1 << 24, device=1)
+    st1 = pk.CacheStreams(i32(2, 4, device=1), i32(2, device=1), i32(3, device=1), 5, 3)
+    p = f(9, 512)
+
+    def refused(*calls):
+        for call in calls:
+            with pytest.raises(pk.PkHipError) as e:
+                call()
+            assert e.value.code == pk.PK_HIP_EINVAL
+
+    monkeypatch.setattr(pk, "_device", lambda: 0)
+    refused(lambda: pk.CacheStreams(i32(2, 4), i32(2, device=1), i32(3), 5, 3),
+            lambda: pk.CacheStreams(i32(2, 4), i32(2), i32(3, device=1), 5, 3),
+            lambda: cache.append(0, kv1, kv, st, 0), lambda: cache.append(0, kv, kv1, st, 0),
+            lambda: cache.append(0, kv, kv, st1, 0), lambda: cache.read(0, kv, kv1, st, 0),
+            lambda: cache.read(0, kv, kv, st1, 0), lambda: cache.attention(q1, 0, q, st, 8, ws, stream=0),
+            lambda: cache.attention(q, 0, q1, st, 8, ws, stream=0), lambda: cache.attention(q, 0, q, st1, 8, ws, stream=0),
+            lambda: cache.attention(q, 0, q, st, 8, ws1, stream=0),
+            lambda: cache.attention(q, 0, q, st, 8, ws, (f(9, 512, device=1), 4, b, b), stream=0),
+            lambda: cache.attention(q, 0, q, st, 8, ws, (p, 4, b1, b), stream=0),
+            lambda: cache.attention(q, 0, q, st, 8, ws, (p, 4, b, b1), stream=0),
+            lambda: cache.move([(0, 1)], i32(2, 4, device=1), stream=0), lambda: cache.move([(0, 1)], None, other, 0),
+            lambda: pk.PagePool(8).compact(cache, i32(2, 4, device=1)))
+    monkeypatch.setattr(pk, "_device", lambda: 1)
+    refused(lambda: cache.append(0, kv, kv, st, 0), lambda: cache.read(0, kv, kv, st, 0),
+            lambda: cache.attention(q, 0, q, st, 8, ws, stream=0), lambda: cache.move([(0, 1)], stream=0))
 
 
 def test_reference_round_trip():
