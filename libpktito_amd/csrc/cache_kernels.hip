@@ -626,29 +626,30 @@ __device__ __forceinline__ bool share_of(const CacheAttention &a, Share &s, uint
 /* the wave's number in its workgroup, known to be the same in all its lanes */
 __device__ __forceinline__ uint32_t wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
-/* The pages that a wave takes, every fourth of its workgroup's: 64 table
+/* The pages that a wave takes, every W-th of its workgroup of W waves: 64 table
  * entries at a time, one a lane, those that are no page of the pool passed
  * over. */
+template <int W>
 struct Walk {
     int32_t first, ids;
     uint64_t left;
 
     __device__ __forceinline__ Walk(const CacheAttention &a, const Share &s)
-        : first(s.pa + (int32_t)wave_id() - 4 * 64), ids(0), left(0) {}
+        : first(s.pa + (int32_t)wave_id() - W * 64), ids(0), left(0) {}
 
     /* the next page and its place in the pool; false, and pg and id as they were, after the last */
     __device__ __forceinline__ bool next(const CacheAttention &a, const Share &s, int32_t &pg, int32_t &id) {
         while (left == 0) {
-            if (first + 4 * 64 >= s.pb)
+            if (first + W * 64 >= s.pb)
                 return false;
-            first += 4 * 64;
-            const int32_t mine = first + 4 * (int32_t)(threadIdx.x & 63);
+            first += W * 64;
+            const int32_t mine = first + W * (int32_t)(threadIdx.x & 63);
             ids = mine < s.pb ? a.st.table[(uint64_t)s.b * a.st.max_pages + mine] : -1;
             left = __ballot(cache_page_ok(ids, a.pages));
         }
         const int at = __builtin_ctzll(left);
         left &= left - 1;
-        pg = first + 4 * at;
+        pg = first + W * at;
         id = __builtin_amdgcn_readlane(ids, at);
         return true;
     }
@@ -704,18 +705,18 @@ __device__ __forceinline__ v4f normal(v4f y, float l) {
 
 /* The workgroup's waves met: into the outputs, or with several splits into
  * the workspace (R rows of dk sums, then R pairs of maximum and sum). */
-template <int R, int NS>
+template <int R, int NS, int W>
 __device__ __forceinline__ void finish(const CacheAttention &a, const Share &s, float (*part)[R][32 * NS + 4],
                                        float (*tops)[R], float (*sums)[R]) {
     constexpr uint32_t dk = 32 * NS;
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < R * dk / 4; i += 256) {
+    for (uint32_t i = threadIdx.x; i < R * dk / 4; i += 64 * W) {
         const uint32_t r = i / (dk / 4), c = i % (dk / 4) * 4;
         const int32_t rr = s.rr0 + (int32_t)r;
         if (rr >= s.nrows)
             continue;
         float m, l;
-        const v4f y = joined<4>(4, [&](int n, float &top, float &sum, v4f *o) {
+        const v4f y = joined<W>(W, [&](int n, float &top, float &sum, v4f *o) {
             top = tops[n][r], sum = sums[n][r];
             if (o)
                 *o = *(const v4f *)&part[n][r][c];
@@ -801,12 +802,12 @@ constexpr float kSlack = 8.0f;
  * spill: 233). Short calls take 10 to 12 us whatever their bytes: a launch,
  * the stream, its table, a page's loads and three pages a wave. */
 enum { kNone, kMade, kOwn };
-template <int NS, int POS>
-__global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
+template <int NS, int POS, int W>
+__global__ __launch_bounds__(64 * W) void cache_few_kernel(CacheAttention a) {
     constexpr uint32_t dk = 32 * NS, record = kPage * dk + 4 * kPage;
     constexpr uint32_t kRow = 72;           /* bfloat16 a row of pieces: 64 and a pad against bank conflicts */
-    __shared__ float part[4][4][dk + 4], tops[4][4], sums[4][4];
-    __shared__ __attribute__((aligned(16))) uint16_t prob[4][12][kRow];
+    __shared__ float part[W][4][dk + 4], tops[W][4], sums[W][4];
+    __shared__ __attribute__((aligned(16))) uint16_t prob[W][12][kRow];
     Share s;
     if (!share_of<4>(a, s, a.splits))
         return;
@@ -901,7 +902,7 @@ __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
         vs = *(const v2u *)(rec + cache_value_scale_at(dk, 4 * c));
     };
 
-    Walk walk(a, s);
+    Walk<W> walk(a, s);
     int32_t pg = 0, id = 0;
     bool more = walk.next(a, s, pg, id);
     if (more) {
@@ -988,7 +989,7 @@ __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
 #pragma unroll
     for (int dt = 0; dt < 2 * NS; dt++)
         part[wave][w][16 * dt + c] = (o[dt][2] + o[dt][1]) + o[dt][0];
-    finish<4, NS>(a, s, part, tops, sums);
+    finish<4, NS, W>(a, s, part, tops, sums);
 }
 
 /* More rows: 16 a workgroup, its four waves a page each in turn with the
@@ -1002,12 +1003,12 @@ __global__ __launch_bounds__(256) void cache_few_kernel(CacheAttention a) {
  * quarters of the cycles at two waves a SIMD (235 registers). Measured and no
  * faster: a page's first product under the page before's softmax (130), the
  * products at another wave priority (127, 129), the queries' pieces in LDS
- * (126; for three waves, 250: spills), eight waves (147; 13.2 against 14.2 us
- * where 16 streams of 14 rows leave half the CUs idle). */
-template <int NS, bool POS>
-__global__ __launch_bounds__(256) void cache_many_kernel(CacheAttention a) {
+ * (126; for three waves, 250: spills), eight waves (147; where 16 streams of 14
+ * rows leave half the CUs idle, eight take 12.8 and four 14.5). */
+template <int NS, bool POS, int W>
+__global__ __launch_bounds__(64 * W) void cache_many_kernel(CacheAttention a) {
     constexpr uint32_t dk = 32 * NS, record = kPage * dk + 4 * kPage;
-    __shared__ float part[4][16][dk + 4], tops[4][16], sums[4][16];
+    __shared__ float part[W][16][dk + 4], tops[W][16], sums[W][16];
     Share sh;
     if (!share_of<16>(a, sh, a.splits))
         return;
@@ -1072,7 +1073,7 @@ __global__ __launch_bounds__(256) void cache_many_kernel(CacheAttention a) {
             vs[kt] = *(const v2u *)(rec + cache_value_scale_at(dk, 16 * kt + 4 * w));
     };
 
-    Walk walk(a, sh);
+    Walk<W> walk(a, sh);
     int32_t pg = 0, id = 0;
     bool more = walk.next(a, sh, pg, id);
     if (more) {
@@ -1162,7 +1163,7 @@ __global__ __launch_bounds__(256) void cache_many_kernel(CacheAttention a) {
 #pragma unroll
     for (int dt = 0; dt < 2 * NS; dt++)
         *(v4f *)&part[wave][lane % 16][16 * dt + 4 * w] = o[dt];
-    finish<16, NS>(a, sh, part, tops, sums);
+    finish<16, NS, W>(a, sh, part, tops, sums);
 }
 
 /* ----------------------------------------------------------------- move --- */
@@ -1257,16 +1258,30 @@ int launch_cache_read(const uint8_t *data, uint32_t pages, uint32_t G, uint32_t 
 /* workgroups of 256 in a launch's first dimension, under 2^32 threads */
 constexpr uint64_t kMostGroups = (1u << 24) - 1;
 
-/* How a call's rows are dealt: tiles of four rows where a stream has at most
- * four a kept head, else of 16; and splits of a tile's pages where the tiles
- * are fewer than two workgroups a CU and a wave would take eight pages or more
- * one after another. Joining the splits costs 4 to 5 us, a wave's page about
- * one: one frame against 704 pages takes 873 us unsplit, 17 over 64 splits a
- * head (19 over 96, 22 over 128); 16 streams of 17 pages 11 unsplit, 15 over
- * two; 512 tiles of 12 pages 11.7 unsplit, 19 over two. */
+/* How a call's rows are dealt. Tiles of four rows where a stream has at most
+ * four a kept head, else of 16. With up to 256 tiles, a workgroup a CU, the
+ * waves that a CU holds are found in two ways: workgroups of eight waves, which
+ * meet in LDS, where a wave then takes a page or more (four rows' pages are
+ * short work, so 10 pages of 128 dimensions or 20 of 64), and splits of a
+ * tile's pages, joined for 4 to 5 us by a launch of their own, from 32 pages
+ * on, so many that a wave takes two pages or more. As many splits of four waves
+ * as two a CU allow only where that is an odd number, so that those of eight
+ * waves leave CUs idle, and against none from 80 pages on.
+ *
+ * Heads of 128, four rows: 256 tiles of 33 pages 16.2 us with eight waves, 16.7
+ * with four, 19.4 in two splits of four; 192 of 16 8.6 and 9.0 (heads of 64 7.7
+ * and 7.3); 32 of 70 unsplit with four 23.7, in eight splits 10.7, in nine 11.5.
+ * 16 rows: 256 of 33 19.4 with eight, in two splits of four 26.4; 192 of 24 15.1
+ * with eight and 15.8 with four, of 8 9.2 and 9.1; 320 of 24 27.4 and 22.8 (more
+ * tiles than CUs). 168 tiles of one row unsplit with eight waves and in three splits of
+ * four: 33 pages 12.7 and 14.6, 80 23.7 and 26.0 (16 rows 30.6 and 30.5), 300
+ * 71 and 69 (103 and 95; heads of 64 47 and 39); 96 tiles in two of eight and
+ * in five of four: 33 pages 11.7 and 11.2, 300 43.7 and 44.1 (16 rows 55 and
+ * 49). One frame against 704 pages of one stream: 873 us unsplit. */
 struct Deal {
     uint32_t rows, tiles, splits;           /* rows a tile, a stream's tiles a kept head, a tile's splits */
     uint32_t pages;                         /* pages a tile can reach */
+    uint32_t waves;                         /* waves a workgroup of the attention */
     uint64_t units;
     bool own;                               /* a row's position scores made where they are used */
 };
@@ -1276,16 +1291,23 @@ struct Deal {
  * 7.2 us so and 8.9 with a launch of their own, by 181 10.0 and 9.0; 16 rows
  * by 71 7.3 and 9.1, 64 rows 13.6 and 10.6 (each stream reads the table
  * itself, in pieces of 16 bytes). */
-static Deal deal(const CacheStreams &st, uint32_t G, uint32_t H, int32_t left, int32_t right) {
+static Deal deal(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, int32_t left, int32_t right) {
     Deal d;
     const uint32_t rows = st.max_T * (H / G);
     d.rows = rows <= 4 ? 4 : 16;
     d.tiles = (rows + d.rows - 1) / d.rows;
     d.units = (uint64_t)st.B * G * d.tiles;
     d.pages = cache_tile_pages(st.max_pages, left, right);
-    const uint64_t want = d.units ? 512 / d.units : 1;
     d.own = rows == 1 && st.B <= 16 && left + right < 100;
-    d.splits = d.pages < 32 ? 1 : (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({ want, (d.pages + 7) / 8, 128 }));
+    d.splits = 1, d.waves = 4;
+    if (d.units == 0 || d.units > 256)
+        return d;
+    const uint32_t eights = (uint32_t)(256 / d.units), fours = (uint32_t)(512 / d.units);
+    const bool odd = fours % 2 && d.pages >= (eights == 1 ? 80 : 32);
+    if (d.pages >= 32)
+        d.splits = std::min({ odd ? fours : eights, (d.pages + 7) / 8, 128u });
+    if (!odd && (d.rows == 4 ? (uint64_t)d.pages * dk > 1280u * d.splits : d.pages > 8 * d.splits))
+        d.waves = 8;
     return d;
 }
 
@@ -1316,12 +1338,12 @@ static Space space(const CacheStreams &st, uint32_t H, uint32_t dk, bool positio
 
 size_t cache_attention_workspace(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, bool positions,
                                  int32_t left, int32_t right) {
-    const Space s = space(st, H, dk, positions, (uint32_t)left + (uint32_t)right + 1, deal(st, G, H, left, right));
+    const Space s = space(st, H, dk, positions, (uint32_t)left + (uint32_t)right + 1, deal(st, G, H, dk, left, right));
     return s.place + s.halved + s.parts;
 }
 
-bool cache_attention_fits(const CacheStreams &st, uint32_t G, uint32_t H, int32_t left, int32_t right) {
-    const Deal d = deal(st, G, H, left, right);
+bool cache_attention_fits(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, int32_t left, int32_t right) {
+    const Deal d = deal(st, G, H, dk, left, right);
     return d.units <= kMostGroups / d.splits && ((uint32_t)left + (uint32_t)right) / 64 < kMostGroups;
 }
 
@@ -1354,16 +1376,17 @@ static void attend(const CacheAttention &a, const Deal &d, hipStream_t s) {
         }
     }
     const uint32_t grid = (uint32_t)(d.units * d.splits);
+    const uint32_t threads = 64 * d.waves;
     if (d.rows == 4 && a.p && d.own)
-        cache_few_kernel<NS, kOwn><<<grid, 256, 0, s>>>(a);
+        cache_few_kernel<NS, kOwn, 4><<<grid, threads, 0, s>>>(a);
     else if (d.rows == 4 && a.p)
-        cache_few_kernel<NS, kMade><<<grid, 256, 0, s>>>(a);
+        (d.waves == 8 ? cache_few_kernel<NS, kMade, 8> : cache_few_kernel<NS, kMade, 4>)<<<grid, threads, 0, s>>>(a);
     else if (d.rows == 4)
-        cache_few_kernel<NS, kNone><<<grid, 256, 0, s>>>(a);
+        (d.waves == 8 ? cache_few_kernel<NS, kNone, 8> : cache_few_kernel<NS, kNone, 4>)<<<grid, threads, 0, s>>>(a);
     else if (a.p)
-        cache_many_kernel<NS, true><<<grid, 256, 0, s>>>(a);
+        (d.waves == 8 ? cache_many_kernel<NS, true, 8> : cache_many_kernel<NS, true, 4>)<<<grid, threads, 0, s>>>(a);
     else
-        cache_many_kernel<NS, false><<<grid, 256, 0, s>>>(a);
+        (d.waves == 8 ? cache_many_kernel<NS, false, 8> : cache_many_kernel<NS, false, 4>)<<<grid, threads, 0, s>>>(a);
     if (d.splits > 1) {
         if (d.rows == 4)
             cache_join_kernel<4, NS><<<dim3(grid / d.splits, std::min(d.rows, a.st.max_T * (a.H / a.G))), 256, 0, s>>>(a);
@@ -1381,7 +1404,7 @@ int launch_cache_attention(const CacheAttentionCall &c, hipStream_t s) {
     a.scale = 1.0f / sqrtf((float)c.dk);
     a.p = c.p, a.bias_u = c.bias_u, a.bias_w = c.bias_w;
     a.bw = (uint32_t)c.left + (uint32_t)c.right + 1;
-    const Deal d = deal(c.st, c.G, c.H, c.left, c.right);
+    const Deal d = deal(c.st, c.G, c.H, c.dk, c.left, c.right);
     a.tiles = d.tiles, a.splits = d.splits;
     const Space sp = space(c.st, c.H, c.dk, c.p != nullptr, a.bw, d);
     a.place = (float *)c.ws;

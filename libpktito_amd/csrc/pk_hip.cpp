@@ -1666,7 +1666,7 @@ static int attention_window(const pk_hip_cache *c, const pk_hip_streams *st, uin
     }
     *l = (int32_t)lo;
     *r = (int32_t)hi;
-    if (!pkq8::cache_attention_fits(streams_of(st), c->heads, H, *l, *r))
+    if (!pkq8::cache_attention_fits(streams_of(st), c->heads, H, c->dk, *l, *r))
         return fail(PK_HIP_EINVAL, "%s: %u streams of up to %u rows, %u heads: more than a launch holds", who, st->B,
                     st->max_T, H);
     return PK_HIP_OK;

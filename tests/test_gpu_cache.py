@@ -301,6 +301,29 @@ def test_long_stream(hip, torch):
         w.check(4, left=2000)
 
 
+@pytest.mark.parametrize("B,H,G,T,dk,pages", [
+    (3, 2, 2, 1, 128, 12), (3, 2, 2, 3, 64, 22), (32, 8, 8, 1, 32, 44),     # tiles of four rows, eight waves
+    (16, 8, 8, 1, 128, 33), (1, 2, 1, 2, 96, 300),                          # in splits of eight waves
+    (19, 8, 8, 1, 64, 80), (12, 8, 8, 1, 32, 34),                           # in three and five splits of four
+    (3, 2, 2, 20, 128, 9), (2, 2, 1, 64, 32, 31), (16, 8, 8, 17, 32, 33),   # tiles of 16 rows, eight waves
+    (8, 8, 4, 9, 64, 35), (1, 1, 1, 40, 96, 120),                           # in splits
+    (17, 8, 8, 16, 32, 81), (33, 8, 8, 1, 32, 40),                          # in three splits; more tiles than CUs
+])
+@pytest.mark.parametrize("with_positions", [False, True])
+def test_pages_dealt(hip, torch, B, H, G, T, dk, pages, with_positions):
+    """Each way that a tile's pages are dealt to waves and workgroups. All streams
+    read one stream's pages, each with holes of its own; the last one has fewer."""
+    say("dealt", B, H, G, T, dk, pages, with_positions)
+    total = 64 * pages - 5
+    w = World(hip, torch, [total - T] * (B - 1) + [total - T - (70 if B > 1 else 0)], [T] * B, G, dk, seed=pages)
+    w.table[:] = w.table[0]
+    w.fill(upto=[total] + [0] * (B - 1))
+    for b in range(B):
+        w.table[b, (7 * b + 3) % pages] = w.table[b, (11 * b + 1) % pages] = -1
+    w.upload()
+    w.check(H, w.positions(H, total, T) if with_positions else None)
+
+
 @pytest.mark.parametrize("seed", range(24))
 def test_any_call(hip, torch, seed):
     """Calls drawn over the documented ranges: streams, lengths, rows, heads,
