@@ -436,8 +436,10 @@ size_t pk_hip_cache_bytes(uint32_t layers, uint32_t pages, uint32_t heads, uint3
  *   row0   [B + 1]: stream b's rows are [row0[b], row0[b + 1]), its frames
  *          [len[b], len[b] + T) with T = row0[b + 1] - row0[b], which may be 0
  * rows is the call's number of rows and max_T at least the longest stream's T
- * (rows a stream has beyond max_T or beyond rows take no part, and frames
- * past 64 max_pages have no page). Rows of no stream are left as they were.
+ * (rows a stream has beyond max_T or beyond rows take no part). Frames past 64
+ * max_pages have no page: they are not kept, and their rows attend those that
+ * the table holds; a len past 64 max_pages counts as that. Rows of no stream
+ * are left as they were.
  * No two streams of a call may have one row or write one page. max_pages up
  * to 2^24, B up to 65535, rows up to 2^21, and B x max_T x heads what a launch
  * holds (refused otherwise): in a write or read 2^28 pages of all streams and

@@ -497,9 +497,8 @@ __global__ __launch_bounds__(64 * W, 4) void cache_place_kernel(CacheAttention a
         const int32_t r0 = max(sp.r0, (int32_t)n0), r1 = min(sp.r0 + sp.T, (int32_t)(n0 + kRows));
         if (r0 >= r1)
             continue;
-        const int32_t p0 = sp.len + r0 - sp.r0, p1 = sp.len + r1 - 1 - sp.r0;
-        lo = min(lo, a.left - p1);
-        hi = max(hi, a.left + sp.total - 1 - p0);
+        lo = min(lo, place_lo(sp, r1, a.left));
+        hi = max(hi, place_hi(sp, r0, a.left));
     }
     lo = -wave_max(-lo), hi = wave_max(hi);
     if (lane == 0)

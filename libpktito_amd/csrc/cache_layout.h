@@ -150,6 +150,13 @@ PK_HD CacheSpan cache_span(const CacheStreams &s, int32_t row0, int32_t row1, in
  * frames are neither written nor attended */
 PK_HD bool cache_page_ok(int32_t id, uint32_t pages) { return (uint32_t)id < pages; }
 
+/* The furthest back that a row of a call can attend. A stream's frames may
+ * outgrow its table: then the last rows lie past every frame that the table
+ * holds, and the first of those is this far behind. */
+PK_HD int32_t cache_most_left(uint32_t max_pages, uint32_t max_T) {
+    return (int32_t)(max_pages * kPage - 1 + max_T);
+}
+
 /* The frames a row at position pos attends: [lo, hi], empty if lo > hi. */
 PK_HD int32_t cache_lo(int32_t pos, int32_t left) { return pos > left ? pos - left : 0; }
 PK_HD int32_t cache_hi(int32_t pos, int32_t right, int32_t total) {
@@ -173,6 +180,14 @@ PK_HD uint32_t cache_tile_pages(uint32_t max_pages, int32_t left, int32_t right)
  * up to 31 past bw. */
 constexpr uint32_t kPlacePad = 80;
 PK_HD uint32_t place_stride(uint32_t bw) { return (bw + 2 * kPlacePad + 15) / 16 * 16; }
+
+/* the distances x that the call's rows [r0, r1) of a stream need, all of its
+ * frames: the last row's of frame 0, the first one's of the last frame (which
+ * is under max_T ahead of it, so that left is added to a small number) */
+PK_HD int32_t place_lo(const CacheSpan &sp, int32_t r1, int32_t left) { return left - (sp.len + r1 - 1 - sp.r0); }
+PK_HD int32_t place_hi(const CacheSpan &sp, int32_t r0, int32_t left) {
+    return left + (sp.total - 1 - (sp.len + r0 - sp.r0));
+}
 
 }  // namespace pkq8
 

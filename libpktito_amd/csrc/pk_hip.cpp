@@ -1644,8 +1644,8 @@ int pk_hip_cache_read_dev(const pk_hip_cache *c, uint32_t layer, float *k, size_
     return PK_HIP_OK;
 }
 
-/* The window that an attention's rows have: the asked one, no wider than a
- * stream can be or than the positions' table reaches. */
+/* The window that an attention's rows have: the asked one, no wider than the
+ * rows can reach or than the positions' table does. */
 static int attention_window(const pk_hip_cache *c, const pk_hip_streams *st, uint32_t H, const pk_hip_positions *pos,
                             uint32_t left, uint32_t right, const char *who, int32_t *l, int32_t *r) {
     int e;
@@ -1655,7 +1655,8 @@ static int attention_window(const pk_hip_cache *c, const pk_hip_streams *st, uin
         (uint64_t)st->max_T * (H / c->heads) > 0x3fffffff)
         return fail(PK_HIP_EINVAL, "%s: H = %u heads of 32, 64, 96 or 128 dimensions, a multiple of the kept ones, at "
                                    "most 2^30 rows of a kept head a stream", who, H);
-    uint32_t lo = std::min(left, st->max_pages * pkq8::kPage - 1), hi = std::min(right, st->max_T ? st->max_T - 1 : 0);
+    uint32_t lo = std::min(left, (uint32_t)pkq8::cache_most_left(st->max_pages, st->max_T));
+    uint32_t hi = std::min(right, st->max_T ? st->max_T - 1 : 0);
     if (pos) {
         if (!pos->p || !pos->bias_u || !pos->bias_w || (((uintptr_t)pos->p | (uintptr_t)pos->bias_u |
             (uintptr_t)pos->bias_w) & 15) || pos->center >= pos->n)

@@ -30,4 +30,15 @@ void t_span(uint32_t max_pages, uint32_t rows, uint32_t max_T, int32_t row0, int
     out[0] = p.r0, out[1] = p.T, out[2] = p.len, out[3] = p.total;
 }
 
+/* out: the call's r0, T, len, total, then the distances that its rows [a, b) need with this left */
+int32_t t_most_left(uint32_t max_pages, uint32_t max_T) { return cache_most_left(max_pages, max_T); }
+void t_places(uint32_t max_pages, uint32_t rows, uint32_t max_T, int32_t row0, int32_t row1, int32_t len, int32_t a,
+              int32_t b, int32_t left, int32_t *out) {
+    CacheStreams s = {};
+    s.max_pages = max_pages, s.rows = rows, s.max_T = max_T;
+    const CacheSpan p = cache_span(s, row0, row1, len);
+    out[0] = p.r0, out[1] = p.T, out[2] = p.len, out[3] = p.total;
+    out[4] = place_lo(p, p.r0 + b, left), out[5] = place_hi(p, p.r0 + a, left);
+}
+
 }

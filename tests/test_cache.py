@@ -483,3 +483,28 @@ def test_reference_round_trip():
                 want, _, _ = cr.kept(x[:, which], 2)
                 got = pool.read(0, 1, h)[which]
                 assert np.array_equal(got, want[:, h * dk:(h + 1) * dk])
+
+
+def test_windows_reach_the_first_frame(layout):
+    """Streams that outgrow their tables, up to the largest: the widest window has
+    frame 0 in it for every row, the narrower ones theirs, and the distances
+    between a block's rows and the frames are right (the build stops at sums that
+    pass 32 bits)."""
+    i, u = ctypes.c_int32, ctypes.c_uint32
+    layout.t_most_left.restype, layout.t_most_left.argtypes = i, [u, u]
+    layout.t_places.restype, layout.t_places.argtypes = None, [u, u, u, i, i, i, i, i, i, ctypes.POINTER(i)]
+    r, out = random.Random(6), (i * 6)()
+    for _ in range(20000):
+        max_pages = r.choice([1, 2, 100, 1 << 24])
+        cap = 64 * max_pages
+        T = r.choice([1, 4, 300, 1 << 21])
+        n = r.choice([0, cap, cap - 1, max(0, cap - T), r.randint(0, cap)])
+        most = layout.t_most_left(max_pages, T)
+        t0 = r.choice([0, T - 1, r.randint(0, T - 1)])
+        t1 = r.randint(t0, T - 1)
+        left = r.choice([most, min(most, cap), cap - 1, r.randint(0, most)])
+        layout.t_places(max_pages, T, T, 0, T, n, t0, t1 + 1, left, out)
+        _, rows, ln, total, lo, hi = out
+        assert (rows, ln, total) == (T, n, min(n + T, cap))
+        assert layout.t_lo(ln + t1, most) == 0 and layout.t_lo(ln + t1, left) == max(0, ln + t1 - left)
+        assert lo == left - (ln + t1) and hi == left + total - 1 - (ln + t0)

@@ -780,3 +780,41 @@ def test_nothing_to_do(hip, torch):
     st = hip.CacheStreams(z.reshape(0, 1), z, torch.zeros(1, dtype=torch.int32, device="cuda"), 0, 0)
     e = torch.empty(0, 128, device="cuda")
     assert w.cache.attention_workspace(st, 2, None) == 0
+
+
+# ------------------------------------------------- rows past the table --
+
+@pytest.mark.parametrize("lens,T,max_pages", [
+    ([60, 64, 10, 0], 1, 1), ([60, 64, 63], 4, 1), ([60, 64, 0], 10, 1),
+    ([128, 120, 64], 40, 2), ([0, 100], 300, 2), ([1, 64], 90, 1),
+])
+@pytest.mark.parametrize("with_positions", [False, True])
+def test_rows_past_the_table(hip, torch, lens, T, max_pages, with_positions):
+    """A stream that outgrows its table: its last rows' frames have no page, and
+    the rows attend what the table holds, the first frame included."""
+    say("past the table", lens, T, max_pages, with_positions)
+    w = World(hip, torch, lens, [T] * len(lens), 2, 64, seed=50 + T, first=1, tail=1, max_pages=max_pages)
+    w.fill()
+    cap = 64 * max_pages
+    for left, right in ((None, None), (None, 0), (cap - 1, None), (cap, None), (cap + 2, 0), (5, 3)):
+        w.check(4 if T < 10 else 2, w.positions(4 if T < 10 else 2, max(lens) + T, T) if with_positions else None, left,
+                right)
+    if with_positions:                          # what the table of positions reaches, on both sides of the cap
+        for back in (cap - 1, cap, cap + 1):
+            w.check(2, w.positions(2, back, 2))
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_any_call_past_the_table(hip, torch, seed):
+    """Drawn calls whose tables are narrower than some of their streams."""
+    r = random.Random(1000 + seed)
+    dk, (H, G) = r.choice(DKS), r.choice([(1, 1), (2, 2), (4, 1), (6, 3)])
+    max_pages, B = r.choice([1, 1, 2, 3]), r.choice([1, 3, 18])
+    Ts = [r.choice([1, 2, 3, r.randint(1, 70)]) for _ in range(B)]
+    lens = [max(0, 64 * max_pages - r.choice([0, 1, 5, r.randint(0, 64 * max_pages)])) for _ in range(B)]
+    say("any past", seed, dk, H, G, lens, Ts, max_pages)
+    w = World(hip, torch, lens, Ts, G, dk, seed=seed, first=r.randint(0, 2), tail=r.randint(0, 2), max_pages=max_pages)
+    w.fill()
+    left, right = (r.choice([None, None, 0, 64 * max_pages, r.randint(0, 400)]) for _ in range(2))
+    pos = w.positions(H, r.choice([64 * max_pages, 300, 40]), r.choice([70, 2])) if r.random() < 0.6 else None
+    w.check(H, pos, left, right)
