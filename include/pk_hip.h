@@ -521,7 +521,11 @@ int pk_hip_cache_move_dev(const pk_hip_cache *dst, const pk_hip_cache *src, cons
  *            number in use, at most cap of them; the pool's own counts move at
  *            once, so the caller's next calls are pk_hip_cache_move_dev with
  *            them and the tables (in stream order before any later write).
- *            Returns how many in *n. */
+ *            Returns how many in *n.
+ *   restore  the counts as before a compact that gave these pairs, for a move
+ *            that was refused. Refused itself, and then nothing is changed,
+ *            where a page that the compact freed is held again, or one that it
+ *            filled is free */
 typedef struct pk_hip_pool pk_hip_pool;
 int pk_hip_pool_create(pk_hip_pool **pool, uint32_t pages);
 void pk_hip_pool_destroy(pk_hip_pool *pool);
@@ -531,6 +535,7 @@ int pk_hip_pool_share(pk_hip_pool *pool, const int32_t *ids, uint32_t n);
 int pk_hip_pool_release(pk_hip_pool *pool, const int32_t *ids, uint32_t n);
 uint32_t pk_hip_pool_holders(const pk_hip_pool *pool, int32_t id);
 int pk_hip_pool_compact(pk_hip_pool *pool, int32_t *pairs, uint32_t cap, uint32_t *n);
+int pk_hip_pool_restore(pk_hip_pool *pool, const int32_t *pairs, uint32_t n);
 
 /* Measurement aids, with no counterpart in the reference: the floors a
  * small product's time is read against. pk_hip_empty_dev launches an empty

@@ -209,6 +209,7 @@ _SIGS = {
     "pk_hip_pool_holders": (ctypes.c_uint32, [ctypes.c_void_p, ctypes.c_int32]),
     "pk_hip_pool_compact": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32,
                                            ctypes.POINTER(ctypes.c_uint32)]),
+    "pk_hip_pool_restore": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32]),
     "pk_hip_joint_dev": (ctypes.c_int, [ctypes.c_void_p] * 6 + [ctypes.c_uint32, ctypes.c_uint32, ctypes.c_void_p]),
     "pk_hip_layer_dev": (ctypes.c_int, [ctypes.POINTER(LayerW), ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p,
                                         ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p, ctypes.c_size_t,
@@ -949,12 +950,17 @@ class PagePool:
         self._fits(cache)
         if most is not None and most < 0:
             raise PkHipError(PK_HIP_EINVAL, f"compact: at most {most} pages")
-        _table(table, cache.device)                     # refused before the pool's own counts have moved
+        _table(table, cache.device)
+        cache.move([], table, stream=stream)            # what a move would be refused for, before the counts move
         cap = self.pages if most is None else min(most, self.pages)
         pairs = (ctypes.c_int32 * max(2, 2 * cap))()
         n = ctypes.c_uint32(0)
         _check(lib().pk_hip_pool_compact(self.handle, pairs, cap, ctypes.byref(n)))
         moved = [(pairs[2 * i], pairs[2 * i + 1]) for i in range(n.value)]
         if moved:
-            cache.move(moved, table, stream=stream)
+            try:
+                cache.move(moved, table, stream=stream)
+            except Exception:
+                _check(lib().pk_hip_pool_restore(self.handle, pairs, n))
+                raise
         return moved

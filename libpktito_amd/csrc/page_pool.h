@@ -83,9 +83,7 @@ public:
             if (to >= top)
                 break;
             const uint32_t from = top - 1;
-            take(to);
-            give(from);
-            std::swap(holders_[to], holders_[from]);
+            relocate(from, to);
             pairs[2 * n] = (int32_t)from;
             pairs[2 * n + 1] = (int32_t)to;
             n++;
@@ -93,7 +91,32 @@ public:
         return n;
     }
 
+    /* undoes compact's pairs, the last first, if each page that one was moved
+     * from is still free and the page it went to held */
+    bool restore(const int32_t *pairs, uint32_t n) {
+        std::lock_guard<std::mutex> lk(mu_);
+        uint32_t i = n;
+        for (; i > 0; i--) {
+            const uint32_t from = (uint32_t)pairs[2 * i - 2], to = (uint32_t)pairs[2 * i - 1];
+            if (from >= holders_.size() || to >= from || holders_[from] != 0 || holders_[to] == 0)
+                break;
+            relocate(to, from);
+        }
+        if (i > 0) {                        /* as it was */
+            for (; i < n; i++)
+                relocate((uint32_t)pairs[2 * i], (uint32_t)pairs[2 * i + 1]);
+            return false;
+        }
+        return true;
+    }
+
 private:
+    /* page `from` in use becomes page `to`, which is free */
+    void relocate(uint32_t from, uint32_t to) {
+        take(to);
+        give(from);
+        std::swap(holders_[to], holders_[from]);
+    }
     /* the lowest free page; there is one */
     uint32_t lowest() {
         while (free_[low_] == 0)

@@ -1819,6 +1819,12 @@ int pk_hip_pool_compact(pk_hip_pool *pool, int32_t *pairs, uint32_t cap, uint32_
     return PK_HIP_OK;
 }
 
+int pk_hip_pool_restore(pk_hip_pool *pool, const int32_t *pairs, uint32_t n) {
+    if (!pool || (n && !pairs) || !pool->pages.restore(pairs, n))
+        return fail(PK_HIP_EINVAL, "pool_restore: the pairs of a compaction, the pages that it freed still free");
+    return PK_HIP_OK;
+}
+
 int pk_hip_empty_dev(void *stream) {
     int e = pk_hip_init();
     if (e)

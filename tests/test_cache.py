@@ -508,3 +508,90 @@ def test_windows_reach_the_first_frame(layout):
         assert (rows, ln, total) == (T, n, min(n + T, cap))
         assert layout.t_lo(ln + t1, most) == 0 and layout.t_lo(ln + t1, left) == max(0, ln + t1 - left)
         assert lo == left - (ln + t1) and hi == left + total - 1 - (ln + t0)
+
+
+class _Fails(_Moves):
+    """Stands for a cache that refuses every move (its device is not the current
+    one), or the launch of one."""
+    def __init__(self, pages, where):
+        super().__init__(pages)
+        self.where = where
+
+    def move(self, pairs, table=None, source=None, stream=None):
+        if pairs or self.where == "device":
+            raise RuntimeError(self.where)
+
+
+@pytest.mark.parametrize("where", ["device", "launch"])
+@pytest.mark.parametrize("most", [None, 1])
+def test_compact_that_fails_leaves_the_pool(where, most):
+    """Pages whose copy is refused stay their streams': the counts are as they were
+    and the next pages given out are others."""
+    import libpktito_amd as pk
+    p = pk.PagePool(200)
+    held = p.alloc(150)
+    p.share([149, 149, 100])
+    p.release([i for i in held if i not in (100, 130, 149, 3)])
+    before = [p.holders(i) for i in range(200)]
+    with pytest.raises(RuntimeError):
+        p.compact(_Fails(200, where), None, most)
+    assert [p.holders(i) for i in range(200)] == before and p.free_pages == 196
+    assert p.alloc(5) == [0, 1, 2, 4, 5]
+
+
+def test_compact_on_another_device_leaves_the_pool(monkeypatch):
+    """The current device is another than the cache's: refused with nothing moved."""
+    import torch
+    import libpktito_amd as pk
+    cache, _ = _wrapped(pk, torch)
+    monkeypatch.setattr(pk, "_device", lambda: 1)
+    p = pk.PagePool(8)
+    p.release(p.alloc(5)[:3])
+    with pytest.raises(pk.PkHipError) as e:
+        p.compact(cache, _Device(torch.int32, 2, 4))
+    assert e.value.code == pk.PK_HIP_EINVAL
+    assert [p.holders(i) for i in range(8)] == [0, 0, 0, 1, 1, 0, 0, 0] and p.alloc(1) == [0]
+
+
+def test_pool_restore():
+    """A compaction undone: all of it or its last pairs, in any state of the other
+    pages; refused, with nothing changed, where it is not undone so."""
+    import libpktito_amd as pk
+    l = pk.lib()
+    r = random.Random(7)
+
+    def restore(p, pairs):
+        flat = (ctypes.c_int32 * max(1, 2 * len(pairs)))(*[i for pair in pairs for i in pair])
+        return l.pk_hip_pool_restore(p.handle, flat, len(pairs))
+
+    for pages in (1, 5, 64, 130):
+        for _ in range(60):
+            p = pk.PagePool(pages)
+            held = p.alloc(r.randint(0, pages))
+            p.share(r.choices(held, k=3) if held else [])
+            for i in held:
+                if r.random() < 0.5:
+                    p.release([i] * p.holders(i))
+            counts = lambda: [p.holders(i) for i in range(pages)]
+            before, free = counts(), p.free_pages
+            pairs = (ctypes.c_int32 * (2 * pages))()
+            n = ctypes.c_uint32()
+            assert l.pk_hip_pool_compact(p.handle, pairs, pages, ctypes.byref(n)) == 0
+            moves = [(pairs[2 * i], pairs[2 * i + 1]) for i in range(n.value)]
+            after = counts()
+            if moves:
+                f, t = moves[0]
+                for bad in ([(f, f)], [(t, f)], [(f, pages)], [(pages, t)], [(-1, t)], moves + [(f, t)], moves[:1] * 2):
+                    assert restore(p, bad) == pk.PK_HIP_EINVAL and counts() == after and p.free_pages == free
+            assert restore(p, []) == pk.PK_HIP_OK and counts() == after
+            assert restore(p, moves) == pk.PK_HIP_OK and counts() == before and p.free_pages == free
+            if free:                            # the lowest free page is found again
+                assert p.alloc(1) == [before.index(0)]
+    p = pk.PagePool(4)
+    p.release([p.alloc(3)[0]])
+    pairs, n = (ctypes.c_int32 * 8)(), ctypes.c_uint32()
+    l.pk_hip_pool_compact(p.handle, pairs, 4, ctypes.byref(n))
+    assert n.value == 1 and p.alloc(1) == [pairs[0]]        # given out since
+    assert restore(p, [(pairs[0], pairs[1])]) == pk.PK_HIP_EINVAL and p.free_pages == 1
+    assert l.pk_hip_pool_restore(None, pairs, 1) == pk.PK_HIP_EINVAL
+    assert l.pk_hip_pool_restore(p.handle, None, 1) == pk.PK_HIP_EINVAL
