@@ -327,8 +327,7 @@ struct CacheAttention {
     const float *p, *bias_u, *bias_w;
     float *place;                           /* the position scores, [rows][H][place_stride(bw)] */
     uint32_t bw;
-    void *halved;                           /* the table's operands, [H][tiles of 16][steps][2][64 lanes], and its exponents */
-    int32_t *halved_expo;
+    void *pieces;                           /* the table cut beforehand, [H][tiles of 16][steps][3][64 lanes] of 16 bytes */
     /* a stream's tiles of rows a kept head, workgroups that share a tile's pages, what they leave each other */
     uint32_t tiles, splits;
     float *parts;
@@ -338,52 +337,35 @@ __device__ __forceinline__ uint64_t unit_of(const CacheAttention &a, uint32_t b,
     return ((uint64_t)b * a.tiles + tile) * a.G + g;
 }
 
-/* A row of floats cut in two float16 for a product of floats with floats: times
- * the power of two that puts the row's largest magnitude into [2^14, 2^15),
- * its nearest float16 and the nearest of what is left, so that every value is
- * kept to 2^-22 of itself, or of 2^-17 of the row's largest where that is more
- * (float16's own last places). Three products of pieces are taken, and the
- * exponents of both rows put back at the end. */
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-struct Halves {
-    v8h hi, lo;
-};
-
-/* the exponent e with 2^e <= top < 2^(e + 1), kept where 2^(14 - e) is a normal number (0 for a row of zeros, or
- * with a NaN or an infinity, which its products then are too) */
-__device__ __forceinline__ int row_exponent(uint32_t top_bits) {
-    const int e = (int)(top_bits >> 23) - 127;
-    return e == 128 || top_bits == 0 ? 0 : max(e, -112);
-}
-
-/* the largest magnitude, NaNs passed over (they are in the pieces) */
-__device__ __forceinline__ float largest(const float (&x)[8]) {
-    float m = fmaxf(fabsf(x[0]), fabsf(x[1]));
+/* Floats cut for a product of floats with floats: each piece the nearest
+ * bfloat16 of what the ones before leave, so that the second is at most 2^-8
+ * of the float's power of two, the third 2^-17, and the three sum to it exactly
+ * (down to 2^-126, where pieces end). Of the nine products of two floats'
+ * pieces the six largest are taken: those left out are 2^-24 of the product at
+ * most, as much as a 32-bit product's own rounding. Whatever the other
+ * dimensions hold: a row has no exponent in common. */
+__device__ __forceinline__ Pieces cut_near(const float (&x)[8]) {
+    Pieces r;
+    uint32_t w[3][4];
 #pragma unroll
-    for (int i = 2; i < 8; i++)
-        m = fmaxf(m, fabsf(x[i]));
-    return m;
-}
-
-__device__ __forceinline__ Halves halve(const float (&x)[8], int e) {
-    const float s = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-    Halves r;
+    for (int i = 0; i < 4; i++) {
+        v2f_c a = { x[2 * i], x[2 * i + 1] };
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float v = x[i] * s;
-        r.hi[i] = (_Float16)v;
-        r.lo[i] = (_Float16)(v - (float)r.hi[i]);
+        for (int n = 0; n < 3; n++) {
+            w[n][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(a, v2bf));
+            a.x -= __uint_as_float(w[n][i] << 16);
+            a.y -= __uint_as_float(w[n][i] & 0xffff0000u);
+        }
     }
+#pragma unroll
+    for (int n = 0; n < 3; n++)
+        r.p[n] = __builtin_bit_cast(v8bf, v4u{ w[n][0], w[n][1], w[n][2], w[n][3] });
     return r;
-}
-
-__device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
 /* Sixteen rows of the positions' table for one head as the matrix
  * instruction's operand: lane l has dimensions 32 s + 8 (l / 16) of row l % 16
- * in step s, and that row's exponent. */
+ * in step s. */
 template <int NS>
 struct PlaceTile {
     v4f p[NS][2];
@@ -396,44 +378,33 @@ struct PlaceTile {
             p[s][0] = src[8 * s], p[s][1] = src[8 * s + 1];
     }
 
-    __device__ __forceinline__ int halves(Halves (&out)[NS]) const {
-        float x[NS][8], most = 0.0f;
+    __device__ __forceinline__ void pieces(Pieces (&out)[NS]) const {
 #pragma unroll
         for (int s = 0; s < NS; s++) {
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                x[s][j] = p[s][j / 4][j % 4];
-            most = fmaxf(most, largest(x[s]));
+            const float x[8] = { p[s][0][0], p[s][0][1], p[s][0][2], p[s][0][3], p[s][1][0], p[s][1][1], p[s][1][2], p[s][1][3] };
+            out[s] = cut_near(x);
         }
-        int top = mag_bits(most);
-        top = max(top, __shfl_xor(top, 16));
-        top = max(top, __shfl_xor(top, 32));
-        const int e = row_exponent((uint32_t)top);
-#pragma unroll
-        for (int s = 0; s < NS; s++)
-            out[s] = halve(x[s], e);
-        return e;
     }
 };
 
-/* The table halved once for a call whose rows would do it many times over: a
- * wave a tile of a head, its operands 1 KB in a row each, then the exponents. */
+/* The table cut once for a call whose rows would do it many times over: a wave
+ * a tile of a head, its operands 1 KB in a row each. */
 template <int NS>
-__global__ __launch_bounds__(256) void cache_halve_kernel(CacheAttention a) {
+__global__ __launch_bounds__(256) void cache_cut_kernel(CacheAttention a) {
     const uint32_t tiles = (a.bw + 15) / 16, lane = threadIdx.x & 63;
     const uint32_t h = blockIdx.y, tile = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (tile >= tiles)
         return;
     PlaceTile<NS> t;
     t.load(a, h, 16 * tile);
-    Halves ph[NS];
-    const int e = t.halves(ph);
-    v8h *to = (v8h *)a.halved + ((uint64_t)h * tiles + tile) * (NS * 2 * 64) + lane;
+    Pieces ph[NS];
+    t.pieces(ph);
+    v8bf *to = (v8bf *)a.pieces + ((uint64_t)h * tiles + tile) * (NS * 3 * 64) + lane;
 #pragma unroll
     for (int s = 0; s < NS; s++)
-        to[128 * s] = ph[s].hi, to[128 * s + 64] = ph[s].lo;
-    if (lane < 16)
-        a.halved_expo[((uint64_t)h * tiles + tile) * 16 + lane] = e;
+#pragma unroll
+        for (int n = 0; n < 3; n++)
+            to[64 * (3 * s + n)] = ph[s].p[n];
 }
 
 /* The maximum over the wave, in every lane (all of them active). */
@@ -451,27 +422,35 @@ __device__ __forceinline__ int wave_max(int v) {
  * of 2), of every row at every distance that it needs, into the workspace:
  * the same rows of p serve every stream, so this is one product of all rows by
  * the table, read once, where the attention reads its own stream's pages only.
- * A workgroup of W waves takes 16 RT rows of a head, halved into the matrix
- * instruction's operands in LDS, and walks `steps` runs of 16 MT W distances;
- * a wave takes MT tiles of 16 of each, so that an operand read from LDS serves
- * MT. PRE: the table's rows come halved.
+ * A workgroup of four waves takes 16 RT rows of a head, cut into the matrix
+ * instruction's operands in LDS, and walks `steps` runs of 64 MT distances; a
+ * wave takes MT tiles of 16 of each, so that an operand read from LDS serves
+ * MT. PRE: the table's rows come cut.
  *
- * At 2624 rows by up to 3750 distances it takes 91 us (and the halving 10) for
- * 280 MB of scores: 57 without its stores, which is its operands' and
- * instructions' latency (the matrix cores are busy a third of it), the stores
- * on top at the rate that memory takes them. At 256 rows by 4500 it takes 28
- * us, and at few rows a chain of two memory round trips and a launch, 4.5.
+ * At 2624 rows by up to 3750 distances it takes 121 us, 110 at best (and the
+ * cutting 11), for 280 MB of scores: its products alone take 94 at the 1134
+ * TFLOP/s that a bfloat16 product of 8192 cubed reaches here. Of two float16
+ * pieces with an exponent a row three products do, in 97 us, but what is small
+ * beside its row's largest loses its bits. At 256 rows by 4500 it takes 28 us,
+ * and at few rows a chain of two memory round trips and a launch, 7. The
+ * shapes of a workgroup are within a few us of each other: 8 waves, 128 rows
+ * and two tiles a wave 132 us, three tiles 126, 96 rows and 6 waves 147.
  * Measured and taken back: a lane's four scores stored at the frames' own
  * places (16 bytes at any multiple of 4: each step twice as long), one float a
- * lane stored there (as long as now, and the attention no faster), the next
- * step's rows loaded ahead (registers: 12 -> 15 us at 128 rows by 751), and
- * six products of three bfloat16 pieces (14 -> 16 us there, 142 at 2624 rows
- * without the halving apart, against 124). */
-template <int NS, int RT, int W, int MT, bool PRE>
-__global__ __launch_bounds__(64 * W, 4) void cache_place_kernel(CacheAttention a, int32_t steps) {
+ * lane stored there (as long as now, and the attention no faster), stores
+ * through the caches (the attention of 256 streams 171 -> 190 us). */
+
+/* waves a SIMD: registers for three where a wave keeps two tiles of the table, as
+ * LDS has room for (48 KB a workgroup of 64 rows of 128) */
+constexpr int kPlaceWaves = 4;
+constexpr int place_residency(int MT) { return MT == 1 ? 4 : 3; }
+
+template <int NS, int RT, int MT, bool PRE>
+__global__ __launch_bounds__(64 * kPlaceWaves, place_residency(MT)) void cache_place_kernel(CacheAttention a, int32_t steps) {
+    constexpr int W = kPlaceWaves;
     constexpr int kRows = 16 * RT, kRun = 16 * MT * W, kThreads = 64 * W, kFill = kRows * 16 / kThreads;
-    __shared__ v8h frag[RT][NS][2][64];
-    __shared__ int32_t need[W][2], expo[kRows];
+    __shared__ v8bf frag[RT][NS][3][64];
+    __shared__ int32_t need[W][2];
     const uint32_t h = blockIdx.y, n0 = blockIdx.z * kRows;
     const int32_t x0 = (int32_t)blockIdx.x * (kRun * steps), x1 = min(x0 + kRun * steps, (int32_t)a.bw);
     const uint32_t dk = 32 * NS, stride = place_stride(a.bw);
@@ -511,14 +490,12 @@ __global__ __launch_bounds__(64 * W, 4) void cache_place_kernel(CacheAttention a
 #pragma unroll
         for (int j = 0; j < 8; j++)
             x[j] = (qv[i][j / 4][j % 4] + bias[j / 4][j % 4]) * c2;
-        const int e = row_exponent((uint32_t)group_max_nonneg<16>(mag_bits(largest(x))));
-        const Halves c = halve(x, e);
+        const Pieces c = cut_near(x);
         if (part < 4 * NS) {                /* a row's parts in different banks */
-            frag[row / 16][part / 4][0][16 * (part % 4) + (row % 16 ^ part)] = c.hi;
-            frag[row / 16][part / 4][1][16 * (part % 4) + (row % 16 ^ part)] = c.lo;
+#pragma unroll
+            for (int n = 0; n < 3; n++)
+                frag[row / 16][part / 4][n][16 * (part % 4) + (row % 16 ^ part)] = c.p[n];
         }
-        if (part == 0)
-            expo[row] = e;
     }
     __syncthreads();
     int32_t from = need[0][0], to = need[0][1];
@@ -529,19 +506,18 @@ __global__ __launch_bounds__(64 * W, 4) void cache_place_kernel(CacheAttention a
     for (int32_t x = x0 + 16 * MT * (int32_t)wave; x < x1 && x <= to; x += kRun) {
         if (from >= x + 16 * MT)
             continue;
-        Halves ph[MT][NS];
-        int pe[MT][4];
+        Pieces ph[MT][NS];
         if constexpr (PRE) {
             const uint32_t tiles = (a.bw + 15) / 16;
 #pragma unroll
             for (int i = 0; i < MT; i++) {
                 const uint32_t tile = min((uint32_t)x / 16 + i, tiles - 1);
-                const v8h *src = (const v8h *)a.halved + ((uint64_t)h * tiles + tile) * (NS * 2 * 64) + lane;
+                const v8bf *src = (const v8bf *)a.pieces + ((uint64_t)h * tiles + tile) * (NS * 3 * 64) + lane;
 #pragma unroll
                 for (int s = 0; s < NS; s++)
-                    ph[i][s].hi = src[128 * s], ph[i][s].lo = src[128 * s + 64];
-                const int4 e = *(const int4 *)(a.halved_expo + ((uint64_t)h * tiles + tile) * 16 + 4 * w);
-                pe[i][0] = e.x, pe[i][1] = e.y, pe[i][2] = e.z, pe[i][3] = e.w;
+#pragma unroll
+                    for (int n = 0; n < 3; n++)
+                        ph[i][s].p[n] = src[64 * (3 * s + n)];
             }
         } else {
             PlaceTile<NS> t[MT];
@@ -549,12 +525,8 @@ __global__ __launch_bounds__(64 * W, 4) void cache_place_kernel(CacheAttention a
             for (int i = 0; i < MT; i++)
                 t[i].load(a, h, (uint32_t)x + 16 * i);
 #pragma unroll
-            for (int i = 0; i < MT; i++) {
-                const int e = t[i].halves(ph[i]);
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    pe[i][r] = __shfl(e, 4 * w + r);
-            }
+            for (int i = 0; i < MT; i++)
+                t[i].pieces(ph[i]);
         }
 #pragma unroll 1
         for (uint32_t rt = 0; 16 * rt < rows; rt++) {
@@ -562,26 +534,32 @@ __global__ __launch_bounds__(64 * W, 4) void cache_place_kernel(CacheAttention a
 #pragma unroll
             for (int s = 0; s < NS; s++) {
                 const uint32_t at = 16 * w + (lane % 16 ^ (4 * s + w));
-                const v8h qh = frag[rt][s][0][at], ql = frag[rt][s][1][at];
+                const v8bf q0 = frag[rt][s][0][at], q1 = frag[rt][s][1][at], q2 = frag[rt][s][2][at];
 #pragma unroll
-                for (int i = 0; i < MT; i++) {
-                    acc[i] = mfma(ph[i][s].lo, qh, acc[i]);
-                    acc[i] = mfma(ph[i][s].hi, ql, acc[i]);
-                    acc[i] = mfma(ph[i][s].hi, qh, acc[i]);
-                }
+                for (int i = 0; i < MT; i++)
+                    acc[i] = mfma(ph[i][s].p[2], q0, acc[i]);
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+                    acc[i] = mfma(ph[i][s].p[1], q1, acc[i]);
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+                    acc[i] = mfma(ph[i][s].p[0], q2, acc[i]);
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+                    acc[i] = mfma(ph[i][s].p[1], q0, acc[i]);
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+                    acc[i] = mfma(ph[i][s].p[0], q1, acc[i]);
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+                    acc[i] = mfma(ph[i][s].p[0], q0, acc[i]);
             }
             const uint32_t row = 16 * rt + lane % 16;
-            const int qe = expo[row];
             float *to_row = a.place + ((uint64_t)(n0 + row) * a.H + h) * stride + kPlacePad + x + 4 * w;
             if (row < rows) {
 #pragma unroll
-                for (int i = 0; i < MT; i++) {
-                    v4f y;
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        y[r] = __builtin_ldexpf(acc[i][r], pe[i][r] + qe - 28);
-                    __builtin_nontemporal_store(y, (v4f *)(to_row + 16 * i));
-                }
+                for (int i = 0; i < MT; i++)
+                    __builtin_nontemporal_store(acc[i], (v4f *)(to_row + 16 * i));
             }
         }
     }
@@ -1286,10 +1264,10 @@ struct Deal {
 };
 
 /* A row's position scores are made where they are used for single rows of few
- * streams with a narrow window: a launch fewer. One row by 71 distances takes
- * 7.2 us so and 8.9 with a launch of their own, by 181 10.0 and 9.0; 16 rows
- * by 71 7.3 and 9.1, 64 rows 13.6 and 10.6 (each stream reads the table
- * itself, in pieces of 16 bytes). */
+ * streams with a narrow window: a launch fewer. A call of one row by 71
+ * distances takes 7.7 us so and 10.0 with a launch of their own, by 181 11.5 and
+ * 11.7; 16 rows by 71 8.0 and 9.8, by 181 12.1 and 11.6; 64 rows by 71 14.3 and
+ * 12.4 (each stream reads the table itself, in pieces of 16 bytes). */
 static Deal deal(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, int32_t left, int32_t right) {
     Deal d;
     const uint32_t rows = st.max_T * (H / G);
@@ -1310,25 +1288,27 @@ static Deal deal(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, in
     return d;
 }
 
-/* From this many rows on, the position scores are made of a table halved
- * beforehand, 128 rows a workgroup: with 2624 rows by 3750 distances 10 + 91
- * us, without 128; with 384 by 767 4 + 8, without 12. */
-static bool place_halved(uint32_t rows) { return rows >= 512; }
+/* From this many scores a head on, the position scores are made of a table cut
+ * beforehand: a launch more, and 64 rows' share of the cutting less for each 64
+ * rows. Whole calls of 8 heads of 128 with it and without: 2624 rows by 3750
+ * distances 260 and 267 us, 1000 by 3450 105 and 117, 1920 by 2280 134 and 152;
+ * 1000 by 2300 56 and 52, 600 by 2600 67 and 64, 600 by 1500 38 and 36. */
+static bool place_cut(uint32_t rows, uint32_t bw) { return (uint64_t)rows * bw >= 2600000; }
 
-static size_t halved_bytes(uint32_t H, uint32_t bw, uint32_t dk) {
-    return (size_t)H * ((bw + 15) / 16) * 16 * (4 * dk + 4);
+static size_t pieces_bytes(uint32_t H, uint32_t bw, uint32_t dk) {
+    return (size_t)H * ((bw + 15) / 16) * 16 * (6 * dk);
 }
 
 /* The workspace's parts, in bytes, one after another (each a multiple of 16). */
 struct Space {
-    size_t place, halved, parts;
+    size_t place, pieces, parts;
 };
 
 static Space space(const CacheStreams &st, uint32_t H, uint32_t dk, bool positions, uint32_t bw, const Deal &d) {
     Space s = { 0, 0, 0 };
     if (positions && !d.own) {
         s.place = (size_t)st.rows * H * place_stride(bw) * sizeof(float);
-        s.halved = place_halved(st.rows) ? halved_bytes(H, bw, dk) : 0;
+        s.pieces = place_cut(st.rows, bw) ? pieces_bytes(H, bw, dk) : 0;
     }
     if (d.splits > 1)
         s.parts = (size_t)d.units * d.splits * d.rows * (dk + 2) * sizeof(float);
@@ -1338,7 +1318,7 @@ static Space space(const CacheStreams &st, uint32_t H, uint32_t dk, bool positio
 size_t cache_attention_workspace(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, bool positions,
                                  int32_t left, int32_t right) {
     const Space s = space(st, H, dk, positions, (uint32_t)left + (uint32_t)right + 1, deal(st, G, H, dk, left, right));
-    return s.place + s.halved + s.parts;
+    return s.place + s.pieces + s.parts;
 }
 
 bool cache_attention_fits(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, int32_t left, int32_t right) {
@@ -1346,32 +1326,34 @@ bool cache_attention_fits(const CacheStreams &st, uint32_t G, uint32_t H, uint32
     return d.units <= kMostGroups / d.splits && ((uint32_t)left + (uint32_t)right) / 64 < kMostGroups;
 }
 
-template <int NS, int RT, int W, int MT, bool PRE>
+template <int NS, int RT, int MT, bool PRE>
 static void place(const CacheAttention &a, hipStream_t s) {
-    /* Two runs one after another in a workgroup, whose rows' operands are then made once for both, where that takes
-     * fewer steps in a row over the rounds of workgroups that the chip holds, those operands counted as a step (36 runs
-     * by 32: in one round of two steps 28 us, in two of one 33; 2624 rows by 3750 in steps of one, two and five 97, 92
-     * and 103: lengths differ, and longer steps even them out less). */
-    constexpr uint32_t kRun = 16 * MT * W, kHeld = 256 * 16 / W;
+    /* Runs one after another in a workgroup, whose rows' operands are then made once for all of them, as many as take the
+     * fewest steps in a row over the rounds of workgroups that the chip holds, those operands counted as a step (2624
+     * rows by 3750: 154 us with one run, 134 with two, 125 with five, which it takes; 160 rows by 900: 8.7 with one,
+     * which it takes, 11.9 with two, 21.0 with five). */
+    constexpr uint32_t kRun = 16 * MT * kPlaceWaves, kHeld = 256 * 4 * place_residency(MT) / kPlaceWaves;
     const uint32_t runs = (a.bw + kRun - 1) / kRun, blocks = (a.st.rows + 16 * RT - 1) / (16 * RT);
     auto rounds = [&](uint32_t n) { return ((uint64_t)((runs + n - 1) / n) * a.H * blocks + kHeld - 1) / kHeld * (n + 1); };
-    const uint32_t steps = rounds(2) < rounds(1) ? 2 : 1;
-    cache_place_kernel<NS, RT, W, MT, PRE><<<dim3((runs + steps - 1) / steps, a.H, blocks), 64 * W, 0, s>>>(a, (int32_t)steps);
+    uint32_t steps = 1;
+    for (uint32_t n = 2; n <= 8; n++)
+        steps = rounds(n) < rounds(steps) ? n : steps;
+    cache_place_kernel<NS, RT, MT, PRE><<<dim3((runs + steps - 1) / steps, a.H, blocks), 64 * kPlaceWaves, 0, s>>>(a, (int32_t)steps);
 }
 
 template <int NS>
 static void attend(const CacheAttention &a, const Deal &d, hipStream_t s) {
     if (a.p && !d.own) {
-        if (place_halved(a.st.rows)) {
-            cache_halve_kernel<NS><<<dim3(((a.bw + 15) / 16 + 3) / 4, a.H), 256, 0, s>>>(a);
-            place<NS, 8, 8, 2, true>(a, s);
+        if (place_cut(a.st.rows, a.bw)) {
+            cache_cut_kernel<NS><<<dim3(((a.bw + 15) / 16 + 3) / 4, a.H), 256, 0, s>>>(a);
+            place<NS, 4, 2, true>(a, s);
         } else if (a.st.rows <= 16 || (uint64_t)((a.st.rows + 15) / 16) * ((a.bw + 15) / 16) * a.H <= 4096) {
             /* up to four tiles of 16 by 16 a SIMD: one workgroup's pass from the table's rows to the last store is what
-             * takes time, and 16 rows have the shortest (128 rows by 751 distances 8.1 us, with 64 rows 10.7; 256 by
-             * 4500 58 and 30) */
-            place<NS, 1, 4, 1, false>(a, s);
+             * takes time, and 16 rows have the shortest (128 rows by 751 distances 7.4 us, with 64 rows 8.4; 256 by
+             * 4500 47 and 29) */
+            place<NS, 1, 1, false>(a, s);
         } else {
-            place<NS, 4, 4, 2, false>(a, s);
+            place<NS, 4, 2, false>(a, s);
         }
     }
     const uint32_t grid = (uint32_t)(d.units * d.splits);
@@ -1407,9 +1389,8 @@ int launch_cache_attention(const CacheAttentionCall &c, hipStream_t s) {
     a.tiles = d.tiles, a.splits = d.splits;
     const Space sp = space(c.st, c.H, c.dk, c.p != nullptr, a.bw, d);
     a.place = (float *)c.ws;
-    a.halved = (char *)c.ws + sp.place;
-    a.halved_expo = (int32_t *)((char *)a.halved + (size_t)c.H * ((a.bw + 15) / 16) * 16 * 4 * c.dk);
-    a.parts = (float *)((char *)c.ws + sp.place + sp.halved);
+    a.pieces = (char *)c.ws + sp.place;
+    a.parts = (float *)((char *)c.ws + sp.place + sp.pieces);
     switch (c.dk / 32) {
     case 1: attend<1>(a, d, s); break;
     case 2: attend<2>(a, d, s); break;

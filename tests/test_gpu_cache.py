@@ -818,3 +818,101 @@ def test_any_call_past_the_table(hip, torch, seed):
     left, right = (r.choice([None, None, 0, 64 * max_pages, r.randint(0, 400)]) for _ in range(2))
     pos = w.positions(H, r.choice([64 * max_pages, 300, 40]), r.choice([70, 2])) if r.random() < 0.6 else None
     w.check(H, pos, left, right)
+
+
+# ----------------------------------------- position scores' precision --
+
+SHAPES = [                                      # lens, Ts, dk, the window: each way that position scores are made
+    ([90], [1], 64, 70),                        # where they are used
+    ([60 + b for b in range(17)], [1] * 17, 64, 70),
+    ([100, 7], [3, 20], 128, None),             # 16 rows a workgroup
+    ([1300, 900], [150, 20], 32, None),         # many distances, more rows a workgroup
+    ([40, 0], [300, 240], 96, None),
+    ([60], [1200], 32, None),                   # the table cut beforehand
+]
+
+
+@pytest.mark.parametrize("lens,Ts,dk,left", SHAPES, ids=str)
+@pytest.mark.parametrize("wide", ["queries", "positions", "both"])
+@pytest.mark.parametrize("ratio", [1e4, 1e6, 1e12])
+def test_position_scores_of_wide_rows(hip, torch, lens, Ts, dk, left, wide, ratio):
+    """Rows of queries and of the table that are far larger in one dimension than
+    in the others, where the other factor (and the keys) have a zero: the score is
+    the small dimensions', and is held as a 32-bit sum holds it."""
+    say("wide rows", lens, Ts, dk, left, wide, ratio)
+    w = World(hip, torch, lens, Ts, 1, dk, seed=60)
+    big = 5
+    std = w.g.standard_normal
+    for b in range(len(lens)):
+        for f in range(lens[b] + Ts[b]):
+            k, v = std((2, dk)).astype(np.float32)
+            k[big] = k[big + 1] = 0
+            w.pool.write(0, w.table[b, f // 64], f % 64, 1e-3 * k, v)
+    w.upload()
+    far = max(a + t for a, t in zip(lens, Ts))
+    p, c, u, b = w.positions(1, far, max(Ts))
+    q = std((w.rows, dk)).astype(np.float32)
+    u, b = 0 * u, (0.1 * b).astype(np.float32)
+    q[:, big:big + 2], b[big:big + 2], p[:, big:big + 2] = 0, 0, 0
+    if wide != "positions":                     # queries: the rest by ratio smaller, the table by as much larger
+        q[:, big] = ratio * (1 + np.abs(std(w.rows)))
+    if wide != "queries":
+        p[:, big + 1] = ratio * (1 + np.abs(std(len(p))))
+    if wide == "queries":
+        q /= np.float32(ratio)
+        b = (b / np.float32(ratio)).astype(np.float32)
+        p = (p * np.float32(ratio)).astype(np.float32)
+    elif wide == "positions":
+        p /= np.float32(ratio)
+        q, b = (q * np.float32(ratio)).astype(np.float32), (b * np.float32(ratio)).astype(np.float32)
+        # content: keys in proportion, or the products of the larger queries would be all there is
+        w.pool.data[..., 64 * dk:64 * dk + 128] = 0
+        w.upload()
+    w.check(1, (p, c, u, b), left, q=q)
+
+
+@pytest.mark.parametrize("lens,Ts,dk,left", SHAPES, ids=str)
+def test_position_scores_of_one_dimension(hip, torch, lens, Ts, dk, left):
+    """Queries with one dimension set, no content scores: a position score is one
+    product. Relative to it the scale to powers of two is off by three roundings
+    (its factors' and its own), the scaled query by one, the product by one (two
+    where pieces make it: what is left out of them, and their sum, which may cut
+    where it should round), the exponential's argument by two: 10 of 2^-24 of the
+    largest score at most, twice for the maximum's. Each row's largest scores are
+    of one, so that what the exponentials and the output's sums add (a page's
+    rescaling, n terms) is the rest."""
+    say("one dimension", lens, Ts, dk, left)
+    w = World(hip, torch, lens, Ts, 1, dk, seed=61)
+    std = w.g.standard_normal
+    for b in range(len(lens)):
+        for f in range(lens[b] + Ts[b]):
+            w.pool.write(0, w.table[b, f // 64], f % 64, np.zeros(dk, np.float32), std(dk).astype(np.float32))
+    w.upload()
+    far = max(a + t for a, t in zip(lens, Ts))
+    p, c, u, b = w.positions(1, far, max(Ts))
+    q = np.zeros((w.rows, dk), np.float32)
+    at = np.arange(w.rows) % dk
+    q[np.arange(w.rows), at] = 2 * std(w.rows) * np.sqrt(dk)
+    got = w.attend(q, 1, (p, c, 0 * u, 0 * b), left)
+    for s in range(len(lens)):
+        total = lens[s] + Ts[s]
+        v = np.concatenate([w.pool.read(0, w.table[s, i], 0)[1] for i in range(-(-total // 64))])[:total]
+        for t in range(Ts[s]):
+            row, pos = w.row0[s] + t, lens[s] + t
+            j = np.arange(max(0, pos - left) if left is not None else 0, total)
+            x = p[c - pos + j, at[row]].astype(np.float64) * float(q[row, at[row]]) / np.sqrt(dk)
+            e = np.exp(x - x.max())
+            want = e @ v[j] / e.sum()
+            tol = (2 * 10 * (np.abs(x).max() + 1) + 2 * (3 * len(j) + 4 * (len(j) // 64 + 8))) * 2.0 ** -24
+            assert (np.abs(got[row] - want) <= tol * 2 * (e @ np.abs(v[j])) / e.sum()).all(), (s, t)
+
+
+@pytest.mark.parametrize("dk,H,G", [(32, 1, 1), (64, 2, 1), (96, 2, 2), (128, 1, 1)])
+@pytest.mark.parametrize("left", [None, 1000])
+def test_table_cut_beforehand(hip, torch, dk, H, G, left):
+    """Rows and distances enough for the table's pieces to be made once, the last
+    block of rows and the last run of distances in part."""
+    say("cut beforehand", dk, H, G, left)
+    w = World(hip, torch, [60, 3], [1201, 24], G, dk, seed=62, first=2, tail=1)
+    w.fill()
+    w.check(H, w.positions(H, 1270, 1201), left)
