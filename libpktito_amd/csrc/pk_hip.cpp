@@ -1735,27 +1735,29 @@ int pk_hip_cache_move_dev(const pk_hip_cache *dst, const pk_hip_cache *src, cons
         return fail(PK_HIP_EINVAL, "cache_move_dev: pairs set, and a table only where src and dst are one cache");
     if (n > dst->pages)
         return fail(PK_HIP_EINVAL, "cache_move_dev: %u pairs onto %u pages: one is copied to twice", n, dst->pages);
+    for (uint32_t i = 0; i < n; i++)
+        if ((uint32_t)pairs[2 * i] >= src->pages || (uint32_t)pairs[2 * i + 1] >= dst->pages)
+            return fail(PK_HIP_EINVAL, "cache_move_dev: pair %u is pages %d and %d, of %u and %u", i, pairs[2 * i],
+                        pairs[2 * i + 1], src->pages, dst->pages);
     try {
-        /* bit 0: copied to, bit 1: copied from (of src, which is dst where it matters) */
-        std::vector<uint8_t> seen(same ? src->pages : std::max(src->pages, dst->pages), 0);
-        for (uint32_t i = 0; i < n; i++) {
-            const uint32_t f = (uint32_t)pairs[2 * i], t = (uint32_t)pairs[2 * i + 1];
-            if (f >= src->pages || t >= dst->pages)
-                return fail(PK_HIP_EINVAL, "cache_move_dev: pair %u is pages %d and %d, of %u and %u", i, (int)f, (int)t,
-                            src->pages, dst->pages);
-            if (seen[t] & 1)
-                return fail(PK_HIP_EINVAL, "cache_move_dev: page %u is copied to twice", t);
-            seen[t] |= 1;
-            if (table && (seen[f] & 2))
-                return fail(PK_HIP_EINVAL, "cache_move_dev: page %u moves to two places", f);
-            seen[f] |= 2;
+        std::vector<int32_t> from(n), to(n);
+        for (uint32_t i = 0; i < n; i++)
+            from[i] = pairs[2 * i], to[i] = pairs[2 * i + 1];
+        std::sort(from.begin(), from.end());
+        std::sort(to.begin(), to.end());
+        const auto twice = std::adjacent_find(to.begin(), to.end());
+        if (twice != to.end())
+            return fail(PK_HIP_EINVAL, "cache_move_dev: page %d is copied to twice", *twice);
+        const auto two = table ? std::adjacent_find(from.begin(), from.end()) : from.end();
+        if (two != from.end())
+            return fail(PK_HIP_EINVAL, "cache_move_dev: page %d moves to two places", *two);
+        for (uint32_t i = 0, j = 0; same && i < n && j < n;) {
+            if (from[i] == to[j])
+                return fail(PK_HIP_EINVAL, "cache_move_dev: page %d is copied from and to", from[i]);
+            from[i] < to[j] ? i++ : j++;
         }
-        if (same)
-            for (uint32_t i = 0; i < n; i++)
-                if (seen[(uint32_t)pairs[2 * i]] & 1)
-                    return fail(PK_HIP_EINVAL, "cache_move_dev: page %d is copied from and to", (int)pairs[2 * i]);
     } catch (...) {
-        return fail(PK_HIP_ENOMEM, "cache_move_dev: host memory for %u pages", dst->pages);
+        return fail(PK_HIP_ENOMEM, "cache_move_dev: host memory for %u pairs", n);
     }
     if ((e = pk_hip_init()))
         return e;

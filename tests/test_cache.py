@@ -5,6 +5,7 @@ import ctypes
 import os
 import random
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -595,3 +596,46 @@ def test_pool_restore():
     assert restore(p, [(pairs[0], pairs[1])]) == pk.PK_HIP_EINVAL and p.free_pages == 1
     assert l.pk_hip_pool_restore(None, pairs, 1) == pk.PK_HIP_EINVAL
     assert l.pk_hip_pool_restore(p.handle, None, 1) == pk.PK_HIP_EINVAL
+
+
+def test_move_takes_memory_for_its_pairs():
+    """One page of the largest pool: the host memory that the checks take goes by
+    the pairs, not by the pool (a child process with 256 MB to spare, no device)."""
+    child = """
+import ctypes, resource, sys
+sys.path.insert(0, sys.argv[1])
+import libpktito_amd as pk
+l = pk.lib()
+c = pk.Cache(4096, 1, 1 << 30, 1, 32)
+pairs = (ctypes.c_int32 * 4)((1 << 30) - 1, 5, 7, 6)
+used = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (used + (256 << 20),) * 2)
+for n in (0, 1, 2):
+    e = l.pk_hip_cache_move_dev(ctypes.byref(c), ctypes.byref(c), pairs, n, None, 0, None)
+    print(e, l.pk_hip_last_error().decode())
+    assert e == pk.PK_HIP_ENODEV
+"""
+    r = subprocess.run([sys.executable, "-c", child, ROOT], env=os.environ | {"PKTITO_HIP_DISABLE": "1"},
+                       capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_move_checks_many_pairs():
+    """Pairs in any order, some thousand of them: what is refused is found wherever
+    it is, and nothing else is."""
+    import libpktito_amd as pk
+    r = random.Random(8)
+    n = 3000
+    c = pk.Cache(4096, 1, 2 * n, 1, 32)
+    ids = r.sample(range(2 * n), 2 * n)
+
+    def move(pairs, table=None):
+        flat = (ctypes.c_int32 * (2 * len(pairs)))(*[i for pair in pairs for i in pair])
+        return pk.lib().pk_hip_cache_move_dev(ctypes.byref(c), ctypes.byref(c), flat, len(pairs), table, 16, None)
+
+    good = list(zip(ids[:n], ids[n:]))
+    for i, j in (r.sample(range(n), 2) for _ in range(20)):
+        for bad, table in (((good[j][0], good[i][1]), None), ((good[i][1], good[j][1]), None),
+                           ((good[j][0], good[j][0]), None), ((good[i][0], good[j][1]), 4096)):
+            pairs = good[:j] + [bad] + good[j + 1:]
+            assert move(pairs, table) == pk.PK_HIP_EINVAL, (i, j, bad)
