@@ -868,14 +868,13 @@ class DeviceCache:
         source (this cache by default), to one of this cache; with table, an
         int32 device tensor, its entries that name a page moved follow it
         (pk_hip_cache_move_dev)."""
-        flat = [i for pair in pairs for i in pair]
-        n = len(flat)
-        if n != 2 * len(pairs):
+        if any(len(pair) != 2 for pair in pairs):
             raise PkHipError(PK_HIP_EINVAL, "pairs of pages (from, to)")
+        flat = [i for pair in pairs for i in pair]
         _table(table, self.device)
         source = source or self
         _check(lib().pk_hip_cache_move_dev(ctypes.byref(self.st), ctypes.byref(source.st),
-                                           _page_ids(flat), n // 2, _dptr(table),
+                                           _page_ids(flat), len(pairs), _dptr(table),
                                            table.numel() if table is not None else 0, self._queue(stream, source)))
 
 

@@ -639,3 +639,15 @@ def test_move_checks_many_pairs():
                            ((good[j][0], good[j][0]), None), ((good[i][0], good[j][1]), 4096)):
             pairs = good[:j] + [bad] + good[j + 1:]
             assert move(pairs, table) == pk.PK_HIP_EINVAL, (i, j, bad)
+
+
+def test_pairs_that_are_none_are_refused(monkeypatch):
+    """Each of them two pages, not all of them together."""
+    import torch
+    import libpktito_amd as pk
+    monkeypatch.setattr(pk, "_device", lambda: 0)
+    cache, _ = _wrapped(pk, torch)
+    for pairs in ([(1,), (2, 3, 4)], [(0, 1, 2, 3), ()], [(0,), (1,)], [(0, 1), (2,), (3, 4, 5)]):
+        with pytest.raises(pk.PkHipError) as e:
+            cache.move(pairs, stream=0)
+        assert e.value.code == pk.PK_HIP_EINVAL and "pairs" in str(e.value)
