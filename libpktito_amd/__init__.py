@@ -788,8 +788,9 @@ class DeviceCache:
         _is(data, "uint8", "cache", None)
         for v, what in ((layers, "layers"), (pages, "pages"), (heads, "heads"), (dk, "dk")):
             _u32(v, what)
-        if not data.is_contiguous() or data.numel() < max(1, cache_bytes(layers, pages, heads, dk)):
-            raise PkHipError(PK_HIP_EINVAL, f"cache: {cache_bytes(layers, pages, heads, dk)} contiguous bytes (heads of "
+        need = cache_bytes(layers, pages, heads, dk)
+        if not need or not data.is_contiguous() or data.numel() < need:
+            raise PkHipError(PK_HIP_EINVAL, f"cache: {need} contiguous bytes (0: sizes that are not taken; heads are of "
                                             "32, 64, 96 or 128 dimensions)")
         self.data, self.heads, self.dk, self.device = data, int(heads), int(dk), data.get_device()
         self.st = Cache(data.data_ptr(), layers, pages, heads, dk)

@@ -651,3 +651,14 @@ def test_pairs_that_are_none_are_refused(monkeypatch):
         with pytest.raises(pk.PkHipError) as e:
             cache.move(pairs, stream=0)
         assert e.value.code == pk.PK_HIP_EINVAL and "pairs" in str(e.value)
+
+
+def test_sizes_that_no_call_takes_are_refused_at_once():
+    """Sizes that have no number of bytes, whatever memory is given with them."""
+    import torch
+    import libpktito_amd as pk
+    big = _Device(torch.uint8, 1 << 40)
+    for sizes in ((2, 8, 4, 48), (2, 8, 4, 0), (0, 8, 4, 64), (2, 0, 4, 64), (2, 8, 0, 64), (2, 8, 1025, 64)):
+        with pytest.raises(pk.PkHipError) as e:
+            pk.DeviceCache(big, *sizes)
+        assert e.value.code == pk.PK_HIP_EINVAL
