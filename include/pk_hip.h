@@ -439,12 +439,11 @@ size_t pk_hip_cache_bytes(uint32_t layers, uint32_t pages, uint32_t heads, uint3
  * (rows a stream has beyond max_T or beyond rows take no part). Frames past 64
  * max_pages have no page: they are not kept, and their rows attend those that
  * the table holds; a len past 64 max_pages counts as that. Rows of no stream
- * are left as they were.
- * No two streams of a call may have one row or write one page. max_pages up
- * to 2^24, B up to 65535, rows up to 2^21, and B x max_T x heads what a launch
- * holds (refused otherwise): in a write or read 2^28 pages of all streams and
- * heads, ceil((max_T + 63) / 64) a stream, in an attention 2^24 tiles of their
- * rows. */
+ * are left as they were. No two streams of a call may have one row or write
+ * one page. max_pages 1 to 2^24, B up to 65535 (with none, table and len may be
+ * NULL), rows up to 2^21, and B x max_T x heads what a launch holds (refused
+ * otherwise): in a write or read 2^28 pages of all streams and heads,
+ * ceil((max_T + 63) / 64) a stream, in an attention 2^24 tiles of their rows. */
 typedef struct {
     const int32_t *table, *len, *row0;
     uint32_t B, max_pages, rows, max_T;

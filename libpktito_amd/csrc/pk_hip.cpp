@@ -1561,8 +1561,8 @@ static int check_cache(const pk_hip_cache *c, const char *who) {
 }
 
 static int check_streams(const pk_hip_streams *st, const char *who) {
-    if (!st || !st->table || !st->len || !st->row0 || st->max_pages == 0 || st->max_pages > 1u << 24 || st->B > 65535 ||
-        st->rows > 1u << 21 || st->max_T > st->rows)
+    if (!st || (st->B && (!st->table || !st->len)) || !st->row0 || st->max_pages == 0 || st->max_pages > 1u << 24 ||
+        st->B > 65535 || st->rows > 1u << 21 || st->max_T > st->rows)
         return fail(PK_HIP_EINVAL, "%s: streams with their table, len and row0, 1 to 2^24 pages a stream, up to 65535 "
                                    "streams and 2^21 rows, max_T up to rows", who);
     return PK_HIP_OK;

@@ -662,3 +662,17 @@ def test_sizes_that_no_call_takes_are_refused_at_once():
         with pytest.raises(pk.PkHipError) as e:
             pk.DeviceCache(big, *sizes)
         assert e.value.code == pk.PK_HIP_EINVAL
+
+
+@pytest.mark.parametrize("rows", [0, 5])
+def test_steps_without_streams(rows):
+    """No streams: their table and lengths are empty, which torch gives no address,
+    and there is nothing to do (or no device to do it on)."""
+    import libpktito_amd as pk
+    none = {} if rows else dict(k=None, v=None, o=None, q=None)
+    calls = _calls(pk, B=0, table=None, len=None, rows=rows, max_T=0, **none)
+    for e in ALL:
+        assert calls[e]() in (pk.PK_HIP_OK, pk.PK_HIP_ENODEV), (e, pk.lib().pk_hip_last_error())
+    calls = _calls(pk, B=0, table=None, len=None, row0=None, rows=rows, max_T=0, **none)
+    for e in ALL:
+        assert calls[e]() == pk.PK_HIP_EINVAL

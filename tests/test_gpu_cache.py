@@ -916,3 +916,24 @@ def test_table_cut_beforehand(hip, torch, dk, H, G, left):
     w = World(hip, torch, [60, 3], [1201, 24], G, dk, seed=62, first=2, tail=1)
     w.fill()
     w.check(H, w.positions(H, 1270, 1201), left)
+
+
+def test_step_without_streams(hip, torch):
+    """A step that no stream takes part in: every call returns and nothing moves."""
+    say("no streams")
+    w = World(hip, torch, [10, 20], [1, 2], 2, 64, seed=63)
+    w.fill()
+    before = w.data.clone()
+    z = torch.zeros(0, dtype=torch.int32, device="cuda")
+    for rows in (0, 3):
+        st = hip.CacheStreams(z.reshape(0, 1), z, torch.zeros(1, dtype=torch.int32, device="cuda"), rows, 0)
+        a, o = torch.ones(rows, 128, device="cuda"), torch.full((rows, 256), 7.25, device="cuda")
+        q, p, b = torch.ones(rows, 256, device="cuda"), torch.ones(9, 256, device="cuda"), torch.ones(256, device="cuda")
+        w.cache.append(0, a, a, st)
+        w.cache.read(0, a, a.clone(), st)
+        assert w.cache.attention_workspace(st, 4, None) == 0
+        w.cache.attention(o, 0, q, st, 4, None)
+        ws = torch.empty(max(1, w.cache.attention_workspace(st, 4, (p, 4, b, b))), dtype=torch.uint8, device="cuda")
+        w.cache.attention(o, 0, q, st, 4, ws, (p, 4, b, b))
+        torch.cuda.synchronize()
+        assert (a == 1).all() and (o == 7.25).all() and torch.equal(w.data, before)
