@@ -1323,8 +1323,10 @@ size_t cache_attention_workspace(const CacheStreams &st, uint32_t G, uint32_t H,
 
 bool cache_attention_fits(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, int32_t left, int32_t right) {
     const Deal d = deal(st, G, H, dk, left, right);
-    return d.units <= kMostGroups / d.splits && ((uint32_t)left + (uint32_t)right) / 64 < kMostGroups;
+    return d.units <= kMostGroups / d.splits;
 }
+
+bool cache_places_fit(int32_t left, int32_t right) { return ((uint32_t)left + (uint32_t)right) / 64 < kMostGroups; }
 
 template <int NS, int RT, int MT, bool PRE>
 static void place(const CacheAttention &a, hipStream_t s) {

@@ -1670,6 +1670,8 @@ static int attention_window(const pk_hip_cache *c, const pk_hip_streams *st, uin
     if (!pkq8::cache_attention_fits(streams_of(st), c->heads, H, c->dk, *l, *r))
         return fail(PK_HIP_EINVAL, "%s: %u streams of up to %u rows, %u heads: more than a launch holds", who, st->B,
                     st->max_T, H);
+    if (pos && !pkq8::cache_places_fit(*l, *r))
+        return fail(PK_HIP_EINVAL, "%s: position scores by %u distances: more than a launch holds", who, lo + hi + 1);
     return PK_HIP_OK;
 }
 

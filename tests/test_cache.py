@@ -676,3 +676,16 @@ def test_steps_without_streams(rows):
     calls = _calls(pk, B=0, table=None, len=None, row0=None, rows=rows, max_T=0, **none)
     for e in ALL:
         assert calls[e]() == pk.PK_HIP_EINVAL
+
+
+@pytest.mark.parametrize("max_pages,T", [(1 << 24, 1), (1 << 24, 5), ((1 << 24) - 2, 5), (1 << 24, 0)])
+def test_widest_tables(max_pages, T):
+    """Every frame of the widest table may be attended without positions. The calls
+    end at an output that is not aligned, which is looked at after the window."""
+    import libpktito_amd as pk
+    r = ctypes.byref
+    c, st = pk.Cache(4096, 2, 8, 4, 64), pk.Streams(4096, 4096, 4096, 2, max_pages, 5, T)
+    for left, right in ((pk.UNLIMITED, pk.UNLIMITED), (64 * max_pages, 0), (1 << 30, 3)):
+        assert pk.lib().pk_hip_attention_cache_dev(4100, 512, 8192, 512, r(c), 1, r(st), 8, None, left, right, 4096, 1 << 40,
+                                                   None) == pk.PK_HIP_EINVAL
+        assert b"aligned" in pk.lib().pk_hip_last_error(), pk.lib().pk_hip_last_error()
