@@ -486,11 +486,12 @@ typedef struct {
  * memory (of the same cache, streams' counts, H, pos, left and right),
  * 16-byte aligned, of no matter before and after; calls that overlap in time
  * need workspaces of their own (0 bytes: none is needed, or the sizes are not
- * taken). Products and sums in 32 bits: what enters them is not rounded below
- * that, and a position score's products are held to 2^-24 of themselves, as
- * 32-bit ones are, but for what of a query, of a position's row or of a value is
- * under 2^-122, which may be dropped (of numbers under 2^-99, their last bits).
- * Values of 2^100 and more may pass the largest float in a sum. */
+ * taken; position scores take 2^48 bytes at most). Products and sums in 32
+ * bits: what enters them is not rounded below that, and a position score's
+ * products are held to 2^-24 of themselves, as 32-bit ones are, but for what of
+ * a query, of a position's row or of a value is under 2^-122, which may be
+ * dropped (of numbers under 2^-99, their last bits). Values of 2^100 and more
+ * may pass the largest float in a sum. */
 size_t pk_hip_attention_cache_workspace(const pk_hip_cache *c, const pk_hip_streams *st, uint32_t H,
                                         const pk_hip_positions *pos, uint32_t left, uint32_t right);
 int pk_hip_attention_cache_dev(float *o, size_t os, const float *q, size_t qs, const pk_hip_cache *c, uint32_t layer,

@@ -1326,7 +1326,11 @@ bool cache_attention_fits(const CacheStreams &st, uint32_t G, uint32_t H, uint32
     return d.units <= kMostGroups / d.splits;
 }
 
-bool cache_places_fit(int32_t left, int32_t right) { return ((uint32_t)left + (uint32_t)right) / 64 < kMostGroups; }
+bool cache_places_fit(const CacheStreams &st, uint32_t H, int32_t left, int32_t right) {
+    const uint32_t bw = (uint32_t)left + (uint32_t)right + 1;
+    const uint64_t row = (uint64_t)H * place_stride(bw) * sizeof(float);        /* under 2^50 */
+    return (bw - 1) / 64 < kMostGroups && (st.rows == 0 || row <= (1ull << 48) / st.rows);
+}
 
 template <int NS, int RT, int MT, bool PRE>
 static void place(const CacheAttention &a, hipStream_t s) {

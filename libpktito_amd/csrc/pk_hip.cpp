@@ -1670,8 +1670,9 @@ static int attention_window(const pk_hip_cache *c, const pk_hip_streams *st, uin
     if (!pkq8::cache_attention_fits(streams_of(st), c->heads, H, c->dk, *l, *r))
         return fail(PK_HIP_EINVAL, "%s: %u streams of up to %u rows, %u heads: more than a launch holds", who, st->B,
                     st->max_T, H);
-    if (pos && !pkq8::cache_places_fit(*l, *r))
-        return fail(PK_HIP_EINVAL, "%s: position scores by %u distances: more than a launch holds", who, lo + hi + 1);
+    if (pos && !pkq8::cache_places_fit(streams_of(st), H, *l, *r))
+        return fail(PK_HIP_EINVAL, "%s: position scores of %u rows, %u heads, by %u distances: more than a launch or a "
+                                   "workspace of 2^48 bytes holds", who, st->rows, H, lo + hi + 1);
     return PK_HIP_OK;
 }
 

@@ -237,8 +237,8 @@ size_t cache_attention_workspace(const CacheStreams &st, uint32_t G, uint32_t H,
                                  int32_t left, int32_t right);
 /* whether a launch holds the call's workgroups */
 bool cache_attention_fits(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, int32_t left, int32_t right);
-/* and those of its position scores */
-bool cache_places_fit(int32_t left, int32_t right);
+/* and those of its position scores, in a workspace of 2^48 bytes at most */
+bool cache_places_fit(const CacheStreams &st, uint32_t H, int32_t left, int32_t right);
 int launch_cache_attention(const CacheAttentionCall &c, hipStream_t s);
 /* n pairs (from, to) of pages, in every layer (dlayer, slayer bytes a layer) */
 int launch_cache_move(uint8_t *dst, uint64_t dlayer, const uint8_t *src, uint64_t slayer, uint32_t layers,

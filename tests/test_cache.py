@@ -689,3 +689,25 @@ def test_widest_tables(max_pages, T):
         assert pk.lib().pk_hip_attention_cache_dev(4100, 512, 8192, 512, r(c), 1, r(st), 8, None, left, right, 4096, 1 << 40,
                                                    None) == pk.PK_HIP_EINVAL
         assert b"aligned" in pk.lib().pk_hip_last_error(), pk.lib().pk_hip_last_error()
+@pytest.mark.parametrize("H,n", [
+    (32768, (1 << 26) - 160),                   # 2^64 bytes of scores: none would be left
+    (32768, (1 << 26) - 144),                   # and 2^38 more
+    (65532, 0xffffffff), (4, 0xffffffff),       # the widest tables; the last one's scores would pass 2^48 bytes only
+])
+def test_workspaces_past_what_a_size_holds(H, n):
+    """Position scores whose bytes pass what a size holds have no workspace, and a
+    call of them is refused, not run in the one that the last bits give."""
+    import libpktito_amd as pk
+    rows, r = 1 << 21, ctypes.byref
+    c = pk.Cache(4096, 2, 8, 4, 32)
+    st = pk.Streams(4096, 4096, 4096, 1, 1 << 24, rows, 1)
+    for center in {min(n - 1, (1 << 30) - 1), n - 1}:
+        pos = pk.Positions(4096, 4096, 4096, n, center)
+        args = (r(st), H, r(pos), pk.UNLIMITED, 0)
+        assert pk.lib().pk_hip_attention_cache_workspace(r(c), *args) == 0
+        assert pk.lib().pk_hip_attention_cache_dev(4096, H * 32, 8192, H * 32, r(c), 1, *args, 4096, 1 << 62,
+                                                   None) == pk.PK_HIP_EINVAL
+        assert b"workspace" in pk.lib().pk_hip_last_error()
+    # the largest position table that 288 GB hold beside its queries is taken: 2^31 of its numbers
+    st.rows, pos = 64, pk.Positions(4096, 4096, 4096, 1 << 24, (1 << 24) - 1)
+    assert pk.lib().pk_hip_attention_cache_workspace(r(c), r(st), 4, r(pos), pk.UNLIMITED, 0) >= 64 * 4 * 4 << 24
