@@ -1243,18 +1243,21 @@ constexpr uint64_t kMostGroups = (1u << 24) - 1;
  * tile's pages, joined for 4 to 5 us by a launch of their own, from 32 pages
  * on, so many that a wave takes two pages or more. As many splits of four waves
  * as two a CU allow only where that is an odd number, so that those of eight
- * waves leave CUs idle, and against none from 80 pages on.
+ * waves leave CUs idle, and against none from 120 pages on (100 of 16 rows).
  *
  * Heads of 128, four rows: 256 tiles of 33 pages 16.2 us with eight waves, 16.7
  * with four, 19.4 in two splits of four; 192 of 16 8.6 and 9.0 (heads of 64 7.7
  * and 7.3); 32 of 70 unsplit with four 23.7, in eight splits 10.7, in nine 11.5.
  * 16 rows: 256 of 33 19.4 with eight, in two splits of four 26.4; 192 of 24 15.1
  * with eight and 15.8 with four, of 8 9.2 and 9.1; 320 of 24 27.4 and 22.8 (more
- * tiles than CUs). 168 tiles of one row unsplit with eight waves and in three splits of
- * four: 33 pages 12.7 and 14.6, 80 23.7 and 26.0 (16 rows 30.6 and 30.5), 300
- * 71 and 69 (103 and 95; heads of 64 47 and 39); 96 tiles in two of eight and
- * in five of four: 33 pages 11.7 and 11.2, 300 43.7 and 44.1 (16 rows 55 and
- * 49). One frame against 704 pages of one stream: 873 us unsplit. */
+ * tiles than CUs). 152 tiles of four rows unsplit with eight waves and in three
+ * splits of four: 100 pages 26.1 and 27.5, 120 30.3 and 30.6, 300 66 and 62 (136
+ * tiles of 120 30.5 and 28.7, 168 30.7 and 32.7; heads of 64 22.4 and 21.5). 136
+ * tiles of 16 rows: 80 pages 31.3 and 29.6, 120 42 and 36.5 (heads of 64 21.8 and
+ * 22.8, 29.2 and 27.2; of 32 17.8 and 20.1, 24.4 and 24.6). 96 tiles in two of
+ * eight and in five of four: 33 pages 12.1 and 12.0, 300 42.2 and 42.5 (16 rows 56
+ * and 50; heads of 32 29.8 and 25.4). One frame against 704 pages of one stream:
+ * 16.4 in 32 splits of eight waves, unsplit 141, with four waves 200. */
 struct Deal {
     uint32_t rows, tiles, splits;           /* rows a tile, a stream's tiles a kept head, a tile's splits */
     uint32_t pages;                         /* pages a tile can reach */
@@ -1280,7 +1283,7 @@ static Deal deal(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, in
     if (d.units == 0 || d.units > 256)
         return d;
     const uint32_t eights = (uint32_t)(256 / d.units), fours = (uint32_t)(512 / d.units);
-    const bool odd = fours % 2 && d.pages >= (eights == 1 ? 80 : 32);
+    const bool odd = fours % 2 && d.pages >= (eights > 1 ? 32 : d.rows == 4 ? 120 : 100);
     if (d.pages >= 32)
         d.splits = std::min({ odd ? fours : eights, (d.pages + 7) / 8, 128u });
     if (!odd && (d.rows == 4 ? (uint64_t)d.pages * dk > 1280u * d.splits : d.pages > 8 * d.splits))

@@ -937,3 +937,21 @@ def test_step_without_streams(hip, torch):
         w.cache.attention(o, 0, q, st, 4, ws, (p, 4, b, b))
         torch.cuda.synchronize()
         assert (a == 1).all() and (o == 7.25).all() and torch.equal(w.data, before)
+
+
+@pytest.mark.parametrize("B,H,G,T,dk,pages", [
+    (17, 8, 8, 2, 32, 120), (21, 8, 8, 4, 32, 119),     # tiles of four rows, in three splits from 120 pages
+    (17, 8, 8, 16, 32, 100), (17, 8, 8, 5, 32, 99),     # of 16 rows, from 100
+])
+def test_pages_dealt_in_odd_splits(hip, torch, B, H, G, T, dk, pages):
+    """On both sides of the pages from which three workgroups share a tile's. All
+    streams read one stream's pages, each with a hole of its own."""
+    say("odd splits", B, H, G, T, dk, pages)
+    total = 64 * pages - 5
+    w = World(hip, torch, [total - T] * B, [T] * B, G, dk, seed=pages)
+    w.table[:] = w.table[0]
+    w.fill(upto=[total] + [0] * (B - 1))
+    for b in range(B):
+        w.table[b, (7 * b + 3) % pages] = -1
+    w.upload()
+    w.check(H)
