@@ -428,17 +428,18 @@ __device__ __forceinline__ int wave_max(int v) {
  * MT. PRE: the table's rows come cut.
  *
  * At 2624 rows by up to 3750 distances it takes 121 us, 110 at best (and the
- * cutting 11), for 280 MB of scores: its products alone take 94 at the 1134
- * TFLOP/s that a bfloat16 product of 8192 cubed reaches here. Of two float16
- * pieces with an exponent a row three products do, in 97 us, but what is small
- * beside its row's largest loses its bits. At 256 rows by 4500 it takes 28 us,
- * and at few rows a chain of two memory round trips and a launch, 7. The
- * shapes of a workgroup are within a few us of each other: 8 waves, 128 rows
- * and two tiles a wave 132 us, three tiles 126, 96 rows and 6 waves 147.
- * Measured and taken back: a lane's four scores stored at the frames' own
- * places (16 bytes at any multiple of 4: each step twice as long), one float a
- * lane stored there (as long as now, and the attention no faster), stores
- * through the caches (the attention of 256 streams 171 -> 190 us). */
+ * cutting 11), for 280 MB of scores: its products alone take 91 at the 1134
+ * TFLOP/s that a bfloat16 product of 8192 cubed reaches here, and the matrix
+ * cores are busy half of its cycles. Of two float16 pieces with an exponent a
+ * row three products do, in 97 us, but what is small beside its row's largest
+ * loses its bits. At 256 rows by 4500 it takes 28 us, and at few rows a chain of
+ * two memory round trips and a launch, 7. The shapes of a workgroup are within a
+ * few us of each other: 8 waves, 128 rows and two tiles a wave 132 us, three
+ * tiles 126, 96 rows and 6 waves 147. Measured and taken back: a lane's four
+ * scores stored at the frames' own places (16 bytes at any multiple of 4: each
+ * step twice as long), one float a lane stored there (as long as now, and the
+ * attention no faster), stores through the caches (the attention of 256 streams
+ * 171 -> 190 us). */
 
 /* waves a SIMD: registers for three where a wave keeps two tiles of the table, as
  * LDS has room for (48 KB a workgroup of 64 rows of 128) */
@@ -975,13 +976,14 @@ __global__ __launch_bounds__(64 * W) void cache_few_kernel(CacheAttention a) {
  * the second product takes them.
  *
  * Four files of 500 to 750 rows after 2200 to 3000 frames, 8 heads of 128:
- * 124 us, 265 TFLOP/s as an fp32 product counts them. Instructions bound it:
- * 515 vector ones a page and 16 rows, 96 of them products, issue in three
- * quarters of the cycles at two waves a SIMD (235 registers). Measured and no
- * faster: a page's first product under the page before's softmax (130), the
- * products at another wave priority (127, 129), the queries' pieces in LDS
- * (126; for three waves, 250: spills), eight waves (147; where 16 streams of 14
- * rows leave half the CUs idle, eight take 12.8 and four 14.5). */
+ * 135 us (123 at best), 243 TFLOP/s as an fp32 product counts them. Instructions
+ * bound it: of 525 vector ones a page and 16 rows 96 are products, which keep the
+ * matrix cores busy 44% of the cycles, and the others issue in 49%, with two waves
+ * a SIMD (235 registers) to overlap them. Measured and no faster, at best: a
+ * page's first product under the page before's softmax (130), the products at
+ * another wave priority (127, 129), the queries' pieces in LDS (126; for three
+ * waves, 250: spills), eight waves (147; where 16 streams of 14 rows leave half
+ * the CUs idle, eight take 12.8 and four 14.5). */
 template <int NS, bool POS, int W>
 __global__ __launch_bounds__(64 * W) void cache_many_kernel(CacheAttention a) {
     constexpr uint32_t dk = 32 * NS, record = kPage * dk + 4 * kPage;

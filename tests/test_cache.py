@@ -711,3 +711,21 @@ def test_workspaces_past_what_a_size_holds(H, n):
     # the largest position table that 288 GB hold beside its queries is taken: 2^31 of its numbers
     st.rows, pos = 64, pk.Positions(4096, 4096, 4096, 1 << 24, (1 << 24) - 1)
     assert pk.lib().pk_hip_attention_cache_workspace(r(c), r(st), 4, r(pos), pk.UNLIMITED, 0) >= 64 * 4 * 4 << 24
+
+
+def test_how_far_kept_values_are_off(layout):
+    """Half a level's step of a scale that is up to 2^-7 over a sixth of the head's
+    largest magnitude: a sixth of that and 2^-7 more, a twenty-fourth so up to two
+    levels. Tops just over a bfloat16's six-fold come near it."""
+    g = np.random.default_rng(9)
+    most = 0.0
+    for _ in range(3000):
+        top = np.float32(6.0 * (1 + 2.0 ** -20)) if g.random() < 0.1 else np.float32(abs(g.standard_normal()) + 0.1)
+        d = float(np.uint32(layout.t_scale(float(top)) << 16).view(np.float32))
+        for x in (np.float32(v) for v in (g.uniform(-1, 1) * float(top), 5 * d, 1.25 * d, float(top))):
+            if abs(x) > top:
+                continue
+            off = abs(layout.t_level(layout.t_code(float(x), d)) * d - float(x)) / float(top)
+            assert off <= (1 + 2.0 ** -7) / (24 if abs(x) <= 2 * d else 6)
+            most = max(most, off)
+    assert most > 1 / 6
