@@ -955,3 +955,33 @@ def test_pages_dealt_in_odd_splits(hip, torch, B, H, G, T, dk, pages):
         w.table[b, (7 * b + 3) % pages] = -1
     w.upload()
     w.check(H)
+
+
+def test_graph_with_the_table_cut_beforehand(hip, torch):
+    """A call of many rows captured, replayed with other queries, positions and
+    lengths in the same memory and the program's own work between: each replay is
+    the eager call's bits, on a stream of its own too."""
+    say("graph, cut beforehand")
+    w = World(hip, torch, [60, 3], [1201, 24], 1, 32, seed=64)
+    w.fill()
+    p, c, u, b = w.positions(1, 1270, 1201)
+    pos = (w.dev(p), c, w.dev(u), w.dev(b))
+    q = w.dev(w.g.standard_normal((w.rows, 32)).astype(np.float32))
+    o = torch.empty_like(q)
+    need = w.cache.attention_workspace(w.streams, 1, pos)
+    ws = [torch.full((need,), 0xff, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        w.cache.attention(o, 0, q, w.streams, 1, ws[0], pos)
+    side, eager = torch.cuda.Stream(), torch.empty_like(q)
+    for i in range(4):
+        q.copy_(w.dev(w.g.standard_normal((w.rows, 32)).astype(np.float32)))
+        pos[0].mul_(0.9)
+        w.streams.len[0] = 60 - 7 * i
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            w.cache.attention(eager, 0, q, w.streams, 1, ws[1], pos)
+        torch.cuda.synchronize()
+        assert torch.equal(o, eager) and torch.isfinite(o).all(), i
+        (torch.randn(512, 512, device="cuda") @ torch.randn(512, 512, device="cuda")).sum().item()
