@@ -537,6 +537,41 @@ uint32_t pk_hip_pool_holders(const pk_hip_pool *pool, int32_t id);
 int pk_hip_pool_compact(pk_hip_pool *pool, int32_t *pairs, uint32_t cap, uint32_t *n);
 int pk_hip_pool_restore(pk_hip_pool *pool, const int32_t *pairs, uint32_t n);
 
+/* ------------------------------------------- audio without an end --- */
+
+/* The attention of whole segments with a sliding window and sinks, for audio
+ * too long for every frame to attend to every other: frame t of a segment of T
+ * attends the frames j < T with j <= t + right and either j >= t - left or j <
+ * sinks (the segment's first frames, which stay visible behind the window).
+ * Scores are
+ *   ((q + u) . k + (q + w) . p[center - min(t - j, left)]) / sqrt(dk)
+ * (pk_hip_positions; a sink behind the window takes the position of
+ * distance left) or q . k / sqrt(dk) with pos NULL; each row is the softmax's
+ * weighted values, in one launch whose time goes by the window. With pos,
+ * distances that p has no row for are not attended: left is at most center,
+ * right at most n - 1 - center. left and right may be PK_HIP_UNLIMITED.
+ * q and o are [rows][H * dk], k and v [rows][G * dk], H a multiple of G (each
+ * kept head shared among H / G consecutive ones), dk 32, 64, 96 or 128; row r
+ * of x at x + r * its stride (qs, ks, vs, os), 16-byte aligned, strides
+ * multiples of 4. o may be q with os = qs; an o that shares memory with k, v or
+ * the positions is refused. Rows of no segment are left as they were. Products
+ * and sums in 32 bits, not held to a bit pattern (pk_hip_attention_dev's are
+ * the reference's, core/encoder.c:280-327, which has no window). A row's
+ * outputs depend on the frames that it attends alone, whatever the others hold.
+ *
+ * The segments of a call: row0 [B + 1] in device memory, read when the kernel
+ * runs, segment b's rows [row0[b], row0[b + 1]) of rows in all; max_T at least
+ * the longest one's T (what is beyond max_T or beyond rows takes no part). B up
+ * to 65535, rows up to 2^21, and B x H x ceil(max_T / 16) under 2^24. */
+typedef struct {
+    const int32_t *row0;
+    uint32_t B, rows, max_T;
+} pk_hip_segments;
+int pk_hip_attention_window_dev(float *o, size_t os, const float *q, size_t qs, const float *k, size_t ks,
+                                const float *v, size_t vs, const pk_hip_segments *sg, uint32_t H, uint32_t G,
+                                uint32_t dk, const pk_hip_positions *pos, uint32_t left, uint32_t right,
+                                uint32_t sinks, void *stream);
+
 /* Measurement aids, with no counterpart in the reference: the floors a
  * small product's time is read against. pk_hip_empty_dev launches an empty
  * kernel; pk_hip_stream_read_dev reads the bytes at p (16-byte aligned,

@@ -90,6 +90,12 @@ class Positions(ctypes.Structure):
                 ("n", ctypes.c_uint32), ("center", ctypes.c_uint32)]
 
 
+class SegmentRows(ctypes.Structure):
+    """pk_hip_segments: the segments of an attention with a window."""
+    _fields_ = [("row0", ctypes.c_void_p), ("B", ctypes.c_uint32), ("rows", ctypes.c_uint32),
+                ("max_T", ctypes.c_uint32)]
+
+
 CACHE_PAGE = 64
 UNLIMITED = 0xffffffff
 
@@ -198,6 +204,9 @@ _SIGS = {
                                                   ctypes.c_uint32, ctypes.POINTER(Positions), ctypes.c_uint32,
                                                   ctypes.c_uint32, ctypes.c_void_p, ctypes.c_size_t,
                                                   ctypes.c_void_p]),
+    "pk_hip_attention_window_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_size_t] * 4 +
+                                    [ctypes.POINTER(SegmentRows)] + [ctypes.c_uint32] * 3 +
+                                    [ctypes.POINTER(Positions)] + [ctypes.c_uint32] * 3 + [ctypes.c_void_p]),
     "pk_hip_cache_move_dev": (ctypes.c_int, [ctypes.POINTER(Cache), ctypes.POINTER(Cache), ctypes.c_void_p,
                                              ctypes.c_uint32, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "pk_hip_pool_create": (ctypes.c_int, [ctypes.POINTER(ctypes.c_void_p), ctypes.c_uint32]),
@@ -779,6 +788,22 @@ class CacheStreams:
                           self.rows, self.max_T)
 
 
+def _positions(positions, H, dk, device):
+    """(p [n, H * dk], center, bias_u, bias_w) as the C side takes them."""
+    if positions is None:
+        return None
+    p, center, u, w = positions
+    n = max(1, _u32(H, "H")) * dk
+    _is(p, "float32", "p", device)
+    _is(u, "float32", "bias_u", device)
+    _is(w, "float32", "bias_w", device)
+    rows, rest = divmod(p.numel(), n)
+    if rest or u.numel() != n or w.numel() != n or not (p.is_contiguous() and u.is_contiguous() and
+                                                        w.is_contiguous()):
+        raise PkHipError(PK_HIP_EINVAL, f"positions: p [n, {n}] and biases [{n}], contiguous")
+    return Positions(p.data_ptr(), u.data_ptr(), w.data_ptr(), rows, _u32(center, "center"))
+
+
 class DeviceCache:
     """Keys and values of streams of live audio, kept in 4 bits in pages of
     CACHE_PAGE frames (pk_hip_cache): data a contiguous uint8 device tensor of
@@ -831,18 +856,7 @@ class DeviceCache:
                                                       _reach(left, "left"), _reach(right, "right"))
 
     def _positions(self, positions, H):
-        if positions is None:
-            return None
-        p, center, u, w = positions
-        n = max(1, _u32(H, "H")) * self.dk
-        _is(p, "float32", "p", self.device)
-        _is(u, "float32", "bias_u", self.device)
-        _is(w, "float32", "bias_w", self.device)
-        rows, rest = divmod(p.numel(), n)
-        if rest or u.numel() != n or w.numel() != n or not (p.is_contiguous() and u.is_contiguous() and
-                                                            w.is_contiguous()):
-            raise PkHipError(PK_HIP_EINVAL, f"positions: p [n, {n}] and biases [{n}], contiguous")
-        return Positions(p.data_ptr(), u.data_ptr(), w.data_ptr(), rows, _u32(center, "center"))
+        return _positions(positions, H, self.dk, self.device)
 
     def attention(self, o, layer, q, streams, H, ws, positions=None, left=None, right=None, stream=None):
         """The attention of the rows q [rows, H * dk] to their streams' kept
@@ -964,3 +978,39 @@ class PagePool:
                 _check(lib().pk_hip_pool_restore(self.handle, pairs, n))
                 raise
         return moved
+
+
+# ------------------------------------------------- audio without an end ---
+
+class Segments:
+    """The segments of an attention with a window (pk_hip_segments): an int32
+    device tensor row0 [B + 1], the call's number of rows and its longest
+    segment's. row0 is read when the kernel runs."""
+
+    def __init__(self, row0, rows, max_T):
+        _is(row0, "int32", "row0", None)
+        if row0.dim() != 1 or not row0.is_contiguous() or row0.shape[0] < 1:
+            raise PkHipError(PK_HIP_EINVAL, "segments: row0 [B + 1], contiguous")
+        self.row0, self.device = row0, row0.get_device()
+        self.rows, self.max_T = _u32(int(rows), "rows"), _u32(int(max_T), "max_T")
+        self.st = SegmentRows(row0.data_ptr(), row0.shape[0] - 1, self.rows, self.max_T)
+
+
+def attention_window_dev(o, q, k, v, segments, H, dk, positions=None, left=None, right=None, sinks=0, stream=None):
+    """The attention of whole segments with a window and sinks, into o [rows,
+    H * dk] (pk_hip_attention_window_dev): q [rows, H * dk], k and v [rows, G *
+    dk], positions (p [n, H * dk], center, bias_u, bias_w) or None, left and
+    right the frames attended behind and ahead (None: all), sinks the first
+    frames that stay visible."""
+    n, w, device = segments.rows, _u32(H, "H") * _u32(dk, "dk"), segments.device
+    if _device() != device:
+        raise PkHipError(PK_HIP_EINVAL, f"segments on device {device}, with {_device()} the current one")
+    G, rest = divmod(k.shape[-1] if k.dim() else 0, max(1, dk))
+    if rest:
+        raise PkHipError(PK_HIP_EINVAL, f"k: rows of heads of {dk}, not {tuple(k.shape)}")
+    pos = _positions(positions, H, dk, device)
+    _check(lib().pk_hip_attention_window_dev(*_rows(o, n, w, "o", device), *_rows(q, n, w, "q", device),
+                                             *_rows(k, n, G * dk, "k", device), *_rows(v, n, G * dk, "v", device),
+                                             ctypes.byref(segments.st), H, G, dk, ctypes.byref(pos) if pos else None,
+                                             _reach(left, "left"), _reach(right, "right"), _u32(sinks, "sinks"),
+                                             _stream(stream)))

@@ -1644,6 +1644,14 @@ int pk_hip_cache_read_dev(const pk_hip_cache *c, uint32_t layer, float *k, size_
     return PK_HIP_OK;
 }
 
+static int check_positions(const pk_hip_positions *pos, const char *who) {
+    if (!pos->p || !pos->bias_u || !pos->bias_w || (((uintptr_t)pos->p | (uintptr_t)pos->bias_u |
+        (uintptr_t)pos->bias_w) & 15) || pos->center >= pos->n)
+        return fail(PK_HIP_EINVAL, "%s: positions with p and both biases 16-byte aligned, the center one of the "
+                                   "rows", who);
+    return PK_HIP_OK;
+}
+
 /* The window that an attention's rows have: the asked one, no wider than the
  * rows can reach or than the positions' table does. */
 static int attention_window(const pk_hip_cache *c, const pk_hip_streams *st, uint32_t H, const pk_hip_positions *pos,
@@ -1658,10 +1666,8 @@ static int attention_window(const pk_hip_cache *c, const pk_hip_streams *st, uin
     uint32_t lo = std::min(left, (uint32_t)pkq8::cache_most_left(st->max_pages, st->max_T));
     uint32_t hi = std::min(right, st->max_T ? st->max_T - 1 : 0);
     if (pos) {
-        if (!pos->p || !pos->bias_u || !pos->bias_w || (((uintptr_t)pos->p | (uintptr_t)pos->bias_u |
-            (uintptr_t)pos->bias_w) & 15) || pos->center >= pos->n)
-            return fail(PK_HIP_EINVAL, "%s: positions with p and both biases 16-byte aligned, the center one of the "
-                                       "rows", who);
+        if ((e = check_positions(pos, who)))
+            return e;
         lo = std::min(lo, pos->center);
         hi = std::min(hi, pos->n - 1 - pos->center);
     }
@@ -1719,6 +1725,75 @@ int pk_hip_attention_cache_dev(float *o, size_t os, const float *q, size_t qs, c
     a.ws = ws;
     PK_LAUNCH(pkq8::launch_cache_attention(a, (hipStream_t)stream), "cache attention launch");
     g_kernel = "cache_attention";
+    return PK_HIP_OK;
+}
+
+/* Rows of floats: n of width w, stride s apart. */
+struct FloatRows {
+    const float *p;
+    uint64_t s, w, n;
+};
+
+/* Whether two share memory, as far as is seen without a walk over them: rows
+ * between each other's (one stride, as of matrices side by side) do not. */
+static bool rows_meet(const FloatRows &a, const FloatRows &b) {
+    if (!a.n || !b.n)
+        return false;
+    const uintptr_t a0 = (uintptr_t)a.p, b0 = (uintptr_t)b.p, f = sizeof(float);
+    if (a0 + ((a.n - 1) * a.s + a.w) * f <= b0 || b0 + ((b.n - 1) * b.s + b.w) * f <= a0)
+        return false;
+    if (a.s != b.s || a.s < a.w || a.s < b.w)
+        return true;
+    const uintptr_t step = a.s * f, past = a0 < b0 ? (b0 - a0) % step : (step - (a0 - b0) % step) % step;
+    return past < a.w * f || past + b.w * f > step;
+}
+
+int pk_hip_attention_window_dev(float *o, size_t os, const float *q, size_t qs, const float *k, size_t ks,
+                                const float *v, size_t vs, const pk_hip_segments *sg, uint32_t H, uint32_t G,
+                                uint32_t dk, const pk_hip_positions *pos, uint32_t left, uint32_t right,
+                                uint32_t sinks, void *stream) {
+    static const char who[] = "attention_window_dev";
+    int e;
+    if (!sg || !sg->row0 || sg->B > 65535 || sg->rows > 1u << 21 || sg->max_T > sg->rows)
+        return fail(PK_HIP_EINVAL, "%s: segments with their row0, up to 65535 of them and 2^21 rows, max_T up to rows", who);
+    if (G == 0 || G > 1024 || !pkq8::cache_dk_ok(dk) || H == 0 || H > 65535 || H % G)
+        return fail(PK_HIP_EINVAL, "%s: H = %u heads of 32, 64, 96 or 128 dimensions, a multiple of the G = %u of keys and "
+                                   "values (1 to 1024)", who, H, G);
+    if (!pkq8::window_fits(sg->B, sg->max_T, H))
+        return fail(PK_HIP_EINVAL, "%s: %u segments of up to %u rows, %u heads: more than a launch holds", who, sg->B,
+                    sg->max_T, H);
+    const uint64_t width = (uint64_t)H * dk, kept = (uint64_t)G * dk;
+    const uint32_t n = sg->rows, most = sg->max_T ? sg->max_T - 1 : 0;
+    if (n && ((e = check_rows(o, os, width, n, who, "o")) || (e = check_rows(q, qs, width, n, who, "q")) ||
+              (e = check_rows(k, ks, kept, n, who, "k")) || (e = check_rows(v, vs, kept, n, who, "v"))))
+        return e;
+    pkq8::WindowCall a = {};
+    uint32_t lo = std::min(left, most), hi = std::min(right, most);
+    if (pos) {
+        if ((e = check_positions(pos, who)))
+            return e;
+        lo = std::min(lo, pos->center);
+        hi = std::min(hi, pos->n - 1 - pos->center);
+        a.p = pos->p + (pos->center - lo) * width;
+        a.bias_u = pos->bias_u, a.bias_w = pos->bias_w;
+    }
+    const FloatRows out = { o, os, width, n };
+    if ((const float *)o == q ? os != qs && n > 1 : rows_meet(out, { q, qs, width, n }))
+        return fail(PK_HIP_EINVAL, "%s: an output that is not its queries, with their stride, apart from them", who);
+    if (rows_meet(out, { k, ks, kept, n }) || rows_meet(out, { v, vs, kept, n }) ||
+        (pos && (rows_meet(out, { pos->p, width, width, pos->n }) || rows_meet(out, { pos->bias_u, width, width, 1 }) ||
+                 rows_meet(out, { pos->bias_w, width, width, 1 }))))
+        return fail(PK_HIP_EINVAL, "%s: an output apart from the keys, the values and the positions", who);
+    if ((e = pk_hip_init()))
+        return e;
+    if (sg->B == 0 || sg->max_T == 0)
+        return PK_HIP_OK;
+    a.o = o, a.os = os, a.q = q, a.qs = qs, a.k = k, a.ks = ks, a.v = v, a.vs = vs;
+    a.row0 = sg->row0, a.B = sg->B, a.rows = n, a.max_T = sg->max_T;
+    a.H = H, a.G = G, a.dk = dk;
+    a.left = (int32_t)lo, a.right = (int32_t)hi, a.sinks = (int32_t)std::min(sinks, sg->max_T);
+    PK_LAUNCH(pkq8::launch_window(a, (hipStream_t)stream), "window attention launch");
+    g_kernel = "attention_window";
     return PK_HIP_OK;
 }
 

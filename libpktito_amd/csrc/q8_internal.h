@@ -245,6 +245,23 @@ int launch_cache_move(uint8_t *dst, uint64_t dlayer, const uint8_t *src, uint64_
                       uint32_t page_bytes, const int32_t *pairs, uint32_t n, int32_t *table, uint64_t entries,
                       hipStream_t s);
 
+/* Attention with a window and sinks over whole segments (window_kernels.hip);
+ * left, right and sinks clipped to what can occur, p at distance left's row
+ * (NULL: content scores alone). Arguments checked by the caller; 0, -2 for
+ * shapes no kernel takes, -1 for a failed launch. */
+struct WindowCall {
+    float *o;
+    const float *q, *k, *v;
+    uint64_t os, qs, ks, vs;
+    const int32_t *row0;
+    uint32_t B, rows, max_T, H, G, dk;
+    int32_t left, right, sinks;
+    const float *p, *bias_u, *bias_w;
+};
+int launch_window(const WindowCall &c, hipStream_t s);
+/* whether a launch holds the call's workgroups */
+bool window_fits(uint32_t B, uint32_t max_T, uint32_t H);
+
 /* Measurement aids (diag_kernels.hip): an empty launch; a streaming read of
  * bytes (a multiple of 16) at p, 16-byte aligned. */
 int launch_empty(hipStream_t s);
