@@ -572,6 +572,77 @@ int pk_hip_attention_window_dev(float *o, size_t os, const float *q, size_t qs, 
                                 uint32_t dk, const pk_hip_positions *pos, uint32_t left, uint32_t right,
                                 uint32_t sinks, void *stream);
 
+/* The plan of a step of a cache's streams, made on the device: what each stream
+ * brings in, and out come the descriptor that the cache's calls take
+ * (pk_hip_streams), pages taken from a pool for new frames, and pages that the
+ * window has left given back to it, with nothing for the host to wait for or to
+ * send, so that a captured graph of plan, append and attention runs a stream's
+ * steps one after another. It stands beside the host's pool (pk_hip_pool_*): a
+ * cache's pages are one's or the other's, and pages of this one have one holder.
+ *
+ * B streams (places that requests come and go in), device memory throughout, 4
+ * byte aligned, each a call's own while it runs:
+ *   add    [B]: the frames that each stream brings; negative counts as 0
+ *   fresh  [B], or NULL for none: not 0 where a stream begins anew: whatever
+ *          pages its place held go back, and it brings its first frames (a
+ *          stream that ends: fresh, and nothing added)
+ *   state  [B][2], kept between calls: the stream's frames so far, and the column
+ *          of its table before which the window has given back all but the
+ *          sinks'; zeros at first
+ *   pool   [2 + pages], kept: the number of the first free page's place, how many
+ *          are free, and a ring of places of free pages' ids (at first 0, pages,
+ *          and every id): a queue, taken from its front and given back to its end
+ *   table  [B][max_pages], kept: as in pk_hip_streams; entries are written as
+ *          pages are taken (the id) and given back (-1)
+ *   len, row0   [B], [B + 1], written: as in pk_hip_streams, for this call's rows
+ *   slot   [rows], or NULL, written: each row's place in the pool, 64 times its
+ *          page and its frame's number in it; -1 for rows of no stream or page
+ *   told   [4], written: the call's rows, frames asked for that got none (beyond
+ *          max_T a stream, rows in all, or 64 max_pages frames of a stream; those
+ *          of the last streams in order), pages that the pool did not have
+ *          (their frames have a hole), pages free now
+ * First, in the order of streams and columns, pages go back: those of columns
+ * whose frames are all more than left behind the stream's first new one and that
+ * hold no sink (left PK_HIP_UNLIMITED: none), and those of fresh streams. Then, in
+ * that order, every column that the new frames begin gets a page. A window that
+ * grows from one call to the next does not bring pages back, and sinks that
+ * become fewer stay held until their stream ends. Numbers that no call leaves
+ * (counts below 0 or too great, ids outside the pool) are read as the nearest
+ * that can be, and never make it write outside of the arrays. max_pages 1 to
+ * 2^24, B up to 65535, rows up to 2^21, max_T up to rows, pages 1 to 2^24. */
+typedef struct {
+    int32_t *table, *len, *row0, *state, *pool, *slot, *told;
+    uint32_t B, max_pages, rows, max_T, pages;
+} pk_hip_plan;
+int pk_hip_cache_plan_dev(const pk_hip_plan *p, const int32_t *add, const int32_t *fresh, uint32_t left,
+                          uint32_t sinks, void *stream);
+
+/* How sure a recognizer is of its tokens: for each of `rows` rows of cols logits
+ * (row r at x + r xs; any 4-byte alignment and stride, so the tokens' or the
+ * durations' columns of the joint's logits serve as they are,
+ * core/decoder.c:81-101), where asked for,
+ *   lp       [rows][m]: the log probabilities of the given tokens [rows][m] (-1
+ *            is none and gets 0; any other id outside [0, cols) gets a NaN)
+ *   entropy  [rows]: of the row's distribution, in nats
+ *   top      [rows][k]: the k most probable ids, the most probable first, of
+ *            equal logits the lowest id, NaN last; and with top_lp [rows][k]
+ *            their log probabilities
+ * Computed in 32 bits from the differences to the row's largest logit, whose own
+ * term is left out of the sum and added by log1p: a token that is all but certain
+ * keeps its small log probability. A logit may be -infinity (probability 0, log
+ * probability -infinity); in a row with a NaN, with an infinity, or with nothing
+ * but -infinity every probability and the entropy are NaN, and the order is the
+ * logits' all the same. Outputs that share memory with the logits or the tokens
+ * are refused. cols 1 to 2^20, k up to 32 and up to cols, rows up to 2^21 and
+ * under 2^24 with a row's every 8192 columns counted. ws:
+ * pk_hip_logprobs_workspace(rows, cols, k) bytes of device memory (0 for up to
+ * 8192 columns), 16-byte aligned, of no matter before and after; calls that
+ * overlap in time need workspaces of their own. */
+size_t pk_hip_logprobs_workspace(uint32_t rows, uint32_t cols, uint32_t k);
+int pk_hip_logprobs_dev(const float *x, size_t xs, uint32_t rows, uint32_t cols, const int32_t *tokens, uint32_t m,
+                        float *lp, float *entropy, uint32_t k, int32_t *top, float *top_lp, void *ws, size_t ws_bytes,
+                        void *stream);
+
 /* Measurement aids, with no counterpart in the reference: the floors a
  * small product's time is read against. pk_hip_empty_dev launches an empty
  * kernel; pk_hip_stream_read_dev reads the bytes at p (16-byte aligned,

@@ -96,6 +96,12 @@ class SegmentRows(ctypes.Structure):
                 ("max_T", ctypes.c_uint32)]
 
 
+class Plan(ctypes.Structure):
+    """pk_hip_plan: the arrays of a plan of a cache's streams."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("table", "len", "row0", "state", "pool", "slot", "told")] +
+                [(n, ctypes.c_uint32) for n in ("B", "max_pages", "rows", "max_T", "pages")])
+
+
 CACHE_PAGE = 64
 UNLIMITED = 0xffffffff
 
@@ -207,6 +213,13 @@ _SIGS = {
     "pk_hip_attention_window_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_size_t] * 4 +
                                     [ctypes.POINTER(SegmentRows)] + [ctypes.c_uint32] * 3 +
                                     [ctypes.POINTER(Positions)] + [ctypes.c_uint32] * 3 + [ctypes.c_void_p]),
+    "pk_hip_cache_plan_dev": (ctypes.c_int, [ctypes.POINTER(Plan), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32,
+                                             ctypes.c_uint32, ctypes.c_void_p]),
+    "pk_hip_logprobs_workspace": (ctypes.c_size_t, [ctypes.c_uint32] * 3),
+    "pk_hip_logprobs_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_uint32, ctypes.c_uint32,
+                                           ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p, ctypes.c_void_p,
+                                           ctypes.c_uint32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                           ctypes.c_size_t, ctypes.c_void_p]),
     "pk_hip_cache_move_dev": (ctypes.c_int, [ctypes.POINTER(Cache), ctypes.POINTER(Cache), ctypes.c_void_p,
                                              ctypes.c_uint32, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "pk_hip_pool_create": (ctypes.c_int, [ctypes.POINTER(ctypes.c_void_p), ctypes.c_uint32]),
@@ -1014,3 +1027,91 @@ def attention_window_dev(o, q, k, v, segments, H, dk, positions=None, left=None,
                                              ctypes.byref(segments.st), H, G, dk, ctypes.byref(pos) if pos else None,
                                              _reach(left, "left"), _reach(right, "right"), _u32(sinks, "sinks"),
                                              _stream(stream)))
+
+
+class CachePlan:
+    """The plan of a step of a cache's streams, made on the device
+    (pk_hip_cache_plan_dev): int32 device tensors, contiguous, table [B,
+    max_pages], state [B, 2], pool [2 + pages] and, for rows' places in the pool,
+    slot [rows]. `streams` is the descriptor that the cache's calls take, as the
+    last step made it; `told` [4] the rows, the frames that got none, the pages
+    that were missing and those that are free."""
+
+    def __init__(self, table, state, pool, rows, max_T, slot=None):
+        import torch
+        _is(table, "int32", "table", None)
+        device = table.get_device()
+        for t, what in ((table, "table"), (state, "state"), (pool, "pool"), (slot, "slot")):
+            if t is not None:
+                _is(t, "int32", what, device)
+                if not t.is_contiguous():
+                    raise PkHipError(PK_HIP_EINVAL, f"{what} is not contiguous")
+        B = table.shape[0] if table.dim() == 2 else -1
+        if B < 0 or tuple(state.shape) != (B, 2) or pool.dim() != 1 or pool.shape[0] < 3 or (
+                slot is not None and tuple(slot.shape) != (rows,)):
+            raise PkHipError(PK_HIP_EINVAL, "plan: table [B, max_pages], state [B, 2], pool [2 + pages], slot [rows]")
+        new = lambda n: torch.zeros(n, dtype=torch.int32, device=table.device)
+        self.streams = CacheStreams(table, new(B), new(B + 1), rows, max_T)
+        self.table, self.state, self.pool, self.slot, self.told = table, state, pool, slot, new(4)
+        self.device = device
+        self.st = Plan(table.data_ptr(), self.streams.len.data_ptr(), self.streams.row0.data_ptr(), state.data_ptr(),
+                       pool.data_ptr(), _dptr(slot), self.told.data_ptr(), B, table.shape[1], self.streams.rows,
+                       self.streams.max_T, pool.shape[0] - 2)
+
+    @classmethod
+    def empty(cls, pages, B, max_pages, rows, max_T, slots=False, device="cuda"):
+        """B places without streams over a pool of free pages."""
+        import torch
+        new = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device=device)
+        pool = torch.cat([torch.tensor([0, pages]), torch.arange(pages)]).to(torch.int32).to(device)
+        return cls(new(B, max_pages).fill_(-1), new(B, 2), pool, rows, max_T, new(rows) if slots else None)
+
+    def step(self, add, fresh=None, left=None, sinks=0, stream=None):
+        """The next call's rows: add [B] frames of each stream, fresh [B] not 0
+        where one begins anew, left the frames that the window reaches back (None:
+        all are kept), sinks the first frames that stay."""
+        B = self.st.B
+        for t, what in ((add, "add"), (fresh, "fresh")):
+            if t is not None or what == "add":
+                _is(t, "int32", what, self.device)
+                if tuple(t.shape) != (B,) or not t.is_contiguous():
+                    raise PkHipError(PK_HIP_EINVAL, f"{what}: [{B}], contiguous")
+        if _device() != self.device:
+            raise PkHipError(PK_HIP_EINVAL, f"a plan on device {self.device}, with {_device()} the current one")
+        _check(lib().pk_hip_cache_plan_dev(ctypes.byref(self.st), add.data_ptr(), _dptr(fresh), _reach(left, "left"),
+                                           _u32(sinks, "sinks"), _stream(stream)))
+
+
+def logprobs_workspace(rows, cols, k):
+    """Bytes of workspace logprobs_dev takes."""
+    return lib().pk_hip_logprobs_workspace(_u32(rows, "rows"), _u32(cols, "cols"), _u32(k, "k"))
+
+
+def logprobs_dev(x, tokens=None, lp=None, entropy=None, top=None, top_lp=None, ws=None, stream=None):
+    """How sure rows of logits are (pk_hip_logprobs_dev): x [rows, cols] float32,
+    its columns dense; tokens [rows, m] int32 and their log probabilities into lp
+    [rows, m]; the entropy into entropy [rows]; the k most probable ids into top
+    [rows, k] int32, their log probabilities into top_lp [rows, k]; each where it
+    is given. ws a uint8 tensor of logprobs_workspace(rows, cols, k) bytes."""
+    _is(x, "float32", "x", None)
+    device = x.get_device()
+    if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
+        raise PkHipError(PK_HIP_EINVAL, f"x: [rows, cols], its rows dense, not {tuple(x.shape)}")
+    rows, cols = x.shape
+    m, k = (0 if t is None else t.shape[-1] if t.dim() == 2 else -1 for t in (tokens, top))
+    for t, dtype, shape, what in ((tokens, "int32", (rows, m), "tokens"), (lp, "float32", (rows, m), "lp"),
+                                  (entropy, "float32", (rows,), "entropy"), (top, "int32", (rows, k), "top"),
+                                  (top_lp, "float32", (rows, k), "top_lp")):
+        if t is not None:
+            _is(t, dtype, what, device)
+            if tuple(t.shape) != shape or not t.is_contiguous():
+                raise PkHipError(PK_HIP_EINVAL, f"{what}: {shape}, contiguous, not {tuple(t.shape)}")
+    if ws is not None:
+        _is(ws, "uint8", "ws", device)
+        if not ws.is_contiguous():
+            raise PkHipError(PK_HIP_EINVAL, "ws is not contiguous")
+    if _device() != device:
+        raise PkHipError(PK_HIP_EINVAL, f"logits on device {device}, with {_device()} the current one")
+    _check(lib().pk_hip_logprobs_dev(x.data_ptr(), x.stride(0) if rows > 1 else cols, rows, cols, _dptr(tokens), m,
+                                     _dptr(lp), _dptr(entropy), k, _dptr(top), _dptr(top_lp), _dptr(ws),
+                                     ws.numel() if ws is not None else 0, _stream(stream)))

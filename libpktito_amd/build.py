@@ -7,7 +7,9 @@ shared library: the kernels (csrc/q8_kernels.hip, the quantizer, repack and
 products; csrc/layer_kernels.hip, the device-resident layer's float kernels;
 csrc/dec_kernels.hip, the decoder's fused per-token launches;
 csrc/cache_kernels.hip, the 4-bit cache of keys and values and its attention;
-csrc/window_kernels.hip, the attention with a window over whole segments)
+csrc/window_kernels.hip, the attention with a window over whole segments;
+csrc/plan_kernels.hip, the cache's tables of a step; csrc/prob_kernels.hip, log
+probabilities of rows of logits)
 and the runtime (csrc/pk_hip.cpp). The flags are part of the path's contract:
   -ffp-contract=off    no multiply and add the code writes apart is fused: the
                        epilogue's operations are the reference's, one rounding
@@ -33,7 +35,7 @@ ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libpkhip.so")
 SOURCES = [os.path.join(HERE, "csrc", n)
            for n in ("q8_kernels.hip", "q8_stream.hip", "layer_kernels.hip", "dec_kernels.hip", "cache_kernels.hip",
-                       "window_kernels.hip", "diag_kernels.hip", "pk_hip.cpp")]
+                       "window_kernels.hip", "plan_kernels.hip", "prob_kernels.hip", "diag_kernels.hip", "pk_hip.cpp")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 FLAGS = [

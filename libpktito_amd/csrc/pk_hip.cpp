@@ -1797,6 +1797,78 @@ int pk_hip_attention_window_dev(float *o, size_t os, const float *q, size_t qs, 
     return PK_HIP_OK;
 }
 
+int pk_hip_cache_plan_dev(const pk_hip_plan *p, const int32_t *add, const int32_t *fresh, uint32_t left,
+                          uint32_t sinks, void *stream) {
+    static const char who[] = "cache_plan_dev";
+    int e;
+    if (!p || (p->B && (!add || !p->table || !p->len || !p->state)) || !p->row0 || !p->pool || !p->told)
+        return fail(PK_HIP_EINVAL, "%s: a plan with its table, len, row0, state, pool and told, and what streams add", who);
+    if ((((uintptr_t)add | (uintptr_t)fresh | (uintptr_t)p->table | (uintptr_t)p->len | (uintptr_t)p->row0 |
+          (uintptr_t)p->state | (uintptr_t)p->pool | (uintptr_t)p->slot | (uintptr_t)p->told) & 3))
+        return fail(PK_HIP_EINVAL, "%s: arrays 4-byte aligned", who);
+    if (p->max_pages == 0 || p->max_pages > 1u << 24 || p->pages == 0 || p->pages > 1u << 24 || p->B > 65535 ||
+        p->rows > 1u << 21 || p->max_T > p->rows)
+        return fail(PK_HIP_EINVAL, "%s: 1 to 2^24 pages of the pool and of a stream, up to 65535 streams and 2^21 rows, "
+                                   "max_T up to rows", who);
+    if ((e = pk_hip_init()))
+        return e;
+    pkq8::PlanCall c = {};
+    c.add = add, c.fresh = fresh;
+    c.state = p->state, c.pool = p->pool, c.table = p->table, c.len = p->len, c.row0 = p->row0, c.slot = p->slot;
+    c.told = p->told;
+    c.B = p->B, c.max_pages = p->max_pages, c.rows = p->rows, c.max_T = p->max_T, c.pages = p->pages;
+    c.left = left == PK_HIP_UNLIMITED ? -1 : (int64_t)left;
+    c.kept = std::min((uint32_t)(((uint64_t)sinks + pkq8::kPage - 1) / pkq8::kPage), p->max_pages);
+    PK_LAUNCH(pkq8::launch_plan(c, (hipStream_t)stream), "plan launch");
+    g_kernel = "cache_plan";
+    return PK_HIP_OK;
+}
+
+size_t pk_hip_logprobs_workspace(uint32_t rows, uint32_t cols, uint32_t k) {
+    if (cols == 0 || cols > pkq8::kMostLogits || k > pkq8::kMostAlternatives || k > cols || rows > 1u << 21 ||
+        !pkq8::answer_fits(rows, cols))
+        return 0;
+    return pkq8::answer_workspace(rows, cols, k);
+}
+
+int pk_hip_logprobs_dev(const float *x, size_t xs, uint32_t rows, uint32_t cols, const int32_t *tokens, uint32_t m,
+                        float *lp, float *entropy, uint32_t k, int32_t *top, float *top_lp, void *ws, size_t ws_bytes,
+                        void *stream) {
+    static const char who[] = "logprobs_dev";
+    int e;
+    if (cols == 0 || cols > pkq8::kMostLogits || k > pkq8::kMostAlternatives || k > cols || rows > 1u << 21 ||
+        !pkq8::answer_fits(rows, cols))
+        return fail(PK_HIP_EINVAL, "%s: 1 to 2^20 columns, not %u, up to 32 alternatives and as many as columns, not %u, up to "
+                                   "2^21 rows and under 2^24 by 8192 columns, not %u", who, cols, k, rows);
+    if (m > 65535 || (rows && ((m ? !tokens || !lp : tokens || lp) || (k ? !top : top || top_lp) || (!m && !entropy && !k))))
+        return fail(PK_HIP_EINVAL, "%s: tokens and lp where m is set (up to 65535), top where k is, and something asked for",
+                    who);
+    if (rows && (!x || ((uintptr_t)x & 3) || (rows > 1 && xs < cols)))
+        return fail(PK_HIP_EINVAL, "%s: logits 4-byte aligned, rows at least %u apart", who, cols);
+    if (((uintptr_t)tokens | (uintptr_t)lp | (uintptr_t)entropy | (uintptr_t)top | (uintptr_t)top_lp) & 3)
+        return fail(PK_HIP_EINVAL, "%s: tokens and outputs 4-byte aligned", who);
+    const FloatRows in[2] = { { x, xs, cols, rows }, { (const float *)tokens, m, m, m ? rows : 0 } };
+    const FloatRows out[4] = { { lp, m, m, m ? rows : 0 }, { entropy, 1, 1, entropy ? rows : 0 },
+                               { (const float *)top, k, k, k ? rows : 0 }, { top_lp, k, k, top_lp ? rows : 0 } };
+    for (int i = 0; i < 4; i++)
+        for (int j = 0; j < 4; j++)
+            if ((j < 2 && rows_meet(out[i], in[j])) || (j < i && rows_meet(out[i], out[j])))
+                return fail(PK_HIP_EINVAL, "%s: outputs apart from the logits, the tokens and each other", who);
+    const size_t need = pkq8::answer_workspace(rows, cols, k);
+    if (need && (!ws || ((uintptr_t)ws & 15) || ws_bytes < need))
+        return fail(PK_HIP_EINVAL, "%s: 16-byte aligned workspace of %zu bytes, %zu needed", who, ws_bytes, need);
+    if ((e = pk_hip_init()))
+        return e;
+    if (rows == 0)
+        return PK_HIP_OK;
+    pkq8::AnswerCall c = {};
+    c.x = x, c.xs = xs, c.rows = rows, c.cols = cols, c.tokens = tokens, c.m = m;
+    c.lp = lp, c.entropy = entropy, c.k = k, c.top = top, c.top_lp = top_lp, c.ws = ws;
+    PK_LAUNCH(pkq8::launch_answer(c, (hipStream_t)stream), "log probabilities launch");
+    g_kernel = "logprobs";
+    return PK_HIP_OK;
+}
+
 int pk_hip_cache_move_dev(const pk_hip_cache *dst, const pk_hip_cache *src, const int32_t *pairs, uint32_t n,
                           int32_t *table, size_t entries, void *stream) {
     int e;

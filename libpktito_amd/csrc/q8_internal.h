@@ -262,6 +262,35 @@ int launch_window(const WindowCall &c, hipStream_t s);
 /* whether a launch holds the call's workgroups */
 bool window_fits(uint32_t B, uint32_t max_T, uint32_t H);
 
+/* Rows of logits: log probabilities of given tokens, entropy, the k most
+ * probable (prob_kernels.hip); as above. */
+struct AnswerCall {
+    const float *x;
+    uint64_t xs;
+    uint32_t rows, cols;
+    const int32_t *tokens;
+    uint32_t m;
+    float *lp, *entropy;
+    uint32_t k;
+    int32_t *top;
+    float *top_lp;
+    void *ws;
+};
+constexpr uint32_t kMostAlternatives = 32, kMostLogits = 1u << 20;
+size_t answer_workspace(uint32_t rows, uint32_t cols, uint32_t k);
+bool answer_fits(uint32_t rows, uint32_t cols);
+int launch_answer(const AnswerCall &c, hipStream_t s);
+
+/* The plan of a step of a cache's streams (plan_kernels.hip); as above. */
+struct PlanCall {
+    const int32_t *add, *fresh;
+    int32_t *state, *pool, *table, *len, *row0, *slot, *told;
+    uint32_t B, max_pages, rows, max_T, pages;
+    int64_t left;                           /* -1: no end */
+    uint32_t kept;                          /* the sinks' columns */
+};
+int launch_plan(const PlanCall &c, hipStream_t s);
+
 /* Measurement aids (diag_kernels.hip): an empty launch; a streaming read of
  * bytes (a multiple of 16) at p, 16-byte aligned. */
 int launch_empty(hipStream_t s);

@@ -85,8 +85,8 @@ class Tensor:
     def is_contiguous(self):
         return self.dense
 
-    def stride(self):
-        return self.strides
+    def stride(self, i=None):
+        return self.strides if i is None else self.strides[i]
 
     def data_ptr(self):
         return 16
