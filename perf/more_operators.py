@@ -438,7 +438,7 @@ def run(state):
                                          s["left"], s["right"], case["sinks"])
         else:
             s["cache"].attention(s["o"], 0, s["q"], s["streams"], case["H"], s["ws"], s["at"], s["left"], s["right"],
-                                 case["sinks"])
+                                 sinks=case["sinks"])
         return s["o"]
     if kind == "answer":
         return _plain_answer(s)
