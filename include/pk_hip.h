@@ -572,6 +572,18 @@ int pk_hip_attention_window_dev(float *o, size_t os, const float *q, size_t qs, 
                                 uint32_t dk, const pk_hip_positions *pos, uint32_t left, uint32_t right,
                                 uint32_t sinks, void *stream);
 
+/* The same over the cache (pk_hip_attention_cache_dev), for its streams' steps:
+ * the row of frame t also attends its stream's frames j < sinks, j <= t + right,
+ * that lie behind the window and whose page the stream holds; their position
+ * scores take distance left's row. sinks 0, or a window that all frames are in,
+ * is pk_hip_attention_cache_dev. Arguments, outputs and arithmetic are that
+ * one's, with the workspace of this one's arguments. */
+size_t pk_hip_attention_sinks_workspace(const pk_hip_cache *c, const pk_hip_streams *st, uint32_t H,
+                                        const pk_hip_positions *pos, uint32_t left, uint32_t right, uint32_t sinks);
+int pk_hip_attention_sinks_dev(float *o, size_t os, const float *q, size_t qs, const pk_hip_cache *c, uint32_t layer,
+                               const pk_hip_streams *st, uint32_t H, const pk_hip_positions *pos, uint32_t left,
+                               uint32_t right, uint32_t sinks, void *ws, size_t ws_bytes, void *stream);
+
 /* The plan of a step of a cache's streams, made on the device: what each stream
  * brings in, and out come the descriptor that the cache's calls take
  * (pk_hip_streams), pages taken from a pool for new frames, and pages that the

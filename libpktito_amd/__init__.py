@@ -210,6 +210,13 @@ _SIGS = {
                                                   ctypes.c_uint32, ctypes.POINTER(Positions), ctypes.c_uint32,
                                                   ctypes.c_uint32, ctypes.c_void_p, ctypes.c_size_t,
                                                   ctypes.c_void_p]),
+    "pk_hip_attention_sinks_workspace": (ctypes.c_size_t, [ctypes.POINTER(Cache), ctypes.POINTER(Streams),
+                                                           ctypes.c_uint32, ctypes.POINTER(Positions)] +
+                                         [ctypes.c_uint32] * 3),
+    "pk_hip_attention_sinks_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_size_t,
+                                                  ctypes.POINTER(Cache), ctypes.c_uint32, ctypes.POINTER(Streams),
+                                                  ctypes.c_uint32, ctypes.POINTER(Positions)] + [ctypes.c_uint32] * 3 +
+                                   [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "pk_hip_attention_window_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_size_t] * 4 +
                                     [ctypes.POINTER(SegmentRows)] + [ctypes.c_uint32] * 3 +
                                     [ctypes.POINTER(Positions)] + [ctypes.c_uint32] * 3 + [ctypes.c_void_p]),
@@ -857,37 +864,37 @@ class DeviceCache:
                                            *_rows(k, n, w, "k", self.device), *_rows(v, n, w, "v", self.device),
                                            ctypes.byref(streams.st), self._queue(stream, streams)))
 
-    def attention_workspace(self, streams, H, positions, left=None, right=None):
+    def attention_workspace(self, streams, H, positions, left=None, right=None, sinks=0):
         """Bytes of workspace an attention takes; positions as for attention,
         or True for a table that reaches as far as left and right do."""
         if positions is True:
             pos = Positions(16, 16, 16, 0xffffffff, 0x7fffffff)
         else:
             pos = self._positions(positions or None, H)
-        return lib().pk_hip_attention_cache_workspace(ctypes.byref(self.st), ctypes.byref(streams.st), _u32(H, "H"),
-                                                      ctypes.byref(pos) if pos else None,
-                                                      _reach(left, "left"), _reach(right, "right"))
+        return lib().pk_hip_attention_sinks_workspace(ctypes.byref(self.st), ctypes.byref(streams.st), _u32(H, "H"),
+                                                      ctypes.byref(pos) if pos else None, _reach(left, "left"),
+                                                      _reach(right, "right"), _u32(sinks, "sinks"))
 
     def _positions(self, positions, H):
         return _positions(positions, H, self.dk, self.device)
 
-    def attention(self, o, layer, q, streams, H, ws, positions=None, left=None, right=None, stream=None):
+    def attention(self, o, layer, q, streams, H, ws, positions=None, left=None, right=None, stream=None, sinks=0):
         """The attention of the rows q [rows, H * dk] to their streams' kept
-        frames, into o (pk_hip_attention_cache_dev); ws a uint8 tensor of
+        frames, into o (pk_hip_attention_sinks_dev); ws a uint8 tensor of
         attention_workspace(...) bytes, positions (p [n, H * dk], center,
         bias_u, bias_w) or None, left and right the frames attended behind and
-        ahead (None: all)."""
+        ahead (None: all), sinks the first frames that stay visible."""
         n, w = streams.rows, H * self.dk
         pos = self._positions(positions, H)
         if ws is not None:
             _is(ws, "uint8", "ws", self.device)
             if not ws.is_contiguous():                   # an expanded one has fewer bytes than elements
                 raise PkHipError(PK_HIP_EINVAL, "ws is not contiguous")
-        _check(lib().pk_hip_attention_cache_dev(*_rows(o, n, w, "o", self.device), *_rows(q, n, w, "q", self.device),
+        _check(lib().pk_hip_attention_sinks_dev(*_rows(o, n, w, "o", self.device), *_rows(q, n, w, "q", self.device),
                                                 ctypes.byref(self.st),
                                                 _u32(layer, "layer"), ctypes.byref(streams.st), _u32(H, "H"),
                                                 ctypes.byref(pos) if pos else None,
-                                                _reach(left, "left"), _reach(right, "right"),
+                                                _reach(left, "left"), _reach(right, "right"), _u32(sinks, "sinks"),
                                                 _dptr(ws), ws.numel() if ws is not None else 0,
                                                 self._queue(stream, streams)))
 

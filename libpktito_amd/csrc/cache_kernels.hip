@@ -321,7 +321,7 @@ struct CacheAttention {
     const uint8_t *data;                    /* the layer's records */
     uint32_t pages, G, H, dk;
     CacheStreams st;
-    int32_t left, right;                    /* clipped to what can occur */
+    int32_t left, right, sinks;             /* clipped to what can occur */
     float scale;                            /* 1 / sqrt(dk) */
     /* positions (p NULL: none), p's first row the distance left's */
     const float *p, *bias_u, *bias_w;
@@ -478,7 +478,7 @@ __global__ __launch_bounds__(64 * kPlaceWaves, place_residency(MT)) void cache_p
         if (r0 >= r1)
             continue;
         lo = min(lo, place_lo(sp, r1, a.left));
-        hi = max(hi, place_hi(sp, r0, a.left));
+        hi = max(hi, a.sinks ? max(place_hi(sp, r0, a.left), 0) : place_hi(sp, r0, a.left));
     }
     lo = -wave_max(-lo), hi = wave_max(hi);
     if (lane == 0)
@@ -575,10 +575,16 @@ struct Share {
     uint32_t g, b, grp, split;
     int32_t nrows, rr0;                     /* the stream's rows, the tile's first */
     int32_t pa, pb;                         /* the workgroup's pages, [pa, pb) of the stream */
+    int32_t far, skip;                      /* with sinks: of those that the tile reaches, the first `far` of which hold
+                                             * sinks before the window, and the others are `skip` further on */
     uint64_t unit;                          /* the tile among all of the call's */
+
+    /* page n of those, as one of the stream */
+    template <bool SINKS>
+    __device__ __forceinline__ int32_t page(int32_t n) const { return !SINKS ? n : n < far ? n : n + skip; }
 };
 
-template <int R>
+template <int R, bool SINKS>
 __device__ __forceinline__ bool share_of(const CacheAttention &a, Share &s, uint32_t splits) {
     uint32_t i = blockIdx.x;
     s.g = i % a.G, i /= a.G;
@@ -594,9 +600,12 @@ __device__ __forceinline__ bool share_of(const CacheAttention &a, Share &s, uint
     const int32_t t0 = s.rr0 / (int32_t)s.grp, t1 = min(s.rr0 + R - 1, s.nrows - 1) / (int32_t)s.grp;
     const int32_t j0 = cache_lo(s.sp.len + t0, a.left), j1 = cache_hi(s.sp.len + t1, a.right, s.sp.total);
     const int32_t p0 = j0 / (int32_t)kPage, p1 = j1 < j0 ? p0 : j1 / (int32_t)kPage + 1;
-    const int32_t each = (p1 - p0 + (int32_t)splits - 1) / (int32_t)splits;
-    s.pa = min(p0 + (int32_t)s.split * each, p1);
-    s.pb = min(s.pa + each, p1);
+    s.far = SINKS ? cache_far_pages(a.sinks, p0, j1) : 0;
+    s.skip = p0 - s.far;
+    const int32_t n0 = SINKS ? 0 : p0, n1 = SINKS ? s.far + p1 - p0 : p1;
+    const int32_t each = (n1 - n0 + (int32_t)splits - 1) / (int32_t)splits;
+    s.pa = min(n0 + (int32_t)s.split * each, n1);
+    s.pb = min(s.pa + each, n1);
     s.unit = unit_of(a, s.b, tile, s.g);
     return true;
 }
@@ -607,7 +616,7 @@ __device__ __forceinline__ uint32_t wave_id() { return __builtin_amdgcn_readfirs
 /* The pages that a wave takes, every W-th of its workgroup of W waves: 64 table
  * entries at a time, one a lane, those that are no page of the pool passed
  * over. */
-template <int W>
+template <int W, bool SINKS>
 struct Walk {
     int32_t first, ids;
     uint64_t left;
@@ -622,16 +631,26 @@ struct Walk {
                 return false;
             first += W * 64;
             const int32_t mine = first + W * (int32_t)(threadIdx.x & 63);
-            ids = mine < s.pb ? a.st.table[(uint64_t)s.b * a.st.max_pages + mine] : -1;
+            ids = mine < s.pb ? a.st.table[(uint64_t)s.b * a.st.max_pages + s.page<SINKS>(mine)] : -1;
             left = __ballot(cache_page_ok(ids, a.pages));
         }
         const int at = __builtin_ctzll(left);
         left &= left - 1;
-        pg = first + W * at;
+        pg = s.page<SINKS>(first + W * at);
         id = __builtin_amdgcn_readlane(ids, at);
         return true;
     }
 };
+
+/* Four frames' position scores at `at`, the first of them `ahead` frames before
+ * the window: those that are, sinks, take the score of the window's first. */
+__device__ __forceinline__ v4f far_places(const float *at, int32_t ahead) {
+    v4f x;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        x[i] = at[max(ahead, i)];
+    return x;
+}
 
 __device__ __forceinline__ float bf_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
@@ -721,7 +740,7 @@ __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttention a) {
     __shared__ v4f part[kGroups][kCols];
     __shared__ float tops[kGroups], sums[kGroups];
     Share s;
-    if (!share_of<R>(a, s, 1))
+    if (!share_of<R, false>(a, s, 1))
         return;
     const uint32_t r = blockIdx.y, group = threadIdx.x / kCols, c = threadIdx.x % kCols;
     const int32_t rr = s.rr0 + (int32_t)r;
@@ -780,14 +799,14 @@ constexpr float kSlack = 8.0f;
  * spill: 233). Short calls take 10 to 12 us whatever their bytes: a launch,
  * the stream, its table, a page's loads and three pages a wave. */
 enum { kNone, kMade, kOwn };
-template <int NS, int POS, int W>
+template <int NS, int POS, int W, bool SINKS>
 __global__ __launch_bounds__(64 * W) void cache_few_kernel(CacheAttention a) {
     constexpr uint32_t dk = 32 * NS, record = kPage * dk + 4 * kPage;
     constexpr uint32_t kRow = 72;           /* bfloat16 a row of pieces: 64 and a pad against bank conflicts */
     __shared__ float part[W][4][dk + 4], tops[W][4], sums[W][4];
     __shared__ __attribute__((aligned(16))) uint16_t prob[W][12][kRow];
     Share s;
-    if (!share_of<4>(a, s, a.splits))
+    if (!share_of<4, SINKS>(a, s, a.splits))
         return;
     const uint32_t lane = threadIdx.x & 63, wave = wave_id(), w = lane / 16, c = lane % 16;
 
@@ -860,8 +879,13 @@ __global__ __launch_bounds__(64 * W) void cache_few_kernel(CacheAttention a) {
             for (int st = 0; st < NS; st++)
                 kw[kt][st] = ((const uint32_t *)(rec + cache_key_at(dk, 4 * c + kt) + w * (4 * NS)))[st];
         ks = *(const v2u *)(rec + cache_key_scale_at(dk, 4 * c));
-        if constexpr (POS == kMade)
-            add = *(const v4f_u *)(place + pg * (int32_t)kPage);
+        if constexpr (POS == kMade) {
+            if (SINKS && pg * (int32_t)kPage < a.sinks) {
+                add = far_places(place + pg * (int32_t)kPage, pos - a.left - (pg * (int32_t)kPage + 4 * (int32_t)c));
+            } else {
+                add = *(const v4f_u *)(place + pg * (int32_t)kPage);
+            }
+        }
         if constexpr (POS == kOwn) {
 #pragma unroll
             for (int kt = 0; kt < 4; kt++) {
@@ -880,7 +904,7 @@ __global__ __launch_bounds__(64 * W) void cache_few_kernel(CacheAttention a) {
         vs = *(const v2u *)(rec + cache_value_scale_at(dk, 4 * c));
     };
 
-    Walk<W> walk(a, s);
+    Walk<W, SINKS> walk(a, s);
     int32_t pg = 0, id = 0;
     bool more = walk.next(a, s, pg, id);
     if (more) {
@@ -910,7 +934,7 @@ __global__ __launch_bounds__(64 * W) void cache_few_kernel(CacheAttention a) {
 #pragma unroll
         for (int kt = 0; kt < 4; kt++) {
             const float v = __builtin_fmaf((acc[kt][2] + acc[kt][1]) + acc[kt][0], bf_of(ks, kt), add[kt]);
-            x[kt] = j + kt >= lo && j + kt <= hi ? v : -INFINITY;
+            x[kt] = (j + kt >= lo || (SINKS && j + kt < a.sinks)) && j + kt <= hi ? v : -INFINITY;
             best = fmaxf(best, x[kt]);
         }
         more = walk.next(a, s, pg, id);
@@ -984,12 +1008,12 @@ __global__ __launch_bounds__(64 * W) void cache_few_kernel(CacheAttention a) {
  * another wave priority (127, 129), the queries' pieces in LDS (126; for three
  * waves, 250: spills), eight waves (147; where 16 streams of 14 rows leave half
  * the CUs idle, eight take 12.8 and four 14.5). */
-template <int NS, bool POS, int W>
+template <int NS, bool POS, int W, bool SINKS>
 __global__ __launch_bounds__(64 * W) void cache_many_kernel(CacheAttention a) {
     constexpr uint32_t dk = 32 * NS, record = kPage * dk + 4 * kPage;
     __shared__ float part[W][16][dk + 4], tops[W][16], sums[W][16];
     Share sh;
-    if (!share_of<16>(a, sh, a.splits))
+    if (!share_of<16, SINKS>(a, sh, a.splits))
         return;
     const CacheSpan &sp = sh.sp;
     const uint32_t lane = threadIdx.x & 63, wave = wave_id(), w = lane / 16;
@@ -1039,8 +1063,13 @@ __global__ __launch_bounds__(64 * W) void cache_many_kernel(CacheAttention a) {
             for (int st = 0; st < NS; st++)
                 kw[kt][st] = ((const uint32_t *)(rec + cache_key_at(dk, 16 * kt + lane % 16) + w * (4 * NS)))[st];
             ks[kt] = *(const v2u *)(rec + cache_key_scale_at(dk, 16 * kt + 4 * w));
-            if constexpr (POS)
-                add[kt] = *(const v4f_u *)(place + pg * (int32_t)kPage + 16 * kt);
+            if constexpr (POS) {
+                const int32_t f = pg * (int32_t)kPage + 16 * kt;
+                if (SINKS && pg * (int32_t)kPage < a.sinks)
+                    add[kt] = far_places(place + f, pos - a.left - (f + 4 * (int32_t)w));
+                else
+                    add[kt] = *(const v4f_u *)(place + f);
+            }
         }
     };
     auto load_values = [&](const uint8_t *rec) {
@@ -1052,7 +1081,7 @@ __global__ __launch_bounds__(64 * W) void cache_many_kernel(CacheAttention a) {
             vs[kt] = *(const v2u *)(rec + cache_value_scale_at(dk, 16 * kt + 4 * w));
     };
 
-    Walk<W> walk(a, sh);
+    Walk<W, SINKS> walk(a, sh);
     int32_t pg = 0, id = 0;
     bool more = walk.next(a, sh, pg, id);
     if (more) {
@@ -1083,7 +1112,7 @@ __global__ __launch_bounds__(64 * W) void cache_many_kernel(CacheAttention a) {
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 const int32_t f = j + 16 * (i / 4) + i % 4;
-                s[i / 4][i % 4] = f >= lo && f <= hi ? s[i / 4][i % 4] : -INFINITY;
+                s[i / 4][i % 4] = (f >= lo || (SINKS && f < a.sinks)) && f <= hi ? s[i / 4][i % 4] : -INFINITY;
             }
         }
         more = walk.next(a, sh, pg, id);
@@ -1273,13 +1302,13 @@ struct Deal {
  * distances takes 7.7 us so and 10.0 with a launch of their own, by 181 11.5 and
  * 11.7; 16 rows by 71 8.0 and 9.8, by 181 12.1 and 11.6; 64 rows by 71 14.3 and
  * 12.4 (each stream reads the table itself, in pieces of 16 bytes). */
-static Deal deal(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, int32_t left, int32_t right) {
+static Deal deal(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, int32_t left, int32_t right, int32_t sinks) {
     Deal d;
     const uint32_t rows = st.max_T * (H / G);
     d.rows = rows <= 4 ? 4 : 16;
     d.tiles = (rows + d.rows - 1) / d.rows;
     d.units = (uint64_t)st.B * G * d.tiles;
-    d.pages = cache_tile_pages(st.max_pages, left, right);
+    d.pages = std::min(cache_tile_pages(st.max_pages, left, right) + ((uint32_t)sinks + kPage - 1) / kPage, st.max_pages);
     d.own = rows == 1 && st.B <= 16 && left + right < 100;
     d.splits = 1, d.waves = 4;
     if (d.units == 0 || d.units > 256)
@@ -1321,13 +1350,15 @@ static Space space(const CacheStreams &st, uint32_t H, uint32_t dk, bool positio
 }
 
 size_t cache_attention_workspace(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, bool positions,
-                                 int32_t left, int32_t right) {
-    const Space s = space(st, H, dk, positions, (uint32_t)left + (uint32_t)right + 1, deal(st, G, H, dk, left, right));
+                                 int32_t left, int32_t right, int32_t sinks) {
+    const Space s = space(st, H, dk, positions, (uint32_t)left + (uint32_t)right + 1,
+                          deal(st, G, H, dk, left, right, sinks));
     return s.place + s.pieces + s.parts;
 }
 
-bool cache_attention_fits(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, int32_t left, int32_t right) {
-    const Deal d = deal(st, G, H, dk, left, right);
+bool cache_attention_fits(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, int32_t left, int32_t right,
+                          int32_t sinks) {
+    const Deal d = deal(st, G, H, dk, left, right, sinks);
     return d.units <= kMostGroups / d.splits;
 }
 
@@ -1352,7 +1383,7 @@ static void place(const CacheAttention &a, hipStream_t s) {
     cache_place_kernel<NS, RT, MT, PRE><<<dim3((runs + steps - 1) / steps, a.H, blocks), 64 * kPlaceWaves, 0, s>>>(a, (int32_t)steps);
 }
 
-template <int NS>
+template <int NS, bool SINKS>
 static void attend(const CacheAttention &a, const Deal &d, hipStream_t s) {
     if (a.p && !d.own) {
         if (place_cut(a.st.rows, a.bw)) {
@@ -1370,15 +1401,15 @@ static void attend(const CacheAttention &a, const Deal &d, hipStream_t s) {
     const uint32_t grid = (uint32_t)(d.units * d.splits);
     const uint32_t threads = 64 * d.waves;
     if (d.rows == 4 && a.p && d.own)
-        cache_few_kernel<NS, kOwn, 4><<<grid, threads, 0, s>>>(a);
+        cache_few_kernel<NS, kOwn, 4, SINKS><<<grid, threads, 0, s>>>(a);
     else if (d.rows == 4 && a.p)
-        (d.waves == 8 ? cache_few_kernel<NS, kMade, 8> : cache_few_kernel<NS, kMade, 4>)<<<grid, threads, 0, s>>>(a);
+        (d.waves == 8 ? cache_few_kernel<NS, kMade, 8, SINKS> : cache_few_kernel<NS, kMade, 4, SINKS>)<<<grid, threads, 0, s>>>(a);
     else if (d.rows == 4)
-        (d.waves == 8 ? cache_few_kernel<NS, kNone, 8> : cache_few_kernel<NS, kNone, 4>)<<<grid, threads, 0, s>>>(a);
+        (d.waves == 8 ? cache_few_kernel<NS, kNone, 8, SINKS> : cache_few_kernel<NS, kNone, 4, SINKS>)<<<grid, threads, 0, s>>>(a);
     else if (a.p)
-        (d.waves == 8 ? cache_many_kernel<NS, true, 8> : cache_many_kernel<NS, true, 4>)<<<grid, threads, 0, s>>>(a);
+        (d.waves == 8 ? cache_many_kernel<NS, true, 8, SINKS> : cache_many_kernel<NS, true, 4, SINKS>)<<<grid, threads, 0, s>>>(a);
     else
-        (d.waves == 8 ? cache_many_kernel<NS, false, 8> : cache_many_kernel<NS, false, 4>)<<<grid, threads, 0, s>>>(a);
+        (d.waves == 8 ? cache_many_kernel<NS, false, 8, SINKS> : cache_many_kernel<NS, false, 4, SINKS>)<<<grid, threads, 0, s>>>(a);
     if (d.splits > 1) {
         if (d.rows == 4)
             cache_join_kernel<4, NS><<<dim3(grid / d.splits, std::min(d.rows, a.st.max_T * (a.H / a.G))), 256, 0, s>>>(a);
@@ -1392,21 +1423,21 @@ int launch_cache_attention(const CacheAttentionCall &c, hipStream_t s) {
     a.o = c.o, a.os = c.os, a.q = c.q, a.qs = c.qs;
     a.data = c.data, a.pages = c.pages, a.G = c.G, a.H = c.H, a.dk = c.dk;
     a.st = c.st;
-    a.left = c.left, a.right = c.right;
+    a.left = c.left, a.right = c.right, a.sinks = c.sinks;
     a.scale = 1.0f / sqrtf((float)c.dk);
     a.p = c.p, a.bias_u = c.bias_u, a.bias_w = c.bias_w;
     a.bw = (uint32_t)c.left + (uint32_t)c.right + 1;
-    const Deal d = deal(c.st, c.G, c.H, c.dk, c.left, c.right);
+    const Deal d = deal(c.st, c.G, c.H, c.dk, c.left, c.right, c.sinks);
     a.tiles = d.tiles, a.splits = d.splits;
     const Space sp = space(c.st, c.H, c.dk, c.p != nullptr, a.bw, d);
     a.place = (float *)c.ws;
     a.pieces = (char *)c.ws + sp.place;
     a.parts = (float *)((char *)c.ws + sp.place + sp.pieces);
     switch (c.dk / 32) {
-    case 1: attend<1>(a, d, s); break;
-    case 2: attend<2>(a, d, s); break;
-    case 3: attend<3>(a, d, s); break;
-    case 4: attend<4>(a, d, s); break;
+    case 1: a.sinks ? attend<1, true>(a, d, s) : attend<1, false>(a, d, s); break;
+    case 2: a.sinks ? attend<2, true>(a, d, s) : attend<2, false>(a, d, s); break;
+    case 3: a.sinks ? attend<3, true>(a, d, s) : attend<3, false>(a, d, s); break;
+    case 4: a.sinks ? attend<4, true>(a, d, s) : attend<4, false>(a, d, s); break;
     default: return -2;
     }
     return hipPeekAtLastError() == hipSuccess ? 0 : -1;

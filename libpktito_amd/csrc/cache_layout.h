@@ -164,6 +164,14 @@ PK_HD int32_t cache_hi(int32_t pos, int32_t right, int32_t total) {
     return h < (int64_t)total - 1 ? (int32_t)h : total - 1;
 }
 
+/* The pages that hold sinks and lie before a window's first, p0, j1 the last
+ * frame that any row of the tile attends (-1: none). */
+PK_HD int32_t cache_far_pages(int32_t sinks, int32_t p0, int32_t j1) {
+    const int32_t n = sinks < j1 + 1 ? sinks : j1 + 1;
+    const int32_t pages = n > 0 ? (n - 1) / (int32_t)kPage + 1 : 0;
+    return pages < p0 ? pages : p0;
+}
+
 /* The pages that a tile of rows reaches, at most: its rows' positions are up
  * to 15 apart, so its frames are at most left + right + 16 in a row, which
  * touch one page more than they fill. */

@@ -1655,7 +1655,8 @@ static int check_positions(const pk_hip_positions *pos, const char *who) {
 /* The window that an attention's rows have: the asked one, no wider than the
  * rows can reach or than the positions' table does. */
 static int attention_window(const pk_hip_cache *c, const pk_hip_streams *st, uint32_t H, const pk_hip_positions *pos,
-                            uint32_t left, uint32_t right, const char *who, int32_t *l, int32_t *r) {
+                            uint32_t left, uint32_t right, uint32_t sinks, const char *who, int32_t *l, int32_t *r,
+                            int32_t *n) {
     int e;
     if ((e = check_streams(st, who)))
         return e;
@@ -1673,7 +1674,9 @@ static int attention_window(const pk_hip_cache *c, const pk_hip_streams *st, uin
     }
     *l = (int32_t)lo;
     *r = (int32_t)hi;
-    if (!pkq8::cache_attention_fits(streams_of(st), c->heads, H, c->dk, *l, *r))
+    /* no frame is behind a window that reaches as far as any row can */
+    *n = lo < (uint32_t)pkq8::cache_most_left(st->max_pages, st->max_T) ? (int32_t)std::min(sinks, st->max_pages * pkq8::kPage) : 0;
+    if (!pkq8::cache_attention_fits(streams_of(st), c->heads, H, c->dk, *l, *r, *n))
         return fail(PK_HIP_EINVAL, "%s: %u streams of up to %u rows, %u heads: more than a launch holds", who, st->B,
                     st->max_T, H);
     if (pos && !pkq8::cache_places_fit(streams_of(st), H, *l, *r))
@@ -1682,35 +1685,40 @@ static int attention_window(const pk_hip_cache *c, const pk_hip_streams *st, uin
     return PK_HIP_OK;
 }
 
-size_t pk_hip_attention_cache_workspace(const pk_hip_cache *c, const pk_hip_streams *st, uint32_t H,
-                                        const pk_hip_positions *pos, uint32_t left, uint32_t right) {
-    int32_t l, r;
-    if (attention_window(c, st, H, pos, left, right, "attention_cache_workspace", &l, &r))
+size_t pk_hip_attention_sinks_workspace(const pk_hip_cache *c, const pk_hip_streams *st, uint32_t H,
+                                        const pk_hip_positions *pos, uint32_t left, uint32_t right, uint32_t sinks) {
+    int32_t l, r, n;
+    if (attention_window(c, st, H, pos, left, right, sinks, "attention_cache_workspace", &l, &r, &n))
         return 0;
-    return pkq8::cache_attention_workspace(streams_of(st), c->heads, H, c->dk, pos != nullptr, l, r);
+    return pkq8::cache_attention_workspace(streams_of(st), c->heads, H, c->dk, pos != nullptr, l, r, n);
 }
 
-int pk_hip_attention_cache_dev(float *o, size_t os, const float *q, size_t qs, const pk_hip_cache *c, uint32_t layer,
-                               const pk_hip_streams *st, uint32_t H, const pk_hip_positions *pos, uint32_t left,
-                               uint32_t right, void *ws, size_t ws_bytes, void *stream) {
+size_t pk_hip_attention_cache_workspace(const pk_hip_cache *c, const pk_hip_streams *st, uint32_t H,
+                                        const pk_hip_positions *pos, uint32_t left, uint32_t right) {
+    return pk_hip_attention_sinks_workspace(c, st, H, pos, left, right, 0);
+}
+
+static int attention_cache(float *o, size_t os, const float *q, size_t qs, const pk_hip_cache *c, uint32_t layer,
+                           const pk_hip_streams *st, uint32_t H, const pk_hip_positions *pos, uint32_t left,
+                           uint32_t right, uint32_t sinks, void *ws, size_t ws_bytes, void *stream, const char *who) {
     int e;
     pkq8::CacheAttentionCall a = {};
-    if ((e = check_cache(c, "attention_cache_dev")) ||
-        (e = attention_window(c, st, H, pos, left, right, "attention_cache_dev", &a.left, &a.right)))
+    if ((e = check_cache(c, who)) ||
+        (e = attention_window(c, st, H, pos, left, right, sinks, who, &a.left, &a.right, &a.sinks)))
         return e;
     if (layer >= c->layers)
-        return fail(PK_HIP_EINVAL, "attention_cache_dev: layer %u of %u", layer, c->layers);
+        return fail(PK_HIP_EINVAL, "%s: layer %u of %u", who, layer, c->layers);
     const uint64_t width = (uint64_t)H * c->dk;
-    if (st->rows && ((e = check_rows(o, os, width, st->rows, "attention_cache_dev", "o")) ||
-                     (e = check_rows(q, qs, width, st->rows, "attention_cache_dev", "q"))))
+    if (st->rows && ((e = check_rows(o, os, width, st->rows, who, "o")) ||
+                     (e = check_rows(q, qs, width, st->rows, who, "q"))))
         return e;
     if ((const float *)o == q && os != qs)
-        return fail(PK_HIP_EINVAL, "attention_cache_dev: an output over its queries has their stride");
+        return fail(PK_HIP_EINVAL, "%s: an output over its queries has their stride", who);
     a.st = streams_of(st);
-    const size_t need = pkq8::cache_attention_workspace(a.st, c->heads, H, c->dk, pos != nullptr, a.left, a.right);
+    const size_t need = pkq8::cache_attention_workspace(a.st, c->heads, H, c->dk, pos != nullptr, a.left, a.right,
+                                                         a.sinks);
     if (need && (!ws || ((uintptr_t)ws & 15) || ws_bytes < need))
-        return fail(PK_HIP_EINVAL, "attention_cache_dev: 16-byte aligned workspace of %zu bytes, %zu needed", ws_bytes,
-                    need);
+        return fail(PK_HIP_EINVAL, "%s: 16-byte aligned workspace of %zu bytes, %zu needed", who, ws_bytes, need);
     if ((e = pk_hip_init()))
         return e;
     if (st->B == 0 || st->max_T == 0)
@@ -1726,6 +1734,20 @@ int pk_hip_attention_cache_dev(float *o, size_t os, const float *q, size_t qs, c
     PK_LAUNCH(pkq8::launch_cache_attention(a, (hipStream_t)stream), "cache attention launch");
     g_kernel = "cache_attention";
     return PK_HIP_OK;
+}
+
+int pk_hip_attention_cache_dev(float *o, size_t os, const float *q, size_t qs, const pk_hip_cache *c, uint32_t layer,
+                               const pk_hip_streams *st, uint32_t H, const pk_hip_positions *pos, uint32_t left,
+                               uint32_t right, void *ws, size_t ws_bytes, void *stream) {
+    return attention_cache(o, os, q, qs, c, layer, st, H, pos, left, right, 0, ws, ws_bytes, stream,
+                           "attention_cache_dev");
+}
+
+int pk_hip_attention_sinks_dev(float *o, size_t os, const float *q, size_t qs, const pk_hip_cache *c, uint32_t layer,
+                               const pk_hip_streams *st, uint32_t H, const pk_hip_positions *pos, uint32_t left,
+                               uint32_t right, uint32_t sinks, void *ws, size_t ws_bytes, void *stream) {
+    return attention_cache(o, os, q, qs, c, layer, st, H, pos, left, right, sinks, ws, ws_bytes, stream,
+                           "attention_sinks_dev");
 }
 
 /* Rows of floats: n of width w, stride s apart. */

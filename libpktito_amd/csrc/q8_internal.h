@@ -229,14 +229,15 @@ struct CacheAttentionCall {
     const uint8_t *data;
     uint32_t pages, G, H, dk;
     CacheStreams st;
-    int32_t left, right;
+    int32_t left, right, sinks;
     const float *p, *bias_u, *bias_w;
     void *ws;
 };
 size_t cache_attention_workspace(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, bool positions,
-                                 int32_t left, int32_t right);
+                                 int32_t left, int32_t right, int32_t sinks);
 /* whether a launch holds the call's workgroups */
-bool cache_attention_fits(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, int32_t left, int32_t right);
+bool cache_attention_fits(const CacheStreams &st, uint32_t G, uint32_t H, uint32_t dk, int32_t left, int32_t right,
+                          int32_t sinks);
 /* and those of its position scores, in a workspace of 2^48 bytes at most */
 bool cache_places_fit(const CacheStreams &st, uint32_t H, int32_t left, int32_t right);
 int launch_cache_attention(const CacheAttentionCall &c, hipStream_t s);

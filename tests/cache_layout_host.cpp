@@ -18,6 +18,7 @@ uint32_t t_key_scale_at(uint32_t dk, uint32_t f) { return cache_key_scale_at(dk,
 uint32_t t_value_scale_at(uint32_t dk, uint32_t f) { return cache_value_scale_at(dk, f); }
 int t_page_ok(int32_t id, uint32_t pages) { return cache_page_ok(id, pages); }
 uint32_t t_tile_pages(uint32_t max_pages, int32_t left, int32_t right) { return cache_tile_pages(max_pages, left, right); }
+int32_t t_far_pages(int32_t sinks, int32_t p0, int32_t j1) { return cache_far_pages(sinks, p0, j1); }
 uint32_t t_place_stride(uint32_t bw) { return place_stride(bw); }
 uint32_t t_place_pad(void) { return kPlacePad; }
 int32_t t_lo(int32_t pos, int32_t left) { return cache_lo(pos, left); }
