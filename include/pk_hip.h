@@ -553,7 +553,7 @@ int pk_hip_pool_restore(pk_hip_pool *pool, const int32_t *pairs, uint32_t n);
  * q and o are [rows][H * dk], k and v [rows][G * dk], H a multiple of G (each
  * kept head shared among H / G consecutive ones), dk 32, 64, 96 or 128; row r
  * of x at x + r * its stride (qs, ks, vs, os), 16-byte aligned, strides
- * multiples of 4. o may be q with os = qs; an o that shares memory with k, v or
+ * multiples of 4, ks and vs up to 2^25. o may be q with os = qs; an o that shares memory with k, v or
  * the positions is refused. Rows of no segment are left as they were. Products
  * and sums in 32 bits, not held to a bit pattern (pk_hip_attention_dev's are
  * the reference's, core/encoder.c:280-327, which has no window). A row's

@@ -1789,6 +1789,8 @@ int pk_hip_attention_window_dev(float *o, size_t os, const float *q, size_t qs, 
     if (n && ((e = check_rows(o, os, width, n, who, "o")) || (e = check_rows(q, qs, width, n, who, "q")) ||
               (e = check_rows(k, ks, kept, n, who, "k")) || (e = check_rows(v, vs, kept, n, who, "v"))))
         return e;
+    if (n > 1 && std::max(ks, vs) > 1u << 25)
+        return fail(PK_HIP_EINVAL, "%s: keys and values with strides up to 2^25 floats", who);
     pkq8::WindowCall a = {};
     uint32_t lo = std::min(left, most), hi = std::min(right, most);
     if (pos) {
@@ -1810,7 +1812,7 @@ int pk_hip_attention_window_dev(float *o, size_t os, const float *q, size_t qs, 
         return e;
     if (sg->B == 0 || sg->max_T == 0)
         return PK_HIP_OK;
-    a.o = o, a.os = os, a.q = q, a.qs = qs, a.k = k, a.ks = ks, a.v = v, a.vs = vs;
+    a.o = o, a.os = os, a.q = q, a.qs = qs, a.k = k, a.ks = n > 1 ? ks : 0, a.v = v, a.vs = n > 1 ? vs : 0;
     a.row0 = sg->row0, a.B = sg->B, a.rows = n, a.max_T = sg->max_T;
     a.H = H, a.G = G, a.dk = dk;
     a.left = (int32_t)lo, a.right = (int32_t)hi, a.sinks = (int32_t)std::min(sinks, sg->max_T);

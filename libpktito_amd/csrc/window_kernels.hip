@@ -21,29 +21,31 @@ typedef float w4f __attribute__((ext_vector_type(4)));
 struct WindowAttention {
     float *o;
     const float *q, *k, *v;
-    uint64_t os, qs, ks, vs;
+    const float *p, *bias_u, *bias_w;       /* p's first row the distance left's; NULL: no positions */
     const int32_t *row0;
+    uint64_t os, qs, ks, vs;
     uint32_t B, rows, max_T, H, G;
     int32_t left, right, sinks;             /* clipped to what can occur */
-    float scale;                            /* log2(e) / sqrt(dk) */
-    const float *p, *bias_u, *bias_w;       /* p's first row the distance left's; NULL: no positions */
-    uint32_t bw;                            /* its rows, left + right + 1 */
+    uint32_t bw;                            /* the rows of p, left + right + 1 */
     uint32_t tiles;                         /* a segment's tiles of rows */
+    float scale;                            /* log2(e) / sqrt(dk) */
 };
 
-/* A workgroup's part: rows [i0, i0 + R) of a segment of T at row r0, one head. */
+/* A wave's part: rows [i0, i0 + R) of a segment of T at row r0, one head; its
+ * workgroup has N tiles one after another. */
 struct WindowTile {
     int32_t r0, T, i0;
     uint32_t h, g;
 };
 
-template <int R>
-__device__ __forceinline__ bool window_tile(const WindowAttention &a, WindowTile &s) {
+template <int R, int N>
+__device__ __forceinline__ bool window_tile(const WindowAttention &a, WindowTile &s, uint32_t tile) {
     uint32_t i = blockIdx.x;
     s.h = i % a.H, i /= a.H;
     s.g = s.h / (a.H / a.G);
-    s.i0 = (int32_t)(i % a.tiles) * R;
-    const uint32_t b = i / a.tiles;
+    const uint32_t groups = (a.tiles + N - 1) / N;
+    s.i0 = (int32_t)(i % groups * N + tile) * R;
+    const uint32_t b = i / groups;
     s.r0 = cache_clip(a.row0[b], 0, (int32_t)a.rows);
     s.T = cache_clip(cache_clip(a.row0[b + 1], 0, (int32_t)a.rows) - s.r0, 0, (int32_t)a.max_T);
     return s.i0 < s.T;
@@ -74,10 +76,10 @@ struct WindowShape {
  * table's first row). */
 template <int NS, bool POS>
 struct WindowQueries {
-    w4f c[2 * NS], p[POS ? 2 * NS : 1];
+    w4f c[2 * NS];
     float behind;
 
-    __device__ __forceinline__ void load(const WindowAttention &a, const WindowTile &s, int32_t i) {
+    __device__ __forceinline__ void load(const WindowAttention &a, const WindowTile &s, int32_t i, w4f (*at_place)[64]) {
         constexpr uint32_t dk = 32 * NS;
         const uint32_t w = (threadIdx.x & 63) / 16;
         const float *src = a.q + (uint64_t)(s.r0 + min(i, s.T - 1)) * a.qs + s.h * dk + 4 * w;
@@ -88,12 +90,13 @@ struct WindowQueries {
             if constexpr (POS) {
                 const uint32_t d = s.h * dk + 4 * w + 16 * t;
                 c[t] = (x + *(const w4f *)(a.bias_u + d)) * a.scale;
-                p[t] = (x + *(const w4f *)(a.bias_w + d)) * a.scale;
+                const w4f p = (x + *(const w4f *)(a.bias_w + d)) * a.scale;
+                at_place[t][threadIdx.x & 63] = p;
                 if (a.sinks) {
                     const w4f far = *(const w4f *)(a.p + d);
 #pragma unroll
                     for (int j = 0; j < 4; j++)
-                        behind = __builtin_fmaf(p[t][j], far[j], behind);
+                        behind = __builtin_fmaf(p[j], far[j], behind);
                 }
             } else {
                 c[t] = x * a.scale;
@@ -121,7 +124,7 @@ __device__ __forceinline__ void window_softmax(w4f (&s)[KT], float &top, float &
     if (__any(best > top + kWindowSlack)) {
         best = fmaxf(best, __shfl_xor(best, 16));
         best = fmaxf(best, __shfl_xor(best, 32));
-        const float now = fmaxf(top, best);
+        const float now = best > top + kWindowSlack ? best : top;   /* by the query's own scores: no other row's bits */
         const float scale = __builtin_amdgcn_exp2f(top - (now == -INFINITY ? 0.0f : now));
         top = now;
         sum *= scale;
@@ -143,183 +146,268 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_wave_barrier();
 }
 
-/* Sixteen rows a workgroup, its waves a run of 32 frames each in turn, met in
- * LDS at the end: for calls of few tiles, where one wave's pass over a row's
- * frames is what takes time. Operands come straight from memory. A frame j's
- * place scores are products with 47 rows of the table, x = left - (row - j); a
- * lane's are another column's, so they pass through LDS. */
+/* Sixteen rows a tile, W waves to a tile, each a run of its steps of 16 frames:
+ * the sinks' steps first, then the window's, which begins at the tile's first
+ * frame of it whatever that is a multiple of (no step is taken for alignment).
+ * Operands come straight from memory: 24 KB a step for 96 matrix instructions,
+ * whose 3072 cycles hide the loads of the step after, each issued into the
+ * registers of this one's as those have been used.
+ *
+ * A frame j's place scores are products with the rows x = left - (row - j) of
+ * the table, 31 of them for 16 rows and frames; the first 16 of those are the
+ * step before's last, so each step makes 16 more. A lane's are another column's
+ * than its scores', so they pass through LDS. */
 template <int NS, bool POS, int W>
-__global__ __launch_bounds__(64 * W, 1) void window_few_kernel(WindowAttention a) {
+__global__ __launch_bounds__(W > 4 ? 64 * W : 256, 2) void window_kernel(WindowAttention a) {
     using S = WindowShape<NS>;
-    constexpr int KT = 2, kKeys = 16 * KT, PT = KT + 1, kRow = 16 * PT + 4;
-    __shared__ __attribute__((aligned(16))) float part[W][16][S::dk + 4];
-    __shared__ __attribute__((aligned(16))) float place[POS ? W : 1][16][kRow];
-    __shared__ float tops[W][16], sums[W][16];
-    WindowTile s;
-    if (!window_tile<16>(a, s))
-        return;
+    constexpr int kWaves = W > 4 ? W : 4, kTiles = kWaves / W, kRow = 36;
+    __shared__ __attribute__((aligned(16))) float place[POS ? kWaves : 1][16][kRow];
+    __shared__ __attribute__((aligned(16))) float rows[kWaves][16][S::dk + 4];
+    __shared__ w4f query[POS ? kWaves : 1][S::NT][64];      /* the place's operands, which registers have no room for */
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    WindowTile s;
+    if (!window_tile<16, kTiles>(a, s, wave / W))
+        return;
     const int32_t c = (int32_t)(lane % 16), w = (int32_t)(lane / 16), i = s.i0 + c;
     WindowQueries<NS, POS> q;
-    q.load(a, s, i);
-    float top = -INFINITY, sum = 0.0f;
-    w4f o[2 * NS] = {};
+    q.load(a, s, i, query[POS ? wave : 0]);
+    float top, sum;
+    w4f o[2 * NS];
 
-    /* the runs that the tile reaches: the sinks' first, then the window's */
-    const int32_t w0 = max(s.i0 - a.left, 0) / kKeys, w1 = min(s.i0 + 15 + a.right, s.T - 1) / kKeys + 1;
-    const int32_t ns = min((min(a.sinks, s.T) + kKeys - 1) / kKeys, w0);
-    const int32_t runs = ns + w1 - w0;
-#pragma unroll 1
-    for (int32_t n = (int32_t)wave; n < runs; n += W) {
-        const int32_t j0 = kKeys * (n < ns ? n : n - ns + w0);
-        w4f x[KT] = {};
+    /* the window's frames [lo, hi] of any of the rows, the sinks [0, far) before them, the steps of both */
+    const int32_t lo = max(s.i0 - a.left, 0), hi = min(s.i0 + 15 + a.right, s.T - 1), far = min(a.sinks, lo);
+    const int32_t ns = (far + 15) / 16, steps = ns + (hi - lo) / 16 + 1, each = (steps + W - 1) / W;
+    const int32_t n0 = min((int32_t)(wave % W) * each, steps), n1 = min(n0 + each, steps);
+    const int32_t last = min(i + a.right, s.T - 1);         /* the lane's query's */
+    auto first_of = [&](int32_t n) { return n < ns ? 16 * n : lo + 16 * (n - ns); };
+
+    w4f key[2][NS], pos[2][NS], before;
+    typename S::vec v[4][S::NB];
+    /* Sixteen rows of keys or of the table, 128 bytes of one to eight lanes (to a lane of its own the 16 bytes that the
+     * instruction wants of it, each row's would be cache lookups of their own, four times as many), put where operands are
+     * read from. Offsets from a step's first row are 32 bits, as no stride passes 2^25 floats. */
+    const int32_t lr = (int32_t)(lane / 8), lc = 4 * (int32_t)(lane % 8);
+    auto load_keys = [&](int32_t n) {
+        const int32_t j0 = first_of(n);
+        const float *src = a.k + (uint64_t)(s.r0 + j0) * a.ks + s.g * S::dk + lc;
 #pragma unroll
-        for (int kt = 0; kt < KT; kt++) {
-            const float *src = a.k + (uint64_t)(s.r0 + min(j0 + 16 * kt + c, s.T - 1)) * a.ks + s.g * S::dk + 4 * w;
-            w4f key[S::NT];
+        for (int half = 0; half < 2; half++) {
+            const uint32_t off = (uint32_t)min(lr + 8 * half, s.T - 1 - j0) * (uint32_t)a.ks;
 #pragma unroll
-            for (int t = 0; t < S::NT; t++)
-                key[t] = *(const w4f *)(src + 16 * t);
-#pragma unroll
-            for (int t = 0; t < S::NT; t++)
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    x[kt] = wmfma(key[t][j], q.c[t][j], x[kt]);
+            for (int t = 0; t < NS; t++)
+                key[half][t] = *(const w4f *)(src + off + 32 * t);
         }
+    };
+    auto put = [&](const w4f (&x)[2][NS]) {
+        wave_sync();
+#pragma unroll
+        for (int half = 0; half < 2; half++)
+#pragma unroll
+            for (int t = 0; t < NS; t++)
+                *(w4f *)&rows[wave][lr + 8 * half][lc + 32 * t] = x[half][t];
+        wave_sync();
+    };
+    auto operand = [&](int t) { return *(const w4f *)&rows[wave][c][16 * t + 4 * w]; };
+    const uint32_t value_off = 4 * (uint32_t)w * (uint32_t)a.vs + S::VW * c;
+    auto load_values = [&](int32_t n) {
+        const int32_t j0 = first_of(n);
+        const float *src = a.v + (uint64_t)(s.r0 + j0) * a.vs + s.g * S::dk;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const uint32_t off = j0 + 15 < s.T ? value_off + r * (uint32_t)a.vs
+                                               : (uint32_t)min(4 * w + r, s.T - 1 - j0) * (uint32_t)a.vs + S::VW * c;
+#pragma unroll
+            for (int b = 0; b < S::NB; b++)
+                v[r][b] = *(const typename S::vec *)(src + off + 16 * S::VW * b);
+        }
+    };
+    /* the table's rows x to x + 15 */
+    auto load_places = [&](int32_t x) {
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const uint32_t row = (uint32_t)cache_clip(x + lr + 8 * half, 0, (int32_t)a.bw - 1);
+            const float *src = a.p + (uint64_t)row * (a.H * S::dk) + s.h * S::dk + lc;
+#pragma unroll
+            for (int t = 0; t < NS; t++)
+                pos[half][t] = *(const w4f *)(src + 32 * t);
+        }
+    };
+    auto places = [&]() {
+        w4f r = {};
+#pragma unroll
+        for (int t = 0; t < S::NT; t++) {
+            const w4f x = operand(t), y = query[wave][t][lane];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                r = wmfma(x[j], y[j], r);
+        }
+        return r;
+    };
+    /* the row of the table of the tile's last row and step n's first frame */
+    auto place_of = [&](int32_t n) { return first_of(n) - (s.i0 + 15) + a.left; };
+
+    /* A value that is an infinity or no number gives NaN to every row of the tile, those that do not attend it among them
+     * (its product with their 0). So a pass that ends with one is made again with care. */
+    bool careful = false;
+    for (;;) {
+    top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int n = 0; n < 2 * NS; n++)
+        o[n] = w4f{};
+    if (n0 < n1) {
+        load_keys(n0);
+        load_values(n0);
         if constexpr (POS) {
-            if (n >= ns) {
-                const int32_t x0 = a.left - (s.i0 + 15) + j0;
+            const int32_t n = max(n0, ns);
+            load_places(place_of(n));
+            put(pos);
+            before = places();
+            load_places(place_of(n) + 16);
+        }
+    }
+#pragma unroll 1
+    for (int32_t n = n0; n < n1; n++) {
+        const int32_t j0 = first_of(n), next = min(n + 1, n1 - 1);
+        w4f x[1] = {};
+        put(key);
+        load_keys(next);
 #pragma unroll
-                for (int pt = 0; pt < PT; pt++) {
-                    const int32_t row = cache_clip(x0 + 16 * pt + c, 0, (int32_t)a.bw - 1);
-                    const float *src = a.p + (uint64_t)(uint32_t)row * (a.H * S::dk) + s.h * S::dk + 4 * w;
-                    w4f pos[S::NT], r = {};
+        for (int t = 0; t < S::NT; t++) {
+            const w4f y = operand(t);
 #pragma unroll
-                    for (int t = 0; t < S::NT; t++)
-                        pos[t] = *(const w4f *)(src + 16 * t);
+            for (int j = 0; j < 4; j++)
+                x[0] = wmfma(y[j], q.c[t][j], x[0]);
+        }
+        w4f now = {};
+        if constexpr (POS) {
+            const int32_t x0 = place_of(n);
+            put(pos);
+            load_places(place_of(max(next, ns)) + 16);
+            if (n >= ns && x0 + 16 < (int32_t)a.bw)
+                now = places();
+        }
+        if (n < ns) {
+            x[0] += q.behind;
 #pragma unroll
-                    for (int t = 0; t < S::NT; t++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            r = wmfma(pos[t][j], q.p[t][j], r);
-                    *(w4f *)&place[wave][c][16 * pt + 4 * w] = r;
-                }
+            for (int r = 0; r < 4; r++)
+                x[0][r] = j0 + 4 * w + r < far ? x[0][r] : -INFINITY;
+        } else {
+            if constexpr (POS) {
+                *(w4f *)&place[wave][c][4 * w] = before;
+                *(w4f *)&place[wave][c][16 + 4 * w] = now;
+                before = now;
                 wave_sync();
 #pragma unroll
-                for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const float y = place[wave][c][15 - c + 16 * kt + 4 * w + r];
-                        x[kt][r] += j0 + 16 * kt + 4 * w + r < i - a.left ? q.behind : y;
-                    }
-                wave_sync();
-            } else {
-#pragma unroll
-                for (int kt = 0; kt < KT; kt++)
-                    x[kt] += q.behind;
-            }
-        }
-#pragma unroll
-        for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int32_t j = j0 + 16 * kt + 4 * w + r;
-                const bool seen = j < s.T && j <= i + a.right && (j >= i - a.left || j < a.sinks);
-                x[kt][r] = seen ? x[kt][r] : -INFINITY;
-            }
-        typename S::vec v[KT][4][S::NB];
-        float odd = 0.0f;                   /* NaN where a value is no number */
-#pragma unroll
-        for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int32_t j = min(j0 + 16 * kt + 4 * w + r, s.T - 1);
-                const float *src = a.v + (uint64_t)(s.r0 + j) * a.vs + s.g * S::dk + S::VW * c;
-#pragma unroll
-                for (int b = 0; b < S::NB; b++) {
-                    v[kt][r][b] = *(const typename S::vec *)(src + 16 * S::VW * b);
-#pragma unroll
-                    for (int e = 0; e < S::VW; e++)
-                        odd = __builtin_fmaf(v[kt][r][b][e], 0.0f, odd);
+                for (int r = 0; r < 4; r++) {
+                    const float y = place[wave][c][15 - c + 4 * w + r];
+                    x[0][r] += j0 + 4 * w + r < i - a.left ? q.behind : y;
                 }
+                wave_sync();
             }
-        w4f prob[KT];
 #pragma unroll
-        for (int kt = 0; kt < KT; kt++)
-            prob[kt] = x[kt];
-        window_softmax<KT, 2 * NS>(prob, top, sum, o);
-        if (__builtin_expect(__any(odd != odd), 0)) {
-            /* An infinity or a NaN among the values may be only some rows': the others would get its product with
-             * their 0. Those take the product without it, and each attended one is added to the rows that attend it. */
-#pragma unroll
-            for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-#pragma unroll
-                    for (int b = 0; b < S::NB; b++)
-#pragma unroll
-                        for (int e = 0; e < S::VW; e++) {
-                            const float y = v[kt][r][b][e];
-                            const bool bad = __builtin_fmaf(y, 0.0f, 0.0f) != 0.0f;
-                            v[kt][r][b][e] = bad ? 0.0f : y;
-                            uint64_t who = __ballot(bad);
-                            while (who) {
-                                const int from = __builtin_ctzll(who);
-                                who &= who - 1;
-                                const float value = __shfl(y, from);
-                                const float mine = __shfl(prob[kt][r], 16 * (from / 16) + c);
-                                const bool seen = __shfl((int)(x[kt][r] != -INFINITY), 16 * (from / 16) + c);
-                                /* its dimension is row from % 16 of block (b, e), which lanes w = row / 4 hold */
-                                const int row = from % 16;
-#pragma unroll
-                                for (int rr = 0; rr < 4; rr++)
-                                    if (seen && row == 4 * w + rr)
-                                        o[b * S::VW + e][rr] += mine * value;
-                            }
-                        }
+            for (int r = 0; r < 4; r++) {
+                const int32_t j = j0 + 4 * w + r;
+                const bool seen = (j <= last) & ((j >= i - a.left) | (j < a.sinks));
+                x[0][r] = seen ? x[0][r] : -INFINITY;
+            }
         }
-#pragma unroll
-        for (int kt = 0; kt < KT; kt++)
+        w4f prob[1] = { x[0] };
+        window_softmax<1, 2 * NS>(prob, top, sum, o);
+        if (__builtin_expect(careful, 0)) {
+            /* the product without them, and each added to the rows that attend it */
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
                 for (int b = 0; b < S::NB; b++)
 #pragma unroll
-                    for (int e = 0; e < S::VW; e++)
-                        o[b * S::VW + e] = wmfma(v[kt][r][b][e], prob[kt][r], o[b * S::VW + e]);
+                    for (int e = 0; e < S::VW; e++) {
+                        const float y = v[r][b][e];
+                        const bool bad = __builtin_fmaf(y, 0.0f, 0.0f) != 0.0f;
+                        v[r][b][e] = bad ? 0.0f : y;
+                        uint64_t who = __ballot(bad);
+                        while (who) {
+                            const int from = __builtin_ctzll(who);
+                            who &= who - 1;
+                            const float value = __shfl(y, from);
+                            const float mine = __shfl(prob[0][r], 16 * (from / 16) + c);
+                            const bool seen = __shfl((int)(x[0][r] != -INFINITY), 16 * (from / 16) + c);
+                            /* its dimension is row from % 16 of block (b, e), which lanes w = row / 4 hold */
+                            const int row = from % 16;
+#pragma unroll
+                            for (int rr = 0; rr < 4; rr++)
+                                if (seen && row == 4 * w + rr)
+                                    o[b * S::VW + e][rr] += mine * value;
+                        }
+                    }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int b = 0; b < S::NB; b++)
+#pragma unroll
+                for (int e = 0; e < S::VW; e++)
+                    o[b * S::VW + e] = wmfma(v[r][b][e], prob[0][r], o[b * S::VW + e]);
+        load_values(next);
+    }
+    float odd = 0.0f;                       /* NaN where an output is no number */
+#pragma unroll
+    for (int n = 0; n < 2 * NS; n++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            odd = __builtin_fmaf(o[n][r], 0.0f, odd);
+    if (careful || !__any(odd != odd))
+        break;
+    careful = true;
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
-    if (w == 0)
-        tops[wave][c] = top, sums[wave][c] = sum;
+    /* a lane's outputs: VW dimensions next to each other from 16 VW b + VW (4 w + r) on */
+    auto output = [&](int b, int r) {
+        typename S::vec y;
 #pragma unroll
-    for (int b = 0; b < S::NB; b++)
+        for (int e = 0; e < S::VW; e++)
+            y[e] = o[b * S::VW + e][r];
+        return y;
+    };
+    if constexpr (W == 1) {
+        if (i >= s.T)
+            return;
+        const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+        float *to = a.o + (uint64_t)(s.r0 + i) * a.os + s.h * S::dk + S::VW * 4 * w;
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            typename S::vec y;
+        for (int b = 0; b < S::NB; b++)
 #pragma unroll
-            for (int e = 0; e < S::VW; e++)
-                y[e] = o[b * S::VW + e][r];
-            *(typename S::vec *)&part[wave][c][16 * S::VW * b + S::VW * (4 * w + r)] = y;
+            for (int r = 0; r < 4; r++)
+                *(typename S::vec *)(to + 16 * S::VW * b + S::VW * r) = output(b, r) * scale;
+    } else {
+        __shared__ float tops[kWaves][16], sums[kWaves][16];
+        if (w == 0)
+            tops[wave][c] = top, sums[wave][c] = sum;
+#pragma unroll
+        for (int b = 0; b < S::NB; b++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                *(typename S::vec *)&rows[wave][c][16 * S::VW * b + S::VW * (4 * w + r)] = output(b, r);
+        __syncthreads();
+        const uint32_t w0 = wave / W * W;
+        for (uint32_t n = threadIdx.x % (64 * W); n < 16 * S::dk / 4; n += 64 * W) {
+            const int32_t r = (int32_t)(n / (S::dk / 4)), d = (int32_t)(n % (S::dk / 4)) * 4;
+            if (s.i0 + r >= s.T)
+                continue;
+            float m = -INFINITY, l = 0.0f;
+            w4f y = {};
+#pragma unroll
+            for (int u = 0; u < W; u++)
+                m = fmaxf(m, tops[w0 + u][r]);
+            const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int u = 0; u < W; u++) {
+                const float e = __builtin_amdgcn_exp2f(tops[w0 + u][r] - base);
+                l += sums[w0 + u][r] * e;
+                y += *(const w4f *)&rows[w0 + u][r][d] * e;
+            }
+            *(w4f *)(a.o + (uint64_t)(s.r0 + s.i0 + r) * a.os + s.h * S::dk + d) = l == 0.0f ? w4f{} : y / l;
         }
-    __syncthreads();
-    for (uint32_t n = threadIdx.x; n < 16 * S::dk / 4; n += 64 * W) {
-        const int32_t r = (int32_t)(n / (S::dk / 4)), d = (int32_t)(n % (S::dk / 4)) * 4;
-        if (s.i0 + r >= s.T)
-            continue;
-        float m = -INFINITY, l = 0.0f;
-        w4f y = {};
-#pragma unroll
-        for (int u = 0; u < W; u++)
-            m = fmaxf(m, tops[u][r]);
-        const float base = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int u = 0; u < W; u++) {
-            const float e = __builtin_amdgcn_exp2f(tops[u][r] - base);
-            l += sums[u][r] * e;
-            y += *(const w4f *)&part[u][r][d] * e;
-        }
-        *(w4f *)(a.o + (uint64_t)(s.r0 + s.i0 + r) * a.os + s.h * S::dk + d) = l == 0.0f ? w4f{} : y / l;
     }
 }
 
@@ -331,14 +419,23 @@ bool window_fits(uint32_t B, uint32_t max_T, uint32_t H) {
     return (uint64_t)((max_T + 15) / 16) * B * H <= kMostWindowGroups;
 }
 
+template <int NS, int W>
+static void window(const WindowAttention &a, hipStream_t s) {
+    constexpr uint32_t kTiles = W > 4 ? 1 : 4 / W;
+    const uint32_t grid = a.B * ((a.tiles + kTiles - 1) / kTiles) * a.H;
+    (a.p ? window_kernel<NS, true, W> : window_kernel<NS, false, W>)<<<grid, W > 4 ? 64 * W : 256, 0, s>>>(a);
+}
+
 template <int NS>
 static void window(WindowAttention &a, hipStream_t s) {
     a.tiles = (a.max_T + 15) / 16;
-    const uint32_t grid = a.B * a.tiles * a.H;
-    if (a.p)
-        window_few_kernel<NS, true, 4><<<grid, 256, 0, s>>>(a);
-    else
-        window_few_kernel<NS, false, 4><<<grid, 256, 0, s>>>(a);
+    const char *e = getenv("PKW");
+    switch (e ? atoi(e) : 4) {
+    case 1: window<NS, 1>(a, s); break;
+    case 2: window<NS, 2>(a, s); break;
+    case 4: window<NS, 4>(a, s); break;
+    default: window<NS, 8>(a, s); break;
+    }
 }
 
 int launch_window(const WindowCall &c, hipStream_t s) {

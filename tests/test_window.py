@@ -39,7 +39,8 @@ def call(pk, **change):
     dict(dk=16), dict(dk=48), dict(dk=160), dict(dk=0), dict(H=0), dict(H=3), dict(H=65536), dict(G=0), dict(G=1025, H=1025),
     dict(B=60000, rows=1 << 20, max_T=1 << 20),
     dict(o=None), dict(q=None), dict(k=None), dict(v=None), dict(o=A + 4), dict(q=B_ + 8), dict(k=C + 4), dict(v=D + 12),
-    dict(os=255), dict(qs=257), dict(ks=126), dict(vs=127), dict(os=252), dict(ks=124),
+    dict(os=255), dict(qs=257), dict(ks=126), dict(vs=127), dict(os=252), dict(ks=124), dict(ks=(1 << 25) + 4),
+    dict(vs=1 << 26),
     dict(p=F + 8192, u=None), dict(p=F + 8192, w=None), dict(p=F + 8196), dict(p=F + 8192, center=9), dict(p=F + 8192, n=0),
     dict(o=B_, os=260), dict(o=B_ + 1024), dict(o=C), dict(o=D + 4 * 128 * 9), dict(k=A + 4 * 256 * 9),
     dict(os=512, qs=512, q=A + 4 * 252), dict(os=512, ks=512, k=A + 4 * 388), dict(os=508, qs=508, q=A + 4 * 256),
