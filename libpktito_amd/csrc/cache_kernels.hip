@@ -2,6 +2,7 @@
  * write of a chunk's keys and values, their read-back, the attention of a
  * chunk's rows to everything kept, and the move of pages. */
 #include "cache_layout.h"
+#include "pieces.h"
 #include "q8_device.h"
 #include "q8_internal.h"
 
@@ -14,12 +15,7 @@
 
 namespace pkq8 {
 
-typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
-typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
-typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v4f_u __attribute__((ext_vector_type(4), aligned(4)));
-typedef float v2f_c __attribute__((ext_vector_type(2)));
-typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ CacheSpan span_of(const CacheStreams &s, uint32_t b) {
@@ -277,10 +273,6 @@ __global__ __launch_bounds__(256) void cache_read_kernel(uint8_t *data, uint32_t
  * after the first piece and 8 after the second). Three products of exact
  * terms, added in 32 bits: what an fp32 product of the same values gives, at
  * a third of the bfloat16 rate, five times the fp32 matrix rate. */
-struct Pieces {
-    v8bf p[3];
-};
-
 __device__ __forceinline__ Pieces cut(const float (&x)[8]) {
     Pieces r;
     uint32_t w[3][4];
@@ -310,10 +302,6 @@ __device__ __forceinline__ v8bf levels(uint32_t w) {
     return v8bf{ a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y };
 }
 
-__device__ __forceinline__ v4f mfma(v8bf a, v8bf b, v4f c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
-
 struct CacheAttention {
     float *o;
     const float *q;
@@ -335,32 +323,6 @@ struct CacheAttention {
 
 __device__ __forceinline__ uint64_t unit_of(const CacheAttention &a, uint32_t b, uint32_t tile, uint32_t g) {
     return ((uint64_t)b * a.tiles + tile) * a.G + g;
-}
-
-/* Floats cut for a product of floats with floats: each piece the nearest
- * bfloat16 of what the ones before leave, so that the second is at most 2^-8
- * of the float's power of two, the third 2^-17, and the three sum to it exactly
- * (down to 2^-126, where pieces end). Of the nine products of two floats'
- * pieces the six largest are taken: those left out are 2^-24 of the product at
- * most, as much as a 32-bit product's own rounding. Whatever the other
- * dimensions hold: a row has no exponent in common. */
-__device__ __forceinline__ Pieces cut_near(const float (&x)[8]) {
-    Pieces r;
-    uint32_t w[3][4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        v2f_c a = { x[2 * i], x[2 * i + 1] };
-#pragma unroll
-        for (int n = 0; n < 3; n++) {
-            w[n][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(a, v2bf));
-            a.x -= __uint_as_float(w[n][i] << 16);
-            a.y -= __uint_as_float(w[n][i] & 0xffff0000u);
-        }
-    }
-#pragma unroll
-    for (int n = 0; n < 3; n++)
-        r.p[n] = __builtin_bit_cast(v8bf, v4u{ w[n][0], w[n][1], w[n][2], w[n][3] });
-    return r;
 }
 
 /* Sixteen rows of the positions' table for one head as the matrix

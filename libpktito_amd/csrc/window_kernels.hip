@@ -1,10 +1,10 @@
 /* Attention with a sliding window and sinks over whole segments: every row
  * attends the frames of a window around it and the segment's first few, so an
  * hour of audio in one piece costs its frames times the window. Products and
- * sums in 32 bits on the fp32 matrix instruction: it rounds as a fused multiply
- * and add does, takes floats of any magnitude as they are, and a product of
- * three bfloat16 pieces by three would gain a fifth of its time at best and lose
- * that in the cutting. */
+ * sums in 32 bits, whatever the floats' magnitudes: on the fp32 matrix
+ * instruction, which rounds as a fused multiply and add does, or where many rows
+ * can share the cutting on the bfloat16 one. */
+#include "pieces.h"
 #include "q8_internal.h"
 
 #include <hip/hip_runtime.h>
@@ -15,8 +15,6 @@
 #pragma clang fp contract(off)
 
 namespace pkq8 {
-
-typedef float w4f __attribute__((ext_vector_type(4)));
 
 struct WindowAttention {
     float *o;
@@ -51,7 +49,7 @@ __device__ __forceinline__ bool window_tile(const WindowAttention &a, WindowTile
     return s.i0 < s.T;
 }
 
-__device__ __forceinline__ w4f wmfma(float x, float y, w4f c) {
+__device__ __forceinline__ v4f wmfma(float x, float y, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(x, y, c, 0, 0, 0);
 }
 
@@ -76,24 +74,24 @@ struct WindowShape {
  * table's first row). */
 template <int NS, bool POS>
 struct WindowQueries {
-    w4f c[2 * NS];
+    v4f c[2 * NS];
     float behind;
 
-    __device__ __forceinline__ void load(const WindowAttention &a, const WindowTile &s, int32_t i, w4f (*at_place)[64]) {
+    __device__ __forceinline__ void load(const WindowAttention &a, const WindowTile &s, int32_t i, v4f (*at_place)[64]) {
         constexpr uint32_t dk = 32 * NS;
         const uint32_t w = (threadIdx.x & 63) / 16;
         const float *src = a.q + (uint64_t)(s.r0 + min(i, s.T - 1)) * a.qs + s.h * dk + 4 * w;
         behind = 0.0f;
 #pragma unroll
         for (int t = 0; t < 2 * NS; t++) {
-            const w4f x = *(const w4f *)(src + 16 * t);
+            const v4f x = *(const v4f *)(src + 16 * t);
             if constexpr (POS) {
                 const uint32_t d = s.h * dk + 4 * w + 16 * t;
-                c[t] = (x + *(const w4f *)(a.bias_u + d)) * a.scale;
-                const w4f p = (x + *(const w4f *)(a.bias_w + d)) * a.scale;
+                c[t] = (x + *(const v4f *)(a.bias_u + d)) * a.scale;
+                const v4f p = (x + *(const v4f *)(a.bias_w + d)) * a.scale;
                 at_place[t][threadIdx.x & 63] = p;
                 if (a.sinks) {
-                    const w4f far = *(const w4f *)(a.p + d);
+                    const v4f far = *(const v4f *)(a.p + d);
 #pragma unroll
                     for (int j = 0; j < 4; j++)
                         behind = __builtin_fmaf(p[j], far[j], behind);
@@ -116,7 +114,7 @@ constexpr float kWindowSlack = 8.0f;
 /* Scores of a query with 16 KT frames, -infinity where not attended, into the
  * running softmax: the exponentials in their place. */
 template <int KT, int NO>
-__device__ __forceinline__ void window_softmax(w4f (&s)[KT], float &top, float &sum, w4f (&o)[NO]) {
+__device__ __forceinline__ void window_softmax(v4f (&s)[KT], float &top, float &sum, v4f (&o)[NO]) {
     float best = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 4 * KT; i++)
@@ -149,31 +147,34 @@ __device__ __forceinline__ void wave_sync() {
 /* Sixteen rows a tile, W waves to a tile, each a run of its steps of 16 frames:
  * the sinks' steps first, then the window's, which begins at the tile's first
  * frame of it whatever that is a multiple of (no step is taken for alignment).
- * Operands come straight from memory: 24 KB a step for 96 matrix instructions,
- * whose 3072 cycles hide the loads of the step after, each issued into the
- * registers of this one's as those have been used.
+ * Operands come from memory, 24 KB a step, each load issued into the registers
+ * of the step before as those have been used.
  *
  * A frame j's place scores are products with the rows x = left - (row - j) of
  * the table, 31 of them for 16 rows and frames; the first 16 of those are the
  * step before's last, so each step makes 16 more. A lane's are another column's
- * than its scores', so they pass through LDS. */
+ * than its scores', so they pass through LDS.
+ *
+ * An hour (45000 frames, 8 heads of 128, 128 + 128 + 1 frames and 16 sinks, 75.6
+ * GFLOP): 785 us, 96 TFLOP/s of the 154 that an fp32 product reaches. The matrix
+ * instructions are busy 63% of it; vector instructions, LDS and loads hold them up,
+ * two waves a SIMD or one (4900 and 5400 clocks a step, of which 3072 are theirs).
+ * Keys by lanes that use them took 910 (53 cache lookups a load, 16 now). Measured
+ * and no faster: the shared cutting of the kernel below (820: four barriers a step),
+ * 32 rows a wave cut into pieces in its registers (850, a wave a SIMD). */
 template <int NS, bool POS, int W>
-__global__ __launch_bounds__(W > 4 ? 64 * W : 256, 2) void window_kernel(WindowAttention a) {
+__global__ __launch_bounds__(256, 2) void window_kernel(WindowAttention a) {
     using S = WindowShape<NS>;
-    constexpr int kWaves = W > 4 ? W : 4, kTiles = kWaves / W, kRow = 36;
+    static_assert(W == 1 || W == 4, "a workgroup's four waves have a tile each, or one");
+    constexpr int kWaves = 4, kTiles = kWaves / W, kRow = 36;
     __shared__ __attribute__((aligned(16))) float place[POS ? kWaves : 1][16][kRow];
     __shared__ __attribute__((aligned(16))) float rows[kWaves][16][S::dk + 4];
-    __shared__ w4f query[POS ? kWaves : 1][S::NT][64];      /* the place's operands, which registers have no room for */
+    __shared__ v4f query[POS ? kWaves : 1][S::NT][64];      /* the place's operands, which registers have no room for */
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     WindowTile s;
     if (!window_tile<16, kTiles>(a, s, wave / W))
         return;
     const int32_t c = (int32_t)(lane % 16), w = (int32_t)(lane / 16), i = s.i0 + c;
-    WindowQueries<NS, POS> q;
-    q.load(a, s, i, query[POS ? wave : 0]);
-    float top, sum;
-    w4f o[2 * NS];
-
     /* the window's frames [lo, hi] of any of the rows, the sinks [0, far) before them, the steps of both */
     const int32_t lo = max(s.i0 - a.left, 0), hi = min(s.i0 + 15 + a.right, s.T - 1), far = min(a.sinks, lo);
     const int32_t ns = (far + 15) / 16, steps = ns + (hi - lo) / 16 + 1, each = (steps + W - 1) / W;
@@ -181,7 +182,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256, 2) void window_kernel(WindowA
     const int32_t last = min(i + a.right, s.T - 1);         /* the lane's query's */
     auto first_of = [&](int32_t n) { return n < ns ? 16 * n : lo + 16 * (n - ns); };
 
-    w4f key[2][NS], pos[2][NS], before;
+    v4f key[2][NS], pos[2][NS], before;
     typename S::vec v[4][S::NB];
     /* Sixteen rows of keys or of the table, 128 bytes of one to eight lanes (to a lane of its own the 16 bytes that the
      * instruction wants of it, each row's would be cache lookups of their own, four times as many), put where operands are
@@ -195,19 +196,19 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256, 2) void window_kernel(WindowA
             const uint32_t off = (uint32_t)min(lr + 8 * half, s.T - 1 - j0) * (uint32_t)a.ks;
 #pragma unroll
             for (int t = 0; t < NS; t++)
-                key[half][t] = *(const w4f *)(src + off + 32 * t);
+                key[half][t] = *(const v4f *)(src + off + 32 * t);
         }
     };
-    auto put = [&](const w4f (&x)[2][NS]) {
+    auto put = [&](const v4f (&x)[2][NS]) {
         wave_sync();
 #pragma unroll
         for (int half = 0; half < 2; half++)
 #pragma unroll
             for (int t = 0; t < NS; t++)
-                *(w4f *)&rows[wave][lr + 8 * half][lc + 32 * t] = x[half][t];
+                *(v4f *)&rows[wave][lr + 8 * half][lc + 32 * t] = x[half][t];
         wave_sync();
     };
-    auto operand = [&](int t) { return *(const w4f *)&rows[wave][c][16 * t + 4 * w]; };
+    auto operand = [&](int t) { return *(const v4f *)&rows[wave][c][16 * t + 4 * w]; };
     const uint32_t value_off = 4 * (uint32_t)w * (uint32_t)a.vs + S::VW * c;
     auto load_values = [&](int32_t n) {
         const int32_t j0 = first_of(n);
@@ -229,14 +230,14 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256, 2) void window_kernel(WindowA
             const float *src = a.p + (uint64_t)row * (a.H * S::dk) + s.h * S::dk + lc;
 #pragma unroll
             for (int t = 0; t < NS; t++)
-                pos[half][t] = *(const w4f *)(src + 32 * t);
+                pos[half][t] = *(const v4f *)(src + 32 * t);
         }
     };
     auto places = [&]() {
-        w4f r = {};
+        v4f r = {};
 #pragma unroll
         for (int t = 0; t < S::NT; t++) {
-            const w4f x = operand(t), y = query[wave][t][lane];
+            const v4f x = operand(t), y = query[wave][t][lane];
 #pragma unroll
             for (int j = 0; j < 4; j++)
                 r = wmfma(x[j], y[j], r);
@@ -246,118 +247,129 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256, 2) void window_kernel(WindowA
     /* the row of the table of the tile's last row and step n's first frame */
     auto place_of = [&](int32_t n) { return first_of(n) - (s.i0 + 15) + a.left; };
 
+    /* the first loads of all */
+    const int32_t x0 = place_of(max(n0, ns));
+    auto begin = [&]() {
+        if constexpr (POS)
+            load_places(x0);
+        load_keys(n0);
+        load_values(n0);
+    };
+    if (n0 < n1)
+        begin();
+    WindowQueries<NS, POS> q;
+    q.load(a, s, i, query[POS ? wave : 0]);
+    float top, sum;
+    v4f o[2 * NS];
     /* A value that is an infinity or no number gives NaN to every row of the tile, those that do not attend it among them
      * (its product with their 0). So a pass that ends with one is made again with care. */
     bool careful = false;
     for (;;) {
-    top = -INFINITY, sum = 0.0f;
+        top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int n = 0; n < 2 * NS; n++)
-        o[n] = w4f{};
-    if (n0 < n1) {
-        load_keys(n0);
-        load_values(n0);
+        for (int n = 0; n < 2 * NS; n++)
+            o[n] = v4f{};
         if constexpr (POS) {
-            const int32_t n = max(n0, ns);
-            load_places(place_of(n));
-            put(pos);
-            before = places();
-            load_places(place_of(n) + 16);
+            if (n0 < n1) {
+                put(pos);
+                load_places(x0 + 16);
+                before = places();
+            }
         }
-    }
 #pragma unroll 1
-    for (int32_t n = n0; n < n1; n++) {
-        const int32_t j0 = first_of(n), next = min(n + 1, n1 - 1);
-        w4f x[1] = {};
-        put(key);
-        load_keys(next);
+        for (int32_t n = n0; n < n1; n++) {
+            const int32_t j0 = first_of(n), next = min(n + 1, n1 - 1);
+            v4f x = {};
+            put(key);
+            load_keys(next);
 #pragma unroll
-        for (int t = 0; t < S::NT; t++) {
-            const w4f y = operand(t);
+            for (int t = 0; t < S::NT; t++) {
+                const v4f y = operand(t);
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                x[0] = wmfma(y[j], q.c[t][j], x[0]);
-        }
-        w4f now = {};
-        if constexpr (POS) {
-            const int32_t x0 = place_of(n);
-            put(pos);
-            load_places(place_of(max(next, ns)) + 16);
-            if (n >= ns && x0 + 16 < (int32_t)a.bw)
-                now = places();
-        }
-        if (n < ns) {
-            x[0] += q.behind;
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-                x[0][r] = j0 + 4 * w + r < far ? x[0][r] : -INFINITY;
-        } else {
+                for (int j = 0; j < 4; j++)
+                    x = wmfma(y[j], q.c[t][j], x);
+            }
+            v4f now = {};
             if constexpr (POS) {
-                *(w4f *)&place[wave][c][4 * w] = before;
-                *(w4f *)&place[wave][c][16 + 4 * w] = now;
-                before = now;
-                wave_sync();
+                const int32_t x0 = place_of(n);
+                put(pos);
+                load_places(place_of(max(next, ns)) + 16);
+                if (n >= ns && x0 + 16 < (int32_t)a.bw)
+                    now = places();
+            }
+            if (n < ns) {
+                x += q.behind;
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    x[r] = j0 + 4 * w + r < far ? x[r] : -INFINITY;
+            } else {
+                if constexpr (POS) {
+                    *(v4f *)&place[wave][c][4 * w] = before;
+                    *(v4f *)&place[wave][c][16 + 4 * w] = now;
+                    before = now;
+                    wave_sync();
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float y = place[wave][c][15 - c + 4 * w + r];
+                        x[r] += j0 + 4 * w + r < i - a.left ? q.behind : y;
+                    }
+                    wave_sync();
+                }
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const float y = place[wave][c][15 - c + 4 * w + r];
-                    x[0][r] += j0 + 4 * w + r < i - a.left ? q.behind : y;
+                    const int32_t j = j0 + 4 * w + r;
+                    const bool seen = (j <= last) & ((j >= i - a.left) | (j < a.sinks));
+                    x[r] = seen ? x[r] : -INFINITY;
                 }
-                wave_sync();
             }
+            v4f prob[1] = { x };
+            window_softmax<1, 2 * NS>(prob, top, sum, o);
+            if (__builtin_expect(careful, 0)) {
+                /* the product without them, and each added to the rows that attend it */
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int32_t j = j0 + 4 * w + r;
-                const bool seen = (j <= last) & ((j >= i - a.left) | (j < a.sinks));
-                x[0][r] = seen ? x[0][r] : -INFINITY;
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int b = 0; b < S::NB; b++)
+#pragma unroll
+                        for (int e = 0; e < S::VW; e++) {
+                            const float y = v[r][b][e];
+                            const bool bad = __builtin_fmaf(y, 0.0f, 0.0f) != 0.0f;
+                            v[r][b][e] = bad ? 0.0f : y;
+                            uint64_t who = __ballot(bad);
+                            while (who) {
+                                const int from = __builtin_ctzll(who);
+                                who &= who - 1;
+                                const float value = __shfl(y, from);
+                                const float mine = __shfl(prob[0][r], 16 * (from / 16) + c);
+                                const bool seen = __shfl((int)(x[r] != -INFINITY), 16 * (from / 16) + c);
+                                /* its dimension is row from % 16 of block (b, e), which lanes w = row / 4 hold */
+                                const int row = from % 16;
+#pragma unroll
+                                for (int rr = 0; rr < 4; rr++)
+                                    if (seen && row == 4 * w + rr)
+                                        o[b * S::VW + e][rr] += mine * value;
+                            }
+                        }
             }
-        }
-        w4f prob[1] = { x[0] };
-        window_softmax<1, 2 * NS>(prob, top, sum, o);
-        if (__builtin_expect(careful, 0)) {
-            /* the product without them, and each added to the rows that attend it */
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
                 for (int b = 0; b < S::NB; b++)
 #pragma unroll
-                    for (int e = 0; e < S::VW; e++) {
-                        const float y = v[r][b][e];
-                        const bool bad = __builtin_fmaf(y, 0.0f, 0.0f) != 0.0f;
-                        v[r][b][e] = bad ? 0.0f : y;
-                        uint64_t who = __ballot(bad);
-                        while (who) {
-                            const int from = __builtin_ctzll(who);
-                            who &= who - 1;
-                            const float value = __shfl(y, from);
-                            const float mine = __shfl(prob[0][r], 16 * (from / 16) + c);
-                            const bool seen = __shfl((int)(x[0][r] != -INFINITY), 16 * (from / 16) + c);
-                            /* its dimension is row from % 16 of block (b, e), which lanes w = row / 4 hold */
-                            const int row = from % 16;
-#pragma unroll
-                            for (int rr = 0; rr < 4; rr++)
-                                if (seen && row == 4 * w + rr)
-                                    o[b * S::VW + e][rr] += mine * value;
-                        }
-                    }
+                    for (int e = 0; e < S::VW; e++)
+                        o[b * S::VW + e] = wmfma(v[r][b][e], prob[0][r], o[b * S::VW + e]);
+            load_values(next);
         }
+        float odd = 0.0f;                   /* NaN where an output is no number */
 #pragma unroll
-        for (int r = 0; r < 4; r++)
+        for (int n = 0; n < 2 * NS; n++)
 #pragma unroll
-            for (int b = 0; b < S::NB; b++)
-#pragma unroll
-                for (int e = 0; e < S::VW; e++)
-                    o[b * S::VW + e] = wmfma(v[r][b][e], prob[0][r], o[b * S::VW + e]);
-        load_values(next);
-    }
-    float odd = 0.0f;                       /* NaN where an output is no number */
-#pragma unroll
-    for (int n = 0; n < 2 * NS; n++)
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-            odd = __builtin_fmaf(o[n][r], 0.0f, odd);
-    if (careful || !__any(odd != odd))
-        break;
-    careful = true;
+            for (int r = 0; r < 4; r++)
+                odd = __builtin_fmaf(o[n][r], 0.0f, odd);
+        if (careful || !__any(odd != odd))
+            break;
+        careful = true;
+        begin();
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
@@ -389,26 +401,239 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256, 2) void window_kernel(WindowA
             for (int r = 0; r < 4; r++)
                 *(typename S::vec *)&rows[wave][c][16 * S::VW * b + S::VW * (4 * w + r)] = output(b, r);
         __syncthreads();
-        const uint32_t w0 = wave / W * W;
-        for (uint32_t n = threadIdx.x % (64 * W); n < 16 * S::dk / 4; n += 64 * W) {
+        for (uint32_t n = threadIdx.x; n < 16 * S::dk / 4; n += 64 * W) {
             const int32_t r = (int32_t)(n / (S::dk / 4)), d = (int32_t)(n % (S::dk / 4)) * 4;
             if (s.i0 + r >= s.T)
                 continue;
             float m = -INFINITY, l = 0.0f;
-            w4f y = {};
+            v4f y = {};
 #pragma unroll
             for (int u = 0; u < W; u++)
-                m = fmaxf(m, tops[w0 + u][r]);
+                m = fmaxf(m, tops[u][r]);
             const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
             for (int u = 0; u < W; u++) {
-                const float e = __builtin_amdgcn_exp2f(tops[w0 + u][r] - base);
-                l += sums[w0 + u][r] * e;
-                y += *(const w4f *)&rows[w0 + u][r][d] * e;
+                const float e = __builtin_amdgcn_exp2f(tops[u][r] - base);
+                l += sums[u][r] * e;
+                y += *(const v4f *)&rows[u][r][d] * e;
             }
-            *(w4f *)(a.o + (uint64_t)(s.r0 + s.i0 + r) * a.os + s.h * S::dk + d) = l == 0.0f ? w4f{} : y / l;
+            *(v4f *)(a.o + (uint64_t)(s.r0 + s.i0 + r) * a.os + s.h * S::dk + d) = l == 0.0f ? v4f{} : y / l;
         }
     }
+}
+
+/* The six products of pieces that count, the smallest first. */
+__device__ __forceinline__ v4f product(const Pieces &x, const Pieces &y, v4f acc) {
+    acc = mfma(x.p[2], y.p[0], acc);
+    acc = mfma(x.p[1], y.p[1], acc);
+    acc = mfma(x.p[0], y.p[2], acc);
+    acc = mfma(x.p[1], y.p[0], acc);
+    acc = mfma(x.p[0], y.p[1], acc);
+    return mfma(x.p[0], y.p[0], acc);
+}
+
+/* Many rows without positions: 64 rows a workgroup, 16 a wave, 32 frames a step
+ * for all of them, on the bfloat16 matrix cores with every float in three pieces
+ * (pieces.h): six products take three eighths of the fp32 instructions' time. The
+ * cutting takes 11 vector instructions for two floats, more than the products if
+ * each wave cut what it uses: so the workgroup cuts a step's keys and values once,
+ * into the operands' own order in LDS, and its four waves read them there. Raw,
+ * they are loaded a step ahead.
+ *
+ * Reductions run over 32 indices, eight a quarter of the wave. Scores: lane l
+ * has dimensions 32 s + 8 (l / 16) + i of key l % 16 of a run of 16 (two runs a
+ * step), queries are the columns. A lane's scores are then its query's with
+ * frames 4 (l / 16) + r of both runs, the eight that it gives the second product,
+ * whose rows are dimensions 32 b + 2 (l % 16) + d of instruction (b, d).
+ *
+ * Four segments of 2001 to 3000 frames, 16 heads of 64 to 4 kept ones, 512 frames
+ * and 8 sinks, 19.6 GFLOP: 155 us, 126 TFLOP/s (220 with fp32 instructions); with
+ * 2000 frames 152, the fp32 instructions' peak. Two products' chains side by side
+ * were no faster. */
+template <int NS>
+__global__ __launch_bounds__(256, 2) void window_many_kernel(WindowAttention a) {
+    constexpr int dk = 32 * NS, kChunks = 4 * NS;
+    constexpr int kEach = (32 * kChunks + 255) / 256;       /* eights of dimensions that a thread cuts */
+    __shared__ v8bf key[2][NS][3][64];
+    __shared__ v8bf value[NS][2][3][64];
+    __shared__ uint32_t odd_step;                           /* the step whose values hold what is no number, and one */
+    WindowTile s;
+    if (!window_tile<64, 1>(a, s, 0))
+        return;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int32_t c = (int32_t)(lane % 16), w = (int32_t)(lane / 16), iw = s.i0 + 16 * (int32_t)wave, i = iw + c;
+
+    Pieces q[NS];                           /* scores in powers of 2 */
+    const float *src = a.q + (uint64_t)(s.r0 + min(i, s.T - 1)) * a.qs + s.h * dk + 8 * w;
+#pragma unroll
+    for (int t = 0; t < NS; t++) {
+        const v4f x = *(const v4f *)(src + 32 * t) * a.scale, y = *(const v4f *)(src + 32 * t + 4) * a.scale;
+        const float z[8] = { x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3] };
+        q[t] = cut_near(z);
+    }
+    float top = -INFINITY, sum = 0.0f;
+    v4f o[2 * NS] = {};
+
+    /* the window's frames [lo, hi] of any of the rows, the sinks [0, far) before them, the steps of both */
+    const int32_t lo = max(s.i0 - a.left, 0), hi = min(s.i0 + 63 + a.right, s.T - 1), far = min(a.sinks, lo);
+    const int32_t ns = (far + 31) / 32, steps = ns + (hi - lo) / 32 + 1;
+    auto first_of = [&](int32_t n) { return n < ns ? 32 * n : lo + 32 * (n - ns); };
+
+    /* a step's raw rows: eights of dimensions of a row by threads side by side; of values two dimensions of eight frames,
+     * which become an operand as they are */
+    v4f raw[kEach][2];
+    v2f_c raw_v[8];
+    auto load_keys = [&](int32_t j0) {
+        const float *src = a.k + (uint64_t)(s.r0 + j0) * a.ks + s.g * dk;
+#pragma unroll
+        for (int e = 0; e < kEach; e++) {
+            const uint32_t n = threadIdx.x + 256 * e;
+            const uint32_t off = (uint32_t)min((int32_t)(n / kChunks), s.T - 1 - j0) * (uint32_t)a.ks + 8 * (n % kChunks);
+            raw[e][0] = *(const v4f *)(src + off);
+            raw[e][1] = *(const v4f *)(src + off + 4);
+        }
+    };
+    auto load_values = [&](int32_t j0) {
+        const float *src = a.v + (uint64_t)(s.r0 + j0) * a.vs + s.g * dk + 32 * (wave % NS) + 2 * c;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            raw_v[k] = *(const v2f_c *)(src + (uint32_t)min(16 * (k / 4) + 4 * w + k % 4, s.T - 1 - j0) * (uint32_t)a.vs);
+    };
+    /* rows cut into operands: chunk n % kChunks of row n / kChunks, at a place of its run of 16 that lets threads side by
+     * side write to banks of their own */
+    auto slot_of = [&](uint32_t row, uint32_t chunk) {
+        return 16 * (chunk % 4) + (row % 16 ^ (chunk * (NS == 1 ? 4 : NS == 2 ? 2 : 1)) % 16);
+    };
+    auto put = [&](const v4f (&x)[kEach][2]) {
+#pragma unroll
+        for (int e = 0; e < kEach; e++) {
+            const uint32_t n = threadIdx.x + 256 * e, row = n / kChunks, chunk = n % kChunks;
+            const float z[8] = { x[e][0][0], x[e][0][1], x[e][0][2], x[e][0][3], x[e][1][0], x[e][1][1], x[e][1][2], x[e][1][3] };
+            const Pieces y = cut_near(z);
+            if (32 * kChunks % 256 == 0 || n < 32 * kChunks)
+#pragma unroll
+                for (int k = 0; k < 3; k++)
+                    key[row / 16][chunk / 4][k][slot_of(row, chunk)] = y.p[k];
+        }
+    };
+    auto operand = [&](int kt, int t) {
+        Pieces x;
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+            x.p[k] = key[kt][t][k][slot_of((uint32_t)c, 4 * t + (uint32_t)w)];
+        return x;
+    };
+    /* An infinity or a NaN among the values may be only some rows': the others would get its product with their 0. The
+     * product is made without it, and the step told. */
+    auto put_values = [&](int32_t n) {
+        float odd = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            odd = __builtin_fmaf(raw_v[k].x, 0.0f, __builtin_fmaf(raw_v[k].y, 0.0f, odd));
+        if (__builtin_expect(__any(odd != odd), 0)) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                raw_v[k].x = __builtin_fmaf(raw_v[k].x, 0.0f, 0.0f) == 0.0f ? raw_v[k].x : 0.0f;
+                raw_v[k].y = __builtin_fmaf(raw_v[k].y, 0.0f, 0.0f) == 0.0f ? raw_v[k].y : 0.0f;
+            }
+            odd_step = (uint32_t)n + 1;
+        }
+        if (wave < NS)
+#pragma unroll
+            for (int d = 0; d < 2; d++) {
+                const float z[8] = { raw_v[0][d], raw_v[1][d], raw_v[2][d], raw_v[3][d], raw_v[4][d], raw_v[5][d], raw_v[6][d], raw_v[7][d] };
+                const Pieces y = cut_near(z);
+#pragma unroll
+                for (int k = 0; k < 3; k++)
+                    value[wave][d][k][lane] = y.p[k];
+            }
+    };
+    if (threadIdx.x == 0)
+        odd_step = 0;
+    load_keys(first_of(0));
+    load_values(first_of(0));
+#pragma unroll 1
+    for (int32_t n = 0; n < steps; n++) {
+        const int32_t j0 = first_of(n), next = first_of(min(n + 1, steps - 1));
+        __syncthreads();
+        put(raw);
+        put_values(n);
+        load_keys(next);
+        load_values(next);
+        __syncthreads();
+        /* whether any of the wave's rows attends any of the frames */
+        const bool busy = n < ns || (j0 + 31 >= iw - a.left && j0 <= iw + 15 + a.right) || j0 < a.sinks;
+        if (!busy)
+            continue;
+        v4f x[2] = {};
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+            for (int t = 0; t < NS; t++)
+                x[kt] = product(operand(kt, t), q[t], x[kt]);
+        if (n < ns) {
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                x[k / 4][k % 4] = j0 + 16 * (k / 4) + 4 * w + k % 4 < far ? x[k / 4][k % 4] : -INFINITY;
+        } else if (j0 < iw + 15 - a.left || j0 + 31 > min(iw + a.right, s.T - 1)) {
+            const int32_t last = min(i + a.right, s.T - 1);
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int32_t j = j0 + 16 * (k / 4) + 4 * w + k % 4;
+                const bool seen = (j <= last) & ((j >= i - a.left) | (j < a.sinks));
+                x[k / 4][k % 4] = seen ? x[k / 4][k % 4] : -INFINITY;
+            }
+        }
+        v4f e[2] = { x[0], x[1] };
+        window_softmax<2, 2 * NS>(e, top, sum, o);
+        if (__builtin_expect(odd_step == (uint32_t)n + 1, 0)) {
+#pragma unroll 1
+            for (int32_t k = 0; k < 32; k++) {              /* each value that is no number, to the rows that attend it */
+                const int32_t j = j0 + k;
+                if (j >= s.T)
+                    break;
+                const float mine = __shfl(k % 4 == 0 ? e[k / 16][0] : k % 4 == 1 ? e[k / 16][1] : k % 4 == 2 ? e[k / 16][2] : e[k / 16][3],
+                                          16 * (k / 4 % 4) + c);
+                const float score = __shfl(k % 4 == 0 ? x[k / 16][0] : k % 4 == 1 ? x[k / 16][1] : k % 4 == 2 ? x[k / 16][2] : x[k / 16][3],
+                                           16 * (k / 4 % 4) + c);
+                const float *src = a.v + (uint64_t)(s.r0 + j) * a.vs + s.g * dk + 8 * w;
+                if (score != -INFINITY)
+#pragma unroll
+                    for (int b = 0; b < NS; b++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+#pragma unroll
+                            for (int d = 0; d < 2; d++) {
+                                const float y = src[32 * b + 2 * r + d];
+                                if (__builtin_fmaf(y, 0.0f, 0.0f) != 0.0f)
+                                    o[2 * b + d][r] += mine * y;
+                            }
+            }
+        }
+        const float z[8] = { e[0][0], e[0][1], e[0][2], e[0][3], e[1][0], e[1][1], e[1][2], e[1][3] };
+        const Pieces prob = cut_near(z);
+#pragma unroll
+        for (int b = 0; b < NS; b++)
+#pragma unroll
+            for (int d = 0; d < 2; d++) {
+                Pieces y;
+#pragma unroll
+                for (int k = 0; k < 3; k++)
+                    y.p[k] = value[b][d][k][lane];
+                o[2 * b + d] = product(y, prob, o[2 * b + d]);
+            }
+    }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (i >= s.T)
+        return;
+    const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+    float *to = a.o + (uint64_t)(s.r0 + i) * a.os + s.h * dk + 8 * w;
+#pragma unroll
+    for (int b = 0; b < NS; b++)
+#pragma unroll
+        for (int r = 0; r < 4; r += 2)
+            *(v4f *)(to + 32 * b + 2 * r) = v4f{ o[2 * b][r], o[2 * b + 1][r], o[2 * b][r + 1], o[2 * b + 1][r + 1] } * scale;
 }
 
 /* ------------------------------------------------------------- launches --- */
@@ -419,22 +644,41 @@ bool window_fits(uint32_t B, uint32_t max_T, uint32_t H) {
     return (uint64_t)((max_T + 15) / 16) * B * H <= kMostWindowGroups;
 }
 
-template <int NS, int W>
-static void window(const WindowAttention &a, hipStream_t s) {
-    constexpr uint32_t kTiles = W > 4 ? 1 : 4 / W;
-    const uint32_t grid = a.B * ((a.tiles + kTiles - 1) / kTiles) * a.H;
-    (a.p ? window_kernel<NS, true, W> : window_kernel<NS, false, W>)<<<grid, W > 4 ? 64 * W : 256, 0, s>>>(a);
+/* A SIMD's waves hardly overlap here (an fp32 matrix instruction holds up every
+ * vector one: four of those between two make 53 clocks of its 32), so what counts
+ * is how many waves the fullest SIMD has and how many steps each takes, with
+ * three for what comes before and after them. Four waves a tile of 8 heads of
+ * 128 with 129 + 128 frames of window: 192 tiles 18.8 us, one wave 43.2; 512 31.3
+ * and 44.0; 752 51.0 and 44.2; 1024 56.0 and 45.5; 3000 151 and 120. With 70 + 13
+ * frames: 512 19.2 and 23.1, 752 32.5 and 24.0; with 511: 752 70.6 and 77.1, 1504
+ * 120 and 136, 3000 232 and 219. */
+static bool tile_split(uint64_t tiles, uint64_t steps) {
+    return (4 * tiles + 1023) / 1024 * ((steps + 3) / 4 + 3) <= (tiles + 1023) / 1024 * (steps + 3);
 }
+
+/* Without positions four waves a tile, or from this many tiles on 64 rows a
+ * workgroup. Heads of 128 with 257 frames: 752 tiles 31.1 and 31.9 us, 1024 36.1 and
+ * 32.1, 3000 91.7 and 67.6; heads of 64: 1024 18.6 and 21.2, 1504 25.7 and 26.6,
+ * 3000 47.8 and 35.5; of 96 1024 30.7 and 26.3; of 32 1504 17.1 and 20.6, 3000 29.9
+ * and 26.8. */
+constexpr uint64_t many_from(int NS) { return NS >= 3 ? 1024 : 2048; }
 
 template <int NS>
 static void window(WindowAttention &a, hipStream_t s) {
     a.tiles = (a.max_T + 15) / 16;
-    const char *e = getenv("PKW");
-    switch (e ? atoi(e) : 4) {
-    case 1: window<NS, 1>(a, s); break;
-    case 2: window<NS, 2>(a, s); break;
-    case 4: window<NS, 4>(a, s); break;
-    default: window<NS, 8>(a, s); break;
+    /* segments are up to max_T long, and together no more than the rows */
+    const uint64_t tiles = std::min((uint64_t)a.B * a.tiles, (uint64_t)a.rows / 16 + a.B) * a.H;
+    const uint32_t reach = std::min((uint32_t)(a.left + a.right) + 16, a.max_T + 15);
+    if (a.p) {
+        if (tile_split(tiles, reach / 16 + ((uint32_t)a.sinks + 15) / 16))
+            window_kernel<NS, true, 4><<<a.B * a.tiles * a.H, 256, 0, s>>>(a);
+        else
+            window_kernel<NS, true, 1><<<a.B * ((a.tiles + 3) / 4) * a.H, 256, 0, s>>>(a);
+    } else if (tiles < many_from(NS)) {
+        window_kernel<NS, false, 4><<<a.B * a.tiles * a.H, 256, 0, s>>>(a);
+    } else {
+        a.tiles = (a.max_T + 63) / 64;
+        window_many_kernel<NS><<<a.B * a.tiles * a.H, 256, 0, s>>>(a);
     }
 }
 

@@ -132,6 +132,35 @@ def test_many_tiles(hip, torch, B, T, H, G, dk, left, right, with_positions):
         assert (np.abs(got[rows] - want) <= bound).all(), (b, i)
 
 
+@pytest.mark.parametrize("dk", DKS)
+@pytest.mark.parametrize("with_positions", [False, True])
+@pytest.mark.parametrize("left,right,sinks", [(100, 20, 40), (33, 0, 0), (3, 70, 1), (700, 0, 5)])
+def test_many_rows(hip, torch, dk, with_positions, left, right, sinks):
+    """Calls of many long tiles of each width: all rows of a head around the segments' ends and some picked ones."""
+    say("rows", dk, with_positions, left, right)
+    r = random.Random(dk + left)
+    c = Call(hip, torch, [1500, 1, 1400, 1203, 70], 8, 2, dk, seed=dk, first=1, tail=4)
+    pos = c.positions(left, right) if with_positions else None
+    got = c.attend(pos, left, right, sinks)
+    assert (got[:1] == MARK).all() and (got[c.row0[-1]:] == MARK).all() and np.isfinite(got).all()
+    for b, T in enumerate(c.Ts):
+        s = slice(c.row0[b], c.row0[b] + T)
+        for i in {0, max(0, T - 6), r.randrange(T), r.randrange(T), min(T - 1, 60), min(T - 1, 126)}:
+            n = min(6, T - i)
+            rows = slice(c.row0[b] + i, c.row0[b] + i + n)
+            want, bound = wr.attend(c.q[rows], i, np.arange(T), c.k[s], c.v[s], 8, dk, pos, left, right, sinks)
+            assert (np.abs(got[rows] - want) <= bound).all(), (b, i)
+
+
+@pytest.mark.parametrize("dk", DKS)
+@pytest.mark.parametrize("with_positions", [False, True])
+def test_many_short_segments(hip, torch, dk, with_positions):
+    say("short", dk, with_positions)
+    r = random.Random(dk)
+    c = Call(hip, torch, [r.choice([0, 1, 16, 17, 33, r.randint(1, 45)]) for _ in range(300)], 4, 2, dk, seed=dk, tail=2)
+    c.check(c.positions(20, 9) if with_positions else None, 20, 9, 3)
+
+
 @pytest.mark.parametrize("seed", range(16))
 def test_any_call(hip, torch, seed):
     r = random.Random(seed)
@@ -147,8 +176,8 @@ def test_any_call(hip, torch, seed):
             r.choice([0, r.randint(1, 5), r.randint(1, 300)]))
 
 
-@pytest.mark.parametrize("T,H", [(120, 2), (1400, 8)])
-@pytest.mark.parametrize("dk", [32, 96, 128])
+@pytest.mark.parametrize("T,H", [(120, 2), (1400, 8), (2200, 16)])
+@pytest.mark.parametrize("dk", DKS)
 def test_what_is_not_attended_does_not_count(hip, torch, T, H, dk):
     """NaN and infinities in keys, values and position rows reach the rows that attend them and no others."""
     say("masked", T, H, dk)
@@ -178,8 +207,8 @@ def test_what_is_not_attended_does_not_count(hip, torch, T, H, dk):
 
 def test_bad_queries_stay_in_their_row(hip, torch):
     say("nan rows")
-    for Ts in ([50, 30], [1200, 700]):
-        c = Call(hip, torch, Ts, 4, 2, 64, seed=18)
+    for Ts, H in (([50, 30], 4), ([1200, 700], 4), ([1200, 1700], 12)):
+        c = Call(hip, torch, Ts, H, 2, 64, seed=18)
         for pos in (None, c.positions(40, 30)):
             clean = c.attend(pos, 40, 30, 2)
             q = c.q.copy()
