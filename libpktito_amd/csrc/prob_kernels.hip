@@ -23,34 +23,108 @@ struct Spread {
     float top, rest, slope;
 };
 
-/* Logits in the order that the alternatives have: greater first, of equals the
- * lower id, NaN last. */
-__device__ __forceinline__ uint64_t rank_key(float x, uint32_t id) {
+/* Logits in the order that the alternatives have, as whole numbers: greater
+ * first, of equals the lower id, NaN last. */
+__device__ __forceinline__ uint32_t ordered(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);       /* -0 is 0 */
-    const uint32_t order = x != x ? 0 : (u & 0x80000000u) ? ~u : u | 0x80000000u;
-    return (uint64_t)order << 32 | (uint32_t)~id;
+    return x != x ? 0 : (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float of_ordered(uint32_t o) {
+    return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ uint64_t rank_key(float x, uint32_t id) {
+    return (uint64_t)ordered(x) << 32 | (uint32_t)~id;
 }
 __device__ __forceinline__ uint32_t key_id(uint64_t k) { return ~(uint32_t)k; }
 
-__device__ __forceinline__ float wave_sum_f(float v) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1)
-        v += __shfl_xor(v, m);
-    return v;
+/* Over the wave, in every lane (all of them active): within 16 lanes by DPP,
+ * then across the rows into lane 63. */
+template <typename F>
+__device__ __forceinline__ uint32_t over_wave(uint32_t v, uint32_t none, F f) {
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, 0xB1, 0xF, 0xF, false));
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, 0x4E, 0xF, 0xF, false));
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, 0x141, 0xF, 0xF, false));
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, 0x140, 0xF, 0xF, false));
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, 0x142, 0xA, 0xF, false));
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, 0x143, 0xC, 0xF, false));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
-__device__ __forceinline__ float wave_max_f(float v) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1)
-        v = fmaxf(v, __shfl_xor(v, m));
-    return v;
+__device__ __forceinline__ float wave_sum_f(float x) {
+    return __uint_as_float(over_wave(__float_as_uint(x), 0, [](uint32_t a, uint32_t b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    }));
 }
-__device__ __forceinline__ uint64_t wave_max_u(uint64_t v) {
+__device__ __forceinline__ float wave_max_f(float x) {
+    return __uint_as_float(over_wave(__float_as_uint(x), 0xff800000u, [](uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }));
+}
+__device__ __forceinline__ uint32_t wave_max_u(uint32_t x) {
+    return over_wave(x, 0, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+__device__ __forceinline__ uint32_t wave_min_u(uint32_t x) {
+    return over_wave(x, ~0u, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+}
+__device__ __forceinline__ uint64_t wave_max_key(uint64_t v) {
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) {
         const uint64_t o = __shfl_xor(v, m);
         v = o > v ? o : v;
     }
     return v;
+}
+
+__device__ __forceinline__ void prob_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+/* The k greatest of a wave's many: each lane knows its own greatest, and what at
+ * least k lanes reach with theirs has k at least that reach it, and few more as a
+ * rule. Found by halving the range between the least and the greatest lane's, until
+ * k to k + 4 lanes do. */
+__device__ __forceinline__ uint32_t reached(uint32_t mine, uint32_t k) {
+    uint32_t lo = wave_min_u(mine), hi = wave_max_u(mine);
+    for (int n = 0; n < 20 && lo < hi; n++) {
+        const uint32_t mid = hi - (hi - lo) / 2;
+        const uint32_t lanes = (uint32_t)__builtin_popcountll(__ballot(mine >= mid));
+        if (lanes >= k)
+            lo = mid;
+        else
+            hi = mid - 1;
+        if (lanes >= k && lanes <= k + 4)
+            break;
+    }
+    return lo;
+}
+
+/* n keys, up to 64 of them in LDS in any order: the i-th greatest in lane i. */
+__device__ __forceinline__ uint64_t sorted(uint64_t *list, uint32_t n) {
+    const uint32_t lane = threadIdx.x & 63;
+    prob_sync();
+    const uint64_t key = lane < n ? list[lane] : 0;
+    const uint32_t lo = (uint32_t)key, hi = (uint32_t)(key >> 32);
+    uint32_t rank = 0;
+    for (uint32_t i = 0; i < n; i++) {
+        const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)hi, i) << 32 |
+                               (uint32_t)__builtin_amdgcn_readlane((int)lo, i);
+        rank += other > key;
+    }
+    if (lane < n)
+        list[rank] = key;
+    prob_sync();
+    return lane < n ? list[lane] : 0;
+}
+
+/* Lanes whose entry is taken put it behind the n in the list, if it is up to 64. */
+__device__ __forceinline__ void gather(uint64_t *list, uint32_t &n, bool taken, uint64_t key) {
+    const uint64_t who = __ballot(taken);
+    if (who == 0)
+        return;
+    const uint32_t at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+    if (taken && at < 64)
+        list[at] = key;
+    n += (uint32_t)__builtin_popcountll(who);
 }
 
 /* x of 4 V consecutive columns' values a wave, of lanes in turn 16 bytes each;
@@ -85,42 +159,53 @@ __device__ __forceinline__ uint32_t column_of(uint32_t c0, int j) {
 /* A wave's columns: the spread, and the k greatest keys (0 where there are
  * fewer), the i-th in lane i. */
 template <int V>
-__device__ __forceinline__ Spread part_of_row(const float (&x)[4 * V], uint32_t c0, uint32_t c1, uint32_t k, uint64_t &best) {
-    uint64_t mine = 0;
+__device__ __forceinline__ Spread part_of_row(const float (&x)[4 * V], uint32_t c0, uint32_t c1, uint32_t k,
+                                              uint64_t *list, uint64_t &best) {
     Spread s;
     float top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 4 * V; j++) {
-        const uint32_t c = column_of<V>(c0, j);
-        const uint64_t key = c < c1 ? rank_key(x[j], c) : 0;
-        mine = key > mine ? key : mine;
+    for (int j = 0; j < 4 * V; j++)
         top = fmaxf(top, x[j]);
-    }
     s.top = wave_max_f(top);
-    uint64_t last = wave_max_u(mine);
-    best = last;
-    const uint32_t first = key_id(last);
     const float base = s.top == -INFINITY ? 0.0f : s.top;
     float rest = 0.0f, slope = 0.0f;
+    uint32_t tops = 0;                      /* logits that are the largest: all but one count among the rest */
+#pragma unroll
+    for (int j = 0; j < 4 * V; j++) {
+        const float d = x[j] - base;
+        float e = __builtin_amdgcn_exp2f(d * kLog2e);
+        const bool is_top = x[j] == s.top;
+        tops += (uint32_t)__builtin_popcountll(__ballot(is_top));
+        e = is_top ? 0.0f : e;
+        rest += e;
+        slope = __builtin_fmaf(e, fmaxf(d, -1e30f), slope);
+    }
+    s.rest = wave_sum_f(rest) + (s.top == -INFINITY ? 0.0f : (float)(tops - 1)), s.slope = wave_sum_f(slope);
+    best = 0;
+    if (k == 0)
+        return s;
+    const float least = of_ordered(reached(ordered(top), k));
+    uint32_t n = 0;
 #pragma unroll
     for (int j = 0; j < 4 * V; j++) {
         const uint32_t c = column_of<V>(c0, j);
-        const float d = x[j] - base;
-        float e = __builtin_amdgcn_exp2f(d * kLog2e);
-        e = c >= c1 || c == first ? 0.0f : e;
-        rest += e;
-        slope = e > 0.0f ? __builtin_fmaf(e, d, slope) : slope;
+        gather(list, n, x[j] >= least && c < c1, rank_key(x[j], c));
     }
-    s.rest = wave_sum_f(rest), s.slope = wave_sum_f(slope);
-    for (uint32_t i = 1; i < k; i++) {
-        mine = 0;
+    if (n >= k && n <= 64) {
+        best = sorted(list, n);
+        return s;
+    }
+    /* many equal ones, or few that are numbers: one after another */
+    uint64_t last = ~0ull;
+    for (uint32_t i = 0; i < k; i++) {
+        uint64_t mine = 0;
 #pragma unroll
         for (int j = 0; j < 4 * V; j++) {
             const uint32_t c = column_of<V>(c0, j);
             const uint64_t key = c < c1 ? rank_key(x[j], c) : 0;
             mine = key < last && key > mine ? key : mine;
         }
-        last = wave_max_u(mine);
+        last = wave_max_key(mine);
         best = (threadIdx.x & 63) == i ? last : best;
     }
     return s;
@@ -166,7 +251,7 @@ __device__ __forceinline__ void answer_row(const Answer &a, uint32_t row, const 
  * the part whose key is the greatest has the row's largest logit, the others'
  * largest count among the rest. */
 __device__ __forceinline__ Spread joined_spread(Spread s, uint64_t key, bool live) {
-    const uint64_t first = wave_max_u(live ? key : 0);
+    const uint64_t first = wave_max_key(live ? key : 0);
     Spread r;
     r.top = wave_max_f(live ? s.top : -INFINITY);
     const float d = s.top - (r.top == -INFINITY ? 0.0f : r.top), e = __builtin_amdgcn_exp2f(d * kLog2e);
@@ -179,31 +264,15 @@ __device__ __forceinline__ Spread joined_spread(Spread s, uint64_t key, bool liv
 /* Rows of up to 256 V columns: a wave each. */
 template <int V>
 __global__ __launch_bounds__(256) void answer_wave_kernel(Answer a) {
-    const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6);
+    __shared__ uint64_t list[4][64];
+    const uint32_t wave = threadIdx.x >> 6, row = blockIdx.x * 4 + wave;
     if (row >= a.rows)
         return;
     float x[4 * V];
     load_part<V>(a.x + row * a.xs, 0, a.cols, x);
     uint64_t best;
-    const Spread s = part_of_row<V>(x, 0, a.cols, a.k, best);
+    const Spread s = part_of_row<V>(x, 0, a.cols, a.k, list[wave], best);
     answer_row(a, row, s, best);
-}
-
-/* The greatest k of n keys, the i-th in lane i. */
-template <typename K>
-__device__ __forceinline__ uint64_t greatest(uint32_t n, uint32_t k, K key) {
-    const uint32_t lane = threadIdx.x & 63;
-    uint64_t last = ~0ull, best = 0;
-    for (uint32_t i = 0; i < max(k, 1u); i++) {
-        uint64_t mine = 0;
-        for (uint32_t j = lane; j < n; j += 64) {
-            const uint64_t y = key(j);
-            mine = y < last && y > mine ? y : mine;
-        }
-        last = wave_max_u(mine);
-        best = lane == i ? last : best;
-    }
-    return best;
 }
 
 /* A workgroup's run of 1024 V columns of a row, its four waves' parts met in
@@ -211,25 +280,35 @@ __device__ __forceinline__ uint64_t greatest(uint32_t n, uint32_t k, K key) {
 template <int V>
 __global__ __launch_bounds__(256) void answer_part_kernel(Answer a) {
     __shared__ Spread spread[4];
-    __shared__ uint64_t keys[4][32];
+    __shared__ uint64_t list[4][64], keys[4][kMostAlternatives], met[kMostAlternatives];
     const uint32_t part = blockIdx.x % a.parts, row = blockIdx.x / a.parts;
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, k = max(a.k, 1u);
     const uint32_t c0 = min((part * 4 + wave) * (256 * V), a.cols), c1 = min(c0 + 256 * V, a.cols);
     float x[4 * V];
     load_part<V>(a.x + row * a.xs, c0, c1, x);
     uint64_t best;
-    const Spread s = part_of_row<V>(x, c0, c1, max(a.k, 1u), best);
-    if (lane < max(a.k, 1u))
+    const Spread s = part_of_row<V>(x, c0, c1, k, list[wave], best);
+    if (lane < k)
         keys[wave][lane] = best;
     if (lane == 0)
         spread[wave] = s;
+    if (threadIdx.x < k)
+        met[threadIdx.x] = 0;
+    __syncthreads();
+    /* a key's place among all is its place in its own list and how many of the others' are greater */
+    if (lane < k && best) {
+        uint32_t rank = lane;
+        for (uint32_t u = 1; u < 4; u++)
+            for (uint32_t i = 0; i < k; i++)
+                rank += keys[(wave + u) % 4][i] > best;
+        if (rank < k)
+            met[rank] = best;
+    }
     __syncthreads();
     if (wave)
         return;
-    const uint32_t k = max(a.k, 1u);
-    const bool live = lane < 4 && keys[lane % 4][0] != 0;
-    const Spread all = joined_spread(spread[lane % 4], keys[lane % 4][0], live);
-    best = greatest(4 * k, k, [&](uint32_t j) { return keys[j / k][j % k]; });
+    const Spread all = joined_spread(spread[lane % 4], keys[lane % 4][0], lane < 4 && keys[lane % 4][0] != 0);
+    best = lane < k ? met[lane] : 0;
     if (a.parts == 1) {
         answer_row(a, row, all, best);
         return;
@@ -242,7 +321,9 @@ __global__ __launch_bounds__(256) void answer_part_kernel(Answer a) {
 
 /* A row's parts met, a wave a row. */
 __global__ __launch_bounds__(64) void answer_join_kernel(Answer a) {
-    const uint32_t row = blockIdx.x, lane = threadIdx.x, k = max(a.k, 1u);
+    constexpr int M = 8;
+    __shared__ uint64_t list[64];
+    const uint32_t row = blockIdx.x, lane = threadIdx.x, k = max(a.k, 1u), all_keys = a.parts * k;
     const Spread *spread = a.spread + (uint64_t)row * a.parts;
     const uint64_t *keys = a.keys + (uint64_t)row * a.parts * k;
     Spread all = { -INFINITY, 0.0f, 0.0f };
@@ -256,9 +337,39 @@ __global__ __launch_bounds__(64) void answer_join_kernel(Answer a) {
             s = spread[n], key = keys[(uint64_t)n * k];
         const bool live = own ? n0 > 0 : n < a.parts && n < n0 + 63;
         all = joined_spread(s, key, live);
-        first = wave_max_u(live ? key : 0);
+        first = wave_max_key(live ? key : 0);
     }
-    const uint64_t best = greatest(a.parts * k, a.k, [&](uint32_t j) { return keys[j]; });
+    uint64_t best = 0;
+    for (uint32_t n0 = 0; a.k && n0 < all_keys; n0 += 64 * M) {     /* the greatest so far, and 64 M keys more */
+        uint64_t key[M + 1], top = best;
+        key[M] = best;
+#pragma unroll
+        for (int j = 0; j < M; j++) {
+            const uint32_t n = n0 + 64 * j + lane;
+            key[j] = n < all_keys ? keys[n] : 0;
+            top = key[j] > top ? key[j] : top;
+        }
+        const uint64_t least = (uint64_t)reached((uint32_t)(top >> 32), k) << 32;
+        uint32_t n = 0;
+#pragma unroll
+        for (int j = 0; j <= M; j++)
+            gather(list, n, key[j] != 0 && key[j] >= least, key[j]);
+        if (n >= k && n <= 64) {
+            best = sorted(list, n);
+        } else {
+            uint64_t last = ~0ull;
+            for (uint32_t i = 0; i < k; i++) {
+                uint64_t mine = 0;
+#pragma unroll
+                for (int j = 0; j <= M; j++)
+                    mine = key[j] < last && key[j] > mine ? key[j] : mine;
+                last = wave_max_key(mine);
+                best = lane == i ? last : lane > i ? 0 : best;
+            }
+        }
+        best = lane < k ? best : 0;
+        prob_sync();
+    }
     answer_row(a, row, all, best);
 }
 
