@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <array>
+#include <utility>
 
 #pragma clang fp contract(off)
 
@@ -117,28 +119,30 @@ __device__ __forceinline__ uint64_t sorted(uint64_t *list, uint32_t n) {
 }
 
 /* Lanes whose entry is taken put it behind the n in the list, if it is up to 64. */
-__device__ __forceinline__ void gather(uint64_t *list, uint32_t &n, bool taken, uint64_t key) {
+template <typename K>
+__device__ __forceinline__ void gather(uint64_t *list, uint32_t &n, bool taken, K key) {
     const uint64_t who = __ballot(taken);
     if (who == 0)
         return;
     const uint32_t at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
     if (taken && at < 64)
-        list[at] = key;
+        list[at] = key();
     n += (uint32_t)__builtin_popcountll(who);
 }
 
-/* x of 4 V consecutive columns' values a wave, of lanes in turn 16 bytes each;
+/* A wave's columns [c0, c1) of a row: 16 bytes a lane in turn V times, then 4
+ * bytes a lane S times (so 1025 columns are 17 values a lane and not 20);
  * -infinity past the end. */
-template <int V>
-__device__ __forceinline__ void load_part(const float *x, uint32_t c0, uint32_t c1, float (&y)[4 * V]) {
+template <int V, int S>
+__device__ __forceinline__ void load_part(const float *x, uint32_t c0, uint32_t c1, float (&y)[4 * V + S]) {
     const uint32_t lane = threadIdx.x & 63;
 #pragma unroll
     for (int j = 0; j < V; j++) {
         const uint32_t c = c0 + 4 * (64 * j + lane);
         p4f t = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
-        if (c + 4 <= c1)
+        if (S > 0 || c + 4 <= c1) {         /* the last columns are behind the whole ones */
             t = *(const p4f_u *)(x + c);
-        else if (c < c1) {
+        } else if (c < c1) {
             t.x = x[c];
             if (c + 1 < c1)
                 t.y = x[c + 1];
@@ -149,29 +153,35 @@ __device__ __forceinline__ void load_part(const float *x, uint32_t c0, uint32_t 
         for (int e = 0; e < 4; e++)
             y[4 * j + e] = t[e];
     }
+#pragma unroll
+    for (int j = 0; j < S; j++) {
+        const uint32_t c = c0 + 256 * V + 64 * j + lane;
+        y[4 * V + j] = c < c1 ? x[c] : -INFINITY;
+    }
 }
 
 template <int V>
-__device__ __forceinline__ uint32_t column_of(uint32_t c0, int j) {
-    return c0 + 4 * (64 * (j / 4) + (threadIdx.x & 63)) + j % 4;
+__device__ __forceinline__ uint32_t column_of(uint32_t c0, int j, uint32_t lane) {
+    return c0 + (j < 4 * V ? 4 * (64 * (j / 4) + lane) + j % 4 : 256 * V + 64 * (j - 4 * V) + lane);
 }
 
 /* A wave's columns: the spread, and the k greatest keys (0 where there are
  * fewer), the i-th in lane i. */
-template <int V>
-__device__ __forceinline__ Spread part_of_row(const float (&x)[4 * V], uint32_t c0, uint32_t c1, uint32_t k,
-                                              uint64_t *list, uint64_t &best) {
+template <int V, int S>
+__device__ __forceinline__ Spread part_of_row(const float (&x)[4 * V + S], const float *row, uint32_t c0, uint32_t c1,
+                                              uint32_t k, uint64_t *list, uint64_t &best) {
+    constexpr int E = 4 * V + S;
     Spread s;
     float top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 4 * V; j++)
+    for (int j = 0; j < E; j++)
         top = fmaxf(top, x[j]);
     s.top = wave_max_f(top);
     const float base = s.top == -INFINITY ? 0.0f : s.top;
     float rest = 0.0f, slope = 0.0f;
     uint32_t tops = 0;                      /* logits that are the largest: all but one count among the rest */
 #pragma unroll
-    for (int j = 0; j < 4 * V; j++) {
+    for (int j = 0; j < E; j++) {
         const float d = x[j] - base;
         float e = __builtin_amdgcn_exp2f(d * kLog2e);
         const bool is_top = x[j] == s.top;
@@ -185,24 +195,25 @@ __device__ __forceinline__ Spread part_of_row(const float (&x)[4 * V], uint32_t 
     if (k == 0)
         return s;
     const float least = of_ordered(reached(ordered(top), k));
-    uint32_t n = 0;
+    uint32_t n = 0, lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));          /* columns are made where one is taken: kept, they would cost half of the waves */
+    if (least > -INFINITY)                  /* what is past the end is not */
 #pragma unroll
-    for (int j = 0; j < 4 * V; j++) {
-        const uint32_t c = column_of<V>(c0, j);
-        gather(list, n, x[j] >= least && c < c1, rank_key(x[j], c));
-    }
+        for (int j = 0; j < E; j++)
+            gather(list, n, x[j] >= least, [&] { return rank_key(x[j], column_of<V>(c0, j, lane)); });
     if (n >= k && n <= 64) {
         best = sorted(list, n);
         return s;
     }
-    /* many equal ones, or few that are numbers: one after another */
+    /* many equal ones, or few that are numbers: one after another, from memory (kept in registers their keys would cost
+     * every row half of its waves) */
     uint64_t last = ~0ull;
+#pragma unroll 1
     for (uint32_t i = 0; i < k; i++) {
         uint64_t mine = 0;
-#pragma unroll
-        for (int j = 0; j < 4 * V; j++) {
-            const uint32_t c = column_of<V>(c0, j);
-            const uint64_t key = c < c1 ? rank_key(x[j], c) : 0;
+#pragma unroll 1
+        for (uint32_t c = c0 + (threadIdx.x & 63); c < c1; c += 64) {
+            const uint64_t key = rank_key(row[c], c);
             mine = key < last && key > mine ? key : mine;
         }
         last = wave_max_key(mine);
@@ -261,17 +272,17 @@ __device__ __forceinline__ Spread joined_spread(Spread s, uint64_t key, bool liv
     return r;
 }
 
-/* Rows of up to 256 V columns: a wave each. */
-template <int V>
+/* Rows of up to 2048 columns, 256 V + 64 S of them: a wave each. */
+template <int V, int S>
 __global__ __launch_bounds__(256) void answer_wave_kernel(Answer a) {
     __shared__ uint64_t list[4][64];
-    const uint32_t wave = threadIdx.x >> 6, row = blockIdx.x * 4 + wave;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = blockIdx.x * 4 + wave;
     if (row >= a.rows)
         return;
-    float x[4 * V];
-    load_part<V>(a.x + row * a.xs, 0, a.cols, x);
+    float x[4 * V + S];
+    load_part<V, S>(a.x + row * a.xs, 0, a.cols, x);
     uint64_t best;
-    const Spread s = part_of_row<V>(x, 0, a.cols, a.k, list[wave], best);
+    const Spread s = part_of_row<V, S>(x, a.x + row * a.xs, 0, a.cols, a.k, list[wave], best);
     answer_row(a, row, s, best);
 }
 
@@ -285,9 +296,9 @@ __global__ __launch_bounds__(256) void answer_part_kernel(Answer a) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, k = max(a.k, 1u);
     const uint32_t c0 = min((part * 4 + wave) * (256 * V), a.cols), c1 = min(c0 + 256 * V, a.cols);
     float x[4 * V];
-    load_part<V>(a.x + row * a.xs, c0, c1, x);
+    load_part<V, 0>(a.x + row * a.xs, c0, c1, x);
     uint64_t best;
-    const Spread s = part_of_row<V>(x, c0, c1, k, list[wave], best);
+    const Spread s = part_of_row<V, 0>(x, a.x + row * a.xs, c0, c1, k, list[wave], best);
     if (lane < k)
         keys[wave][lane] = best;
     if (lane == 0)
@@ -353,7 +364,7 @@ __global__ __launch_bounds__(64) void answer_join_kernel(Answer a) {
         uint32_t n = 0;
 #pragma unroll
         for (int j = 0; j <= M; j++)
-            gather(list, n, key[j] != 0 && key[j] >= least, key[j]);
+            gather(list, n, key[j] != 0 && key[j] >= least, [&] { return key[j]; });
         if (n >= k && n <= 64) {
             best = sorted(list, n);
         } else {
@@ -386,6 +397,14 @@ size_t answer_workspace(uint32_t rows, uint32_t cols, uint32_t k) {
 
 bool answer_fits(uint32_t rows, uint32_t cols) { return (uint64_t)rows * answer_parts(cols) < 1u << 24; }
 
+/* The kernel of rows of 64 n columns, n from 1 to 32. */
+using WaveKernel = void (*)(Answer);
+template <int... N>
+static constexpr std::array<WaveKernel, sizeof...(N)> wave_kernels(std::integer_sequence<int, N...>) {
+    return { answer_wave_kernel<(N + 1) / 4, (N + 1) % 4>... };
+}
+static const std::array<WaveKernel, 32> kWaveKernels = wave_kernels(std::make_integer_sequence<int, 32>());
+
 int launch_answer(const AnswerCall &c, hipStream_t s) {
     Answer a = {};
     a.lp = c.lp, a.entropy = c.entropy, a.top = c.top, a.top_lp = c.top_lp, a.k = c.k;
@@ -394,16 +413,8 @@ int launch_answer(const AnswerCall &c, hipStream_t s) {
     a.keys = (uint64_t *)c.ws;
     a.spread = (Spread *)((char *)c.ws + (size_t)c.rows * a.parts * std::max(c.k, 1u) * sizeof(uint64_t));
     if (c.cols <= 2048) {
-        const uint32_t grid = (c.rows + 3) / 4;
-        switch ((c.cols + 255) / 256) {
-        case 1: answer_wave_kernel<1><<<grid, 256, 0, s>>>(a); break;
-        case 2: answer_wave_kernel<2><<<grid, 256, 0, s>>>(a); break;
-        case 3: answer_wave_kernel<3><<<grid, 256, 0, s>>>(a); break;
-        case 4: answer_wave_kernel<4><<<grid, 256, 0, s>>>(a); break;
-        case 5: answer_wave_kernel<5><<<grid, 256, 0, s>>>(a); break;
-        case 6: answer_wave_kernel<6><<<grid, 256, 0, s>>>(a); break;
-        default: answer_wave_kernel<8><<<grid, 256, 0, s>>>(a); break;
-        }
+        const uint32_t sixtyfours = (c.cols + 63) / 64;
+        kWaveKernels[sixtyfours - 1]<<<(c.rows + 3) / 4, 256, 0, s>>>(a);
     } else {
         answer_part_kernel<8><<<c.rows * a.parts, 256, 0, s>>>(a);
         if (a.parts > 1)
