@@ -12,7 +12,7 @@
  * This library computes both on the GPU with the reference's bits: the int8
  * activations, their scales and every fp32 output are those of the
  * reference's scalar ref backend (backend/ref/kernels.c:24-86) on the same
- * inputs. The entry points come in six groups:
+ * inputs. The entry points come in seven groups:
  *
  *   1. the drop-in: pk_hip_quantize and pk_hip_gemm_q8 take host pointers and
  *      the arguments of the table's quantize and gemm_q8, and return with the
@@ -30,7 +30,10 @@
  *   6. the cache of keys and values, for streams of live audio: the encoder's
  *      attention over frames kept in 4 bits between calls. Its outputs are
  *      computed in 32 bits, not held to a bit pattern (the reference has no
- *      cache).
+ *      cache);
+ *   7. audio without an end: attention with a sliding window and sinks, over
+ *      whole segments and over the cache, a step's tables made on the device,
+ *      and how sure a recognizer is of its tokens. In 32 bits as well.
  *
  * Every function returns PK_HIP_OK or an error code (pk_hip_strerror names it,
  * pk_hip_last_error gives the calling thread's last message); nothing falls
@@ -561,8 +564,8 @@ int pk_hip_pool_restore(pk_hip_pool *pool, const int32_t *pairs, uint32_t n);
  *
  * The segments of a call: row0 [B + 1] in device memory, read when the kernel
  * runs, segment b's rows [row0[b], row0[b + 1]) of rows in all; max_T at least
- * the longest one's T (what is beyond max_T or beyond rows takes no part). B up
- * to 65535, rows up to 2^21, and B x H x ceil(max_T / 16) under 2^24. */
+ * the longest one's T (what is beyond max_T or beyond rows takes no part). No two
+ * segments may have one row. B up to 65535, rows up to 2^21, and B x H x ceil(max_T / 16) under 2^24. */
 typedef struct {
     const int32_t *row0;
     uint32_t B, rows, max_T;
@@ -621,7 +624,8 @@ int pk_hip_attention_sinks_dev(float *o, size_t os, const float *q, size_t qs, c
  * become fewer stay held until their stream ends. Numbers that no call leaves
  * (counts below 0 or too great, ids outside the pool) are read as the nearest
  * that can be, and never make it write outside of the arrays. max_pages 1 to
- * 2^24, B up to 65535, rows up to 2^21, max_T up to rows, pages 1 to 2^24. */
+ * 2^24, B up to 65535 and B x max_pages under 2^32, rows up to 2^21, max_T up to
+ * rows, pages 1 to 2^24. */
 typedef struct {
     int32_t *table, *len, *row0, *state, *pool, *slot, *told;
     uint32_t B, max_pages, rows, max_T, pages;

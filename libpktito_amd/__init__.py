@@ -1094,6 +1094,17 @@ def logprobs_workspace(rows, cols, k):
     return lib().pk_hip_logprobs_workspace(_u32(rows, "rows"), _u32(cols, "cols"), _u32(k, "k"))
 
 
+def _beside(t, dtype, what, device, rows, n=None):
+    """How many columns t [rows, n] has beside rows of logits, with n 0 for
+    [rows]; refuses one that is not dense, or not of these sizes."""
+    _is(t, dtype, what, device)
+    shape = t.shape
+    if len(shape) != (1 if n == 0 else 2) or shape[0] != rows or (n and shape[1] != n) or not t.is_contiguous():
+        want = (rows,) if n == 0 else (rows, "n" if n is None else n)
+        raise PkHipError(PK_HIP_EINVAL, f"{what}: {want}, contiguous, not {tuple(shape)}")
+    return shape[-1]
+
+
 def logprobs_dev(x, tokens=None, lp=None, entropy=None, top=None, top_lp=None, ws=None, stream=None):
     """How sure rows of logits are (pk_hip_logprobs_dev): x [rows, cols] float32,
     its columns dense; tokens [rows, m] int32 and their log probabilities into lp
@@ -1101,18 +1112,18 @@ def logprobs_dev(x, tokens=None, lp=None, entropy=None, top=None, top_lp=None, w
     [rows, k] int32, their log probabilities into top_lp [rows, k]; each where it
     is given. ws a uint8 tensor of logprobs_workspace(rows, cols, k) bytes."""
     _is(x, "float32", "x", None)
-    device = x.get_device()
-    if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
-        raise PkHipError(PK_HIP_EINVAL, f"x: [rows, cols], its rows dense, not {tuple(x.shape)}")
-    rows, cols = x.shape
-    m, k = (0 if t is None else t.shape[-1] if t.dim() == 2 else -1 for t in (tokens, top))
-    for t, dtype, shape, what in ((tokens, "int32", (rows, m), "tokens"), (lp, "float32", (rows, m), "lp"),
-                                  (entropy, "float32", (rows,), "entropy"), (top, "int32", (rows, k), "top"),
-                                  (top_lp, "float32", (rows, k), "top_lp")):
-        if t is not None:
-            _is(t, dtype, what, device)
-            if tuple(t.shape) != shape or not t.is_contiguous():
-                raise PkHipError(PK_HIP_EINVAL, f"{what}: {shape}, contiguous, not {tuple(t.shape)}")
+    device, shape = x.get_device(), x.shape
+    if len(shape) != 2 or (x.stride(1) != 1 and shape[1] > 1):
+        raise PkHipError(PK_HIP_EINVAL, f"x: [rows, cols], its rows dense, not {tuple(shape)}")
+    rows, cols = shape
+    m = 0 if tokens is None else _beside(tokens, "int32", "tokens", device, rows)
+    if lp is not None:
+        _beside(lp, "float32", "lp", device, rows, m)
+    if entropy is not None:
+        _beside(entropy, "float32", "entropy", device, rows, 0)
+    k = 0 if top is None else _beside(top, "int32", "top", device, rows)
+    if top_lp is not None:
+        _beside(top_lp, "float32", "top_lp", device, rows, k)
     if ws is not None:
         _is(ws, "uint8", "ws", device)
         if not ws.is_contiguous():

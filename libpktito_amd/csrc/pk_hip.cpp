@@ -1831,9 +1831,9 @@ int pk_hip_cache_plan_dev(const pk_hip_plan *p, const int32_t *add, const int32_
           (uintptr_t)p->state | (uintptr_t)p->pool | (uintptr_t)p->slot | (uintptr_t)p->told) & 3))
         return fail(PK_HIP_EINVAL, "%s: arrays 4-byte aligned", who);
     if (p->max_pages == 0 || p->max_pages > 1u << 24 || p->pages == 0 || p->pages > 1u << 24 || p->B > 65535 ||
-        p->rows > 1u << 21 || p->max_T > p->rows)
-        return fail(PK_HIP_EINVAL, "%s: 1 to 2^24 pages of the pool and of a stream, up to 65535 streams and 2^21 rows, "
-                                   "max_T up to rows", who);
+        p->rows > 1u << 21 || p->max_T > p->rows || (uint64_t)p->B * p->max_pages >> 32)
+        return fail(PK_HIP_EINVAL, "%s: 1 to 2^24 pages of the pool and of a stream, under 2^32 of all streams, up to 65535 "
+                                   "streams and 2^21 rows, max_T up to rows", who);
     if ((e = pk_hip_init()))
         return e;
     pkq8::PlanCall c = {};
