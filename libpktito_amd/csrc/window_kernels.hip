@@ -422,6 +422,11 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowAttention a) {
     }
 }
 
+/* Floats from here on round to a bfloat16 infinity. Values of them are taken
+ * apart from the others; keys and queries of them give scores that are no number,
+ * in 32 bits beyond what most products of theirs hold too. */
+constexpr float kNoPieces = 0x1.ffp127f;
+
 /* The six products of pieces that count, the smallest first. */
 __device__ __forceinline__ v4f product(const Pieces &x, const Pieces &y, v4f acc) {
     acc = mfma(x.p[2], y.p[0], acc);
@@ -456,7 +461,7 @@ __global__ __launch_bounds__(256, 2) void window_many_kernel(WindowAttention a) 
     constexpr int kEach = (32 * kChunks + 255) / 256;       /* eights of dimensions that a thread cuts */
     __shared__ v8bf key[2][NS][3][64];
     __shared__ v8bf value[NS][2][3][64];
-    __shared__ uint32_t odd_step;                           /* the step whose values hold what is no number, and one */
+    __shared__ uint32_t odd_step;                           /* the step whose values hold what has no pieces, and one */
     WindowTile s;
     if (!window_tile<64, 1>(a, s, 0))
         return;
@@ -523,18 +528,18 @@ __global__ __launch_bounds__(256, 2) void window_many_kernel(WindowAttention a) 
             x.p[k] = key[kt][t][k][slot_of((uint32_t)c, 4 * t + (uint32_t)w)];
         return x;
     };
-    /* An infinity or a NaN among the values may be only some rows': the others would get its product with their 0. The
-     * product is made without it, and the step told. */
+    /* An infinity or a NaN among the values, or a float that has no pieces, may be only some rows': the others would get
+     * its product with their 0. The product is made without it, and the step told. */
     auto put_values = [&](int32_t n) {
-        float odd = 0.0f;
+        float odd = 0.0f;                                   /* infinite, or no number, if one is; if it is, one may be */
 #pragma unroll
         for (int k = 0; k < 8; k++)
-            odd = __builtin_fmaf(raw_v[k].x, 0.0f, __builtin_fmaf(raw_v[k].y, 0.0f, odd));
-        if (__builtin_expect(__any(odd != odd), 0)) {
+            odd = __builtin_fmaf(__builtin_fabsf(raw_v[k].x), 2.0f, __builtin_fmaf(__builtin_fabsf(raw_v[k].y), 2.0f, odd));
+        if (__builtin_expect(__any(!(odd < INFINITY)), 0)) {
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                raw_v[k].x = __builtin_fmaf(raw_v[k].x, 0.0f, 0.0f) == 0.0f ? raw_v[k].x : 0.0f;
-                raw_v[k].y = __builtin_fmaf(raw_v[k].y, 0.0f, 0.0f) == 0.0f ? raw_v[k].y : 0.0f;
+                raw_v[k].x = __builtin_fabsf(raw_v[k].x) < kNoPieces ? raw_v[k].x : 0.0f;
+                raw_v[k].y = __builtin_fabsf(raw_v[k].y) < kNoPieces ? raw_v[k].y : 0.0f;
             }
             odd_step = (uint32_t)n + 1;
         }
@@ -588,7 +593,7 @@ __global__ __launch_bounds__(256, 2) void window_many_kernel(WindowAttention a) 
         window_softmax<2, 2 * NS>(e, top, sum, o);
         if (__builtin_expect(odd_step == (uint32_t)n + 1, 0)) {
 #pragma unroll 1
-            for (int32_t k = 0; k < 32; k++) {              /* each value that is no number, to the rows that attend it */
+            for (int32_t k = 0; k < 32; k++) {              /* each value that was left out, to the rows that attend it */
                 const int32_t j = j0 + k;
                 if (j >= s.T)
                     break;
@@ -605,7 +610,7 @@ __global__ __launch_bounds__(256, 2) void window_many_kernel(WindowAttention a) 
 #pragma unroll
                             for (int d = 0; d < 2; d++) {
                                 const float y = src[32 * b + 2 * r + d];
-                                if (__builtin_fmaf(y, 0.0f, 0.0f) != 0.0f)
+                                if (!(__builtin_fabsf(y) < kNoPieces))
                                     o[2 * b + d][r] += mine * y;
                             }
             }

@@ -205,6 +205,29 @@ def test_what_is_not_attended_does_not_count(hip, torch, T, H, dk):
         assert np.array_equal(got[~hit], clean[~hit]) and np.isnan(got[hit]).all()
 
 
+@pytest.mark.parametrize("T,H", [(120, 2), (1400, 8), (2200, 16)])
+@pytest.mark.parametrize("dk", DKS)
+def test_the_greatest_floats(hip, torch, T, H, dk):
+    """The type's greatest and lowest values as padding, in keys and values and position rows that rows do not attend: all
+    but the rows that attend them keep their bits, and the outputs of theirs that no such value takes part in."""
+    say("greatest", T, H, dk)
+    c = Call(hip, torch, [T, 50], H, H, dk, seed=10)
+    left, right, sinks = 20, 3, 2
+    for pos in (None, c.positions(left, right)):
+        clean = c.attend(pos, left, right, sinks)
+        for x in (np.finfo(np.float32).min, np.finfo(np.float32).max, np.float32(2.0 ** 127 * (2 - 2.0 ** -8))):
+            k, v = c.k.copy(), c.v.copy()
+            v[60, ::7], k[90] = x, x
+            rows = np.arange(c.rows)
+            of_value = (rows >= 60 - right) & (rows <= 60 + left)
+            of_key = (rows >= 90 - right) & (rows <= 90 + left)
+            got = c.attend(pos, left, right, sinks, k=k, v=v)
+            assert np.array_equal(got[~of_value & ~of_key], clean[~of_value & ~of_key])
+            other = np.arange(got.shape[1]) % 7 != 0
+            assert np.array_equal(got[of_value & ~of_key][:, other], clean[of_value & ~of_key][:, other])
+            assert not np.isnan(got[of_value & ~of_key]).any()
+
+
 def test_bad_queries_stay_in_their_row(hip, torch):
     say("nan rows")
     for Ts, H in (([50, 30], 4), ([1200, 700], 4), ([1200, 1700], 12)):
