@@ -624,7 +624,7 @@ int pk_hip_attention_sinks_dev(float *o, size_t os, const float *q, size_t qs, c
  * become fewer stay held until their stream ends. Numbers that no call leaves
  * (counts below 0 or too great, ids outside the pool) are read as the nearest
  * that can be, and never make it write outside of the arrays. max_pages 1 to
- * 2^24, B up to 65535 and B x max_pages under 2^32, rows up to 2^21, max_T up to
+ * 2^24, B up to 65535 and B x max_pages up to 2^31, rows up to 2^21, max_T up to
  * rows, pages 1 to 2^24. */
 typedef struct {
     int32_t *table, *len, *row0, *state, *pool, *slot, *told;

@@ -1685,17 +1685,23 @@ static int attention_window(const pk_hip_cache *c, const pk_hip_streams *st, uin
     return PK_HIP_OK;
 }
 
-size_t pk_hip_attention_sinks_workspace(const pk_hip_cache *c, const pk_hip_streams *st, uint32_t H,
-                                        const pk_hip_positions *pos, uint32_t left, uint32_t right, uint32_t sinks) {
+static size_t attention_workspace(const pk_hip_cache *c, const pk_hip_streams *st, uint32_t H,
+                                  const pk_hip_positions *pos, uint32_t left, uint32_t right, uint32_t sinks,
+                                  const char *who) {
     int32_t l, r, n;
-    if (attention_window(c, st, H, pos, left, right, sinks, "attention_cache_workspace", &l, &r, &n))
+    if (attention_window(c, st, H, pos, left, right, sinks, who, &l, &r, &n))
         return 0;
     return pkq8::cache_attention_workspace(streams_of(st), c->heads, H, c->dk, pos != nullptr, l, r, n);
 }
 
+size_t pk_hip_attention_sinks_workspace(const pk_hip_cache *c, const pk_hip_streams *st, uint32_t H,
+                                        const pk_hip_positions *pos, uint32_t left, uint32_t right, uint32_t sinks) {
+    return attention_workspace(c, st, H, pos, left, right, sinks, "attention_sinks_workspace");
+}
+
 size_t pk_hip_attention_cache_workspace(const pk_hip_cache *c, const pk_hip_streams *st, uint32_t H,
                                         const pk_hip_positions *pos, uint32_t left, uint32_t right) {
-    return pk_hip_attention_sinks_workspace(c, st, H, pos, left, right, 0);
+    return attention_workspace(c, st, H, pos, left, right, 0, "attention_cache_workspace");
 }
 
 static int attention_cache(float *o, size_t os, const float *q, size_t qs, const pk_hip_cache *c, uint32_t layer,
@@ -1831,8 +1837,8 @@ int pk_hip_cache_plan_dev(const pk_hip_plan *p, const int32_t *add, const int32_
           (uintptr_t)p->state | (uintptr_t)p->pool | (uintptr_t)p->slot | (uintptr_t)p->told) & 3))
         return fail(PK_HIP_EINVAL, "%s: arrays 4-byte aligned", who);
     if (p->max_pages == 0 || p->max_pages > 1u << 24 || p->pages == 0 || p->pages > 1u << 24 || p->B > 65535 ||
-        p->rows > 1u << 21 || p->max_T > p->rows || (uint64_t)p->B * p->max_pages >> 32)
-        return fail(PK_HIP_EINVAL, "%s: 1 to 2^24 pages of the pool and of a stream, under 2^32 of all streams, up to 65535 "
+        p->rows > 1u << 21 || p->max_T > p->rows || (uint64_t)p->B * p->max_pages > 1u << 31)
+        return fail(PK_HIP_EINVAL, "%s: 1 to 2^24 pages of the pool and of a stream, up to 2^31 of all streams, up to 65535 "
                                    "streams and 2^21 rows, max_T up to rows", who);
     if ((e = pk_hip_init()))
         return e;

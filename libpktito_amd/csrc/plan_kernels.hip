@@ -96,7 +96,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanCall p) {
         const int32_t behind = p.left < 0 ? 0 : (int32_t)(max((int64_t)start - p.left, (int64_t)0) / kPage);
         const int32_t c0 = fresh ? 0 : max(gone, (int32_t)p.kept), c1 = fresh ? (had + (int32_t)kPage - 1) / (int32_t)kPage : behind;
         const uint32_t n = live ? (uint32_t)max(c1 - c0, 0) : 0;
-        /* under 2^32 all of them: 1024 of up to 2^21 rows, the columns of a table, halves of what is asked */
+        /* up to 2^31 each: 1024 of up to 2^21 rows, the columns of a table, halves of what is asked */
         uint32_t v[4] = { want, n, add & 0xffff, add >> 16 }, all[4];
         scan<4>(v, all, sums);
         const uint64_t upto = rows + v[0];

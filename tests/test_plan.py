@@ -34,7 +34,7 @@ def call(pk, **change):
     dict(add=None), dict(add=32770), dict(fresh=1), dict(table=4097), dict(len=2), dict(row0=3), dict(state=5), dict(pool=6),
     dict(slot=7), dict(told=9), dict(max_pages=0), dict(max_pages=(1 << 24) + 1), dict(pages=0), dict(pages=(1 << 24) + 1),
     dict(B=65536), dict(rows=(1 << 21) + 1), dict(max_T=11),
-    dict(B=256, max_pages=1 << 24),
+    dict(B=256, max_pages=1 << 24), dict(B=129, max_pages=1 << 24), dict(B=257, max_pages=16711935),
 ], ids=str)
 def test_refusals(pk, change):
     code, why = call(pk, **change)
@@ -43,7 +43,7 @@ def test_refusals(pk, change):
 
 @pytest.mark.parametrize("change", [
     dict(), dict(fresh=None), dict(slot=None), dict(left=0xffffffff, sinks=0xffffffff), dict(rows=0, max_T=0),
-    dict(B=0, table=None, len=None, state=None, add=None),
+    dict(B=0, table=None, len=None, state=None, add=None), dict(B=128, max_pages=1 << 24),
 ], ids=str)
 def test_calls_that_are_taken(pk, change):
     import torch
