@@ -156,12 +156,15 @@ __device__ __forceinline__ void wave_sync() {
  * than its scores', so they pass through LDS.
  *
  * An hour (45000 frames, 8 heads of 128, 128 + 128 + 1 frames and 16 sinks, 75.6
- * GFLOP): 785 us, 96 TFLOP/s of the 154 that an fp32 product reaches. The matrix
- * instructions are busy 63% of it; vector instructions, LDS and loads hold them up,
- * two waves a SIMD or one (4900 and 5400 clocks a step, of which 3072 are theirs).
- * Keys by lanes that use them took 910 (53 cache lookups a load, 16 now). Measured
- * and no faster: the shared cutting of the kernel below (820: four barriers a step),
- * 32 rows a wave cut into pieces in its registers (850, a wave a SIMD). */
+ * GFLOP): 797 us, 95 TFLOP/s of the 154 that an fp32 product reaches. The matrix
+ * instructions are busy 64% of it, two waves a SIMD or one (4900 and 5400 clocks a
+ * step, of which 3072 are theirs). What holds them up is the loads, 24 a step whose
+ * results pass into registers: without them the same products take 630; without
+ * masks, places' skew and exponentials 765. Keys by lanes that use them took 910 (53
+ * cache lookups a load, 16 now). Measured and no faster: loads straight to LDS, a step
+ * ahead (840), the sinks merged into the window's steps (820), two chains of products
+ * side by side (805), the shared cutting of the kernel below (820: four barriers a
+ * step), 32 rows a wave cut into pieces in its registers (850, a wave a SIMD). */
 template <int NS, bool POS, int W>
 __global__ __launch_bounds__(256, 2) void window_kernel(WindowAttention a) {
     using S = WindowShape<NS>;
