@@ -228,6 +228,35 @@ def test_the_greatest_floats(hip, torch, T, H, dk):
             assert not np.isnan(got[of_value & ~of_key]).any()
 
 
+@pytest.mark.parametrize("H", [8, 480])
+def test_rows_past_32_bits(hip, torch, H):
+    """Rows 2^25 floats apart, the furthest past 2^33 bytes: the bits of the same rows side by side."""
+    say("far rows", H)
+    G, dk, step = 2, 32, 1 << 25
+    c = Call(hip, torch, [78], H, G, dk, seed=23, first=1, tail=1)
+    mem = torch.empty(c.rows * step, device="cuda")
+    place, views = 0, []
+    for x, w in ((np.full((c.rows, H * dk), MARK, np.float32), H * dk), (c.q, H * dk), (c.k, G * dk), (c.v, G * dk)):
+        views.append(torch.as_strided(mem, (c.rows, w), (step, 1), place))
+        views[-1].copy_(torch.from_numpy(x))
+        place += w
+    segments = hip.Segments(c.dev(c.row0), c.rows, c.max_T)
+    for pos in (None, c.positions(30, 9)):
+        at = None if pos is None else (c.dev(pos[0]), pos[1], c.dev(pos[2]), c.dev(pos[3]))
+        want = c.attend(pos, 30, 9, 3)
+        views[0].fill_(MARK)
+        hip.attention_window_dev(*views, segments, H, dk, at, 30, 9, 3)
+        assert np.array_equal(views[0].cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("H,G", [(2048, 1024), (3001, 1)])
+@pytest.mark.parametrize("with_positions", [False, True])
+def test_many_heads(hip, torch, H, G, with_positions):
+    say("heads", H, G, with_positions)
+    c = Call(hip, torch, [3, 2], H, G, 32, seed=24)
+    c.check(c.positions(2, 1) if with_positions else None, 2, 1, 1)
+
+
 def test_bad_queries_stay_in_their_row(hip, torch):
     say("nan rows")
     for Ts, H in (([50, 30], 4), ([1200, 700], 4), ([1200, 1700], 12)):
