@@ -158,7 +158,7 @@ __device__ __forceinline__ void wave_sync() {
  * An hour (45000 frames, 8 heads of 128, 128 + 128 + 1 frames and 16 sinks, 75.6
  * GFLOP): 797 us, 95 TFLOP/s of the 154 that an fp32 product reaches. The matrix
  * instructions are busy 64% of it, two waves a SIMD or one (4900 and 5400 clocks a
- * step, of which 3072 are theirs). What holds them up is the loads, 24 a step whose
+ * step, of which 3100 are theirs). What holds them up is the loads, 24 a step whose
  * results pass into registers: without them the same products take 630; without
  * masks, places' skew and exponentials 765. Keys by lanes that use them took 910 (53
  * cache lookups a load, 16 now). Measured and no faster: loads straight to LDS, a step
