@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #pragma clang fp contract(off)
 
@@ -426,9 +427,15 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowAttention a) {
 }
 
 /* Floats from here on round to a bfloat16 infinity. Values of them are taken
- * apart from the others; keys and queries of them give scores that are no number,
- * in 32 bits beyond what most products of theirs hold too. */
+ * apart from the others. */
 constexpr float kNoPieces = 0x1.ffp127f;
+
+/* Keys are cut at 2^-40 of what they are and queries at 2^40 of it: every finite
+ * key has pieces then, and what pieces end at, 2^-126, is 2^-162 of a query and
+ * 2^-86 of a key. Against the greatest key that is 2^-34 of a score, and against
+ * queries under this bound 2^-36. Queries from it on are taken as no number, which
+ * gives each of their scores the care below. */
+constexpr float kKeyScale = 0x1p-40f, kQueryScale = 0x1p40f, kMostQuery = 0x1p90f;
 
 /* The six products of pieces that count, the smallest first. */
 __device__ __forceinline__ v4f product(const Pieces &x, const Pieces &y, v4f acc) {
@@ -465,6 +472,7 @@ __global__ __launch_bounds__(256, 2) void window_many_kernel(WindowAttention a) 
     __shared__ v8bf key[2][NS][3][64];
     __shared__ v8bf value[NS][2][3][64];
     __shared__ uint32_t odd_step;                           /* the step whose values hold what has no pieces, and one */
+    __shared__ uint32_t again;
     WindowTile s;
     if (!window_tile<64, 1>(a, s, 0))
         return;
@@ -472,15 +480,19 @@ __global__ __launch_bounds__(256, 2) void window_many_kernel(WindowAttention a) 
     const int32_t c = (int32_t)(lane % 16), w = (int32_t)(lane / 16), iw = s.i0 + 16 * (int32_t)wave, i = iw + c;
 
     Pieces q[NS];                           /* scores in powers of 2 */
-    const float *src = a.q + (uint64_t)(s.r0 + min(i, s.T - 1)) * a.qs + s.h * dk + 8 * w;
+    const float *query = a.q + (uint64_t)(s.r0 + min(i, s.T - 1)) * a.qs + s.h * dk + 8 * w;
+    const float query_scale = a.scale * kQueryScale;
 #pragma unroll
     for (int t = 0; t < NS; t++) {
-        const v4f x = *(const v4f *)(src + 32 * t) * a.scale, y = *(const v4f *)(src + 32 * t + 4) * a.scale;
-        const float z[8] = { x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3] };
+        const v4f x = *(const v4f *)(query + 32 * t) * query_scale, y = *(const v4f *)(query + 32 * t + 4) * query_scale;
+        float z[8] = { x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3] };
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            z[e] = __builtin_fabsf(z[e]) < kMostQuery ? z[e] : __builtin_nanf("");
         q[t] = cut_near(z);
     }
-    float top = -INFINITY, sum = 0.0f;
-    v4f o[2 * NS] = {};
+    float top, sum;
+    v4f o[2 * NS];
 
     /* the window's frames [lo, hi] of any of the rows, the sinks [0, far) before them, the steps of both */
     const int32_t lo = max(s.i0 - a.left, 0), hi = min(s.i0 + 63 + a.right, s.T - 1), far = min(a.sinks, lo);
@@ -516,7 +528,8 @@ __global__ __launch_bounds__(256, 2) void window_many_kernel(WindowAttention a) 
 #pragma unroll
         for (int e = 0; e < kEach; e++) {
             const uint32_t n = threadIdx.x + 256 * e, row = n / kChunks, chunk = n % kChunks;
-            const float z[8] = { x[e][0][0], x[e][0][1], x[e][0][2], x[e][0][3], x[e][1][0], x[e][1][1], x[e][1][2], x[e][1][3] };
+            const v4f u = x[e][0] * kKeyScale, v = x[e][1] * kKeyScale;
+            const float z[8] = { u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3] };
             const Pieces y = cut_near(z);
             if (32 * kChunks % 256 == 0 || n < 32 * kChunks)
 #pragma unroll
@@ -531,21 +544,7 @@ __global__ __launch_bounds__(256, 2) void window_many_kernel(WindowAttention a) 
             x.p[k] = key[kt][t][k][slot_of((uint32_t)c, 4 * t + (uint32_t)w)];
         return x;
     };
-    /* An infinity or a NaN among the values, or a float that has no pieces, may be only some rows': the others would get
-     * its product with their 0. The product is made without it, and the step told. */
-    auto put_values = [&](int32_t n) {
-        float odd = 0.0f;                                   /* infinite, or no number, if one is; if it is, one may be */
-#pragma unroll
-        for (int k = 0; k < 8; k++)
-            odd = __builtin_fmaf(__builtin_fabsf(raw_v[k].x), 2.0f, __builtin_fmaf(__builtin_fabsf(raw_v[k].y), 2.0f, odd));
-        if (__builtin_expect(__any(!(odd < INFINITY)), 0)) {
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                raw_v[k].x = __builtin_fabsf(raw_v[k].x) < kNoPieces ? raw_v[k].x : 0.0f;
-                raw_v[k].y = __builtin_fabsf(raw_v[k].y) < kNoPieces ? raw_v[k].y : 0.0f;
-            }
-            odd_step = (uint32_t)n + 1;
-        }
+    auto put_values = [&]() {
         if (wave < NS)
 #pragma unroll
             for (int d = 0; d < 2; d++) {
@@ -556,83 +555,159 @@ __global__ __launch_bounds__(256, 2) void window_many_kernel(WindowAttention a) 
                     value[wave][d][k][lane] = y.p[k];
             }
     };
-    if (threadIdx.x == 0)
-        odd_step = 0;
-    load_keys(first_of(0));
-    load_values(first_of(0));
-#pragma unroll 1
-    for (int32_t n = 0; n < steps; n++) {
-        const int32_t j0 = first_of(n), next = first_of(min(n + 1, steps - 1));
-        __syncthreads();
-        put(raw);
-        put_values(n);
-        load_keys(next);
-        load_values(next);
-        __syncthreads();
-        /* whether any of the wave's rows attends any of the frames */
-        const bool busy = n < ns || (j0 + 31 >= iw - a.left && j0 <= iw + 15 + a.right) || j0 < a.sinks;
-        if (!busy)
-            continue;
-        v4f x[2] = {};
+    /* With care: an infinity or a NaN among the values, or a float that has no pieces, may be only some rows': the others
+     * got its product with their 0. So the product is made without it, and the step told. */
+    auto leave_out = [&](int32_t n) {
+        bool odd = false;
 #pragma unroll
-        for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-            for (int t = 0; t < NS; t++)
-                x[kt] = product(operand(kt, t), q[t], x[kt]);
-        if (n < ns) {
-#pragma unroll
-            for (int k = 0; k < 8; k++)
-                x[k / 4][k % 4] = j0 + 16 * (k / 4) + 4 * w + k % 4 < far ? x[k / 4][k % 4] : -INFINITY;
-        } else if (j0 < iw + 15 - a.left || j0 + 31 > min(iw + a.right, s.T - 1)) {
-            const int32_t last = min(i + a.right, s.T - 1);
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const int32_t j = j0 + 16 * (k / 4) + 4 * w + k % 4;
-                const bool seen = (j <= last) & ((j >= i - a.left) | (j < a.sinks));
-                x[k / 4][k % 4] = seen ? x[k / 4][k % 4] : -INFINITY;
-            }
-        }
-        v4f e[2] = { x[0], x[1] };
-        window_softmax<2, 2 * NS>(e, top, sum, o);
-        if (__builtin_expect(odd_step == (uint32_t)n + 1, 0)) {
-#pragma unroll 1
-            for (int32_t k = 0; k < 32; k++) {              /* each value that was left out, to the rows that attend it */
-                const int32_t j = j0 + k;
-                if (j >= s.T)
-                    break;
-                const float mine = __shfl(k % 4 == 0 ? e[k / 16][0] : k % 4 == 1 ? e[k / 16][1] : k % 4 == 2 ? e[k / 16][2] : e[k / 16][3],
-                                          16 * (k / 4 % 4) + c);
-                const float score = __shfl(k % 4 == 0 ? x[k / 16][0] : k % 4 == 1 ? x[k / 16][1] : k % 4 == 2 ? x[k / 16][2] : x[k / 16][3],
-                                           16 * (k / 4 % 4) + c);
-                const float *src = a.v + (uint64_t)(s.r0 + j) * a.vs + s.g * dk + 8 * w;
-                if (score != -INFINITY)
-#pragma unroll
-                    for (int b = 0; b < NS; b++)
-#pragma unroll
-                        for (int r = 0; r < 4; r++)
-#pragma unroll
-                            for (int d = 0; d < 2; d++) {
-                                const float y = src[32 * b + 2 * r + d];
-                                if (!(__builtin_fabsf(y) < kNoPieces))
-                                    o[2 * b + d][r] += mine * y;
-                            }
-            }
-        }
-        const float z[8] = { e[0][0], e[0][1], e[0][2], e[0][3], e[1][0], e[1][1], e[1][2], e[1][3] };
-        const Pieces prob = cut_near(z);
-#pragma unroll
-        for (int b = 0; b < NS; b++)
+        for (int k = 0; k < 8; k++)
 #pragma unroll
             for (int d = 0; d < 2; d++) {
-                Pieces y;
-#pragma unroll
-                for (int k = 0; k < 3; k++)
-                    y.p[k] = value[b][d][k][lane];
-                o[2 * b + d] = product(y, prob, o[2 * b + d]);
+                const bool has = __builtin_fabsf(raw_v[k][d]) < kNoPieces;
+                odd |= !has;
+                raw_v[k][d] = has ? raw_v[k][d] : 0.0f;
             }
-    }
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
+        if (odd)
+            odd_step = (uint32_t)n + 1;
+    };
+    /* of the lane's eight of a step's 32 frames that of frame k, as the query's lane has it */
+    auto of_frame = [&](const v4f (&x)[2], int32_t k) {
+        float y = x[0][0];
+#pragma unroll
+        for (int n = 1; n < 8; n++)
+            y = k / 16 * 4 + k % 4 == n ? x[n / 4][n % 4] : y;
+        return __shfl(y, 16 * (k / 4 % 4) + c);
+    };
+    auto add_left_out = [&](int32_t j0, const v4f (&x)[2], const v4f (&e)[2]) {
+#pragma unroll 1
+        for (int32_t k = 0; k < 32 && j0 + k < s.T; k++) {
+            const float mine = of_frame(e, k), score = of_frame(x, k);
+            const float *src = a.v + (uint64_t)(s.r0 + j0 + k) * a.vs + s.g * dk + 8 * w;
+            if (score != -INFINITY)
+#pragma unroll
+                for (int b = 0; b < NS; b++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+#pragma unroll
+                        for (int d = 0; d < 2; d++) {
+                            const float y = src[32 * b + 2 * r + d];
+                            if (!(__builtin_fabsf(y) < kNoPieces))
+                                o[2 * b + d][r] += mine * y;
+                        }
+        }
+    };
+    /* Scores that are no number are made again from the floats themselves: an infinite key has pieces that are none, and
+     * its score may be -infinity. */
+    auto score_again = [&](int32_t j0, v4f (&x)[2]) {
+        bool none = false;
+#pragma unroll
+        for (int n = 0; n < 8; n++)
+            none |= x[n / 4][n % 4] != x[n / 4][n % 4];
+        if (!__any(none))
+            return;
+#pragma unroll 1
+        for (int32_t k = 0; k < 32 && j0 + k < s.T; k++) {
+            const float *key = a.k + (uint64_t)(s.r0 + j0 + k) * a.ks + s.g * dk + 8 * w;
+            float score = 0.0f;
+#pragma unroll 1
+            for (int t = 0; t < 8 * NS; t++)
+                score = __builtin_fmaf(query[32 * (t / 8) + t % 8] * a.scale, key[32 * (t / 8) + t % 8], score);
+            score += __shfl_xor(score, 16);
+            score += __shfl_xor(score, 32);
+#pragma unroll
+            for (int n = 0; n < 8; n++) {
+                const float mine = x[n / 4][n % 4];
+                x[n / 4][n % 4] = mine != mine && k == 16 * (n / 4) + 4 * w + n % 4 ? score : mine;
+            }
+        }
+    };
+    if (threadIdx.x == 0)
+        odd_step = again = 0;
+    auto pass = [&](auto careful) {
+        top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int n = 0; n < 2 * NS; n++)
+            o[n] = v4f{};
+        if constexpr (!careful) {
+            load_keys(first_of(0));
+            load_values(first_of(0));
+        }
+#pragma unroll 1
+        for (int32_t n = 0; n < steps; n++) {
+            const int32_t j0 = first_of(n), next = first_of(min(n + 1, steps - 1));
+            if constexpr (careful) {                /* not ahead: the care needs the registers */
+                load_keys(j0);
+                load_values(j0);
+            }
+            __syncthreads();
+            put(raw);
+            if constexpr (careful)
+                leave_out(n);
+            put_values();
+            if constexpr (!careful) {
+                load_keys(next);
+                load_values(next);
+            }
+            __syncthreads();
+            /* whether any of the wave's rows attends any of the frames */
+            const bool busy = n < ns || (j0 + 31 >= iw - a.left && j0 <= iw + 15 + a.right) || j0 < a.sinks;
+            if (!busy)
+                continue;
+            v4f x[2] = {};
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                for (int t = 0; t < NS; t++)
+                    x[kt] = product(operand(kt, t), q[t], x[kt]);
+            if (n < ns) {
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    x[k / 4][k % 4] = j0 + 16 * (k / 4) + 4 * w + k % 4 < far ? x[k / 4][k % 4] : -INFINITY;
+            } else if (j0 < iw + 15 - a.left || j0 + 31 > min(iw + a.right, s.T - 1)) {
+                const int32_t last = min(i + a.right, s.T - 1);
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const int32_t j = j0 + 16 * (k / 4) + 4 * w + k % 4;
+                    const bool seen = (j <= last) & ((j >= i - a.left) | (j < a.sinks));
+                    x[k / 4][k % 4] = seen ? x[k / 4][k % 4] : -INFINITY;
+                }
+            }
+            if constexpr (careful)
+                score_again(j0, x);
+            v4f e[2] = { x[0], x[1] };
+            window_softmax<2, 2 * NS>(e, top, sum, o);
+            if constexpr (careful)
+                if (odd_step == (uint32_t)n + 1)
+                    add_left_out(j0, x, e);
+            const float z[8] = { e[0][0], e[0][1], e[0][2], e[0][3], e[1][0], e[1][1], e[1][2], e[1][3] };
+            const Pieces prob = cut_near(z);
+#pragma unroll
+            for (int b = 0; b < NS; b++)
+#pragma unroll
+                for (int d = 0; d < 2; d++) {
+                    Pieces y;
+#pragma unroll
+                    for (int k = 0; k < 3; k++)
+                        y.p[k] = value[b][d][k][lane];
+                    o[2 * b + d] = product(y, prob, o[2 * b + d]);
+                }
+        }
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+    };
+    pass(std::false_type());
+    /* An infinity or a NaN among the outputs or in a sum: once more then, with care. */
+    float odd = sum;
+#pragma unroll
+    for (int n = 0; n < 2 * NS; n++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            odd = __builtin_fmaf(o[n][r], 0.0f, odd);
+    if (i < s.T && odd != odd)
+        again = 1;
+    __syncthreads();
+    if (__builtin_expect(again, 0))
+        pass(std::true_type());
     if (i >= s.T)
         return;
     const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;

@@ -1,0 +1,85 @@
+"""Attention with a window and sinks over the whole range of floats: the greatest
+and the lowest ones, infinities, the smallest, in rows that attend them, against 64
+bits (window_ref.attend). Calls of few tiles and of so many that keys and values
+are cut into pieces."""
+import sys
+
+import numpy as np
+import pytest
+
+import window_ref as wr
+from test_gpu_window import Call
+
+pytestmark = pytest.mark.gpu
+DKS = (32, 64, 96, 128)
+FEW, MANY = (120, 2), (2200, 16)
+F32 = np.finfo(np.float32)
+
+
+def say(*a):
+    print("[case]", *a, flush=True)
+    sys.stdout.flush()
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    assert torch.cuda.is_available()
+    return torch
+
+
+def want(c, rows, positions, left, right, sinks, without=()):
+    """The outputs of rows of the first segment and their bound, as if the frames `without` were not there."""
+    frames = np.setdiff1d(np.arange(c.Ts[0]), without)
+    out = [wr.attend(c.q[i:i + 1], i, frames, c.k[frames], c.v[frames], c.H, c.dk, positions, left, right, sinks)
+           for i in rows]
+    return np.concatenate([x[0] for x in out]), np.concatenate([x[1] for x in out])
+
+
+def near(got, ref, bound):
+    off = np.abs(got - ref)
+    assert np.isfinite(got).all() and (off <= bound).all(), (got[off > bound][:4], ref[off > bound][:4], off.max())
+
+
+@pytest.mark.parametrize("T,H", [FEW, MANY])
+@pytest.mark.parametrize("dk", DKS)
+@pytest.mark.parametrize("with_positions", [False, True])
+@pytest.mark.parametrize("lowest", [F32.min, -np.inf, np.float32(-(2.0 ** 127) * (2 - 2.0 ** -8))])
+def test_a_dimension_as_a_mask(hip, torch, T, H, dk, with_positions, lowest):
+    """Frames masked by a key of the type's lowest value (or an infinity) where queries are 1: weight 0, and rows that
+    attend them as if they were not there; one row attends nothing else and is not asked for."""
+    say("mask", T, H, dk, with_positions, lowest)
+    c = Call(hip, torch, [T, 50], H, H, dk, seed=dk)
+    left, right, sinks = 20, 3, 2
+    pos = c.positions(left, right) if with_positions else None
+    at = np.arange(H) * dk + 5
+    c.q[:, at] = 1.0
+    masked = np.array([1, 60, 61, 62, 77, T - 2])
+    c.k[np.ix_(masked, at)] = lowest
+    got = c.attend(pos, left, right, sinks)
+    rows = [0, 1, 30, 58, 59, 60, 61, 62, 70, 77, 79, 82, 83, 97, T - 20, T - 2, T - 1]
+    near(got[rows], *want(c, rows, pos, left, right, sinks, masked))
+
+
+@pytest.mark.parametrize("T,H", [FEW, MANY])
+@pytest.mark.parametrize("dk", DKS)
+@pytest.mark.parametrize("with_positions", [False, True])
+@pytest.mark.parametrize("small,great", [(2.0 ** -126, F32.max), (1e-30, 1e30), (1e-18, 1e18), (1e30, 1e-30), (1e18, 1e-18),
+                                         (F32.max / 4, 2.0 ** -125), (2.0 ** 49, 2.0 ** -50)])
+def test_small_queries_great_keys(hip, torch, T, H, dk, with_positions, small, great):
+    """A dimension whose queries are as small as its keys are great, and the other way round: scores of both signs."""
+    say("scales", T, H, dk, with_positions, small, great)
+    c = Call(hip, torch, [T, 50], H, H, dk, seed=dk)
+    left, right, sinks = 20, 3, 2
+    pos = c.positions(left, right) if with_positions else None
+    at = np.arange(H) * dk + 5
+    if pos:
+        pos[2][at] = pos[3][at] = 0         # the smallest queries stay as small with their biases
+        pos[0][:, at] = 0
+    sign = np.where(c.g.random((c.rows, H)) < 0.5, -1, 1)
+    q = (1 + 0.5 * c.g.random((c.rows, H))) * (small if small < 1 else small / 2)
+    k = sign * (0.5 + 0.5 * c.g.random((c.rows, H))) * great
+    c.q[:, at], c.k[:, at] = q.astype(np.float32), k.astype(np.float32)
+    got = c.attend(pos, left, right, sinks)
+    rows = [0, 1, 30, 59, 60, 77, 100, T - 2, T - 1]
+    near(got[rows], *want(c, rows, pos, left, right, sinks))
