@@ -140,6 +140,93 @@ __device__ __forceinline__ void window_softmax(v4f (&s)[KT], float &top, float &
     }
 }
 
+/* A row by itself in 64 bits, dimension lane + 64 n of it in y[n]: for the outputs that 32 bits do not hold on their way.
+ * Sums of weights and values are before their division up to 2^8 (the slack) and the frames' number times the
+ * greatest value, and scores may be beyond floats. Frames whose score is -infinity have no part, and a row without
+ * others is 0. Two walks over the frames, a frame a lane for the scores, a dimension a lane for the values: about fifty
+ * times what the row costs beside others (the hour below with values of 1e37 in every row 37 ms; where all are no
+ * numbers the walks end early). */
+template <int NS, bool POS>
+__device__ __forceinline__ void window_row(const WindowAttention &a, const WindowTile &s, int32_t i, float (&y)[(NS + 1) / 2]) {
+    constexpr int dk = 32 * NS, N = (NS + 1) / 2;
+    const int32_t lane = (int32_t)(threadIdx.x & 63);
+    const int32_t lo = max(i - a.left, 0), far = min(a.sinks, lo), n = far + min(i + a.right, s.T - 1) - lo + 1;
+    const float *q = a.q + (uint64_t)(s.r0 + i) * a.qs + s.h * dk;
+    auto frame_of = [&](int32_t k) { return k < far ? k : lo + k - far; };
+    auto score_of = [&](int32_t j) {
+        const float *key = a.k + (uint64_t)(s.r0 + j) * a.ks + s.g * dk;
+        const float *place = a.p + (uint64_t)(uint32_t)max(j - i + a.left, 0) * (a.H * dk) + s.h * dk;
+        double score = 0.0;
+#pragma unroll 1
+        for (int d = 0; d < dk; d += 4) {
+            const v4f x = *(const v4f *)(q + d), k = *(const v4f *)(key + d);
+            v4f u = {}, w = {}, p = {};
+            if constexpr (POS) {
+                u = *(const v4f *)(a.bias_u + s.h * dk + d), w = *(const v4f *)(a.bias_w + s.h * dk + d);
+                p = *(const v4f *)(place + d);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                score = __builtin_fma((double)x[e] + u[e], (double)k[e], score);
+                if constexpr (POS)
+                    score = __builtin_fma((double)x[e] + w[e], (double)p[e], score);
+            }
+        }
+        return score * a.scale;
+    };
+    double top = -INFINITY, sum = 0.0, o[N] = {};
+    bool none = false;                      /* a score is no number: no output is */
+#pragma unroll 1
+    for (int32_t k = 0; k < n && !none; k += 64) {
+        const double score = score_of(frame_of(min(k + lane, n - 1)));
+        none = __any(score != score);
+        top = fmax(top, score);
+    }
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1)
+        top = fmax(top, __shfl_xor(top, m));
+    if (none || __builtin_fabs(top) == INFINITY) {
+#pragma unroll
+        for (int u = 0; u < N; u++)
+            y[u] = !none && top < 0.0 ? 0.0f : __builtin_nanf("");
+        return;
+    }
+    bool all = false;                       /* every output is no number already */
+#pragma unroll 1
+    for (int32_t k = 0; k < n && !all; k += 64) {
+        const double e = k + lane < n ? exp2(score_of(frame_of(min(k + lane, n - 1))) - top) : 0.0;
+        sum += e;
+#pragma unroll 1
+        for (int32_t l = 0; l < 64; l++) {
+            const double weight = __shfl(e, l);
+            if (weight == 0.0)
+                continue;
+            const float *v = a.v + (uint64_t)(s.r0 + frame_of(k + l)) * a.vs + s.g * dk;
+#pragma unroll
+            for (int u = 0; u < N; u++)
+                if (lane + 64 * u < dk)
+                    o[u] = __builtin_fma(weight, (double)v[lane + 64 * u], o[u]);
+        }
+        bool mine = true;
+#pragma unroll
+        for (int u = 0; u < N; u++)
+            mine &= o[u] != o[u] || lane + 64 * u >= dk;
+        all = __all(mine);
+    }
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1)
+        sum += __shfl_xor(sum, m);
+#pragma unroll
+    for (int u = 0; u < N; u++)
+        y[u] = (float)(o[u] / sum);
+}
+
+/* The lowest 16 bits: the queries that any of a wave's lanes, a query each 16 of them, is in. */
+__device__ __forceinline__ uint32_t queries_of(bool mine) {
+    const uint64_t lanes = __ballot(mine);
+    return (uint32_t)(lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xffff;
+}
+
 __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -263,7 +350,7 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowAttention a) {
         begin();
     WindowQueries<NS, POS> q;
     q.load(a, s, i, query[POS ? wave : 0]);
-    float top, sum;
+    float top, sum, odd;                    /* odd: NaN where an output is no number */
     v4f o[2 * NS];
     /* A value that is an infinity or no number gives NaN to every row of the tile, those that do not attend it among them
      * (its product with their 0). So a pass that ends with one is made again with care. */
@@ -364,19 +451,25 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowAttention a) {
                         o[b * S::VW + e] = wmfma(v[r][b][e], prob[0][r], o[b * S::VW + e]);
             load_values(next);
         }
-        float odd = 0.0f;                   /* NaN where an output is no number */
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if constexpr (W == 1) {
+            const float scale = 1.0f / sum;                 /* of no weight at all: the outputs' 0 times an infinity */
+#pragma unroll
+            for (int n = 0; n < 2 * NS; n++)
+                o[n] *= scale;
+        }
+        odd = 0.0f;
 #pragma unroll
         for (int n = 0; n < 2 * NS; n++)
 #pragma unroll
             for (int r = 0; r < 4; r++)
                 odd = __builtin_fmaf(o[n][r], 0.0f, odd);
-        if (careful || !__any(odd != odd))
+        if (careful || !__any(i < s.T && odd != odd))
             break;
         careful = true;
         begin();
     }
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
     /* a lane's outputs: VW dimensions next to each other from 16 VW b + VW (4 w + r) on */
     auto output = [&](int b, int r) {
         typename S::vec y;
@@ -386,17 +479,36 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowAttention a) {
         return y;
     };
     if constexpr (W == 1) {
+        /* outputs that are no number even so: from their row by itself */
+        for (uint32_t rows = queries_of(i < s.T && odd != odd); rows; rows &= rows - 1) {
+            const int32_t r = __builtin_ctz(rows);
+            float y[(NS + 1) / 2];
+            window_row<NS, POS>(a, s, s.i0 + r, y);
+#pragma unroll
+            for (int b = 0; b < S::NB; b++)
+#pragma unroll
+                for (int e = 0; e < S::VW; e++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const float again = __shfl(y[16 * S::VW * b / 64], 16 * S::VW * b % 64 + S::VW * (4 * w + k) + e);
+                        const float mine = o[b * S::VW + e][k];
+                        o[b * S::VW + e][k] = c == r && __builtin_fmaf(mine, 0.0f, 0.0f) != 0.0f ? again : mine;
+                    }
+        }
         if (i >= s.T)
             return;
-        const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
         float *to = a.o + (uint64_t)(s.r0 + i) * a.os + s.h * S::dk + S::VW * 4 * w;
 #pragma unroll
         for (int b = 0; b < S::NB; b++)
 #pragma unroll
             for (int r = 0; r < 4; r++)
-                *(typename S::vec *)(to + 16 * S::VW * b + S::VW * r) = output(b, r) * scale;
+                *(typename S::vec *)(to + 16 * S::VW * b + S::VW * r) = output(b, r);
     } else {
+        constexpr int kEach = (16 * S::dk / 4 + 255) / 256;
         __shared__ float tops[kWaves][16], sums[kWaves][16];
+        __shared__ uint32_t odd_rows;
+        if (threadIdx.x == 0)
+            odd_rows = 0;
         if (w == 0)
             tops[wave][c] = top, sums[wave][c] = sum;
 #pragma unroll
@@ -405,23 +517,62 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowAttention a) {
             for (int r = 0; r < 4; r++)
                 *(typename S::vec *)&rows[wave][c][16 * S::VW * b + S::VW * (4 * w + r)] = output(b, r);
         __syncthreads();
-        for (uint32_t n = threadIdx.x; n < 16 * S::dk / 4; n += 64 * W) {
-            const int32_t r = (int32_t)(n / (S::dk / 4)), d = (int32_t)(n % (S::dk / 4)) * 4;
-            if (s.i0 + r >= s.T)
+        v4f y[kEach];
+#pragma unroll
+        for (int n = 0; n < kEach; n++) {
+            const uint32_t at = threadIdx.x + 256 * n;
+            const int32_t r = (int32_t)(at / (S::dk / 4)), d = (int32_t)(at % (S::dk / 4)) * 4;
+            if (at >= 16 * S::dk / 4 || s.i0 + r >= s.T)
                 continue;
-            float m = -INFINITY, l = 0.0f;
-            v4f y = {};
+            float m = -INFINITY, l = 0.0f, e[W];
 #pragma unroll
             for (int u = 0; u < W; u++)
                 m = fmaxf(m, tops[u][r]);
             const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
             for (int u = 0; u < W; u++) {
-                const float e = __builtin_amdgcn_exp2f(tops[u][r] - base);
-                l += sums[u][r] * e;
-                y += *(const v4f *)&rows[u][r][d] * e;
+                e[u] = __builtin_amdgcn_exp2f(tops[u][r] - base);
+                l += sums[u][r] * e[u];
             }
-            *(v4f *)(a.o + (uint64_t)(s.r0 + s.i0 + r) * a.os + s.h * S::dk + d) = l == 0.0f ? v4f{} : y / l;
+            y[n] = v4f{};
+            const float scale = 1.0f / l;
+#pragma unroll
+            for (int u = 0; u < W; u++)
+                y[n] += *(const v4f *)&rows[u][r][d] * (e[u] * scale);
+            float none = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                none = __builtin_fmaf(y[n][k], 0.0f, none);
+            if (none != none)
+                atomicOr(&odd_rows, 1u << r);
+        }
+        __syncthreads();
+        float *again = (float *)query;
+        static_assert(sizeof query >= 16 * S::dk * sizeof(float), "a tile's rows fit");
+        for (uint32_t of = odd_rows; of; of &= of - 1) {
+            const int32_t r = __builtin_ctz(of);
+            if (r % kWaves != (int32_t)wave)
+                continue;
+            float x[(NS + 1) / 2];
+            window_row<NS, POS>(a, s, s.i0 + r, x);
+#pragma unroll
+            for (int u = 0; u < (NS + 1) / 2; u++)
+                if ((int)lane + 64 * u < S::dk)
+                    again[r * S::dk + (int)lane + 64 * u] = x[u];
+        }
+        if (odd_rows)
+            __syncthreads();
+#pragma unroll
+        for (int n = 0; n < kEach; n++) {
+            const uint32_t at = threadIdx.x + 256 * n;
+            const int32_t r = (int32_t)(at / (S::dk / 4)), d = (int32_t)(at % (S::dk / 4)) * 4;
+            if (at >= 16 * S::dk / 4 || s.i0 + r >= s.T)
+                continue;
+            if (odd_rows >> r & 1)
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    y[n][k] = __builtin_fmaf(y[n][k], 0.0f, 0.0f) != 0.0f ? again[r * S::dk + d + k] : y[n][k];
+            *(v4f *)(a.o + (uint64_t)(s.r0 + s.i0 + r) * a.os + s.h * S::dk + d) = y[n];
         }
     }
 }
@@ -491,7 +642,7 @@ __global__ __launch_bounds__(256, 2) void window_many_kernel(WindowAttention a) 
             z[e] = __builtin_fabsf(z[e]) < kMostQuery ? z[e] : __builtin_nanf("");
         q[t] = cut_near(z);
     }
-    float top, sum;
+    float top, sum, odd;                    /* odd: NaN where an output is no number */
     v4f o[2 * NS];
 
     /* the window's frames [lo, hi] of any of the rows, the sinks [0, far) before them, the steps of both */
@@ -599,26 +750,33 @@ __global__ __launch_bounds__(256, 2) void window_many_kernel(WindowAttention a) 
     /* Scores that are no number are made again from the floats themselves: an infinite key has pieces that are none, and
      * its score may be -infinity. */
     auto score_again = [&](int32_t j0, v4f (&x)[2]) {
-        bool none = false;
+        uint32_t none = 0;
 #pragma unroll
         for (int n = 0; n < 8; n++)
-            none |= x[n / 4][n % 4] != x[n / 4][n % 4];
+            none |= x[n / 4][n % 4] != x[n / 4][n % 4] ? 1u << n : 0;
         if (!__any(none))
             return;
 #pragma unroll 1
         for (int32_t k = 0; k < 32 && j0 + k < s.T; k++) {
+            const int32_t at = k / 16 * 4 + k % 4;
+            const bool mine = w == k / 4 % 4 && (none >> at & 1);
+            if (!__any(mine))
+                continue;
             const float *key = a.k + (uint64_t)(s.r0 + j0 + k) * a.ks + s.g * dk + 8 * w;
             float score = 0.0f;
 #pragma unroll 1
-            for (int t = 0; t < 8 * NS; t++)
-                score = __builtin_fmaf(query[32 * (t / 8) + t % 8] * a.scale, key[32 * (t / 8) + t % 8], score);
+            for (int t = 0; t < 2 * NS; t++) {
+                const v4f y = *(const v4f *)(query + 32 * (t / 2) + t % 2 * 4) * a.scale;
+                const v4f z = *(const v4f *)(key + 32 * (t / 2) + t % 2 * 4);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    score = __builtin_fmaf(y[e], z[e], score);
+            }
             score += __shfl_xor(score, 16);
             score += __shfl_xor(score, 32);
 #pragma unroll
-            for (int n = 0; n < 8; n++) {
-                const float mine = x[n / 4][n % 4];
-                x[n / 4][n % 4] = mine != mine && k == 16 * (n / 4) + 4 * w + n % 4 ? score : mine;
-            }
+            for (int n = 0; n < 8; n++)
+                x[n / 4][n % 4] = mine && n == at ? score : x[n / 4][n % 4];
         }
     };
     if (threadIdx.x == 0)
@@ -694,29 +852,46 @@ __global__ __launch_bounds__(256, 2) void window_many_kernel(WindowAttention a) 
         }
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
+        const float scale = 1.0f / sum;                     /* of no weight at all: the outputs' 0 times an infinity */
+        odd = 0.0f;
+#pragma unroll
+        for (int n = 0; n < 2 * NS; n++) {
+            o[n] *= scale;
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                odd = __builtin_fmaf(o[n][r], 0.0f, odd);
+        }
     };
     pass(std::false_type());
-    /* An infinity or a NaN among the outputs or in a sum: once more then, with care. */
-    float odd = sum;
-#pragma unroll
-    for (int n = 0; n < 2 * NS; n++)
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-            odd = __builtin_fmaf(o[n][r], 0.0f, odd);
+    /* An infinity or a NaN among the outputs: once more then, with care, and what is none even so from its row by itself. */
     if (i < s.T && odd != odd)
         again = 1;
     __syncthreads();
-    if (__builtin_expect(again, 0))
+    if (__builtin_expect(again, 0)) {
         pass(std::true_type());
+        for (uint32_t rows = queries_of(i < s.T && odd != odd); rows; rows &= rows - 1) {
+            const int32_t row = __builtin_ctz(rows);
+            float y[(NS + 1) / 2];
+            window_row<NS, false>(a, s, iw + row, y);
+#pragma unroll
+            for (int b = 0; b < NS; b++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int d = 0; d < 2; d++) {
+                        const float y1 = __shfl(y[b / 2], 32 * (b % 2) + 8 * w + 2 * r + d), mine = o[2 * b + d][r];
+                        o[2 * b + d][r] = c == row && __builtin_fmaf(mine, 0.0f, 0.0f) != 0.0f ? y1 : mine;
+                    }
+        }
+    }
     if (i >= s.T)
         return;
-    const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
     float *to = a.o + (uint64_t)(s.r0 + i) * a.os + s.h * dk + 8 * w;
 #pragma unroll
     for (int b = 0; b < NS; b++)
 #pragma unroll
         for (int r = 0; r < 4; r += 2)
-            *(v4f *)(to + 32 * b + 2 * r) = v4f{ o[2 * b][r], o[2 * b + 1][r], o[2 * b][r + 1], o[2 * b + 1][r + 1] } * scale;
+            *(v4f *)(to + 32 * b + 2 * r) = v4f{ o[2 * b][r], o[2 * b + 1][r], o[2 * b][r + 1], o[2 * b + 1][r + 1] };
 }
 
 /* ------------------------------------------------------------- launches --- */

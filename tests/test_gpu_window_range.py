@@ -83,3 +83,73 @@ def test_small_queries_great_keys(hip, torch, T, H, dk, with_positions, small, g
     got = c.attend(pos, left, right, sinks)
     rows = [0, 1, 30, 59, 60, 77, 100, T - 2, T - 1]
     near(got[rows], *want(c, rows, pos, left, right, sinks))
+
+
+def great(c, dims, ceiling):
+    """Values up to the type's greatest in some dimensions of each head; scores that rise by 7.8 powers of two from one 16
+    frames to the next, so sums of weights are far over what they are to the greatest score."""
+    d = np.arange(c.H) * c.dk
+    c.k[:, d + 9] = (7.8 * np.log(2) * (np.arange(c.rows) // 16 % 2))[:, None]
+    c.q[:, d + 9] = np.sqrt(c.dk)
+    sign = np.where(c.g.random((c.rows, c.H)) < 0.5, -1, 1)
+    for n, x in zip(dims, (ceiling, ceiling * sign, ceiling * (2 * c.g.random((c.rows, c.H)) - 1),
+                           np.where(np.arange(c.rows)[:, None] == 60, ceiling, 1.0))):
+        c.v[:, d + n] = np.broadcast_to(x, (c.rows, c.H)).astype(np.float32)
+
+
+@pytest.mark.parametrize("T,H", [FEW, MANY])
+@pytest.mark.parametrize("dk", DKS)
+@pytest.mark.parametrize("with_positions", [False, True])
+@pytest.mark.parametrize("ceiling", [1e30, 1e34, 1e36, float(F32.max)])
+def test_great_values(hip, torch, T, H, dk, with_positions, ceiling):
+    """Outputs that floats hold, of sums that they do not: the other dimensions keep their bits."""
+    say("great", T, H, dk, with_positions, ceiling)
+    c = Call(hip, torch, [T, 50], H, H, dk, seed=dk)
+    left, right, sinks = 70, 33, 2
+    pos = c.positions(left, right) if with_positions else None
+    dims = (0, 7, dk // 2 + 1, dk - 1)
+    great(c, dims, 1.0)
+    clean = c.attend(pos, left, right, sinks)
+    c.g = np.random.default_rng(7)
+    great(c, dims, ceiling)
+    got = c.attend(pos, left, right, sinks)
+    other = np.setdiff1d(np.arange(H * dk), (np.arange(H)[:, None] * dk + np.array(dims)).ravel())
+    assert np.array_equal(got[:, other], clean[:, other])
+    rows = [0, 1, 15, 16, 30, 59, 60, 77, 100, T - 40, T - 2, T - 1]
+    near(got[rows], *want(c, rows, pos, left, right, sinks))
+
+
+@pytest.mark.parametrize("T,H", [FEW, MANY])
+@pytest.mark.parametrize("with_positions", [False, True])
+def test_great_values_in_place(hip, torch, T, H, with_positions):
+    """The same with the output over the queries, which the rows made again still need."""
+    say("great in place", T, H, with_positions)
+    c = Call(hip, torch, [T, 50], H, H, 64, seed=3)
+    pos = c.positions(70, 33) if with_positions else None
+    great(c, (0, 7, 33, 63), float(F32.max))
+    expected = c.attend(pos, 70, 33, 2)
+    q, k, v = c.dev(c.q), c.dev(c.k), c.dev(c.v)
+    at = None if pos is None else (c.dev(pos[0]), pos[1], c.dev(pos[2]), c.dev(pos[3]))
+    hip.attention_window_dev(q, q, k, v, hip.Segments(c.dev(c.row0), c.rows, c.max_T), H, 64, at, 70, 33, 2)
+    torch.cuda.synchronize()
+    assert np.isfinite(expected).all() and np.array_equal(q.cpu().numpy(), expected)
+
+
+@pytest.mark.parametrize("T,H", [FEW, MANY])
+@pytest.mark.parametrize("dk", DKS)
+@pytest.mark.parametrize("with_positions", [False, True])
+def test_scores_that_are_no_floats(hip, torch, T, H, dk, with_positions):
+    """Rows all of whose scores are under the type's lowest are the softmax of them all the same, the value of the frame
+    that is far over the others; rows all of whose scores are -infinity are 0."""
+    say("no floats", T, H, dk, with_positions)
+    c = Call(hip, torch, [T, 50], H, H, dk, seed=dk)
+    left, right, sinks = 20, 3, 2
+    pos = c.positions(left, right) if with_positions else None
+    at = np.arange(H) * dk + 5
+    c.q[30:34, at], c.q[70:72, at] = 1e38, 1.0
+    c.k[:, at] = np.float32(-1e20) * np.arange(1, c.rows + 1, dtype=np.float32)[:, None]
+    got = c.attend(pos, left, right, sinks)
+    assert (got[30:34] == c.v[0]).all()
+    c.k[np.ix_([0, 1, *range(70 - left, 72 + right)], at)] = -np.inf
+    got = c.attend(pos, left, right, sinks)
+    assert (got[70:72] == 0).all()
