@@ -563,7 +563,7 @@ int pk_hip_pool_restore(pk_hip_pool *pool, const int32_t *pairs, uint32_t n);
  * outputs depend on the frames that it attends alone, whatever the others hold.
  * Frames whose score is -infinity have no part, and a row without others is 0.
  * Outputs whose sums or scores pass the greatest float on their way (values from
- * some 10^30 on) are right as well, each such row made by itself in 64 bits: a
+ * some 10^28 on) are right as well, each such row made by itself in 64 bits: a
  * call full of them takes about fifty times as long.
  *
  * The segments of a call: row0 [B + 1] in device memory, read when the kernel

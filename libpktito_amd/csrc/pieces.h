@@ -22,7 +22,7 @@ struct Pieces {
 /* Floats cut for a product of floats with floats: each piece the nearest
  * bfloat16 of what the ones before leave, so that the second is at most 2^-8
  * of the float's power of two, the third 2^-17, and the three sum to it exactly
- * (down to 2^-126, where pieces end). Of the nine products of two floats'
+ * (down to 2^-133, the smallest bfloat16). Of the nine products of two floats'
  * pieces the six largest are taken: those left out are 2^-24 of the product at
  * most, as much as a 32-bit product's own rounding. Whatever the other
  * dimensions hold: a row has no exponent in common. */

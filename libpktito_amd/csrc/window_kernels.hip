@@ -582,11 +582,15 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowAttention a) {
 constexpr float kNoPieces = 0x1.ffp127f;
 
 /* Keys are cut at 2^-40 of what they are and queries at 2^40 of it: every finite
- * key has pieces then, and what pieces end at, 2^-126, is 2^-162 of a query and
- * 2^-86 of a key. Against the greatest key that is 2^-34 of a score, and against
- * queries under this bound 2^-36. Queries from it on are taken as no number, which
+ * key has pieces then, and what pieces end at, 2^-133, is 2^-173 of a query and
+ * 2^-93 of a key. Against the greatest key that is 2^-45 of a score, and against
+ * queries under this bound 2^-43. Queries from it on are taken as no number, which
  * gives each of their scores the care below. */
 constexpr float kKeyScale = 0x1p-40f, kQueryScale = 0x1p40f, kMostQuery = 0x1p90f;
+
+/* Values are cut at 2^16 of what they are: the last bit of the smallest, 2^-149,
+ * is then a bfloat16's 2^-133. */
+constexpr float kValueScale = 0x1p16f;
 
 /* The six products of pieces that count, the smallest first. */
 __device__ __forceinline__ v4f product(const Pieces &x, const Pieces &y, v4f acc) {
@@ -699,7 +703,10 @@ __global__ __launch_bounds__(256, 2) void window_many_kernel(WindowAttention a) 
         if (wave < NS)
 #pragma unroll
             for (int d = 0; d < 2; d++) {
-                const float z[8] = { raw_v[0][d], raw_v[1][d], raw_v[2][d], raw_v[3][d], raw_v[4][d], raw_v[5][d], raw_v[6][d], raw_v[7][d] };
+                float z[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    z[k] = raw_v[k][d] * kValueScale;
                 const Pieces y = cut_near(z);
 #pragma unroll
                 for (int k = 0; k < 3; k++)
@@ -714,7 +721,7 @@ __global__ __launch_bounds__(256, 2) void window_many_kernel(WindowAttention a) 
         for (int k = 0; k < 8; k++)
 #pragma unroll
             for (int d = 0; d < 2; d++) {
-                const bool has = __builtin_fabsf(raw_v[k][d]) < kNoPieces;
+                const bool has = __builtin_fabsf(raw_v[k][d] * kValueScale) < kNoPieces;
                 odd |= !has;
                 raw_v[k][d] = has ? raw_v[k][d] : 0.0f;
             }
@@ -741,7 +748,7 @@ __global__ __launch_bounds__(256, 2) void window_many_kernel(WindowAttention a) 
                     for (int r = 0; r < 4; r++)
 #pragma unroll
                         for (int d = 0; d < 2; d++) {
-                            const float y = src[32 * b + 2 * r + d];
+                            const float y = src[32 * b + 2 * r + d] * kValueScale;
                             if (!(__builtin_fabsf(y) < kNoPieces))
                                 o[2 * b + d][r] += mine * y;
                         }
@@ -852,7 +859,7 @@ __global__ __launch_bounds__(256, 2) void window_many_kernel(WindowAttention a) 
         }
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
-        const float scale = 1.0f / sum;                     /* of no weight at all: the outputs' 0 times an infinity */
+        const float scale = 1.0f / sum * (1.0f / kValueScale);      /* of no weight at all: the outputs' 0 times an infinity */
         odd = 0.0f;
 #pragma unroll
         for (int n = 0; n < 2 * NS; n++) {

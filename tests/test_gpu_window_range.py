@@ -153,3 +153,23 @@ def test_scores_that_are_no_floats(hip, torch, T, H, dk, with_positions):
     c.k[np.ix_([0, 1, *range(70 - left, 72 + right)], at)] = -np.inf
     got = c.attend(pos, left, right, sinks)
     assert (got[70:72] == 0).all()
+
+
+@pytest.mark.parametrize("T,H", [FEW, MANY])
+@pytest.mark.parametrize("dk", DKS)
+@pytest.mark.parametrize("with_positions", [False, True])
+@pytest.mark.parametrize("size", [1e-24, 1e-30, 1e-33, 1e-36, 2.0 ** -125])
+def test_small_values(hip, torch, T, H, dk, with_positions, size):
+    """Values that keep the bits of 32 however small they are, and those of dimensions small beside others."""
+    say("small", T, H, dk, with_positions, size)
+    c = Call(hip, torch, [T, 50], H, H, dk, seed=dk)
+    left, right, sinks = 20, 3, 2
+    pos = c.positions(left, right) if with_positions else None
+    c.v *= np.float32(size)
+    c.v[:, 4::9] *= np.float32(1e20)
+    got = c.attend(pos, left, right, sinks)
+    rows = [0, 1, 30, 59, 60, 77, 100, T - 2, T - 1]
+    ref, bound = want(c, rows, pos, left, right, sinks)
+    # the model's bound has 1e-37 for what ends at 2^-126: here a product or a sum of the 26 that is rounded at 2^-149, and
+    # as many times that again by the weights of up to 2^8 and their sum
+    near(got[rows], ref, bound - 1e-37 + 64 * 2.0 ** -149)
