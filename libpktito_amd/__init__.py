@@ -871,16 +871,19 @@ class DeviceCache:
             pos = Positions(16, 16, 16, 0xffffffff, 0x7fffffff)
         else:
             pos = self._positions(positions or None, H)
-        return lib().pk_hip_attention_sinks_workspace(ctypes.byref(self.st), ctypes.byref(streams.st), _u32(H, "H"),
-                                                      ctypes.byref(pos) if pos else None, _reach(left, "left"),
-                                                      _reach(right, "right"), _u32(sinks, "sinks"))
+        args = (ctypes.byref(self.st), ctypes.byref(streams.st), _u32(H, "H"), ctypes.byref(pos) if pos else None,
+                _reach(left, "left"), _reach(right, "right"))
+        if _u32(sinks, "sinks"):
+            return lib().pk_hip_attention_sinks_workspace(*args, sinks)
+        return lib().pk_hip_attention_cache_workspace(*args)
 
     def _positions(self, positions, H):
         return _positions(positions, H, self.dk, self.device)
 
     def attention(self, o, layer, q, streams, H, ws, positions=None, left=None, right=None, stream=None, sinks=0):
         """The attention of the rows q [rows, H * dk] to their streams' kept
-        frames, into o (pk_hip_attention_sinks_dev); ws a uint8 tensor of
+        frames, into o (pk_hip_attention_cache_dev, with sinks
+        pk_hip_attention_sinks_dev); ws a uint8 tensor of
         attention_workspace(...) bytes, positions (p [n, H * dk], center,
         bias_u, bias_w) or None, left and right the frames attended behind and
         ahead (None: all), sinks the first frames that stay visible."""
@@ -890,13 +893,14 @@ class DeviceCache:
             _is(ws, "uint8", "ws", self.device)
             if not ws.is_contiguous():                   # an expanded one has fewer bytes than elements
                 raise PkHipError(PK_HIP_EINVAL, "ws is not contiguous")
-        _check(lib().pk_hip_attention_sinks_dev(*_rows(o, n, w, "o", self.device), *_rows(q, n, w, "q", self.device),
-                                                ctypes.byref(self.st),
-                                                _u32(layer, "layer"), ctypes.byref(streams.st), _u32(H, "H"),
-                                                ctypes.byref(pos) if pos else None,
-                                                _reach(left, "left"), _reach(right, "right"), _u32(sinks, "sinks"),
-                                                _dptr(ws), ws.numel() if ws is not None else 0,
-                                                self._queue(stream, streams)))
+        args = (*_rows(o, n, w, "o", self.device), *_rows(q, n, w, "q", self.device), ctypes.byref(self.st),
+                _u32(layer, "layer"), ctypes.byref(streams.st), _u32(H, "H"), ctypes.byref(pos) if pos else None,
+                _reach(left, "left"), _reach(right, "right"))
+        space = (_dptr(ws), ws.numel() if ws is not None else 0, self._queue(stream, streams))
+        if _u32(sinks, "sinks"):
+            _check(lib().pk_hip_attention_sinks_dev(*args, sinks, *space))
+        else:
+            _check(lib().pk_hip_attention_cache_dev(*args, *space))
 
     def move(self, pairs, table=None, source=None, stream=None):
         """Copies pages in every layer: pairs [(from, to), ...], from a page of
