@@ -557,7 +557,9 @@ int pk_hip_pool_restore(pk_hip_pool *pool, const int32_t *pairs, uint32_t n);
  * kept head shared among H / G consecutive ones), dk 32, 64, 96 or 128; row r
  * of x at x + r * its stride (qs, ks, vs, os), 16-byte aligned, strides
  * multiples of 4, ks and vs up to 2^25. o may be q with os = qs; an o that shares memory with k, v or
- * the positions is refused. Rows of no segment are left as they were. Products
+ * the positions is refused (rows of one stride may lie between each other's; of
+ * different strides they count as sharing memory wherever their ranges
+ * overlap). Rows of no segment are left as they were. Products
  * and sums in 32 bits, not held to a bit pattern (pk_hip_attention_dev's are
  * the reference's, core/encoder.c:280-327, which has no window). A row's
  * outputs depend on the frames that it attends alone, whatever the others hold.
@@ -652,8 +654,9 @@ int pk_hip_cache_plan_dev(const pk_hip_plan *p, const int32_t *add, const int32_
  * keeps its small log probability. A logit may be -infinity (probability 0, log
  * probability -infinity); in a row with a NaN, with an infinity, or with nothing
  * but -infinity every probability and the entropy are NaN, and the order is the
- * logits' all the same. Outputs that share memory with the logits or the tokens
- * are refused. cols 1 to 2^20, k up to 32 and up to cols, rows up to 2^21 and
+ * logits' all the same. Outputs that share memory with the logits, the tokens
+ * or each other are refused (seen as in pk_hip_attention_window_dev: an output
+ * between the rows of logits is taken only with their stride). cols 1 to 2^20, k up to 32 and up to cols, rows up to 2^21 and
  * under 2^24 with a row's every 8192 columns counted. ws:
  * pk_hip_logprobs_workspace(rows, cols, k) bytes of device memory (0 for up to
  * 8192 columns), 16-byte aligned, of no matter before and after; calls that
