@@ -173,3 +173,40 @@ def test_small_values(hip, torch, T, H, dk, with_positions, size):
     # the model's bound has 1e-37 for what ends at 2^-126: here a product or a sum of the 26 that is rounded at 2^-149, and
     # as many times that again by the weights of up to 2^8 and their sum
     near(got[rows], ref, bound - 1e-37 + 64 * 2.0 ** -149)
+
+
+@pytest.mark.parametrize("dk", [64, 128])
+@pytest.mark.parametrize("kind", ["content", "content, great", "places, great"])
+def test_two_streams_and_a_graph(hip, torch, dk, kind):
+    """Calls of many tiles give the same bits on two streams at once, captured and replayed: without positions, and with
+    values whose rows are made again."""
+    say("streams", dk, kind)
+    H = 4
+    c = Call(hip, torch, [3001, 700, 1, 5100], H, H, dk, seed=24)
+    pos = c.positions(60, 10) if "places" in kind else None
+    if "great" in kind:
+        c.v[1000:1100, ::7], c.v[20, 3] = 1e38, np.nan
+    want_ = c.attend(pos, 60, 10, 4)
+    d = [c.dev(x) for x in (c.q, c.k, c.v)]
+    p = None if pos is None else (c.dev(pos[0]), pos[1], c.dev(pos[2]), c.dev(pos[3]))
+    sg = hip.Segments(c.dev(c.row0), c.rows, c.max_T)
+    o = [torch.zeros_like(d[0]) for _ in range(3)]
+    ss = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i, s in enumerate(ss):
+            with torch.cuda.stream(s):
+                hip.attention_window_dev(o[i], *d, sg, H, dk, p, 60, 10, 4)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        hip.attention_window_dev(o[2], *d, sg, H, dk, p, 60, 10, 4)
+    same = lambda x: np.array_equal(x.cpu().numpy(), want_, equal_nan=True)
+    for _ in range(3):
+        o[2].zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same(o[2])
+        (torch.randn(256, 256, device="cuda") @ torch.randn(256, 256, device="cuda")).sum().item()
+    assert all(same(x) for x in o[:2])
+    assert np.isfinite(want_).all() == (kind == "content")
