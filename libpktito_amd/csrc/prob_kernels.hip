@@ -274,7 +274,8 @@ __device__ __forceinline__ Spread joined_spread(Spread s, uint64_t key, bool liv
 
 /* Rows of up to 2048 columns, 256 V + 64 S of them: a wave each. 45000 rows of
  * 1025 with 8 alternatives, 187 MB: 46 us, 4.1 TB/s of the 6.8 that reads reach;
- * instructions bound it (about 450 a row and wave). 60 with 20 values a lane and
+ * instructions bound it (587 vector and 248 scalar ones a row and wave: all of the
+ * cycles). 60 with 20 values a lane and
  * the ties' keys in registers; 68 with a wave's next row loaded under this one's
  * results (92 registers for 28, five waves a SIMD for eight); 113 with one
  * alternative after another out of all values. */

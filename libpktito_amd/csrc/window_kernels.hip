@@ -244,8 +244,8 @@ __device__ __forceinline__ void wave_sync() {
  * than its scores', so they pass through LDS.
  *
  * An hour (45000 frames, 8 heads of 128, 128 + 128 + 1 frames and 16 sinks, 75.6
- * GFLOP): 797 us, 95 TFLOP/s of the 154 that an fp32 product reaches. The matrix
- * instructions are busy 64% of it, two waves a SIMD or one (4900 and 5400 clocks a
+ * GFLOP): 799 us, 95 TFLOP/s of the 154 that an fp32 product reaches. The matrix
+ * instructions are busy 65% of it, two waves a SIMD or one (4900 and 5400 clocks a
  * step, of which 3100 are theirs). What holds them up is the loads, 24 a step whose
  * results pass into registers: without them the same products take 630; without
  * masks, places' skew and exponentials 765. Keys by lanes that use them took 910 (53
@@ -617,9 +617,9 @@ __device__ __forceinline__ v4f product(const Pieces &x, const Pieces &y, v4f acc
  * whose rows are dimensions 32 b + 2 (l % 16) + d of instruction (b, d).
  *
  * Four segments of 2001 to 3000 frames, 16 heads of 64 to 4 kept ones, 512 frames
- * and 8 sinks, 19.6 GFLOP: 155 us, 126 TFLOP/s (220 with fp32 instructions); with
- * 2000 frames 152, the fp32 instructions' peak. Two products' chains side by side
- * were no faster. */
+ * and 8 sinks, 19.6 GFLOP: 150 to 156 us by the machine, 126 to 131 TFLOP/s (220 us
+ * with fp32 instructions); with 2000 frames 390 us, 131 TFLOP/s. Two products' chains
+ * side by side were no faster. */
 template <int NS>
 __global__ __launch_bounds__(256, 2) void window_many_kernel(WindowAttention a) {
     constexpr int dk = 32 * NS, kChunks = 4 * NS;
