@@ -327,7 +327,9 @@ __device__ __forceinline__ uint64_t unit_of(const CacheAttention &a, uint32_t b,
 
 /* Sixteen rows of the positions' table for one head as the matrix
  * instruction's operand: lane l has dimensions 32 s + 8 (l / 16) of row l % 16
- * in step s. */
+ * in step s. Cut at half of what they are and multiplied by twice the queries: the
+ * greatest floats themselves round to a bfloat16 infinity, which has no other
+ * pieces. */
 template <int NS>
 struct PlaceTile {
     v4f p[NS][2];
@@ -343,7 +345,8 @@ struct PlaceTile {
     __device__ __forceinline__ void pieces(Pieces (&out)[NS]) const {
 #pragma unroll
         for (int s = 0; s < NS; s++) {
-            const float x[8] = { p[s][0][0], p[s][0][1], p[s][0][2], p[s][0][3], p[s][1][0], p[s][1][1], p[s][1][2], p[s][1][3] };
+            const v4f u = p[s][0] * 0.5f, v = p[s][1] * 0.5f;
+            const float x[8] = { u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3] };
             out[s] = cut_near(x);
         }
     }
@@ -445,7 +448,7 @@ __global__ __launch_bounds__(64 * kPlaceWaves, place_residency(MT)) void cache_p
     lo = -wave_max(-lo), hi = wave_max(hi);
     if (lane == 0)
         need[wave][0] = lo, need[wave][1] = hi;
-    const float c2 = a.scale * 1.44269504088896340736f;     /* scores in powers of 2 */
+    const float c2 = 2.0f * (a.scale * 1.44269504088896340736f);        /* scores in powers of 2; the table's rows are halves */
 #pragma unroll
     for (int i = 0; i < kFill; i++) {
         const uint32_t row = row_a + 4 * W * i;
