@@ -210,3 +210,25 @@ def test_two_streams_and_a_graph(hip, torch, dk, kind):
         (torch.randn(256, 256, device="cuda") @ torch.randn(256, 256, device="cuda")).sum().item()
     assert all(same(x) for x in o[:2])
     assert np.isfinite(want_).all() == (kind == "content")
+
+
+@pytest.mark.parametrize("T,H", [FEW, MANY])
+@pytest.mark.parametrize("dk", DKS)
+@pytest.mark.parametrize("with_positions", [False, True])
+@pytest.mark.parametrize("span", [100, 45])
+def test_any_magnitudes(hip, torch, T, H, dk, with_positions, span):
+    """Each dimension of queries, and against it of keys and positions, and of values at a power of two of its own."""
+    say("any magnitudes", T, H, dk, with_positions, span)
+    c = Call(hip, torch, [T, 50], H, H, dk, seed=span)
+    left, right, sinks = 25, 6, 3
+    e = np.float32(2.0) ** c.g.integers(-span, span + 1, H * dk).astype(np.float32)
+    f = np.float32(2.0) ** c.g.integers(-110, 111, H * dk).astype(np.float32)
+    c.q, c.k, c.v = c.q * e, c.k / e, c.v * f
+    pos = None
+    if with_positions:
+        p, center, u, w = c.positions(left, right)
+        pos = (p / e, center, u * e, w * e)
+    got = c.attend(pos, left, right, sinks)
+    rows = [0, 1, 30, 59, 60, 77, 100, T - 2, T - 1]
+    ref, bound = want(c, rows, pos, left, right, sinks)
+    near(got[rows], ref, bound - 1e-37 + 64 * 2.0 ** -149)
